@@ -130,6 +130,65 @@ int ixa_op_topk_ivfpq_l3(const int64_t *in_labels_dev, const float *in_values_de
                          int k, int asc, float *out_values_dev, int64_t *out_labels_dev, void *stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Low-precision operators: what an embedding model answers with becomes codes of 8 or 4 bits with scales (alone,
+ * or as the model's last step behind a residual addition and a root-mean-square norm), is read back, and is scored
+ * against a 4-bit store on the matrix cores.  No counterpart in the reference, whose int8 indexes take vectors that
+ * somebody else has quantised.  As the stage operators above: plain DEVICE pointers, nothing allocated, work only
+ * queued on `stream`.  n = 0 (m = 0) is allowed and queues nothing.  Dimensions 1 ... 16384, rows < 2^31; `ld` is the
+ * distance of two rows in elements (>= the row's length); rows of any alignment are accepted, rows that all start on
+ * 16 bytes are read in wide loads.  Codes start on 16 bytes and rows of codes follow each other without gaps.
+ * ------------------------------------------------------------------------------------------- */
+
+/* element types of float rows, weights and results */
+#define IXA_TYPE_F32 0
+#define IXA_TYPE_F16 1
+#define IXA_TYPE_BF16 2
+
+/* Code formats.
+ * IXA_FORMAT_INT8: d bytes per row and ONE FP32 SCALE per row: value = code * scale, scale = max|x| / 127, codes rounded to
+ *   nearest, halfway to even.  A row with an infinity or a NaN: scale NaN, codes 0.  With a fixed scale (one for all rows, as
+ *   AscendIndexInt8Flat needs them to be comparable) codes are clamped to +-127 and a NaN becomes 0.
+ * IXA_FORMAT_MXFP8 / IXA_FORMAT_MXFP4 (the microscaled formats of the Open Compute Project): blocks of 32 consecutive
+ *   elements of a row, ceil(d / 32) blocks per row, one byte of scale per block: value = number * 2^(byte - 127).  Numbers are
+ *   E4M3 in 32 bytes per block or E2M1 in 16 (element 2 i in the lower half of byte i).  byte = clamp(floor(log2 max|x|) - t +
+ *   127, 0, 254) with t = 8 (E4M3) or 2 (E2M1); numbers are rounded to nearest, halfway to even, and end at 448 or 6.  Elements
+ *   behind the last column are written as 0.  A block with an infinity or a NaN: byte 255 (NaN), numbers 0. */
+#define IXA_FORMAT_INT8 0
+#define IXA_FORMAT_MXFP8 1
+#define IXA_FORMAT_MXFP4 2
+
+/* Bytes of one row's codes, and how many scales it has (fp32 for int8, bytes for the others).  Either may be NULL.  Host
+ * code; touches no GPU. */
+int ixa_code_bytes(int format, int d, int64_t *bytes_per_row, int64_t *scales_per_row);
+
+/* Rows x [n][ld] become codes [n][bytes_per_row] and scales [n][scales_per_row].  fixed_scale: 0, or for int8 the scale of all
+ * rows (1e-30 ... 1e30; scales may then be NULL).  sqr_sum [n] (may be NULL): squared norms of the values the codes stand for,
+ * as ixa_op_mx_product takes them. */
+int ixa_op_quantise(const void *x_dev, int64_t ld, int type, int64_t n, int d, int format, float fixed_scale,
+                    uint8_t *codes_dev, void *scales_dev, float *sqr_sum_dev, void *stream);
+
+/* The values that codes and scales stand for, rounded to `type`, in rows out [n][ld]; a NaN scale gives NaN. */
+int ixa_op_dequantise(const uint8_t *codes_dev, const void *scales_dev, int format, int64_t n, int d, int type,
+                      void *out_dev, int64_t ld, void *stream);
+
+/* h = x + residual (residual may be NULL) is written to sum (may be NULL, may be x or residual themselves) rounded to `type`;
+ * y = h / sqrt(mean(h^2) + eps) * weight (weight [d] may be NULL) becomes codes and scales as above.  x, residual, weight and
+ * sum are all of `type`; the arithmetic is fp32 and y is made from the unrounded h.  eps > 0. */
+int ixa_op_rms_norm_quantise(const void *x_dev, int64_t ld_x, const void *residual_dev, int64_t ld_residual,
+                             const void *weight_dev, int type, int64_t n, int d, float eps, void *sum_dev, int64_t ld_sum,
+                             int format, float fixed_scale, uint8_t *codes_dev, void *scales_dev, float *sqr_sum_dev,
+                             void *stream);
+
+/* Scores of m rows a (a_format IXA_FORMAT_MXFP8 or IXA_FORMAT_MXFP4) against n rows b (IXA_FORMAT_MXFP4), all of d dimensions:
+ * out [m][ld] of out_type = inner products g, or for IXA_METRIC_L2 (a_sqr_sum + b_sqr_sum) - g - g (both norms needed;
+ * ignored for the inner product).  Sums are held in fp32.  A NaN scale makes every score of its row NaN.  fp32 scores are what
+ * ixa_op_topk_flat_fp32 selects from. */
+int ixa_op_mx_product(const uint8_t *a_codes_dev, const uint8_t *a_scales_dev, int a_format, int64_t m,
+                      const uint8_t *b_codes_dev, const uint8_t *b_scales_dev, int64_t n, int d, int metric,
+                      const float *a_sqr_sum_dev, const float *b_sqr_sum_dev, int out_type, void *out_dev, int64_t ld,
+                      void *stream);
+
+/* ---------------------------------------------------------------------------------------------
  * IVFPQ
  * ------------------------------------------------------------------------------------------- */
 

@@ -14,6 +14,7 @@
 
 #include "flat_index.h"
 #include "ivfpq_index.h"
+#include "lowp.h"
 #include "ops.h"
 #include "scan.h"
 
@@ -655,6 +656,55 @@ IXA_EXPORT int ixa_op_topk_ivfpq_l3(const int64_t *in_labels_dev, const float *i
     return guarded([&] {
         ixa::op_topk_ivfpq_l3(in_labels_dev, in_values_dev, tiles, batch, list_k, k, asc, out_values_dev, out_labels_dev,
                               static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_code_bytes(int format, int d, int64_t *bytes_per_row, int64_t *scales_per_row)
+{
+    return guarded([&] {
+        IXA_REQUIRE(format >= ixa::kFormatInt8 && format <= ixa::kFormatMxFp4 && d >= 1 && d <= ixa::kMaxCodeDim,
+                    ixa::kErrInvalidParam, "code_bytes: unsupported code format %d or dims %d (1 ... %d)", format, d,
+                    ixa::kMaxCodeDim);
+        if (bytes_per_row) {
+            *bytes_per_row = ixa::code_bytes(format, d);
+        }
+        if (scales_per_row) {
+            *scales_per_row = format == ixa::kFormatInt8 ? 1 : ixa::mx_blocks(d);
+        }
+    }, false);
+}
+IXA_EXPORT int ixa_op_quantise(const void *x_dev, int64_t ld, int type, int64_t n, int d, int format, float fixed_scale,
+                               uint8_t *codes_dev, void *scales_dev, float *sqr_sum_dev, void *stream)
+{
+    return guarded([&] {
+        ixa::op_quantise(x_dev, ld, type, n, d, format, fixed_scale, codes_dev, scales_dev, sqr_sum_dev,
+                         static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_op_dequantise(const uint8_t *codes_dev, const void *scales_dev, int format, int64_t n, int d, int type,
+                                 void *out_dev, int64_t ld, void *stream)
+{
+    return guarded([&] {
+        ixa::op_dequantise(codes_dev, scales_dev, format, n, d, type, out_dev, ld, static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_op_rms_norm_quantise(const void *x_dev, int64_t ld_x, const void *residual_dev, int64_t ld_residual,
+                                        const void *weight_dev, int type, int64_t n, int d, float eps, void *sum_dev,
+                                        int64_t ld_sum, int format, float fixed_scale, uint8_t *codes_dev, void *scales_dev,
+                                        float *sqr_sum_dev, void *stream)
+{
+    return guarded([&] {
+        ixa::op_rms_norm_quantise(x_dev, ld_x, residual_dev, ld_residual, weight_dev, type, n, d, eps, sum_dev, ld_sum, format,
+                                  fixed_scale, codes_dev, scales_dev, sqr_sum_dev, static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_op_mx_product(const uint8_t *a_codes_dev, const uint8_t *a_scales_dev, int a_format, int64_t m,
+                                 const uint8_t *b_codes_dev, const uint8_t *b_scales_dev, int64_t n, int d, int metric,
+                                 const float *a_sqr_sum_dev, const float *b_sqr_sum_dev, int out_type, void *out_dev,
+                                 int64_t ld, void *stream)
+{
+    return guarded([&] {
+        ixa::op_mx_product(a_codes_dev, a_scales_dev, a_format, m, b_codes_dev, b_scales_dev, n, d, metric, a_sqr_sum_dev,
+                           b_sqr_sum_dev, out_type, out_dev, ld, static_cast<hipStream_t>(stream));
     });
 }
 IXA_EXPORT int ivfpq_search_probes_device(ivfpq_index_t *h, int64_t n, const float *x_dev, const int32_t *probes_dev,

@@ -1,0 +1,644 @@
+// Float rows into codes of 8 or 4 bits with scales, alone or behind a residual addition and a root-mean-square norm, and
+// codes back into float rows.  All three move every byte once and compute little: they are bound by memory, a few rows by
+// the latency of one load and of the sums over a row.
+//
+// Microscaled formats (blocks of 32 elements x_0..x_31 of a row; columns behind the last are zeros):
+//   E = clamp(floor(log2 max|x_i|) - t + 127, 0, 254), t = 2 for E2M1 and 8 for E4M3 (their largest power of two); zeros: 0
+//   code_i = x_i * 2^(127 - E) rounded to the nearest number of the format, halfway to even, beyond the largest to it
+// A block that holds an infinity or a NaN gets E = 255, the scale that stands for NaN, and zero codes.
+// int8: scale = max|x| / 127 over the row, code = x * (127 / max|x|) rounded to the nearest integer, halfway to even; a row
+// that holds an infinity or a NaN gets a NaN scale and zero codes.  With a fixed scale, codes are clamped to +-127, NaN to 0.
+#include "lowp.h"
+
+namespace ixa {
+
+namespace {
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef short s2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256;
+constexpr int kVec = 8;                       // elements a lane handles at a time: four lanes hold one block
+constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr uint32_t kNaNScale = 255;
+
+template <typename T>
+struct Vec8 {
+    T v[kVec];
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *__restrict__ p, int count, bool whole, float (&v)[kVec])
+{
+    if (whole && count == kVec) {
+        constexpr int kWords = kVec * sizeof(T) / 16;
+        uint4 w[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            w[i] = reinterpret_cast<const uint4 *>(p)[i];
+        }
+        const Vec8<T> t = __builtin_bit_cast(Vec8<T>, w);
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            v[i] = (float)t.v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            v[i] = i < count ? (float)p[i] : 0.f;
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *__restrict__ p, int count, bool whole, const float (&v)[kVec])
+{
+    if (whole && count == kVec) {
+        constexpr int kWords = kVec * sizeof(T) / 16;
+        struct Words {
+            uint4 w[kWords];
+        };
+        Vec8<T> t;
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            t.v[i] = (T)v[i];
+        }
+        const Words w = __builtin_bit_cast(Words, t);
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            reinterpret_cast<uint4 *>(p)[i] = w.w[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            if (i < count) {
+                p[i] = (T)v[i];
+            }
+        }
+    }
+}
+
+// lane exchanges inside four, eight and sixteen lanes without the LDS
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kQuadXor1 = 0xb1, kQuadXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// the largest value of four lanes that hold one block
+__device__ __forceinline__ uint32_t quad_max(uint32_t v)
+{
+    v = umax(v, dpp<kQuadXor1>(v));
+    return umax(v, dpp<kQuadXor2>(v));
+}
+
+// Reductions over the L lanes of a row; with L = 256 over the workgroup, through `box` (4 words, a barrier on either side).
+template <int L, typename Op>
+__device__ __forceinline__ uint32_t row_reduce(uint32_t v, uint32_t *box, Op op)
+{
+    v = op(v, dpp<kQuadXor1>(v));
+    v = op(v, dpp<kQuadXor2>(v));
+    v = op(v, dpp<kHalfMirror>(v));
+    v = op(v, dpp<kMirror>(v));
+    if constexpr (L >= 32) {
+        v = op(v, (uint32_t)__shfl_xor((int)v, 16));
+    }
+    if constexpr (L >= 64) {
+        v = op(v, (uint32_t)__shfl_xor((int)v, 32));
+    }
+    if constexpr (L == 256) {
+        __syncthreads();   // the readers of the last reduction are done with the box
+        if ((threadIdx.x & 63) == 0) {
+            box[threadIdx.x >> 6] = v;
+        }
+        __syncthreads();
+        v = op(op(box[0], box[1]), op(box[2], box[3]));
+    }
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float row_sum(float v, uint32_t *box)
+{
+    return __uint_as_float(row_reduce<L>(__float_as_uint(v), box, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+template <int L>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *box)
+{
+    return row_reduce<L>(v, box, umax);
+}
+
+struct RowParams {
+    const void *x, *residual, *weight;
+    int64_t ld_x, ld_residual, ld_sum, n;
+    int d, blocks;
+    float eps, fixed_scale;
+    void *sum;
+    uint8_t *codes;
+    void *scales;
+    float *sqr_sum;
+    int format;
+    bool whole_x, whole_residual, whole_weight, whole_sum;   // rows start on 16 bytes: eight elements in wide loads
+};
+
+// What eight elements become, and their share of the squared norm of what the codes stand for.  `biased`: the block's scale.
+__device__ __forceinline__ float encode_fp4(const float (&y)[kVec], uint32_t biased, bool want_sqr, uint32_t &code)
+{
+    const float scale = biased ? __uint_as_float(biased << 23) : __uint_as_float(0x400000u);
+    code = 0;
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[0], y[1], scale, 0);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], scale, 1);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[4], y[5], scale, 2);
+    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[6], y[7], scale, 3);
+    float ss = 0.f;
+    if (want_sqr) {
+        const f2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0),
+                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 1),
+                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 2),
+                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 3)};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            ss = fmaf(v[i].x, v[i].x, ss);
+            ss = fmaf(v[i].y, v[i].y, ss);
+        }
+    }
+    return ss;
+}
+
+__device__ __forceinline__ float encode_fp8(const float (&y)[kVec], uint32_t biased, bool want_sqr, uint32_t (&code)[2])
+{
+    const float scale = biased ? __uint_as_float(biased << 23) : __uint_as_float(0x400000u);
+    const float top = 448.f * scale;   // the instruction makes a NaN of what lies beyond the largest number
+    float ss = 0.f;
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        s2 c = {0, 0};
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, __builtin_amdgcn_fmed3f(y[4 * w], -top, top),
+                                                     __builtin_amdgcn_fmed3f(y[4 * w + 1], -top, top), scale, false);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, __builtin_amdgcn_fmed3f(y[4 * w + 2], -top, top),
+                                                     __builtin_amdgcn_fmed3f(y[4 * w + 3], -top, top), scale, true);
+        code[w] = __builtin_bit_cast(uint32_t, c);
+        if (want_sqr) {
+            const f2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code[w], scale, false);
+            const f2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code[w], scale, true);
+            ss = fmaf(lo.x, lo.x, ss);
+            ss = fmaf(lo.y, lo.y, ss);
+            ss = fmaf(hi.x, hi.x, ss);
+            ss = fmaf(hi.y, hi.y, ss);
+        }
+    }
+    return ss;
+}
+
+// One row per L lanes (16, 32, 64 or the workgroup's 256), held in registers: C times eight elements per lane, so that a
+// row is read once whatever is computed from it.
+template <typename T, int L, int C, bool NORM>
+__global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
+{
+    __shared__ uint32_t box[4];
+    const int lane = threadIdx.x % L;
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+    if (L < 256 && row >= p.n) {
+        return;   // whole groups of lanes that share no data with others (with L = 256 the grid is the number of rows)
+    }
+    float y[C][kVec];
+    const T *x = static_cast<const T *>(p.x) + row * p.ld_x;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int at = (c * L + lane) * kVec;
+        const int count = min(kVec, max(0, p.d - at));
+        load8(x + (count ? at : 0), count, p.whole_x, y[c]);
+    }
+    if constexpr (NORM) {
+        if (p.residual) {
+            const T *r = static_cast<const T *>(p.residual) + row * p.ld_residual;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const int at = (c * L + lane) * kVec;
+                const int count = min(kVec, max(0, p.d - at));
+                float rv[kVec];
+                load8(r + (count ? at : 0), count, p.whole_residual, rv);
+#pragma unroll
+                for (int i = 0; i < kVec; i++) {
+                    y[c][i] += rv[i];
+                }
+            }
+        }
+        if (p.sum) {
+            // the one rounding of the sum to the rows' type; the norm goes on with the unrounded sum
+            T *o = static_cast<T *>(p.sum) + row * p.ld_sum;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const int at = (c * L + lane) * kVec;
+                const int count = min(kVec, max(0, p.d - at));
+                store8(o + (count ? at : 0), count, p.whole_sum, y[c]);
+            }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+#pragma unroll
+            for (int i = 0; i < kVec; i++) {
+                ss = fmaf(y[c][i], y[c][i], ss);
+            }
+        }
+        ss = row_sum<L>(ss, box);
+        float r = 1.0f / sqrtf(ss / (float)p.d + p.eps);
+        if (ss == __builtin_inff()) {   // finite elements whose squares pass the largest number: once more, 2^-80 as large
+            ss = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+#pragma unroll
+                for (int i = 0; i < kVec; i++) {
+                    y[c][i] *= 0x1p-80f;
+                    ss = fmaf(y[c][i], y[c][i], ss);
+                }
+            }
+            r = 1.0f / sqrtf(row_sum<L>(ss, box) / (float)p.d);
+        }
+        const T *w = static_cast<const T *>(p.weight);
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int at = (c * L + lane) * kVec;
+            const int count = min(kVec, max(0, p.d - at));
+            float wv[kVec];
+            if (w) {
+                load8(w + (count ? at : 0), count, p.whole_weight, wv);
+            }
+#pragma unroll
+            for (int i = 0; i < kVec; i++) {
+                y[c][i] *= r;
+                y[c][i] = w ? y[c][i] * wv[i] : y[c][i];
+            }
+        }
+    }
+    const bool want_sqr = p.sqr_sum != nullptr;
+    float ss = 0.f;
+    if (p.format == kFormatInt8) {
+        float scale = p.fixed_scale, pre = 1.f, inv;
+        bool bad = false;
+        if (scale > 0.f) {
+            inv = 1.0f / scale;
+        } else {
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+#pragma unroll
+                for (int i = 0; i < kVec; i++) {
+                    top = umax(top, __float_as_uint(y[c][i]) & 0x7fffffffu);
+                }
+            }
+            top = row_max<L>(top, box);
+            bad = top >= kInfBits;
+            const float t = __uint_as_float(top);
+            pre = t < 0x1p-90f ? 0x1p64f : 1.f;   // 127 / t would not be finite
+            inv = t > 0.f && !bad ? 127.0f / (t * pre) : 0.f;
+            scale = bad ? __builtin_nanf("") : t / 127.0f;
+        }
+        int sq = 0;
+        uint8_t *o = p.codes + row * p.d;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int at = (c * L + lane) * kVec;
+            const int count = min(kVec, max(0, p.d - at));
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < kVec; i++) {
+                const float v = y[c][i] * pre * inv;
+                const int q = bad || v != v ? 0 : (int)rintf(__builtin_amdgcn_fmed3f(v, -127.f, 127.f));
+                sq += q * q;
+                w[i / 4] |= (uint32_t)(q & 0xff) << (8 * (i % 4));
+            }
+            if (count == kVec && (p.d & 7) == 0) {
+                *reinterpret_cast<uint2 *>(o + at) = make_uint2(w[0], w[1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kVec; i++) {
+                    if (i < count) {
+                        o[at + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+                    }
+                }
+            }
+        }
+        if (lane == 0 && p.scales) {
+            static_cast<float *>(p.scales)[row] = scale;
+        }
+        if (want_sqr) {
+            ss = row_sum<L>((float)sq, box) * scale * scale;   // a lane's sum is at most C * 8 * 127^2: exact in 24 bits
+        }
+    } else {
+        const bool four = p.format == kFormatMxFp4;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < kVec; i++) {
+                top = umax(top, __float_as_uint(y[c][i]) & 0x7fffffffu);
+            }
+            top = quad_max(top);
+            const bool bad = top >= kInfBits;
+            const int e = (int)(top >> 23) - (four ? 2 : 8);
+            const uint32_t biased = (uint32_t)max(e, 0);
+            const int at = (c * L + lane) * kVec, block = at / kMxBlock;
+            if (block >= p.blocks) {
+                continue;   // four lanes at a time
+            }
+            const int64_t slot = row * p.blocks + block;
+            float part;
+            if (four) {
+                uint32_t code;
+                part = encode_fp4(y[c], biased, want_sqr, code);
+                reinterpret_cast<uint32_t *>(p.codes)[slot * 4 + (lane & 3)] = bad ? 0u : code;
+            } else {
+                uint32_t code[2];
+                part = encode_fp8(y[c], biased, want_sqr, code);
+                reinterpret_cast<uint2 *>(p.codes)[slot * 4 + (lane & 3)] = bad ? make_uint2(0, 0) : make_uint2(code[0], code[1]);
+            }
+            ss += bad ? __builtin_nanf("") : part;
+            if ((lane & 3) == 0) {
+                static_cast<uint8_t *>(p.scales)[slot] = (uint8_t)(bad ? kNaNScale : biased);
+            }
+        }
+        if (want_sqr) {
+            ss = row_sum<L>(ss, box);
+        }
+    }
+    if (want_sqr && lane == 0) {
+        p.sqr_sum[row] = ss;
+    }
+}
+
+template <typename T, int L, int C, bool NORM>
+void launch_rows_of(const RowParams &p, hipStream_t s)
+{
+    constexpr int kRows = kThreads / L;
+    const int64_t grid = (p.n + kRows - 1) / kRows;
+    hipLaunchKernelGGL((row_quantise_kernel<T, L, C, NORM>), dim3((unsigned)grid), dim3(kThreads), 0, s, p);
+    check_launch();
+}
+
+template <typename T, bool NORM>
+void launch_rows(const RowParams &p, hipStream_t s)
+{
+    const int d = p.d;
+    if (d <= 128) {
+        launch_rows_of<T, 16, 1, NORM>(p, s);
+    } else if (d <= 256) {
+        launch_rows_of<T, 32, 1, NORM>(p, s);
+    } else if (d <= 512) {
+        launch_rows_of<T, 64, 1, NORM>(p, s);
+    } else if (d <= 1024) {
+        launch_rows_of<T, 64, 2, NORM>(p, s);
+    } else if (d <= 2048) {
+        launch_rows_of<T, 64, 4, NORM>(p, s);
+    } else if (d <= 4096) {
+        launch_rows_of<T, 256, 2, NORM>(p, s);
+    } else if (d <= 8192) {
+        launch_rows_of<T, 256, 4, NORM>(p, s);
+    } else {
+        launch_rows_of<T, 256, 8, NORM>(p, s);
+    }
+}
+
+template <bool NORM>
+void launch_rows(const RowParams &p, int type, hipStream_t s)
+{
+    if (type == kTypeF32) {
+        launch_rows<float, NORM>(p, s);
+    } else if (type == kTypeF16) {
+        launch_rows<_Float16, NORM>(p, s);
+    } else {
+        launch_rows<__bf16, NORM>(p, s);
+    }
+}
+
+size_t type_bytes(int type) { return type == kTypeF32 ? 4 : 2; }
+bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+// rows that all start on 16 bytes
+bool whole_rows(const void *p, int64_t ld, int type) { return aligned(p, 16) && (ld * (int64_t)type_bytes(type)) % 16 == 0; }
+
+void check_rows(const char *op, const void *p, int64_t ld, int type, int64_t n, int d)
+{
+    IXA_REQUIRE(p, kErrInvalidParam, "operator buffers can not be nullptr.");
+    IXA_REQUIRE(aligned(p, type_bytes(type)), kErrInvalidParam, "%s: rows are not aligned to their elements", op);
+    IXA_REQUIRE(ld >= d && ld <= (int64_t)1 << 40, kErrInvalidParam, "%s: rows of %d elements in steps of %ld", op, d, (long)ld);
+    (void)n;
+}
+
+void check_codes(const char *op, int type, int64_t n, int d, int format, const uint8_t *codes, const void *scales, bool fixed)
+{
+    IXA_REQUIRE(type >= kTypeF32 && type <= kTypeBF16, kErrInvalidParam, "%s: unsupported element type %d", op, type);
+    IXA_REQUIRE(format >= kFormatInt8 && format <= kFormatMxFp4, kErrInvalidParam, "%s: unsupported code format %d", op, format);
+    IXA_REQUIRE(n >= 0 && n <= 0x7fffffff && d >= 1 && d <= kMaxCodeDim, kErrInvalidParam,
+                "%s: rows %ld (< 2^31), dims %d (1 ... %d)", op, (long)n, d, kMaxCodeDim);
+    IXA_REQUIRE(codes && (scales || fixed), kErrInvalidParam, "operator buffers can not be nullptr.");
+    IXA_REQUIRE(aligned(codes, 16) && (format != kFormatInt8 || aligned(scales, 4)), kErrInvalidParam,
+                "%s: codes have to start on 16 bytes and fp32 scales on 4", op);
+}
+
+void check_fixed(const char *op, int format, float fixed_scale)
+{
+    IXA_REQUIRE(fixed_scale == 0.f || (format == kFormatInt8 && fixed_scale >= 1e-30f && fixed_scale <= 1e30f),
+                kErrInvalidParam, "%s: a fixed scale (%g) goes with int8 codes and lies in [1e-30, 1e30]", op,
+                (double)fixed_scale);
+}
+
+// ----- codes back into rows ---------------------------------------------------------------------------------------------
+
+struct ReadParams {
+    const uint8_t *codes;
+    const void *scales;
+    int64_t n, ld;
+    int d, blocks, format, chunks, rows;   // chunks of 16 elements per row, rows per workgroup
+    void *out;
+    bool whole;
+};
+
+// Sixteen elements per thread: half a block, so one scale each.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void read_codes_kernel(ReadParams p)
+{
+    const int in = threadIdx.x / min(p.chunks, kThreads);
+    const int64_t row = (int64_t)blockIdx.x * p.rows + in;
+    if (in >= p.rows || row >= p.n) {
+        return;
+    }
+    T *o = static_cast<T *>(p.out) + row * p.ld;
+    for (int c = threadIdx.x - in * min(p.chunks, kThreads); c < p.chunks; c += kThreads) {
+        float v[2][kVec];
+        const int at = c * 16;
+        if (p.format == kFormatInt8) {
+            const float scale = static_cast<const float *>(p.scales)[row];
+            const uint8_t *q = p.codes + row * p.d + at;
+            if ((p.d & 15) == 0) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(q);
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    v[i / 8][i % 8] = (float)(int8_t)(u[i / 4] >> (8 * (i % 4))) * scale;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    v[i / 8][i % 8] = at + i < p.d ? (float)(int8_t)q[i] * scale : 0.f;
+                }
+            }
+        } else {
+            const int64_t slot = row * p.blocks + at / kMxBlock;
+            const uint32_t biased = static_cast<const uint8_t *>(p.scales)[slot];
+            const bool bad = biased == kNaNScale;
+            const float scale = biased ? __uint_as_float(biased << 23) : __uint_as_float(0x400000u);
+            if (p.format == kFormatMxFp8) {
+                const uint4 w = reinterpret_cast<const uint4 *>(p.codes)[slot * 2 + (c & 1)];
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const f2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(u[i], scale, false);
+                    const f2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(u[i], scale, true);
+                    v[i / 2][4 * (i & 1)] = lo.x;
+                    v[i / 2][4 * (i & 1) + 1] = lo.y;
+                    v[i / 2][4 * (i & 1) + 2] = hi.x;
+                    v[i / 2][4 * (i & 1) + 3] = hi.y;
+                }
+            } else {
+                const uint2 w = reinterpret_cast<const uint2 *>(p.codes)[slot * 2 + (c & 1)];
+                const uint32_t u[2] = {w.x, w.y};
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const f2 t[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u[i], scale, 0),
+                                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u[i], scale, 1),
+                                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u[i], scale, 2),
+                                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u[i], scale, 3)};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        v[i][2 * j] = t[j].x;
+                        v[i][2 * j + 1] = t[j].y;
+                    }
+                }
+            }
+            if (bad) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    v[i / 8][i % 8] = __builtin_nanf("");
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int first = at + k * kVec, count = min(kVec, p.d - first);
+            if (count > 0) {
+                store8(o + first, count, p.whole, v[k]);
+            }
+        }
+    }
+}
+
+}  // namespace
+
+void op_quantise(const void *x, int64_t ld, int type, int64_t n, int d, int format, float fixed_scale, uint8_t *codes,
+                 void *scales, float *sqr_sum, hipStream_t s)
+{
+    check_codes("quantise", type, n, d, format, codes, scales, fixed_scale > 0.f);
+    check_rows("quantise", x, ld, type, n, d);
+    check_fixed("quantise", format, fixed_scale);
+    IXA_REQUIRE(aligned(sqr_sum, 4), kErrInvalidParam, "quantise: squared norms are not aligned to their elements");
+    if (n == 0) {
+        return;
+    }
+    RowParams p{};
+    p.x = x;
+    p.ld_x = ld;
+    p.n = n;
+    p.d = d;
+    p.blocks = mx_blocks(d);
+    p.fixed_scale = fixed_scale;
+    p.codes = codes;
+    p.scales = scales;
+    p.sqr_sum = sqr_sum;
+    p.format = format;
+    p.whole_x = whole_rows(x, ld, type);
+    launch_rows<false>(p, type, s);
+}
+
+void op_rms_norm_quantise(const void *x, int64_t ld_x, const void *residual, int64_t ld_residual, const void *weight,
+                          int type, int64_t n, int d, float eps, void *sum, int64_t ld_sum, int format, float fixed_scale,
+                          uint8_t *codes, void *scales, float *sqr_sum, hipStream_t s)
+{
+    check_codes("rms_norm_quantise", type, n, d, format, codes, scales, fixed_scale > 0.f);
+    check_rows("rms_norm_quantise", x, ld_x, type, n, d);
+    if (residual) {
+        check_rows("rms_norm_quantise", residual, ld_residual, type, n, d);
+    }
+    if (sum) {
+        check_rows("rms_norm_quantise", sum, ld_sum, type, n, d);
+    }
+    if (weight) {
+        check_rows("rms_norm_quantise", weight, d, type, 1, d);
+    }
+    check_fixed("rms_norm_quantise", format, fixed_scale);
+    IXA_REQUIRE(eps > 0.f && eps < __builtin_inff(), kErrInvalidParam, "rms_norm_quantise: eps %g has to be positive",
+                (double)eps);
+    IXA_REQUIRE(aligned(sqr_sum, 4), kErrInvalidParam, "rms_norm_quantise: squared norms are not aligned to their elements");
+    if (n == 0) {
+        return;
+    }
+    RowParams p{};
+    p.x = x;
+    p.residual = residual;
+    p.weight = weight;
+    p.ld_x = ld_x;
+    p.ld_residual = ld_residual;
+    p.ld_sum = ld_sum;
+    p.n = n;
+    p.d = d;
+    p.blocks = mx_blocks(d);
+    p.eps = eps;
+    p.fixed_scale = fixed_scale;
+    p.sum = sum;
+    p.codes = codes;
+    p.scales = scales;
+    p.sqr_sum = sqr_sum;
+    p.format = format;
+    p.whole_x = whole_rows(x, ld_x, type);
+    p.whole_residual = whole_rows(residual, ld_residual, type);
+    p.whole_weight = aligned(weight, 16);
+    p.whole_sum = whole_rows(sum, ld_sum, type);
+    launch_rows<true>(p, type, s);
+}
+
+void op_dequantise(const uint8_t *codes, const void *scales, int format, int64_t n, int d, int type, void *out, int64_t ld,
+                   hipStream_t s)
+{
+    check_codes("dequantise", type, n, d, format, codes, scales, false);
+    check_rows("dequantise", out, ld, type, n, d);
+    if (n == 0) {
+        return;
+    }
+    ReadParams p{};
+    p.codes = codes;
+    p.scales = scales;
+    p.n = n;
+    p.ld = ld;
+    p.d = d;
+    p.blocks = mx_blocks(d);
+    p.format = format;
+    p.chunks = (d + 15) / 16;
+    p.rows = p.chunks >= kThreads ? 1 : kThreads / p.chunks;
+    p.out = out;
+    p.whole = whole_rows(out, ld, type);
+    const dim3 grid((unsigned)((n + p.rows - 1) / p.rows));
+    if (type == kTypeF32) {
+        hipLaunchKernelGGL(read_codes_kernel<float>, grid, dim3(kThreads), 0, s, p);
+    } else if (type == kTypeF16) {
+        hipLaunchKernelGGL(read_codes_kernel<_Float16>, grid, dim3(kThreads), 0, s, p);
+    } else {
+        hipLaunchKernelGGL(read_codes_kernel<__bf16>, grid, dim3(kThreads), 0, s, p);
+    }
+    check_launch();
+}
+
+}  // namespace ixa

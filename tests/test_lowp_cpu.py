@@ -1,0 +1,131 @@
+"""Low-precision operators without a GPU: the tests' own reference on hand-worked numbers, and what the entry points refuse
+before they touch the device."""
+import ctypes
+import os
+
+import numpy as np
+import pytest
+
+import lowp_reference as ref
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_reference_rounds_halfway_to_even_and_stops_at_the_largest_number():
+    v = np.array([0, 0.24, 0.25, 0.26, 0.75, 1.25, 1.75, 2.5, 3.5, 4.9, 5.0, 5.1, 7.9])
+    assert ref.round_to(v, ref.MXFP4).tolist() == [0, 0, 0, 1, 2, 2, 4, 4, 6, 6, 6, 7, 7]
+    g = ref.grid(ref.MXFP8)
+    assert g[0x7e] == 448 and g[0x38] == 1 and g[1] == 2.0 ** -9 and len(g) == 127
+    assert ref.round_to(np.array([448.0, 511.0, 2.0 ** -10, 3 * 2.0 ** -10]), ref.MXFP8).tolist() == [126, 126, 0, 2]
+
+
+def test_reference_scales():
+    x = np.zeros((1, 32 * 6))
+    x[0, 0] = 4.0            # 2^2: scale 1
+    x[0, 32] = -7.99         # still 2^2
+    x[0, 64] = 2.0 ** -140   # below 2^-125: the smallest scale
+    x[0, 96] = np.inf
+    x[0, 129] = 3.4e38       # 2^127
+    code, scale = ref.mx_codes(x, ref.MXFP4)
+    assert scale.tolist() == [[127, 127, 0, 255, 252, 0]]
+    assert code[0, 0, 0] == 6 and code[0, 1, 0] == 15 and code[0, 3].max() == 0 and code[0, 4, 1] == 7
+    v = ref.mx_values(ref.pack(code, ref.MXFP4), scale, ref.MXFP4)
+    assert v[0, 0] == 4 and v[0, 32] == -6 and np.isnan(v[0, 96:128]).all() and v[0, 129] == 6 * 2.0 ** 125
+
+
+def test_reference_of_bytes_is_its_own_inverse():
+    rng = np.random.default_rng(3)
+    for fmt in (ref.MXFP4, ref.MXFP8):
+        raw = rng.integers(0, 256, (5, 96 if fmt == ref.MXFP8 else 48), dtype=np.uint8)
+        if fmt == ref.MXFP8:
+            raw[(raw & 127) == 127] = 0
+        assert np.array_equal(ref.pack(ref.unpack(raw, fmt).reshape(5, 3, 32), fmt), raw)
+
+
+@pytest.fixture(scope="module")
+def capi():
+    from indexsdk_amd import _capi
+    if not os.path.exists(_capi.LIB_PATH):
+        import __graft_entry__
+        __graft_entry__.build()
+    _capi.load()
+    return _capi
+
+
+def test_code_bytes(capi):
+    lib = capi.load()
+    for fmt, d, want in ((0, 200, (200, 1)), (1, 200, (224, 7)), (2, 200, (112, 7)), (2, 1, (16, 1)), (1, 16384, (16384, 512))):
+        a, b = ctypes.c_int64(), ctypes.c_int64()
+        assert lib.ixa_code_bytes(fmt, d, ctypes.byref(a), ctypes.byref(b)) == 0 and (a.value, b.value) == want
+    assert lib.ixa_code_bytes(2, 32, None, None) == 0
+    for fmt, d in ((3, 32), (-1, 32), (0, 0), (0, 16385)):
+        assert lib.ixa_code_bytes(fmt, d, None, None) == 2001 and "code_bytes" in lib.ixa_last_error().decode()
+
+
+# Addresses are checked before anything is queued and are never read: these stand for buffers.
+P, ODD, OFF = 1 << 20, (1 << 20) + 1, (1 << 20) + 8
+
+
+def _quantise(**kw):
+    a = dict(x=P, ld=64, type=0, n=4, d=64, format=2, fixed=0.0, codes=P, scales=P, sqr=None)
+    a.update(kw)
+    return "ixa_op_quantise", (a["x"], a["ld"], a["type"], a["n"], a["d"], a["format"], a["fixed"], a["codes"], a["scales"],
+                               a["sqr"], None)
+
+
+def _dequantise(**kw):
+    a = dict(codes=P, scales=P, format=2, n=4, d=64, type=0, out=P, ld=64)
+    a.update(kw)
+    return "ixa_op_dequantise", (a["codes"], a["scales"], a["format"], a["n"], a["d"], a["type"], a["out"], a["ld"], None)
+
+
+def _norm(**kw):
+    a = dict(x=P, ld_x=64, res=P, ld_res=64, weight=P, type=2, n=4, d=64, eps=1e-6, sum=P, ld_sum=64, format=0, fixed=0.0,
+             codes=P, scales=P, sqr=None)
+    a.update(kw)
+    return "ixa_op_rms_norm_quantise", tuple(a.values()) + (None,)
+
+
+def _product(**kw):
+    a = dict(ac=P, asc=P, fa=1, m=4, bc=P, bs=P, n=4, d=64, metric=1, asq=P, bsq=P, type=0, out=P, ld=4)
+    a.update(kw)
+    return "ixa_op_mx_product", tuple(a.values()) + (None,)
+
+
+@pytest.mark.parametrize("call,needle", [
+    (_quantise(x=None), "nullptr"), (_quantise(codes=None), "nullptr"), (_quantise(scales=None), "nullptr"),
+    (_quantise(type=3), "element type"), (_quantise(format=3), "code format"), (_quantise(d=0), "dims"),
+    (_quantise(d=16385, ld=16385), "dims"), (_quantise(n=-1), "rows"), (_quantise(n=1 << 31), "rows"),
+    (_quantise(ld=63), "steps of"), (_quantise(x=ODD), "aligned"), (_quantise(codes=OFF), "16 bytes"),
+    (_quantise(fixed=1.0), "fixed scale"), (_quantise(format=0, fixed=-1.0), "fixed scale"),
+    (_quantise(format=0, fixed=float("nan")), "fixed scale"), (_quantise(format=0, fixed=1e38), "fixed scale"),
+    (_quantise(sqr=ODD), "aligned"), (_quantise(format=0, scales=ODD), "fp32 scales"),
+    (_dequantise(out=None), "nullptr"), (_dequantise(scales=None), "nullptr"), (_dequantise(type=-1), "element type"),
+    (_dequantise(format=9), "code format"), (_dequantise(ld=1), "steps of"), (_dequantise(out=ODD), "aligned"),
+    (_norm(x=None), "nullptr"), (_norm(eps=0.0), "eps"), (_norm(eps=float("inf")), "eps"), (_norm(eps=float("nan")), "eps"),
+    (_norm(ld_res=63), "steps of"), (_norm(ld_sum=63), "steps of"), (_norm(weight=ODD), "aligned"), (_norm(sum=ODD), "aligned"),
+    (_norm(type=7), "element type"), (_norm(format=2, fixed=0.5), "fixed scale"), (_norm(codes=OFF), "16 bytes"),
+    (_product(ac=None), "nullptr"), (_product(out=None), "nullptr"), (_product(fa=0), "code format"),
+    (_product(type=3), "element type"), (_product(d=0), "dims"), (_product(m=-1), "rows"), (_product(n=1 << 31, ld=1 << 31), "rows"),
+    (_product(ld=3), "steps of"), (_product(metric=2), "metric"), (_product(asq=None), "norms"), (_product(bsq=None), "norms"),
+    (_product(bc=OFF), "16 bytes"), (_product(out=ODD), "16 bytes"),
+])
+def test_entry_points_refuse(capi, call, needle):
+    lib = capi.load()
+    name, args = call
+    assert getattr(lib, name)(*args) == 2001
+    assert needle in lib.ixa_last_error().decode()
+
+
+@pytest.mark.parametrize("call", [_quantise(n=0), _dequantise(n=0), _norm(n=0), _product(m=0), _product(n=0, ld=0)])
+def test_no_rows_queue_nothing(capi, call):
+    name, args = call
+    assert getattr(capi.load(), name)(*args) == 0
+
+
+def test_no_device_is_an_error(capi):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    for name, args in (_quantise(), _dequantise(), _norm(), _product()):
+        assert getattr(capi.load(), name)(*args) == 2016 and "no CPU path" in capi.load().ixa_last_error().decode()
