@@ -1,25 +1,29 @@
 // Scores of query rows a against stored rows b in microscaled codes: g[i][j] = sum over k of a[i][k] b[j][k], or the squared
 // distance (|a_i|^2 + |b_j|^2) - g - g in the library's expanded form.
 //
-// v_mfma_scale_f32_32x32x64_f8f6f4 multiplies 32 x 64 by 64 x 32 codes and applies the power-of-two scale of each row's
-// block of 32 itself.  A lane (row l & 31, half h = l >> 5) gives it, in 4 bits, the 16 bytes of block h of its row; in 8
-// bits, bytes 16 h .. 16 h + 15 of block 0 and the same of block 1; and in both the scale of block h.
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 codes and applies the power-of-two scale of each row's
+// block of 32 itself.  A lane (row r = l & 15, quarter g = l >> 4) gives it, in 4 bits, the 16 bytes of block g of its row;
+// in 8 bits, bytes 16 g ... 16 g + 15 of the first and of the second 64; and in both the scale of block g.  The stored rows are
+// its first operand, so that a lane ends up with four scores of one query next to each other.
 //
 // Two 4-bit numbers multiply and add up without any loss in the instruction.  Products of an 8-bit and a 4-bit number span
 // more bits than it keeps (what lies under about 2^-14 of the largest product is dropped: 1e-4 of the sum of magnitudes
 // was measured on random codes), so an 8-bit operand goes in twice: the codes of magnitude 2 and more, then the others.
-// Within either half all products are multiples of the smallest that the instruction keeps (2^8.8 * 6 against 2^-2 * 0.5, and
-// 2 * 6 against 2^-9 * 0.5), and the sums are those of 32 bits.
+// Within either half all products are multiples of the smallest that the instruction keeps (2^8.8 * 6 against 2^-2 * 0.5,
+// and 2 * 6 against 2^-9 * 0.5), and the sums are those of 32 bits.
 #include "lowp.h"
+
+#include <algorithm>
 
 namespace ixa {
 
 namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kE4M3 = 0, kE2M1 = 4;   // operand formats of the instruction
+constexpr int kOne = 127;             // a block scale of 1
 
 struct ProductParams {
     const uint8_t *a_codes, *a_scales, *b_codes, *b_scales;
@@ -29,98 +33,294 @@ struct ProductParams {
     void *out;
 };
 
-// bytes of w whose magnitude is 2 or more (E4M3: exponent field 8 and up) as ones
-__device__ __forceinline__ uint32_t large_bytes(uint32_t w)
-{
-    const uint32_t u = (w >> 6) & 0x01010101u;
-    return (u << 8) - u;
-}
+__device__ __forceinline__ v8i wide(uint4 lo) { return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, 0, 0, 0, 0}; }
 
+// What a lane gives the instruction of one query fragment: 4-bit codes, or the two halves of 8-bit codes.
 template <int FA>
-__device__ __forceinline__ v16f multiply(const uint4 (&a)[FA == kE2M1 ? 1 : 2], uint32_t a_scale, uint4 b, uint32_t b_scale,
-                                         v16f c)
-{
-    const v8i bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-    if constexpr (FA == kE2M1) {
-        const v8i av = {(int)a[0].x, (int)a[0].y, (int)a[0].z, (int)a[0].w, 0, 0, 0, 0};
-        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, kE2M1, kE2M1, 0, (int)a_scale, 0, (int)b_scale);
-    } else {
-        const uint32_t w[8] = {a[0].x, a[0].y, a[0].z, a[0].w, a[1].x, a[1].y, a[1].z, a[1].w};
-        v8i lo, hi;
+struct AFragment;
+template <>
+struct AFragment<kE2M1> {
+    v8i v;
+    __device__ __forceinline__ void set(const uint4 (&w)[1]) { v = wide(w[0]); }
+    __device__ __forceinline__ v4f multiply(int scale, const v8i &b, int b_scale, v4f c) const
+    {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, v, c, kE2M1, kE2M1, 0, b_scale, 0, scale);
+    }
+};
+template <>
+struct AFragment<kE4M3> {
+    v8i small, large;
+    __device__ __forceinline__ void set(const uint4 (&w)[2])
+    {
+        const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const uint32_t mask = large_bytes(w[i]);
-            lo[i] = (int)(w[i] & ~mask);
-            hi[i] = (int)(w[i] & mask);
+            const uint32_t two = u[i] & 0x40404040u;           // exponent field 8 and up: magnitude 2 and more
+            const uint32_t mask = (two << 1) - (two >> 6);     // their seven bits below the sign
+            small[i] = (int)(u[i] & ~mask);
+            large[i] = (int)(u[i] & (mask | 0x80808080u));
         }
-        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(lo, bv, c, kE4M3, kE2M1, 0, (int)a_scale, 0, (int)b_scale);
-        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(hi, bv, c, kE4M3, kE2M1, 0, (int)a_scale, 0, (int)b_scale);
+    }
+    __device__ __forceinline__ v4f multiply(int scale, const v8i &b, int b_scale, v4f c) const
+    {
+        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, small, c, kE2M1, kE4M3, 0, b_scale, 0, scale);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, large, c, kE2M1, kE4M3, 0, b_scale, 0, scale);
+    }
+};
+
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four {
+    T v[4];
+};
+
+// Four scores of query `row` from column `col` on (columns beyond n are left out): products g, or squared distances from
+// the norms.
+template <typename T>
+__device__ __forceinline__ void store_scores(const ProductParams &p, int64_t row, int64_t col, v4f g, float a_sqr,
+                                             const float (&b_sqr)[4])
+{
+    if (p.metric == kMetricL2) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            g[i] = (a_sqr + b_sqr[i]) - g[i] - g[i];
+        }
+    }
+    T *o = static_cast<T *>(p.out) + row * p.ld + col;
+    if (col + 3 < p.n) {
+        *reinterpret_cast<Four<T> *>(o) = Four<T>{{(T)g[0], (T)g[1], (T)g[2], (T)g[3]}};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (col + i < p.n) {
+                o[i] = (T)g[i];
+            }
+        }
     }
 }
 
-// One wavefront per 32 x 32 scores, operands straight from memory.
-template <int FA, typename T>
-__global__ __launch_bounds__(256) void mx_product_kernel(ProductParams p)
+__device__ __forceinline__ void load_norms(const float *sqr, int64_t col, int64_t n, float (&v)[4])
 {
-    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-    const int64_t col_tiles = (p.n + 31) / 32;
+    if (col + 3 < n) {
+        const Four<float> f = *reinterpret_cast<const Four<float> *>(sqr + col);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = f.v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = sqr[min(col + i, n - 1)];
+        }
+    }
+}
+
+// Query fragments in LDS: 16 rows x 64 bytes are 1 KB, rows of four 16-byte pieces, piece q of row r at place
+// q ^ ((r >> 2) & 3): the 16 lanes of a quarter that read one piece of 16 rows find them in 16 different bank groups.
+__device__ __forceinline__ int fragment_place(int r, int q) { return r * 64 + ((q ^ ((r >> 2) & 3)) * 16); }
+
+// Few queries: their codes stay in LDS (MF fragments of 16 rows, all columns), every wavefront streams NF fragments of
+// 16 stored rows at a time straight into the registers that the instruction reads, one step ahead.
+template <int FA, int MF, int NF, typename T>
+__global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int steps, int64_t tiles)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int kHalves = FA == kE2M1 ? 1 : 2;           // 64-byte halves of a row's step
+    constexpr int kRows = MF * 16;
+    constexpr int kStepBytes = kRows * 64 * kHalves;
+    uint8_t *const scales = smem + (size_t)steps * kStepBytes;   // [step][row][block of the step]
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int64_t row0 = (int64_t)blockIdx.y * kRows;
+    const int a_row_bytes = p.blocks * 16 * kHalves;
+    // pieces behind the last block and rows behind the last query are zeros
+    for (int e = threadIdx.x; e < steps * kRows * 4 * kHalves; e += 256) {
+        const int q = e & 3, row = (e >> 2) % kRows, part = (e >> 2) / kRows;   // part: 64 bytes of the row
+        const int byte = part * 64 + q * 16;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (byte < a_row_bytes && row0 + row < p.m) {
+            v = *reinterpret_cast<const uint4 *>(p.a_codes + (row0 + row) * a_row_bytes + byte);
+        }
+        *reinterpret_cast<uint4 *>(smem + (size_t)part * kRows * 64 + (row >> 4) * 1024 + fragment_place(row & 15, q)) = v;
+    }
+    for (int e = threadIdx.x; e < steps * kRows * 4; e += 256) {
+        const int b = (e & 3) + (e / (kRows * 4)) * 4, row = (e >> 2) % kRows;
+        scales[e] = b < p.blocks && row0 + row < p.m ? p.a_scales[(row0 + row) * p.blocks + b] : kOne;
+    }
+    __syncthreads();
+    float a_sqr[MF];
+#pragma unroll
+    for (int i = 0; i < MF; i++) {
+        a_sqr[i] = p.metric == kMetricL2 ? p.a_sqr[min(row0 + i * 16 + r, p.m - 1)] : 0.f;
+    }
+    const int64_t stride = (int64_t)gridDim.x * 4;
+    for (int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); tile < tiles; tile += stride) {
+        const int64_t col0 = tile * (NF * 16);
+        const uint8_t *codes[NF], *bs[NF];
+#pragma unroll
+        for (int j = 0; j < NF; j++) {
+            const int64_t row = min(col0 + j * 16 + r, p.n - 1);
+            codes[j] = p.b_codes + row * p.blocks * 16;
+            bs[j] = p.b_scales + row * p.blocks;
+        }
+        uint4 next[NF];
+        int next_scale[NF];
+        // blocks behind the last one repeat it: the queries' codes are zeros there
+        auto fetch = [&](int t) {
+            const int b = min(t * 4 + g, p.blocks - 1);
+#pragma unroll
+            for (int j = 0; j < NF; j++) {
+                next[j] = *reinterpret_cast<const uint4 *>(codes[j] + b * 16);
+                next_scale[j] = bs[j][b];
+            }
+        };
+        fetch(0);
+        v4f acc[MF][NF] = {};
+        for (int t = 0; t < steps; t++) {
+            v8i b[NF];
+            int b_scale[NF];
+#pragma unroll
+            for (int j = 0; j < NF; j++) {
+                b[j] = wide(next[j]);
+                b_scale[j] = next_scale[j];
+            }
+            if (t + 1 < steps) {
+                fetch(t + 1);
+            }
+#pragma unroll
+            for (int i = 0; i < MF; i++) {
+                uint4 w[kHalves];
+#pragma unroll
+                for (int k = 0; k < kHalves; k++) {
+                    w[k] = *reinterpret_cast<const uint4 *>(smem + (size_t)t * kStepBytes + k * kRows * 64 + i * 1024 +
+                                                            fragment_place(r, g));
+                }
+                const int a_scale = scales[(t * kRows + i * 16 + r) * 4 + g];
+                AFragment<FA> a;
+                a.set(w);
+#pragma unroll
+                for (int j = 0; j < NF; j++) {
+                    acc[i][j] = a.multiply(a_scale, b[j], b_scale[j], acc[i][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NF; j++) {
+            const int64_t col = col0 + j * 16 + g * 4;
+            if (col < p.n) {
+                float b_sqr[4] = {};
+                if (p.metric == kMetricL2) {
+                    load_norms(p.b_sqr, col, p.n, b_sqr);
+                }
+#pragma unroll
+                for (int i = 0; i < MF; i++) {
+                    const int64_t row = row0 + i * 16 + r;
+                    if (row < p.m) {
+                        store_scores<T>(p, row, col, acc[i][j], a_sqr[i], b_sqr);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// One wavefront per 16 x 64 scores, operands straight from memory: any number of columns.
+template <int FA, typename T>
+__global__ __launch_bounds__(256) void mx_direct_kernel(ProductParams p)
+{
+    constexpr int kHalves = FA == kE2M1 ? 1 : 2, NF = 4;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int64_t col_tiles = (p.n + 63) / 64;
     const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t row0 = tile / col_tiles * 32, col0 = tile % col_tiles * 32;
-    if (row0 >= p.m) {
+    const int64_t row = tile / col_tiles * 16 + r, col0 = tile % col_tiles * 64;
+    if (tile / col_tiles * 16 >= p.m) {
         return;
     }
-    const int64_t arow = min(row0 + r, p.m - 1), brow = min(col0 + r, p.n - 1);
-    constexpr int kABytes = FA == kE2M1 ? 16 : 32;
-    const uint8_t *ac = p.a_codes + arow * p.blocks * kABytes, *as = p.a_scales + arow * p.blocks;
-    const uint8_t *bc = p.b_codes + brow * p.blocks * 16, *bs = p.b_scales + brow * p.blocks;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    v16f acc = {};
-    for (int t = 0; t < p.blocks; t += 2) {
-        const bool mine = t + h < p.blocks;   // the second block of the last step may not exist: zero codes, scale 1
-        uint4 a[FA == kE2M1 ? 1 : 2];
-        if constexpr (FA == kE2M1) {
-            a[0] = mine ? *reinterpret_cast<const uint4 *>(ac + (t + h) * 16) : zero;
-        } else {
-            a[0] = *reinterpret_cast<const uint4 *>(ac + t * 32 + h * 16);
-            a[1] = t + 1 < p.blocks ? *reinterpret_cast<const uint4 *>(ac + t * 32 + 32 + h * 16) : zero;
+    const int64_t arow = min(row, p.m - 1);
+    const uint8_t *ac = p.a_codes + arow * p.blocks * 16 * kHalves, *as = p.a_scales + arow * p.blocks;
+    v4f acc[NF] = {};
+    for (int t = 0; t * 4 < p.blocks; t++) {
+        const int b = t * 4 + g, last = min(b, p.blocks - 1);
+        uint4 w[kHalves];
+#pragma unroll
+        for (int k = 0; k < kHalves; k++) {
+            const int byte = (t * kHalves + k) * 64 + g * 16;
+            w[k] = byte < p.blocks * 16 * kHalves ? *reinterpret_cast<const uint4 *>(ac + byte) : make_uint4(0, 0, 0, 0);
         }
-        const uint4 b = mine ? *reinterpret_cast<const uint4 *>(bc + (t + h) * 16) : zero;
-        acc = multiply<FA>(a, mine ? as[t + h] : 127, b, mine ? bs[t + h] : 127, acc);
+        AFragment<FA> a;
+        a.set(w);
+        const int a_scale = b < p.blocks ? as[b] : kOne;
+#pragma unroll
+        for (int j = 0; j < NF; j++) {
+            const int64_t brow = min(col0 + j * 16 + r, p.n - 1) * p.blocks + last;
+            acc[j] = a.multiply(a_scale, wide(*reinterpret_cast<const uint4 *>(p.b_codes + brow * 16)), p.b_scales[brow], acc[j]);
+        }
     }
-    const int64_t col = col0 + r;
-    if (col >= p.n) {
+    if (row >= p.m) {
         return;
     }
     const bool l2 = p.metric == kMetricL2;
-    const float bq = l2 ? p.b_sqr[col] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int64_t row = row0 + 8 * (i / 4) + 4 * h + i % 4;
-        if (row < p.m) {
-            float v = acc[i];
+    for (int j = 0; j < NF; j++) {
+        const int64_t col = col0 + j * 16 + g * 4;
+        if (col < p.n) {
+            float b_sqr[4] = {};
             if (l2) {
-                v = (p.a_sqr[row] + bq) - v - v;
+                load_norms(p.b_sqr, col, p.n, b_sqr);
             }
-            static_cast<T *>(p.out)[row * p.ld + col] = (T)v;
+            store_scores<T>(p, row, col, acc[j], l2 ? p.a_sqr[row] : 0.f, b_sqr);
         }
     }
+}
+
+template <int FA>
+size_t stream_lds(int mf, int steps) { return (size_t)steps * mf * 16 * ((FA == kE2M1 ? 64 : 128) + 4); }
+
+template <int FA, int MF, int NF, typename T>
+void launch_stream(const ProductParams &p, hipStream_t s)
+{
+    const int steps = (p.blocks + 3) / 4;
+    const size_t lds = stream_lds<FA>(MF, steps);
+    const int64_t tiles = (p.n + NF * 16 - 1) / (NF * 16);
+    const void *kern = reinterpret_cast<const void *>(mx_stream_kernel<FA, MF, NF, T>);
+    require_dynamic_lds(kern, lds);
+    const int64_t resident = std::max<int64_t>(1, std::min<int64_t>(6, 160 * 1024 / (int64_t)lds)) * 256;
+    const dim3 grid((unsigned)std::min((tiles + 3) / 4, resident), (unsigned)((p.m + MF * 16 - 1) / (MF * 16)));
+    hipLaunchKernelGGL((mx_stream_kernel<FA, MF, NF, T>), grid, dim3(256), lds, s, p, steps, tiles);
+    check_launch();
+}
+
+template <int FA, typename T>
+void launch_type(const ProductParams &p, hipStream_t s)
+{
+    const int steps = (p.blocks + 3) / 4;
+    const int mf = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
+    if (p.m <= 64 && stream_lds<FA>(mf, steps) <= 80 * 1024) {
+        const bool narrow = p.n <= 16 * 4096;   // too few tiles of 64 rows for every wavefront slot
+        if (mf == 1) {
+            narrow ? launch_stream<FA, 1, 1, T>(p, s) : launch_stream<FA, 1, 4, T>(p, s);
+        } else if (mf == 2) {
+            narrow ? launch_stream<FA, 2, 1, T>(p, s) : launch_stream<FA, 2, 4, T>(p, s);
+        } else {
+            narrow ? launch_stream<FA, 4, 1, T>(p, s) : launch_stream<FA, 4, 4, T>(p, s);
+        }
+        return;
+    }
+    const int64_t tiles = ((p.m + 15) / 16) * ((p.n + 63) / 64);
+    IXA_REQUIRE(tiles <= (int64_t)4 * 0x7fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m,
+                (long)p.n);
+    hipLaunchKernelGGL((mx_direct_kernel<FA, T>), dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, s, p);
+    check_launch();
 }
 
 template <int FA>
 void launch(const ProductParams &p, int out_type, hipStream_t s)
 {
-    const int64_t tiles = ((p.m + 31) / 32) * ((p.n + 31) / 32);
-    IXA_REQUIRE(tiles <= (int64_t)4 * 0x7fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m,
-                (long)p.n);
-    const dim3 grid((unsigned)((tiles + 3) / 4));
     if (out_type == kTypeF32) {
-        hipLaunchKernelGGL((mx_product_kernel<FA, float>), grid, dim3(256), 0, s, p);
+        launch_type<FA, float>(p, s);
     } else if (out_type == kTypeF16) {
-        hipLaunchKernelGGL((mx_product_kernel<FA, _Float16>), grid, dim3(256), 0, s, p);
+        launch_type<FA, _Float16>(p, s);
     } else {
-        hipLaunchKernelGGL((mx_product_kernel<FA, __bf16>), grid, dim3(256), 0, s, p);
+        launch_type<FA, __bf16>(p, s);
     }
-    check_launch();
 }
 
 bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
