@@ -14,6 +14,7 @@
 #include "lowp.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ixa {
 
@@ -42,9 +43,10 @@ template <>
 struct AFragment<kE2M1> {
     v8i v;
     __device__ __forceinline__ void set(const uint4 (&w)[1]) { v = wide(w[0]); }
+    template <int BYTE = 0>   // which byte of the scales' registers
     __device__ __forceinline__ v4f multiply(int scale, const v8i &b, int b_scale, v4f c) const
     {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, v, c, kE2M1, kE2M1, 0, b_scale, 0, scale);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, v, c, kE2M1, kE2M1, BYTE, b_scale, BYTE, scale);
     }
 };
 template <>
@@ -61,10 +63,11 @@ struct AFragment<kE4M3> {
             large[i] = (int)(u[i] & (mask | 0x80808080u));
         }
     }
+    template <int BYTE = 0>
     __device__ __forceinline__ v4f multiply(int scale, const v8i &b, int b_scale, v4f c) const
     {
-        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, small, c, kE2M1, kE4M3, 0, b_scale, 0, scale);
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, large, c, kE2M1, kE4M3, 0, b_scale, 0, scale);
+        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, small, c, kE2M1, kE4M3, BYTE, b_scale, BYTE, scale);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, large, c, kE2M1, kE4M3, BYTE, b_scale, BYTE, scale);
     }
 };
 
@@ -222,51 +225,177 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
     }
 }
 
-// One wavefront per 16 x 64 scores, operands straight from memory: any number of columns.
-template <int FA, typename T>
-__global__ __launch_bounds__(256) void mx_direct_kernel(ProductParams p)
+// Many queries: tiles of WM * 128 queries by WN * 64 stored rows, one wavefront per 128 x 64 of them (8 x 4 fragments).  256
+// columns at a time: the queries' codes and both sides' scales go through two LDS buffers, the stored rows' codes straight
+// into the wavefront that owns them, one step of 128 columns ahead.
+template <int FA, int WM, int WN, typename T>
+__global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
-    constexpr int kHalves = FA == kE2M1 ? 1 : 2, NF = 4;
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int64_t col_tiles = (p.n + 63) / 64;
-    const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t row = tile / col_tiles * 16 + r, col0 = tile % col_tiles * 64;
-    if (tile / col_tiles * 16 >= p.m) {
+    constexpr int kHalves = FA == kE2M1 ? 1 : 2, MF = 8, NF = 4, kThreads = WM * WN * 64;
+    constexpr int kRows = WM * 128, kCols = WN * 64;
+    constexpr int kCodeBytes = kRows * 128 * kHalves;                        // of one buffer
+    constexpr int kPieces = kCodeBytes / 16 / kThreads;                      // 16 bytes each, per thread
+    constexpr int kScaleRows = (kRows + kCols + kThreads - 1) / kThreads;    // rows whose scales a thread brings
+    constexpr int kBuffer = kCodeBytes + (kRows + kCols) * 8;
+    __shared__ __align__(16) uint8_t smem[2 * kBuffer];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+    // workgroup b runs on XCD b mod 8: each gets a contiguous run of tiles, eight query tiles high
+    const int64_t id = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (id >= (int64_t)row_tiles * col_tiles) {
         return;
     }
-    const int64_t arow = min(row, p.m - 1);
-    const uint8_t *ac = p.a_codes + arow * p.blocks * 16 * kHalves, *as = p.a_scales + arow * p.blocks;
-    v4f acc[NF] = {};
-    for (int t = 0; t * 4 < p.blocks; t++) {
-        const int b = t * 4 + g, last = min(b, p.blocks - 1);
-        uint4 w[kHalves];
+    const int64_t band = id / (8 * (int64_t)col_tiles);
+    const int high = min(8, row_tiles - (int)band * 8);
+    const int64_t in = id - band * 8 * col_tiles;
+    const int64_t row0 = (band * 8 + in % high) * kRows, col0 = in / high * kCols;
+    const int steps = (p.blocks + 3) / 4, stages = (steps + 1) / 2;
+    const int a_row_bytes = p.blocks * 16 * kHalves;
+    const bool whole = (p.blocks & 3) == 0;
+
+    uint4 piece[kPieces];
+    uint2 scale[kScaleRows];
+    const uint8_t *const a_base = p.a_codes + row0 * a_row_bytes;
+    const int last_row = (int)min<int64_t>(kRows, p.m - row0) - 1, last_col = (int)min<int64_t>(kCols, p.n - col0) - 1;
+    auto bring = [&](int stage) {   // from memory into registers
 #pragma unroll
-        for (int k = 0; k < kHalves; k++) {
-            const int byte = (t * kHalves + k) * 64 + g * 16;
-            w[k] = byte < p.blocks * 16 * kHalves ? *reinterpret_cast<const uint4 *>(ac + byte) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < kPieces; k++) {
+            const int e = tid + k * kThreads, row = min((e >> 2) % kRows, last_row);
+            const int byte = (stage * 2 * kHalves + (e >> 2) / kRows) * 64 + (e & 3) * 16;
+            piece[k] = make_uint4(0, 0, 0, 0);
+            if (byte < a_row_bytes) {
+                piece[k] = *reinterpret_cast<const uint4 *>(a_base + (uint32_t)(row * a_row_bytes + byte));
+            }
         }
-        AFragment<FA> a;
-        a.set(w);
-        const int a_scale = b < p.blocks ? as[b] : kOne;
+#pragma unroll
+        for (int k = 0; k < kScaleRows; k++) {
+            const int row = tid + k * kThreads;
+            if (row < kRows + kCols) {
+                const uint8_t *from = row < kRows ? p.a_scales + (row0 + min(row, last_row)) * p.blocks
+                                                  : p.b_scales + (col0 + min(row - kRows, last_col)) * p.blocks;
+                uint32_t w[2] = {0x7f7f7f7fu, 0x7f7f7f7fu};
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int b = stage * 8 + u * 4;
+                    if (whole && b < p.blocks) {
+                        __builtin_memcpy(&w[u], from + b, 4);
+                    } else if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            if (b + i < p.blocks) {
+                                w[u] = (w[u] & ~(0xffu << (8 * i))) | (uint32_t)from[b + i] << (8 * i);
+                            }
+                        }
+                    }
+                }
+                scale[k] = make_uint2(w[0], w[1]);
+            }
+        }
+    };
+    auto put = [&](int buffer) {    // from registers into LDS
+        uint8_t *const to = smem + buffer * kBuffer;
+#pragma unroll
+        for (int k = 0; k < kPieces; k++) {
+            const int e = tid + k * kThreads, row = (e >> 2) % kRows;
+            *reinterpret_cast<uint4 *>(to + (e >> 2) / kRows * (kRows * 64) + (row >> 4) * 1024 + fragment_place(row & 15, e & 3)) =
+                piece[k];
+        }
+#pragma unroll
+        for (int k = 0; k < kScaleRows; k++) {
+            const int row = tid + k * kThreads;
+            if (row < kRows + kCols) {   // block g of either step next to each other: one 16-bit read serves both
+                *reinterpret_cast<uint2 *>(to + kCodeBytes + row * 8) =
+                    make_uint2(__builtin_amdgcn_perm(scale[k].y, scale[k].x, 0x05010400u),
+                               __builtin_amdgcn_perm(scale[k].y, scale[k].x, 0x07030602u));
+            }
+        }
+    };
+
+    // the wavefront's stored rows; those behind the last one repeat it
+    const int64_t wave_col = min<int64_t>(col0 + wn * 64, p.n - 1);
+    const uint8_t *const b_base = p.b_codes + wave_col * p.blocks * 16;
+    uint32_t b_row[NF];
+#pragma unroll
+    for (int j = 0; j < NF; j++) {
+        b_row[j] = (uint32_t)(min<int64_t>(j * 16 + r, p.n - 1 - wave_col) * p.blocks * 16);
+    }
+    uint4 next[NF];
+    auto fetch = [&](int t) {
+        const uint32_t b = (uint32_t)min(t * 4 + g, p.blocks - 1) * 16;   // behind the last block: it meets zeros
 #pragma unroll
         for (int j = 0; j < NF; j++) {
-            const int64_t brow = min(col0 + j * 16 + r, p.n - 1) * p.blocks + last;
-            acc[j] = a.multiply(a_scale, wide(*reinterpret_cast<const uint4 *>(p.b_codes + brow * 16)), p.b_scales[brow], acc[j]);
+            next[j] = *reinterpret_cast<const uint4 *>(b_base + (b_row[j] + b));
         }
-    }
-    if (row >= p.m) {
-        return;
+    };
+
+    v4f acc[MF][NF] = {};
+    fetch(0);
+    bring(0);
+    put(0);
+    __syncthreads();
+    for (int stage = 0; stage < stages; stage++) {
+        const uint8_t *const from = smem + (stage & 1) * kBuffer;
+        if (stage + 1 < stages) {
+            bring(stage + 1);
+        }
+        int a_scale[MF], b_scale[NF];
+#pragma unroll
+        for (int i = 0; i < MF; i++) {
+            a_scale[i] = *reinterpret_cast<const uint16_t *>(from + kCodeBytes + (wm * 128 + i * 16 + r) * 8 + g * 2);
+        }
+#pragma unroll
+        for (int j = 0; j < NF; j++) {
+            b_scale[j] = *reinterpret_cast<const uint16_t *>(from + kCodeBytes + (kRows + wn * 64 + j * 16 + r) * 8 + g * 2);
+        }
+        auto step = [&](auto which) {
+            constexpr int u = decltype(which)::value;
+            v8i b[NF];
+#pragma unroll
+            for (int j = 0; j < NF; j++) {
+                b[j] = wide(next[j]);
+            }
+            fetch(min(stage * 2 + u + 1, steps - 1));
+#pragma unroll
+            for (int i = 0; i < MF; i++) {
+                uint4 w[kHalves];
+#pragma unroll
+                for (int k = 0; k < kHalves; k++) {
+                    w[k] = *reinterpret_cast<const uint4 *>(from + (u * kHalves + k) * (kRows * 64) + (wm * 8 + i) * 1024 +
+                                                            fragment_place(r, g));
+                }
+                AFragment<FA> a;
+                a.set(w);
+#pragma unroll
+                for (int j = 0; j < NF; j++) {
+                    acc[i][j] = a.template multiply<u>(a_scale[i], b[j], b_scale[j], acc[i][j]);
+                }
+            }
+        };
+        step(std::integral_constant<int, 0>());
+        if (stage * 2 + 1 < steps) {
+            step(std::integral_constant<int, 1>());
+        }
+        if (stage + 1 < stages) {
+            put((stage + 1) & 1);
+        }
+        __syncthreads();
     }
     const bool l2 = p.metric == kMetricL2;
 #pragma unroll
     for (int j = 0; j < NF; j++) {
-        const int64_t col = col0 + j * 16 + g * 4;
+        const int64_t col = col0 + wn * 64 + j * 16 + g * 4;
         if (col < p.n) {
             float b_sqr[4] = {};
             if (l2) {
                 load_norms(p.b_sqr, col, p.n, b_sqr);
             }
-            store_scores<T>(p, row, col, acc[j], l2 ? p.a_sqr[row] : 0.f, b_sqr);
+#pragma unroll
+            for (int i = 0; i < MF; i++) {
+                const int64_t row = row0 + wm * 128 + i * 16 + r;
+                if (row < p.m) {
+                    store_scores<T>(p, row, col, acc[i][j], l2 ? p.a_sqr[row] : 0.f, b_sqr);
+                }
+            }
         }
     }
 }
@@ -288,6 +417,17 @@ void launch_stream(const ProductParams &p, hipStream_t s)
     check_launch();
 }
 
+template <int FA, int WM, int WN, typename T>
+void launch_tiles(const ProductParams &p, hipStream_t s)
+{
+    const int64_t row_tiles = (p.m + WM * 128 - 1) / (WM * 128), col_tiles = (p.n + WN * 64 - 1) / (WN * 64);
+    const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
+    IXA_REQUIRE(per_xcd <= 0x0fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m, (long)p.n);
+    hipLaunchKernelGGL((mx_tile_kernel<FA, WM, WN, T>), dim3((unsigned)per_xcd * 8), dim3(WM * WN * 64), 0, s, p,
+                       (int)row_tiles, (int)col_tiles, (int)per_xcd);
+    check_launch();
+}
+
 template <int FA, typename T>
 void launch_type(const ProductParams &p, hipStream_t s)
 {
@@ -304,11 +444,11 @@ void launch_type(const ProductParams &p, hipStream_t s)
         }
         return;
     }
-    const int64_t tiles = ((p.m + 15) / 16) * ((p.n + 63) / 64);
-    IXA_REQUIRE(tiles <= (int64_t)4 * 0x7fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m,
-                (long)p.n);
-    hipLaunchKernelGGL((mx_direct_kernel<FA, T>), dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, s, p);
-    check_launch();
+    if (p.m <= 128) {
+        launch_tiles<FA, 1, 4, T>(p, s);
+    } else {
+        launch_tiles<FA, 1, 4, T>(p, s);
+    }
 }
 
 template <int FA>
