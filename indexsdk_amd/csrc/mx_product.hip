@@ -3,8 +3,9 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 codes and applies the power-of-two scale of each row's
 // block of 32 itself.  A lane (row r = l & 15, quarter g = l >> 4) gives it, in 4 bits, the 16 bytes of block g of its row;
-// in 8 bits, bytes 16 g ... 16 g + 15 of the first and of the second 64; and in both the scale of block g.  The stored rows are
-// its first operand, so that a lane ends up with four scores of one query next to each other.
+// in 8 bits, bytes 16 g ... 16 g + 15 of the first and of the second 64; and in both the scale of block g.  A lane ends up with
+// scores of queries 4 g ... 4 g + 3 and stored row r of the fragment; four fragments of stored rows are dealt so that row r of
+// fragment j is row 4 r + j of 64, and the lane holds four scores next to each other: 16 lanes write 256 bytes in a row.
 //
 // Two 4-bit numbers multiply and add up without any loss in the instruction.  Products of an 8-bit and a 4-bit number span
 // more bits than it keeps (what lies under about 2^-14 of the largest product is dropped: 1e-4 of the sum of magnitudes
@@ -22,6 +23,7 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));   // 16 bytes of codes
 
 constexpr int kE4M3 = 0, kE2M1 = 4;   // operand formats of the instruction
 constexpr int kOne = 127;             // a block scale of 1
@@ -34,7 +36,7 @@ struct ProductParams {
     void *out;
 };
 
-__device__ __forceinline__ v8i wide(uint4 lo) { return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, 0, 0, 0, 0}; }
+__device__ __forceinline__ v8i wide(u4 lo) { return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, 0, 0, 0, 0}; }
 
 // What a lane gives the instruction of one query fragment: 4-bit codes, or the two halves of 8-bit codes.
 template <int FA>
@@ -42,17 +44,17 @@ struct AFragment;
 template <>
 struct AFragment<kE2M1> {
     v8i v;
-    __device__ __forceinline__ void set(const uint4 (&w)[1]) { v = wide(w[0]); }
+    __device__ __forceinline__ void set(const u4 (&w)[1]) { v = wide(w[0]); }
     template <int BYTE = 0>   // which byte of the scales' registers
     __device__ __forceinline__ v4f multiply(int scale, const v8i &b, int b_scale, v4f c) const
     {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, v, c, kE2M1, kE2M1, BYTE, b_scale, BYTE, scale);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, b, c, kE2M1, kE2M1, BYTE, scale, BYTE, b_scale);
     }
 };
 template <>
 struct AFragment<kE4M3> {
     v8i small, large;
-    __device__ __forceinline__ void set(const uint4 (&w)[2])
+    __device__ __forceinline__ void set(const u4 (&w)[2])
     {
         const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
 #pragma unroll
@@ -66,63 +68,94 @@ struct AFragment<kE4M3> {
     template <int BYTE = 0>
     __device__ __forceinline__ v4f multiply(int scale, const v8i &b, int b_scale, v4f c) const
     {
-        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, small, c, kE2M1, kE4M3, BYTE, b_scale, BYTE, scale);
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, large, c, kE2M1, kE4M3, BYTE, b_scale, BYTE, scale);
+        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(small, b, c, kE4M3, kE2M1, BYTE, scale, BYTE, b_scale);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(large, b, c, kE4M3, kE2M1, BYTE, scale, BYTE, b_scale);
     }
 };
 
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Four {
-    T v[4];
-};
-
-// Four scores of query `row` from column `col` on (columns beyond n are left out): products g, or squared distances from
-// the norms.
-template <typename T>
-__device__ __forceinline__ void store_scores(const ProductParams &p, int64_t row, int64_t col, v4f g, float a_sqr,
-                                             const float (&b_sqr)[4])
+// N values from `at` on of an array that ends at n: those behind its end repeat the last
+template <int N>
+__device__ __forceinline__ void load_run(const float *from, int64_t at, int64_t n, float (&v)[N])
 {
-    if (p.metric == kMetricL2) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            g[i] = (a_sqr + b_sqr[i]) - g[i] - g[i];
-        }
-    }
-    T *o = static_cast<T *>(p.out) + row * p.ld + col;
-    if (col + 3 < p.n) {
-        *reinterpret_cast<Four<T> *>(o) = Four<T>{{(T)g[0], (T)g[1], (T)g[2], (T)g[3]}};
+    if (at + N <= n) {
+        __builtin_memcpy(v, from + at, sizeof(v));
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (col + i < p.n) {
-                o[i] = (T)g[i];
+        for (int i = 0; i < N; i++) {
+            v[i] = from[min(at + i, n - 1)];
+        }
+    }
+}
+
+// The scores of a lane: queries row ... row + 3 (element i of the accumulators) and columns col ... col + NF - 1 (fragment j).
+template <typename T, int NF>
+__device__ __forceinline__ void store_scores(const ProductParams &p, int64_t row, int64_t col, const v4f (&acc)[NF],
+                                             const float (&b_sqr)[NF])
+{
+    if (row >= p.m || col >= p.n) {
+        return;
+    }
+    const bool l2 = p.metric == kMetricL2;
+    float a_sqr[4] = {};
+    if (l2) {
+        load_run(p.a_sqr, row, p.m, a_sqr);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (row + i < p.m) {
+            T v[NF];
+#pragma unroll
+            for (int j = 0; j < NF; j++) {
+                const float g = acc[j][i];
+                v[j] = (T)(l2 ? (a_sqr[i] + b_sqr[j]) - g - g : g);
+            }
+            T *o = static_cast<T *>(p.out) + (row + i) * p.ld + col;
+            if (col + NF <= p.n) {
+                __builtin_memcpy(o, v, sizeof(v));
+            } else {
+#pragma unroll
+                for (int j = 0; j < NF; j++) {
+                    if (col + j < p.n) {
+                        o[j] = v[j];
+                    }
+                }
             }
         }
     }
 }
 
-__device__ __forceinline__ void load_norms(const float *sqr, int64_t col, int64_t n, float (&v)[4])
+// Fragments in LDS: 16 rows of 64 bytes are 1 KB, four 16-byte pieces per row, piece q of row r at place q ^ ((r >> 1) & 3):
+// eight lanes in a row that read one piece of eight rows find them in all banks.
+__device__ __forceinline__ int fragment_place(int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) * 16); }
+// The same for NF fragments of stored rows dealt as above.  Neighbouring rows, which are written together, lie in fragments
+// of their own: every second one swaps its rows in pairs to be in other banks.
+template <int NF>
+__device__ __forceinline__ int stored_place(int j, int r, int q)
 {
-    if (col + 3 < n) {
-        const Four<float> f = *reinterpret_cast<const Four<float> *>(sqr + col);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[i] = f.v[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[i] = sqr[min(col + i, n - 1)];
-        }
-    }
+    return j * 1024 + (NF > 1 ? r ^ (j & 1) : r) * 64 + ((q ^ ((r >> 1) & 3)) * 16);
 }
 
-// Query fragments in LDS: 16 rows x 64 bytes are 1 KB, rows of four 16-byte pieces, piece q of row r at place
-// q ^ ((r >> 2) & 3): the 16 lanes of a quarter that read one piece of 16 rows find them in 16 different bank groups.
-__device__ __forceinline__ int fragment_place(int r, int q) { return r * 64 + ((q ^ ((r >> 2) & 3)) * 16); }
+// The scales of four blocks from block b on of the row that starts at `from`; behind the last block 1.
+__device__ __forceinline__ uint32_t four_scales(const uint8_t *from, int b, int blocks)
+{
+    uint32_t w = 0x01010101u * kOne;
+    if (b + 4 <= blocks) {
+        __builtin_memcpy(&w, from + b, 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            if (b + i < blocks) {
+                w = (w & ~(0xffu << (8 * i))) | (uint32_t)from[b + i] << (8 * i);
+            }
+        }
+    }
+    return w;
+}
 
-// Few queries: their codes stay in LDS (MF fragments of 16 rows, all columns), every wavefront streams NF fragments of
-// 16 stored rows at a time straight into the registers that the instruction reads, one step ahead.
+// Few queries: their codes stay in LDS (MF fragments of 16 rows, all columns) while every wavefront streams NF fragments of
+// stored rows past them, one step ahead.  The stored rows come in whole pieces of 64 bytes, four lanes each, and change lanes
+// in 1 KB of LDS per fragment that the wavefront has to itself: read the way the instruction wants them, 16 lanes
+// would touch 16 rows at a time.
 template <int FA, int MF, int NF, typename T>
 __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int steps, int64_t tiles)
 {
@@ -132,68 +165,80 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
     constexpr int kStepBytes = kRows * 64 * kHalves;
     uint8_t *const scales = smem + (size_t)steps * kStepBytes;   // [step][row][block of the step]
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint8_t *const turn = scales + (size_t)steps * kRows * 4 + wave * (NF * (1024 + 64));
+    uint8_t *const turn_scales = turn + NF * 1024;
     const int64_t row0 = (int64_t)blockIdx.y * kRows;
-    const int a_row_bytes = p.blocks * 16 * kHalves;
+    const int a_row_bytes = p.blocks * 16 * kHalves, b_row_bytes = p.blocks * 16;
     // pieces behind the last block and rows behind the last query are zeros
     for (int e = threadIdx.x; e < steps * kRows * 4 * kHalves; e += 256) {
         const int q = e & 3, row = (e >> 2) % kRows, part = (e >> 2) / kRows;   // part: 64 bytes of the row
         const int byte = part * 64 + q * 16;
-        uint4 v = make_uint4(0, 0, 0, 0);
+        u4 v = u4{};
         if (byte < a_row_bytes && row0 + row < p.m) {
-            v = *reinterpret_cast<const uint4 *>(p.a_codes + (row0 + row) * a_row_bytes + byte);
+            v = *reinterpret_cast<const u4 *>(p.a_codes + (row0 + row) * a_row_bytes + byte);
         }
-        *reinterpret_cast<uint4 *>(smem + (size_t)part * kRows * 64 + (row >> 4) * 1024 + fragment_place(row & 15, q)) = v;
+        *reinterpret_cast<u4 *>(smem + (size_t)part * kRows * 64 + (row >> 4) * 1024 + fragment_place(row & 15, q)) = v;
     }
-    for (int e = threadIdx.x; e < steps * kRows * 4; e += 256) {
-        const int b = (e & 3) + (e / (kRows * 4)) * 4, row = (e >> 2) % kRows;
-        scales[e] = b < p.blocks && row0 + row < p.m ? p.a_scales[(row0 + row) * p.blocks + b] : kOne;
+    for (int e = threadIdx.x; e < steps * kRows; e += 256) {
+        const int row = e % kRows;
+        reinterpret_cast<uint32_t *>(scales)[e] =
+            row0 + row < p.m ? four_scales(p.a_scales + (row0 + row) * p.blocks, e / kRows * 4, p.blocks) : 0x01010101u * kOne;
     }
     __syncthreads();
-    float a_sqr[MF];
-#pragma unroll
-    for (int i = 0; i < MF; i++) {
-        a_sqr[i] = p.metric == kMetricL2 ? p.a_sqr[min(row0 + i * 16 + r, p.m - 1)] : 0.f;
-    }
     const int64_t stride = (int64_t)gridDim.x * 4;
-    for (int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); tile < tiles; tile += stride) {
+    for (int64_t tile = (int64_t)blockIdx.x * 4 + wave; tile < tiles; tile += stride) {
         const int64_t col0 = tile * (NF * 16);
-        const uint8_t *codes[NF], *bs[NF];
+        const int last = (int)min<int64_t>(NF * 16, p.n - col0) - 1;   // rows behind the last one repeat it
+        const uint8_t *const codes = p.b_codes + col0 * b_row_bytes;
+        uint32_t offset[NF];
 #pragma unroll
-        for (int j = 0; j < NF; j++) {
-            const int64_t row = min(col0 + j * 16 + r, p.n - 1);
-            codes[j] = p.b_codes + row * p.blocks * 16;
-            bs[j] = p.b_scales + row * p.blocks;
+        for (int k = 0; k < NF; k++) {
+            offset[k] = (uint32_t)(min(k * 16 + (lane >> 2), last) * b_row_bytes);
         }
-        uint4 next[NF];
-        int next_scale[NF];
-        // blocks behind the last one repeat it: the queries' codes are zeros there
+        const uint8_t *const scale_row = p.b_scales + (col0 + min(lane, last)) * p.blocks;
+        u4 next[NF];
+        uint32_t next_scale = 0;
+        // pieces behind the last block repeat it: the queries' codes are zeros there
         auto fetch = [&](int t) {
-            const int b = min(t * 4 + g, p.blocks - 1);
+            const uint32_t byte = (uint32_t)min(t * 64 + (lane & 3) * 16, b_row_bytes - 16);
 #pragma unroll
-            for (int j = 0; j < NF; j++) {
-                next[j] = *reinterpret_cast<const uint4 *>(codes[j] + b * 16);
-                next_scale[j] = bs[j][b];
+            for (int k = 0; k < NF; k++) {
+                next[k] = *reinterpret_cast<const u4 *>(codes + (offset[k] + byte));
+            }
+            if (NF == 4 || lane < NF * 16) {
+                next_scale = four_scales(scale_row, t * 4, p.blocks);
             }
         };
         fetch(0);
         v4f acc[MF][NF] = {};
         for (int t = 0; t < steps; t++) {
-            v8i b[NF];
-            int b_scale[NF];
 #pragma unroll
-            for (int j = 0; j < NF; j++) {
-                b[j] = wide(next[j]);
-                b_scale[j] = next_scale[j];
+            for (int k = 0; k < NF; k++) {
+                const int row = k * 16 + (lane >> 2);
+                *reinterpret_cast<u4 *>(turn + stored_place<NF>(row % NF, row / NF, lane & 3)) = next[k];
+            }
+            if (NF == 4 || lane < NF * 16) {
+                reinterpret_cast<uint32_t *>(turn_scales)[(lane % NF) * 16 + lane / NF] = next_scale;
             }
             if (t + 1 < steps) {
                 fetch(t + 1);
             }
+            __builtin_amdgcn_wave_barrier();
+            v8i b[NF];
+            int b_scale[NF];
+#pragma unroll
+            for (int j = 0; j < NF; j++) {
+                b[j] = wide(*reinterpret_cast<const u4 *>(turn + stored_place<NF>(j, r, g)));
+                b_scale[j] = turn_scales[(j * 16 + r) * 4 + g];
+            }
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int i = 0; i < MF; i++) {
-                uint4 w[kHalves];
+                u4 w[kHalves];
 #pragma unroll
                 for (int k = 0; k < kHalves; k++) {
-                    w[k] = *reinterpret_cast<const uint4 *>(smem + (size_t)t * kStepBytes + k * kRows * 64 + i * 1024 +
+                    w[k] = *reinterpret_cast<const u4 *>(smem + (size_t)t * kStepBytes + k * kRows * 64 + i * 1024 +
                                                             fragment_place(r, g));
                 }
                 const int a_scale = scales[(t * kRows + i * 16 + r) * 4 + g];
@@ -205,38 +250,31 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
                 }
             }
         }
+        const int64_t col = col0 + r * NF;
+        float b_sqr[NF] = {};
+        if (p.metric == kMetricL2) {
+            load_run(p.b_sqr, col, p.n, b_sqr);
+        }
 #pragma unroll
-        for (int j = 0; j < NF; j++) {
-            const int64_t col = col0 + j * 16 + g * 4;
-            if (col < p.n) {
-                float b_sqr[4] = {};
-                if (p.metric == kMetricL2) {
-                    load_norms(p.b_sqr, col, p.n, b_sqr);
-                }
-#pragma unroll
-                for (int i = 0; i < MF; i++) {
-                    const int64_t row = row0 + i * 16 + r;
-                    if (row < p.m) {
-                        store_scores<T>(p, row, col, acc[i][j], a_sqr[i], b_sqr);
-                    }
-                }
-            }
+        for (int i = 0; i < MF; i++) {
+            store_scores<T, NF>(p, row0 + i * 16 + g * 4, col, acc[i], b_sqr);
         }
     }
 }
 
-// Many queries: tiles of WM * 128 queries by WN * 64 stored rows, one wavefront per 128 x 64 of them (8 x 4 fragments).  256
-// columns at a time: the queries' codes and both sides' scales go through two LDS buffers, the stored rows' codes straight
-// into the wavefront that owns them, one step of 128 columns ahead.
-template <int FA, int WM, int WN, typename T>
+// Many queries: tiles of WM * 128 queries by WN * 64 stored rows, one wavefront per 128 x 64 of them (8 x 4 fragments).  Codes
+// and scales of both sides go through two LDS buffers of U steps (128 columns each); while one is multiplied, the next is
+// written from registers and the one after it is on its way from memory.
+template <int FA, int WM, int WN, int U, typename T>
 __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
     constexpr int kHalves = FA == kE2M1 ? 1 : 2, MF = 8, NF = 4, kThreads = WM * WN * 64;
     constexpr int kRows = WM * 128, kCols = WN * 64;
-    constexpr int kCodeBytes = kRows * 128 * kHalves;                        // of one buffer
-    constexpr int kPieces = kCodeBytes / 16 / kThreads;                      // 16 bytes each, per thread
-    constexpr int kScaleRows = (kRows + kCols + kThreads - 1) / kThreads;    // rows whose scales a thread brings
-    constexpr int kBuffer = kCodeBytes + (kRows + kCols) * 8;
+    constexpr int kABytes = kRows * 64 * kHalves * U, kBBytes = kCols * 64 * U;
+    constexpr int kAPieces = kABytes / 16 / kThreads, kBPieces = kBBytes / 16 / kThreads;   // per thread
+    constexpr int kScaleRows = (kRows + kCols + kThreads - 1) / kThreads;
+    constexpr int kBuffer = kABytes + kBBytes + (kRows + kCols) * 4 * U;
+    static_assert(U == 1 || U == 2, "the scales of a row's block in a buffer are one read");
     __shared__ __align__(16) uint8_t smem[2 * kBuffer];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
@@ -249,23 +287,26 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
     const int high = min(8, row_tiles - (int)band * 8);
     const int64_t in = id - band * 8 * col_tiles;
     const int64_t row0 = (band * 8 + in % high) * kRows, col0 = in / high * kCols;
-    const int steps = (p.blocks + 3) / 4, stages = (steps + 1) / 2;
-    const int a_row_bytes = p.blocks * 16 * kHalves;
-    const bool whole = (p.blocks & 3) == 0;
+    const int steps = (p.blocks + 3) / 4, stages = (steps + U - 1) / U;
+    const int a_row_bytes = p.blocks * 16 * kHalves, b_row_bytes = p.blocks * 16;
 
-    uint4 piece[kPieces];
-    uint2 scale[kScaleRows];
-    const uint8_t *const a_base = p.a_codes + row0 * a_row_bytes;
+    const uint8_t *const a_base = p.a_codes + row0 * a_row_bytes, *const b_base = p.b_codes + col0 * b_row_bytes;
     const int last_row = (int)min<int64_t>(kRows, p.m - row0) - 1, last_col = (int)min<int64_t>(kCols, p.n - col0) - 1;
-    auto bring = [&](int stage) {   // from memory into registers
+    u4 a_piece[kAPieces], b_piece[kBPieces];
+    uint32_t scale[kScaleRows][U];
+    auto bring = [&](int stage) {   // from memory into registers; queries' codes behind the last block are zeros
 #pragma unroll
-        for (int k = 0; k < kPieces; k++) {
+        for (int k = 0; k < kAPieces; k++) {
             const int e = tid + k * kThreads, row = min((e >> 2) % kRows, last_row);
-            const int byte = (stage * 2 * kHalves + (e >> 2) / kRows) * 64 + (e & 3) * 16;
-            piece[k] = make_uint4(0, 0, 0, 0);
-            if (byte < a_row_bytes) {
-                piece[k] = *reinterpret_cast<const uint4 *>(a_base + (uint32_t)(row * a_row_bytes + byte));
-            }
+            const int byte = (stage * U * kHalves + (e >> 2) / kRows) * 64 + (e & 3) * 16;
+            const u4 v = *reinterpret_cast<const u4 *>(a_base + (uint32_t)(row * a_row_bytes + min(byte, a_row_bytes - 16)));
+            a_piece[k] = byte < a_row_bytes ? v : u4{};
+        }
+#pragma unroll
+        for (int k = 0; k < kBPieces; k++) {
+            const int e = tid + k * kThreads, row = min((e >> 2) % kCols, last_col);
+            const int byte = (stage * U + (e >> 2) / kCols) * 64 + (e & 3) * 16;
+            b_piece[k] = *reinterpret_cast<const u4 *>(b_base + (uint32_t)(row * b_row_bytes + min(byte, b_row_bytes - 16)));
         }
 #pragma unroll
         for (int k = 0; k < kScaleRows; k++) {
@@ -273,94 +314,83 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
             if (row < kRows + kCols) {
                 const uint8_t *from = row < kRows ? p.a_scales + (row0 + min(row, last_row)) * p.blocks
                                                   : p.b_scales + (col0 + min(row - kRows, last_col)) * p.blocks;
-                uint32_t w[2] = {0x7f7f7f7fu, 0x7f7f7f7fu};
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int b = stage * 8 + u * 4;
-                    if (whole && b < p.blocks) {
-                        __builtin_memcpy(&w[u], from + b, 4);
-                    } else if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            if (b + i < p.blocks) {
-                                w[u] = (w[u] & ~(0xffu << (8 * i))) | (uint32_t)from[b + i] << (8 * i);
-                            }
-                        }
-                    }
+                for (int u = 0; u < U; u++) {
+                    scale[k][u] = four_scales(from, (stage * U + u) * 4, p.blocks);
                 }
-                scale[k] = make_uint2(w[0], w[1]);
             }
         }
     };
     auto put = [&](int buffer) {    // from registers into LDS
         uint8_t *const to = smem + buffer * kBuffer;
 #pragma unroll
-        for (int k = 0; k < kPieces; k++) {
+        for (int k = 0; k < kAPieces; k++) {
             const int e = tid + k * kThreads, row = (e >> 2) % kRows;
-            *reinterpret_cast<uint4 *>(to + (e >> 2) / kRows * (kRows * 64) + (row >> 4) * 1024 + fragment_place(row & 15, e & 3)) =
-                piece[k];
+            *reinterpret_cast<u4 *>(to + (e >> 2) / kRows * (kRows * 64) + (row >> 4) * 1024 + fragment_place(row & 15, e & 3)) =
+                a_piece[k];
+        }
+#pragma unroll
+        for (int k = 0; k < kBPieces; k++) {
+            const int e = tid + k * kThreads, row = (e >> 2) % kCols;
+            *reinterpret_cast<u4 *>(to + kABytes + (e >> 2) / kCols * (kCols * 64) + (row >> 6) * 4096 +
+                                       stored_place<NF>(row & 3, (row & 63) >> 2, e & 3)) = b_piece[k];
         }
 #pragma unroll
         for (int k = 0; k < kScaleRows; k++) {
             const int row = tid + k * kThreads;
-            if (row < kRows + kCols) {   // block g of either step next to each other: one 16-bit read serves both
-                *reinterpret_cast<uint2 *>(to + kCodeBytes + row * 8) =
-                    make_uint2(__builtin_amdgcn_perm(scale[k].y, scale[k].x, 0x05010400u),
-                               __builtin_amdgcn_perm(scale[k].y, scale[k].x, 0x07030602u));
+            if (row < kRows + kCols) {
+                const int place = row < kRows ? row : (row & ~63) | ((row & 3) * 16 + ((row & 63) >> 2));
+                uint8_t *const o = to + kABytes + kBBytes + place * 4 * U;
+                if constexpr (U == 2) {   // block g of either step next to each other
+                    *reinterpret_cast<uint2 *>(o) = make_uint2(__builtin_amdgcn_perm(scale[k][1], scale[k][0], 0x05010400u),
+                                                               __builtin_amdgcn_perm(scale[k][1], scale[k][0], 0x07030602u));
+                } else {
+                    *reinterpret_cast<uint32_t *>(o) = scale[k][0];
+                }
             }
         }
     };
-
-    // the wavefront's stored rows; those behind the last one repeat it
-    const int64_t wave_col = min<int64_t>(col0 + wn * 64, p.n - 1);
-    const uint8_t *const b_base = p.b_codes + wave_col * p.blocks * 16;
-    uint32_t b_row[NF];
-#pragma unroll
-    for (int j = 0; j < NF; j++) {
-        b_row[j] = (uint32_t)(min<int64_t>(j * 16 + r, p.n - 1 - wave_col) * p.blocks * 16);
-    }
-    uint4 next[NF];
-    auto fetch = [&](int t) {
-        const uint32_t b = (uint32_t)min(t * 4 + g, p.blocks - 1) * 16;   // behind the last block: it meets zeros
-#pragma unroll
-        for (int j = 0; j < NF; j++) {
-            next[j] = *reinterpret_cast<const uint4 *>(b_base + (b_row[j] + b));
-        }
-    };
+    using Scales = std::conditional_t<U == 2, uint16_t, uint8_t>;
 
     v4f acc[MF][NF] = {};
-    fetch(0);
     bring(0);
     put(0);
+    if (stages > 1) {
+        bring(1);
+    }
     __syncthreads();
     for (int stage = 0; stage < stages; stage++) {
         const uint8_t *const from = smem + (stage & 1) * kBuffer;
         if (stage + 1 < stages) {
-            bring(stage + 1);
+            put((stage + 1) & 1);
         }
+        if (stage + 2 < stages) {
+            bring(stage + 2);
+        }
+        const Scales *const sc = reinterpret_cast<const Scales *>(from + kABytes + kBBytes);
         int a_scale[MF], b_scale[NF];
 #pragma unroll
         for (int i = 0; i < MF; i++) {
-            a_scale[i] = *reinterpret_cast<const uint16_t *>(from + kCodeBytes + (wm * 128 + i * 16 + r) * 8 + g * 2);
+            a_scale[i] = sc[(wm * 128 + i * 16 + r) * 4 + g];
         }
 #pragma unroll
         for (int j = 0; j < NF; j++) {
-            b_scale[j] = *reinterpret_cast<const uint16_t *>(from + kCodeBytes + (kRows + wn * 64 + j * 16 + r) * 8 + g * 2);
+            b_scale[j] = sc[(kRows + wn * 64 + j * 16 + r) * 4 + g];
         }
         auto step = [&](auto which) {
             constexpr int u = decltype(which)::value;
             v8i b[NF];
 #pragma unroll
             for (int j = 0; j < NF; j++) {
-                b[j] = wide(next[j]);
+                b[j] = wide(*reinterpret_cast<const u4 *>(from + kABytes + u * (kCols * 64) + wn * 4096 +
+                                                             stored_place<NF>(j, r, g)));
             }
-            fetch(min(stage * 2 + u + 1, steps - 1));
 #pragma unroll
             for (int i = 0; i < MF; i++) {
-                uint4 w[kHalves];
+                u4 w[kHalves];
 #pragma unroll
                 for (int k = 0; k < kHalves; k++) {
-                    w[k] = *reinterpret_cast<const uint4 *>(from + (u * kHalves + k) * (kRows * 64) + (wm * 8 + i) * 1024 +
+                    w[k] = *reinterpret_cast<const u4 *>(from + (u * kHalves + k) * (kRows * 64) + (wm * 8 + i) * 1024 +
                                                             fragment_place(r, g));
                 }
                 AFragment<FA> a;
@@ -372,42 +402,35 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
             }
         };
         step(std::integral_constant<int, 0>());
-        if (stage * 2 + 1 < steps) {
-            step(std::integral_constant<int, 1>());
-        }
-        if (stage + 1 < stages) {
-            put((stage + 1) & 1);
+        if constexpr (U == 2) {
+            if (stage * 2 + 1 < steps) {
+                step(std::integral_constant<int, 1>());
+            }
         }
         __syncthreads();
     }
-    const bool l2 = p.metric == kMetricL2;
+    const int64_t col = col0 + wn * 64 + r * 4;
+    float b_sqr[NF] = {};
+    if (p.metric == kMetricL2 && col < p.n) {
+        load_run(p.b_sqr, col, p.n, b_sqr);
+    }
 #pragma unroll
-    for (int j = 0; j < NF; j++) {
-        const int64_t col = col0 + wn * 64 + j * 16 + g * 4;
-        if (col < p.n) {
-            float b_sqr[4] = {};
-            if (l2) {
-                load_norms(p.b_sqr, col, p.n, b_sqr);
-            }
-#pragma unroll
-            for (int i = 0; i < MF; i++) {
-                const int64_t row = row0 + wm * 128 + i * 16 + r;
-                if (row < p.m) {
-                    store_scores<T>(p, row, col, acc[i][j], l2 ? p.a_sqr[row] : 0.f, b_sqr);
-                }
-            }
-        }
+    for (int i = 0; i < MF; i++) {
+        store_scores<T, NF>(p, row0 + wm * 128 + i * 16 + g * 4, col, acc[i], b_sqr);
     }
 }
 
 template <int FA>
-size_t stream_lds(int mf, int steps) { return (size_t)steps * mf * 16 * ((FA == kE2M1 ? 64 : 128) + 4); }
+size_t stream_lds(int mf, int nf, int steps)
+{
+    return (size_t)steps * mf * 16 * ((FA == kE2M1 ? 64 : 128) + 4) + 4 * nf * (1024 + 64);
+}
 
 template <int FA, int MF, int NF, typename T>
 void launch_stream(const ProductParams &p, hipStream_t s)
 {
     const int steps = (p.blocks + 3) / 4;
-    const size_t lds = stream_lds<FA>(MF, steps);
+    const size_t lds = stream_lds<FA>(MF, NF, steps);
     const int64_t tiles = (p.n + NF * 16 - 1) / (NF * 16);
     const void *kern = reinterpret_cast<const void *>(mx_stream_kernel<FA, MF, NF, T>);
     require_dynamic_lds(kern, lds);
@@ -417,13 +440,13 @@ void launch_stream(const ProductParams &p, hipStream_t s)
     check_launch();
 }
 
-template <int FA, int WM, int WN, typename T>
+template <int FA, int WM, int WN, int U, typename T>
 void launch_tiles(const ProductParams &p, hipStream_t s)
 {
     const int64_t row_tiles = (p.m + WM * 128 - 1) / (WM * 128), col_tiles = (p.n + WN * 64 - 1) / (WN * 64);
     const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
     IXA_REQUIRE(per_xcd <= 0x0fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m, (long)p.n);
-    hipLaunchKernelGGL((mx_tile_kernel<FA, WM, WN, T>), dim3((unsigned)per_xcd * 8), dim3(WM * WN * 64), 0, s, p,
+    hipLaunchKernelGGL((mx_tile_kernel<FA, WM, WN, U, T>), dim3((unsigned)per_xcd * 8), dim3(WM * WN * 64), 0, s, p,
                        (int)row_tiles, (int)col_tiles, (int)per_xcd);
     check_launch();
 }
@@ -433,7 +456,7 @@ void launch_type(const ProductParams &p, hipStream_t s)
 {
     const int steps = (p.blocks + 3) / 4;
     const int mf = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
-    if (p.m <= 64 && stream_lds<FA>(mf, steps) <= 80 * 1024) {
+    if (p.m <= 64 && stream_lds<FA>(mf, 4, steps) <= 80 * 1024) {
         const bool narrow = p.n <= 16 * 4096;   // too few tiles of 64 rows for every wavefront slot
         if (mf == 1) {
             narrow ? launch_stream<FA, 1, 1, T>(p, s) : launch_stream<FA, 1, 4, T>(p, s);
@@ -445,9 +468,9 @@ void launch_type(const ProductParams &p, hipStream_t s)
         return;
     }
     if (p.m <= 128) {
-        launch_tiles<FA, 1, 4, T>(p, s);
+        launch_tiles<FA, 1, 4, 1, T>(p, s);
     } else {
-        launch_tiles<FA, 1, 4, T>(p, s);
+        launch_tiles<FA, 2, 4, FA == kE2M1 ? 2 : 1, T>(p, s);
     }
 }
 
