@@ -26,7 +26,6 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));   // 16 bytes of codes
 
 constexpr int kE4M3 = 0, kE2M1 = 4;   // operand formats of the instruction
-constexpr int kOne = 127;             // a block scale of 1
 
 struct ProductParams {
     const uint8_t *a_codes, *a_scales, *b_codes, *b_scales;
@@ -34,6 +33,7 @@ struct ProductParams {
     int64_t m, n, ld;
     int blocks, metric;
     void *out;
+    bool lines;   // rows of scores start on 64 bytes
 };
 
 __device__ __forceinline__ v8i wide(u4 lo) { return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, 0, 0, 0, 0}; }
@@ -87,6 +87,9 @@ __device__ __forceinline__ void load_run(const float *from, int64_t at, int64_t 
     }
 }
 
+// Scores are not read again here: where a wavefront's runs are whole lines of 64 bytes they pass the caches by, which leaves
+// these to the codes (2048 x 131072 x 768 to fp32: 360 -> 290 us); rows that start anywhere share lines, which the L2 has
+// to join (1024 x 199999 x 128: 210 us, past the caches 330).
 // The scores of a lane: queries row ... row + 3 (element i of the accumulators) and columns col ... col + NF - 1 (fragment j).
 template <typename T, int NF>
 __device__ __forceinline__ void store_scores(const ProductParams &p, int64_t row, int64_t col, const v4f (&acc)[NF],
@@ -103,7 +106,9 @@ __device__ __forceinline__ void store_scores(const ProductParams &p, int64_t row
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (row + i < p.m) {
-            T v[NF];
+            typedef T Scores __attribute__((ext_vector_type(NF)));
+            typedef T ScoresAnywhere __attribute__((ext_vector_type(NF), aligned(sizeof(T))));
+            Scores v;
 #pragma unroll
             for (int j = 0; j < NF; j++) {
                 const float g = acc[j][i];
@@ -111,7 +116,11 @@ __device__ __forceinline__ void store_scores(const ProductParams &p, int64_t row
             }
             T *o = static_cast<T *>(p.out) + (row + i) * p.ld + col;
             if (col + NF <= p.n) {
-                __builtin_memcpy(o, v, sizeof(v));
+                if (p.lines) {
+                    __builtin_nontemporal_store(v, reinterpret_cast<Scores *>(o));
+                } else {
+                    *reinterpret_cast<ScoresAnywhere *>(o) = v;
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < NF; j++) {
@@ -135,21 +144,27 @@ __device__ __forceinline__ int stored_place(int j, int r, int q)
     return j * 1024 + (NF > 1 ? r ^ (j & 1) : r) * 64 + ((q ^ ((r >> 1) & 3)) * 16);
 }
 
-// The scales of four blocks from block b on of the row that starts at `from`; behind the last block 1.
-__device__ __forceinline__ uint32_t four_scales(const uint8_t *from, int b, int blocks)
+// The scales of one row, four blocks at a time and in two parts so that nothing waits for the load: load_scales brings four
+// bytes from block b on or, at the end of the array, from `last`, where its last four begin (`few`: the number of scales of
+// an array that has less); take_scales shifts and masks them.  Blocks behind the last get scale 0, the smallest power of two:
+// the queries' codes are zeros there.
+__device__ __forceinline__ uint32_t load_scales(const uint8_t *from, const uint8_t *last, int few, int b)
 {
-    uint32_t w = 0x01010101u * kOne;
-    if (b + 4 <= blocks) {
-        __builtin_memcpy(&w, from + b, 4);
+    uint32_t w = 0;
+    if (few == 0) {
+        __builtin_memcpy(&w, from + b < last ? from + b : last, 4);
     } else {
-#pragma unroll
-        for (int i = 0; i < 3; i++) {
-            if (b + i < blocks) {
-                w = (w & ~(0xffu << (8 * i))) | (uint32_t)from[b + i] << (8 * i);
-            }
+        for (int i = 0; i < few; i++) {
+            w |= (uint32_t)last[i] << (8 * i);
         }
     }
     return w;
+}
+__device__ __forceinline__ uint32_t take_scales(uint32_t w, const uint8_t *from, const uint8_t *last, int b, int blocks)
+{
+    const int64_t over = from + b - last;
+    w >>= 8 * (over < 0 ? 0 : over > 3 ? 3 : (int)over);
+    return blocks - b >= 4 ? w : w & ((1u << (8 * max(blocks - b, 0))) - 1u);
 }
 
 // Few queries: their codes stay in LDS (MF fragments of 16 rows, all columns) while every wavefront streams NF fragments of
@@ -182,10 +197,17 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
     }
     for (int e = threadIdx.x; e < steps * kRows; e += 256) {
         const int row = e % kRows;
+        const uint8_t *from = p.a_scales + min(row0 + row, p.m - 1) * p.blocks;
+        const int64_t total = p.m * p.blocks;
+        const uint8_t *last = p.a_scales + (total > 4 ? total - 4 : 0);
+        const int b = e / kRows * 4;
         reinterpret_cast<uint32_t *>(scales)[e] =
-            row0 + row < p.m ? four_scales(p.a_scales + (row0 + row) * p.blocks, e / kRows * 4, p.blocks) : 0x01010101u * kOne;
+            take_scales(load_scales(from, last, total < 4 ? (int)total : 0, b), from, last, b, p.blocks);
     }
     __syncthreads();
+    const int64_t b_total = p.n * p.blocks;
+    const uint8_t *const scale_last = p.b_scales + (b_total > 4 ? b_total - 4 : 0);
+    const int scale_few = b_total < 4 ? (int)b_total : 0;
     const int64_t stride = (int64_t)gridDim.x * 4;
     for (int64_t tile = (int64_t)blockIdx.x * 4 + wave; tile < tiles; tile += stride) {
         const int64_t col0 = tile * (NF * 16);
@@ -196,7 +218,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
         for (int k = 0; k < NF; k++) {
             offset[k] = (uint32_t)(min(k * 16 + (lane >> 2), last) * b_row_bytes);
         }
-        const uint8_t *const scale_row = p.b_scales + (col0 + min(lane, last)) * p.blocks;
+        const uint8_t *const scale_from = p.b_scales + (col0 + min(lane, last)) * p.blocks;
         u4 next[NF];
         uint32_t next_scale = 0;
         // pieces behind the last block repeat it: the queries' codes are zeros there
@@ -207,7 +229,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
                 next[k] = *reinterpret_cast<const u4 *>(codes + (offset[k] + byte));
             }
             if (NF == 4 || lane < NF * 16) {
-                next_scale = four_scales(scale_row, t * 4, p.blocks);
+                next_scale = load_scales(scale_from, scale_last, scale_few, t * 4);
             }
         };
         fetch(0);
@@ -219,7 +241,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
                 *reinterpret_cast<u4 *>(turn + stored_place<NF>(row % NF, row / NF, lane & 3)) = next[k];
             }
             if (NF == 4 || lane < NF * 16) {
-                reinterpret_cast<uint32_t *>(turn_scales)[(lane % NF) * 16 + lane / NF] = next_scale;
+                reinterpret_cast<uint32_t *>(turn_scales)[(lane % NF) * 16 + lane / NF] = take_scales(next_scale, scale_from, scale_last, t * 4, p.blocks);
             }
             if (t + 1 < steps) {
                 fetch(t + 1);
@@ -265,11 +287,11 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
 // Many queries: tiles of WM * 128 queries by WN * 64 stored rows, one wavefront per 128 x 64 of them (8 x 4 fragments).  Codes
 // and scales of both sides go through two LDS buffers of U steps (128 columns each); while one is multiplied, the next is
 // written from registers and the one after it is on its way from memory.
-template <int FA, int WM, int WN, int U, typename T>
-__global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
+template <int FA, int WM, int WN, int MF, int U, typename T>
+__global__ __launch_bounds__(WM * WN * 64, MF == 8 || FA == kE4M3 ? 2 : 3) void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
-    constexpr int kHalves = FA == kE2M1 ? 1 : 2, MF = 8, NF = 4, kThreads = WM * WN * 64;
-    constexpr int kRows = WM * 128, kCols = WN * 64;
+    constexpr int kHalves = FA == kE2M1 ? 1 : 2, NF = 4, kThreads = WM * WN * 64;
+    constexpr int kRows = WM * MF * 16, kCols = WN * 64;
     constexpr int kABytes = kRows * 64 * kHalves * U, kBBytes = kCols * 64 * U;
     constexpr int kAPieces = kABytes / 16 / kThreads, kBPieces = kBBytes / 16 / kThreads;   // per thread
     constexpr int kScaleRows = (kRows + kCols + kThreads - 1) / kThreads;
@@ -278,7 +300,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
     __shared__ __align__(16) uint8_t smem[2 * kBuffer];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
-    // workgroup b runs on XCD b mod 8: each gets a contiguous run of tiles, eight query tiles high
     const int64_t id = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     if (id >= (int64_t)row_tiles * col_tiles) {
         return;
@@ -294,13 +315,25 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
     const int last_row = (int)min<int64_t>(kRows, p.m - row0) - 1, last_col = (int)min<int64_t>(kCols, p.n - col0) - 1;
     u4 a_piece[kAPieces], b_piece[kBPieces];
     uint32_t scale[kScaleRows][U];
-    auto bring = [&](int stage) {   // from memory into registers; queries' codes behind the last block are zeros
+    // the rows whose scales a thread brings
+    const uint8_t *scale_from[kScaleRows], *scale_last[kScaleRows];
+    int scale_few[kScaleRows];
+#pragma unroll
+    for (int k = 0; k < kScaleRows; k++) {
+        const int row = tid + k * kThreads;
+        const bool query = row < kRows;
+        const int64_t total = (query ? p.m : p.n) * p.blocks;
+        const uint8_t *const begin = query ? p.a_scales : p.b_scales;
+        scale_from[k] = begin + (query ? row0 + min(row, last_row) : col0 + min(row - kRows, last_col)) * p.blocks;
+        scale_last[k] = begin + (total > 4 ? total - 4 : 0);
+        scale_few[k] = total < 4 ? (int)total : 0;
+    }
+    auto bring = [&](int stage) {   // from memory into registers
 #pragma unroll
         for (int k = 0; k < kAPieces; k++) {
             const int e = tid + k * kThreads, row = min((e >> 2) % kRows, last_row);
             const int byte = (stage * U * kHalves + (e >> 2) / kRows) * 64 + (e & 3) * 16;
-            const u4 v = *reinterpret_cast<const u4 *>(a_base + (uint32_t)(row * a_row_bytes + min(byte, a_row_bytes - 16)));
-            a_piece[k] = byte < a_row_bytes ? v : u4{};
+            a_piece[k] = *reinterpret_cast<const u4 *>(a_base + (uint32_t)(row * a_row_bytes + min(byte, a_row_bytes - 16)));
         }
 #pragma unroll
         for (int k = 0; k < kBPieces; k++) {
@@ -312,22 +345,21 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
         for (int k = 0; k < kScaleRows; k++) {
             const int row = tid + k * kThreads;
             if (row < kRows + kCols) {
-                const uint8_t *from = row < kRows ? p.a_scales + (row0 + min(row, last_row)) * p.blocks
-                                                  : p.b_scales + (col0 + min(row - kRows, last_col)) * p.blocks;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    scale[k][u] = four_scales(from, (stage * U + u) * 4, p.blocks);
+                    scale[k][u] = load_scales(scale_from[k], scale_last[k], scale_few[k], (stage * U + u) * 4);
                 }
             }
         }
     };
-    auto put = [&](int buffer) {    // from registers into LDS
-        uint8_t *const to = smem + buffer * kBuffer;
+    auto put = [&](int stage) {     // from registers into LDS; queries' codes behind the last block are zeros
+        uint8_t *const to = smem + (stage & 1) * kBuffer;
 #pragma unroll
         for (int k = 0; k < kAPieces; k++) {
             const int e = tid + k * kThreads, row = (e >> 2) % kRows;
+            const int byte = (stage * U * kHalves + (e >> 2) / kRows) * 64 + (e & 3) * 16;
             *reinterpret_cast<u4 *>(to + (e >> 2) / kRows * (kRows * 64) + (row >> 4) * 1024 + fragment_place(row & 15, e & 3)) =
-                a_piece[k];
+                byte < a_row_bytes ? a_piece[k] : u4{};
         }
 #pragma unroll
         for (int k = 0; k < kBPieces; k++) {
@@ -341,6 +373,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
             if (row < kRows + kCols) {
                 const int place = row < kRows ? row : (row & ~63) | ((row & 3) * 16 + ((row & 63) >> 2));
                 uint8_t *const o = to + kABytes + kBBytes + place * 4 * U;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    scale[k][u] = take_scales(scale[k][u], scale_from[k], scale_last[k], (stage * U + u) * 4, p.blocks);
+                }
                 if constexpr (U == 2) {   // block g of either step next to each other
                     *reinterpret_cast<uint2 *>(o) = make_uint2(__builtin_amdgcn_perm(scale[k][1], scale[k][0], 0x05010400u),
                                                                __builtin_amdgcn_perm(scale[k][1], scale[k][0], 0x07030602u));
@@ -362,7 +398,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
     for (int stage = 0; stage < stages; stage++) {
         const uint8_t *const from = smem + (stage & 1) * kBuffer;
         if (stage + 1 < stages) {
-            put((stage + 1) & 1);
+            put(stage + 1);
         }
         if (stage + 2 < stages) {
             bring(stage + 2);
@@ -371,7 +407,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
         int a_scale[MF], b_scale[NF];
 #pragma unroll
         for (int i = 0; i < MF; i++) {
-            a_scale[i] = sc[(wm * 128 + i * 16 + r) * 4 + g];
+            a_scale[i] = sc[((wm * MF + i) * 16 + r) * 4 + g];
         }
 #pragma unroll
         for (int j = 0; j < NF; j++) {
@@ -390,7 +426,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
                 u4 w[kHalves];
 #pragma unroll
                 for (int k = 0; k < kHalves; k++) {
-                    w[k] = *reinterpret_cast<const u4 *>(from + (u * kHalves + k) * (kRows * 64) + (wm * 8 + i) * 1024 +
+                    w[k] = *reinterpret_cast<const u4 *>(from + (u * kHalves + k) * (kRows * 64) + (wm * MF + i) * 1024 +
                                                             fragment_place(r, g));
                 }
                 AFragment<FA> a;
@@ -416,7 +452,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_tile_kernel(ProductParams 
     }
 #pragma unroll
     for (int i = 0; i < MF; i++) {
-        store_scores<T, NF>(p, row0 + wm * 128 + i * 16 + g * 4, col, acc[i], b_sqr);
+        store_scores<T, NF>(p, row0 + (wm * MF + i) * 16 + g * 4, col, acc[i], b_sqr);
     }
 }
 
@@ -440,13 +476,13 @@ void launch_stream(const ProductParams &p, hipStream_t s)
     check_launch();
 }
 
-template <int FA, int WM, int WN, int U, typename T>
+template <int FA, int WM, int WN, int MF, int U, typename T>
 void launch_tiles(const ProductParams &p, hipStream_t s)
 {
-    const int64_t row_tiles = (p.m + WM * 128 - 1) / (WM * 128), col_tiles = (p.n + WN * 64 - 1) / (WN * 64);
+    const int64_t row_tiles = (p.m + WM * MF * 16 - 1) / (WM * MF * 16), col_tiles = (p.n + WN * 64 - 1) / (WN * 64);
     const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
     IXA_REQUIRE(per_xcd <= 0x0fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m, (long)p.n);
-    hipLaunchKernelGGL((mx_tile_kernel<FA, WM, WN, U, T>), dim3((unsigned)per_xcd * 8), dim3(WM * WN * 64), 0, s, p,
+    hipLaunchKernelGGL((mx_tile_kernel<FA, WM, WN, MF, U, T>), dim3((unsigned)per_xcd * 8), dim3(WM * WN * 64), 0, s, p,
                        (int)row_tiles, (int)col_tiles, (int)per_xcd);
     check_launch();
 }
@@ -467,10 +503,13 @@ void launch_type(const ProductParams &p, hipStream_t s)
         }
         return;
     }
-    if (p.m <= 128) {
-        launch_tiles<FA, 1, 4, 1, T>(p, s);
+    const int64_t tiles = ((p.m + 127) / 128) * ((p.n + 255) / 256);
+    if (tiles < 512) {
+        launch_tiles<FA, 1, 4, 4, 1, T>(p, s);
+    } else if (p.m <= 128 || p.blocks <= 64) {
+        launch_tiles<FA, 1, 4, 8, 1, T>(p, s);
     } else {
-        launch_tiles<FA, 2, 4, FA == kE2M1 ? 2 : 1, T>(p, s);
+        launch_tiles<FA, 2, 4, 8, FA == kE2M1 ? 2 : 1, T>(p, s);
     }
 }
 
@@ -512,7 +551,8 @@ void op_mx_product(const uint8_t *a_codes, const uint8_t *a_scales, int a_format
     if (m == 0 || n == 0) {
         return;
     }
-    const ProductParams p{a_codes, a_scales, b_codes, b_scales, a_sqr, b_sqr, m, n, ld, mx_blocks(d), metric, out};
+    const ProductParams p{a_codes, a_scales, b_codes, b_scales, a_sqr, b_sqr, m, n, ld, mx_blocks(d), metric, out,
+                          aligned(out, 64) && ld * (out_type == kTypeF32 ? 4 : 2) % 64 == 0};
     if (a_format == kFormatMxFp4) {
         launch<kE2M1>(p, out_type, s);
     } else {
