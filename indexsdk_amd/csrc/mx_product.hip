@@ -15,6 +15,9 @@
 #include "lowp.h"
 
 #include <algorithm>
+#include <map>
+#include <mutex>
+#include <tuple>
 #include <type_traits>
 
 namespace ixa {
@@ -153,10 +156,8 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t *from, const uint8
     uint32_t w = 0;
     if (few == 0) {
         __builtin_memcpy(&w, from + b < last ? from + b : last, 4);
-    } else {
-        for (int i = 0; i < few; i++) {
-            w |= (uint32_t)last[i] << (8 * i);
-        }
+    } else {   // no loop: around one the compiler waits for every load in flight
+        w = last[0] | (few > 1 ? (uint32_t)last[1] << 8 : 0u) | (few > 2 ? (uint32_t)last[2] << 16 : 0u);
     }
     return w;
 }
@@ -456,6 +457,21 @@ __global__ __launch_bounds__(WM * WN * 64, MF == 8 || FA == kE4M3 ? 2 : 3) void 
     }
 }
 
+// Workgroups of a kernel that the GPU runs at a time.
+int64_t resident_workgroups(const void *kern, int threads, size_t lds)
+{
+    static std::mutex mu;
+    static std::map<std::tuple<const void *, int, size_t>, int64_t> known;
+    std::lock_guard<std::mutex> lock(mu);
+    int64_t &count = known[std::make_tuple(kern, threads, lds)];
+    if (count == 0) {
+        int per_cu = 0;
+        IXA_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, threads, lds));
+        count = std::max(1, per_cu) * 256;
+    }
+    return count;
+}
+
 template <int FA>
 size_t stream_lds(int mf, int nf, int steps)
 {
@@ -470,8 +486,7 @@ void launch_stream(const ProductParams &p, hipStream_t s)
     const int64_t tiles = (p.n + NF * 16 - 1) / (NF * 16);
     const void *kern = reinterpret_cast<const void *>(mx_stream_kernel<FA, MF, NF, T>);
     require_dynamic_lds(kern, lds);
-    const int64_t resident = std::max<int64_t>(1, std::min<int64_t>(6, 160 * 1024 / (int64_t)lds)) * 256;
-    const dim3 grid((unsigned)std::min((tiles + 3) / 4, resident), (unsigned)((p.m + MF * 16 - 1) / (MF * 16)));
+    const dim3 grid((unsigned)std::min((tiles + 3) / 4, resident_workgroups(kern, 256, lds)), (unsigned)((p.m + MF * 16 - 1) / (MF * 16)));
     hipLaunchKernelGGL((mx_stream_kernel<FA, MF, NF, T>), grid, dim3(256), lds, s, p, steps, tiles);
     check_launch();
 }
