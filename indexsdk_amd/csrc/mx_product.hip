@@ -457,6 +457,309 @@ __global__ __launch_bounds__(WM * WN * 64, MF == 8 || FA == kE4M3 ? 2 : 3) void 
     }
 }
 
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+// v_mfma_scale_f32_32x32x64_f8f6f4: 32 x 64 by 64 x 32 codes, lane = row l & 31, half h = l >> 5.  In 4 bits the lane holds the
+// 16 bytes of block h; in 8 bits bytes 16 h ... of block 0 and of block 1; its scores are of stored row l & 31 and queries
+// 8 (i / 4) + 4 h + i mod 4.  It issues at 7.5 PFLOP/s of 4-bit products where the 16 x 16 one stops at 5.8.
+template <int FA, int BYTE>
+__device__ __forceinline__ v16f multiply32(const AFragment<FA> &a, int a_scale, const v8i &b, int b_scale, v16f c)
+{
+    if constexpr (FA == kE2M1) {
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.v, b, c, kE2M1, kE2M1, BYTE, a_scale, BYTE, b_scale);
+    } else {
+        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.small, b, c, kE4M3, kE2M1, BYTE, a_scale, BYTE, b_scale);
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.large, b, c, kE4M3, kE2M1, BYTE, a_scale, BYTE, b_scale);
+    }
+}
+
+// A 16-byte piece of row r of 32 rows of 64 bytes in LDS.  The 32 lanes of a half read one piece of 32 rows; of these, rows
+// 0-3, 12-15, 20-23 and 24-27 go together, and the other sixteen: with this swap they are in all banks.
+__device__ __forceinline__ int wide_place(int r, int q) { return r * 64 + ((q ^ ((r >> 2) & 3)) * 16); }
+
+// Many queries and many columns: tiles of 256 queries by 256 stored rows, four wavefronts of 128 x 128 (4 x 4 fragments of
+// 32 rows), one to a SIMD with 512 registers: twice the products per byte read from LDS of the kernel above.  Codes go
+// from memory straight into a ring of R LDS buffers, one step of 128 columns each, scales into two buffers of four steps.  A
+// half-step of 64 columns reads the next one's fragments of stored rows while it multiplies its own, so that no wavefront
+// meets a barrier without products to do.  Whole groups of four steps and 16-byte aligned scales only.
+template <int FA, int R, typename T>
+__global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int row_tiles, int col_tiles, int64_t per_xcd)
+{
+    constexpr int kHalves = FA == kE2M1 ? 1 : 2, kTile = 256, F = 4;
+    constexpr int kABytes = kTile * 64 * kHalves, kBBytes = kTile * 64, kBuffer = kABytes + kBBytes;
+    constexpr int kScaleBytes = 2 * kTile * 16;                       // of both sides, four steps
+    constexpr int kLoads = 4 * kHalves + 4;                           // 1 KB each, per wavefront and step
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t *const scale_lds = smem + R * kBuffer;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+    const int steps = p.blocks >> 2;
+    const int a_row_bytes = p.blocks * 16 * kHalves, b_row_bytes = p.blocks * 16;
+    // Workgroup b runs on XCD b mod 8: each gets a contiguous run of tiles, eight query tiles high, and its workgroups take
+    // them in turn, so that those at work at a time lie next to each other.
+    const int64_t end = min((int64_t)(blockIdx.x & 7) * per_xcd + per_xcd, (int64_t)row_tiles * col_tiles);
+    int64_t id = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (id >= end) {
+        return;
+    }
+
+    // LDS holds 16 rows of 64 bytes in 1 KB (wide_place); a wavefront loads runs wave, wave + 4, ... of either side, lane l
+    // the piece that belongs at place l & 3 of row l >> 2.  Stored row 4 r + j of each 128 is row r of fragment j, so that
+    // a lane ends up with four scores in a row; rows behind the last one repeat it.
+    const int fr = lane >> 2, fq = (lane & 3) ^ ((fr >> 2) & 3);
+    int64_t row0, col0;
+    const uint8_t *a_base, *b_base, *a_scale_from, *b_scale_from;
+    uint32_t a_from[4], b_from[4];
+    auto set_tile = [&]() {
+        const int64_t band = id / (8 * (int64_t)col_tiles);
+        const int high = min(8, row_tiles - (int)band * 8);
+        const int64_t in = id - band * 8 * col_tiles;
+        row0 = (band * 8 + in % high) * kTile;
+        col0 = in / high * kTile;
+        a_base = p.a_codes + row0 * a_row_bytes;
+        b_base = p.b_codes + col0 * b_row_bytes;
+        const int last_row = (int)min<int64_t>(kTile, p.m - row0) - 1, last_col = (int)min<int64_t>(kTile, p.n - col0) - 1;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            a_from[k] = (uint32_t)(min((wave + 4 * k) * 16 + fr, last_row) * a_row_bytes + fq * 16);
+            const int run = wave + 4 * k;   // of 128 rows run >> 3, fragment (run >> 1) & 3, rows 16 (run & 1) ...
+            b_from[k] = (uint32_t)(min((run >> 3) * 128 + ((run & 1) * 16 + fr) * 4 + ((run >> 1) & 3), last_col) * b_row_bytes + fq * 16);
+        }
+        // rows of scales, 16 bytes each, in the order of the fragments' rows
+        const int scale_run = wave * 2 + (lane >> 5);   // 32 rows: of 128 rows scale_run >> 2, fragment scale_run & 3
+        a_scale_from = p.a_scales + (row0 + min(wave * 64 + lane, last_row)) * p.blocks;
+        b_scale_from = p.b_scales + (col0 + min((scale_run >> 2) * 128 + r * 4 + (scale_run & 3), last_col)) * p.blocks;
+    };
+    auto load_lds = [&](const uint8_t *from, uint8_t *to) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                         (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+    };
+    auto issue = [&](int step, int k) {   // a quarter of a step's codes
+        if (k == 0 && (step & 3) == 0) {
+            uint8_t *const to = scale_lds + (step >> 2 & 1) * kScaleBytes + wave * 1024;
+            load_lds(a_scale_from + step * 4, to);
+            load_lds(b_scale_from + step * 4, to + kTile * 16);
+        }
+        uint8_t *const to = smem + step % R * kBuffer + wave * 1024 + k * 4096;
+#pragma unroll
+        for (int half = 0; half < kHalves; half++) {
+            load_lds(a_base + (step * kHalves + half) * 64 + a_from[k], to + half * (kTile * 64));
+        }
+        load_lds(b_base + step * 64 + b_from[k], to + kABytes);
+    };
+
+    v16f acc[F][F] = {};
+    u4 a[2][2][kHalves], b[2][F];   // of two blocks of two query fragments; of two half-steps
+    auto read_b = [&](int step, int half, int j) {
+        return *reinterpret_cast<const u4 *>(smem + step % R * kBuffer + kABytes + (wn * 4 + j) * 2048 +
+                                             wide_place(r, half * 2 + h));
+    };
+    auto read_a = [&](int step, int half, int i, u4 (&v)[kHalves]) {
+        const uint8_t *const from = smem + step % R * kBuffer + (wm * 4 + i) * 2048;
+        if constexpr (FA == kE2M1) {
+            v[0] = *reinterpret_cast<const u4 *>(from + wide_place(r, half * 2 + h));
+        } else {
+            v[0] = *reinterpret_cast<const u4 *>(from + half * (kTile * 64) + wide_place(r, h));
+            v[1] = *reinterpret_cast<const u4 *>(from + half * (kTile * 64) + wide_place(r, 2 + h));
+        }
+    };
+    // blocks h of four half-steps in the bytes of one register, two registers for four steps, of row r of a fragment
+    const uint32_t pick = 0x06040200u + 0x01010101u * h;
+    auto read_scales = [&](int step, int row) {
+        return *reinterpret_cast<const u4 *>(scale_lds + (step >> 2 & 1) * kScaleBytes + (row + r) * 16);
+    };
+    auto block_scales = [&](u4 w, int (&sc)[2]) {
+        sc[0] = (int)__builtin_amdgcn_perm(w[1], w[0], pick);
+        sc[1] = (int)__builtin_amdgcn_perm(w[3], w[2], pick);
+    };
+    int a_scale[F][2], b_scale[F][2], a_scale_next[F][2], b_scale_next[F][2];
+    const int a_row = wm * 128, b_row = kTile + wn * 128;
+
+    auto one = [&](int step, auto which) {
+        constexpr int u = decltype(which)::value;
+        const int after = u < 3 ? step + 1 : min(step + 1, steps - 1);
+        // every wavefront is done with the step before: its place in the ring is free
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        auto half_step = [&](auto which_half) {
+            constexpr int half = decltype(which_half)::value;
+            const int next_step = half == 0 ? step : after;
+#pragma unroll
+            for (int i = 0; i < F; i += 2) {   // eight products at a time
+                AFragment<FA> f;
+                f.set(a[i >> 1][0]);
+                acc[i][0] = multiply32<FA, (u & 1) * 2 + half>(f, a_scale[i][u >> 1], wide(b[half][0]), b_scale[0][u >> 1], acc[i][0]);
+                // the reads for the next eight start behind the first of these, whose operands were waited for with all
+                // others in flight, and have the time of the other seven
+                asm volatile("" : "+a"(acc[i][0]) : : "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                if (step + R - 1 < steps) {
+                    issue(step + R - 1, half * 2 + (i >> 1));
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    read_a(i == 0 ? step : next_step, i == 0 ? half : half ^ 1, i == 0 ? 2 + k : k, a[(i >> 1) ^ 1][k]);
+                    b[half ^ 1][i + k] = read_b(next_step, half ^ 1, i + k);
+                }
+                u4 ws[2][2];
+                if constexpr (u == 3 && half == 1) {
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        ws[k][0] = read_scales(after, a_row + (i + k) * 32);
+                        ws[k][1] = read_scales(after, b_row + (i + k) * 32);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    if (k == 1) {
+                        f.set(a[i >> 1][1]);
+                    }
+#pragma unroll
+                    for (int j = 1 - k; j < F; j++) {
+                        acc[i + k][j] = multiply32<FA, (u & 1) * 2 + half>(f, a_scale[i + k][u >> 1], wide(b[half][j]),
+                                                                           b_scale[j][u >> 1], acc[i + k][j]);
+                    }
+                }
+                asm volatile(""
+                             : "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]), "+a"(acc[i + 1][0]), "+a"(acc[i + 1][1]),
+                               "+a"(acc[i + 1][2]), "+a"(acc[i + 1][3])
+                             :
+                             : "memory");
+                if constexpr (u == 3 && half == 1) {
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        block_scales(ws[k][0], a_scale_next[i + k]);
+                        block_scales(ws[k][1], b_scale_next[i + k]);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        half_step(std::integral_constant<int, 0>());
+        // the other half reads ahead from the next step: its codes have to be there, what was issued later (half of a step's
+        // loads and R - 3 steps' before) may be on its way
+        if (step + R - 1 < steps) {
+            constexpr int kLater = (R - 3) * kLoads + kLoads / 2;
+            __builtin_amdgcn_s_waitcnt(0x0f70 | (kLater & 15) | (kLater >> 4) << 14);
+        } else {
+            __builtin_amdgcn_s_waitcnt(0x0f70);
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        half_step(std::integral_constant<int, 1>());
+        if constexpr (u == 3) {
+#pragma unroll
+            for (int i = 0; i < F; i++) {
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    a_scale[i][k] = a_scale_next[i][k];
+                    b_scale[i][k] = b_scale_next[i][k];
+                }
+            }
+        }
+    };
+    auto begin = [&]() {
+        set_tile();
+#pragma unroll
+        for (int k = 0; k < R - 1; k++) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                issue(k, q);
+            }
+        }
+    };
+    begin();
+    for (;;) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < F; j++) {
+            b[0][j] = read_b(0, 0, j);
+            block_scales(read_scales(0, b_row + j * 32), b_scale[j]);
+            block_scales(read_scales(0, a_row + j * 32), a_scale[j]);
+        }
+        read_a(0, 0, 0, a[0][0]);
+        read_a(0, 0, 1, a[0][1]);
+        for (int step = 0; step < steps; step += 4) {
+            one(step, std::integral_constant<int, 0>());
+            one(step + 1, std::integral_constant<int, 1>());
+            one(step + 2, std::integral_constant<int, 2>());
+            one(step + 3, std::integral_constant<int, 3>());
+        }
+        // the next tile's first codes are on their way while this one's scores leave, once nobody reads the last step's
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int64_t row = row0 + wm * 128 + h * 4, col = col0 + wn * 128 + r * 4;
+        const bool inside = row0 + kTile <= p.m && col0 + kTile <= p.n && p.lines;
+        id += gridDim.x >> 3;
+        if (id < end) {
+            begin();
+        }
+        float b_sqr[4] = {};
+        if (p.metric == kMetricL2 && col < p.n) {
+            load_run(p.b_sqr, col, p.n, b_sqr);
+        }
+        if (inside) {
+            const bool l2 = p.metric == kMetricL2;
+            typedef T Scores __attribute__((ext_vector_type(4)));
+            T *o = static_cast<T *>(p.out) + row * p.ld + col;
+            const int64_t up = p.ld * (int64_t)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < F; i++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    float a_sqr[4] = {};
+                    if (l2) {
+                        load_run(p.a_sqr, row + i * 32 + k * 8, p.m, a_sqr);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        Scores v;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float x = acc[i][j][4 * k + e];
+                            v[j] = (T)(l2 ? (a_sqr[e] + b_sqr[j]) - x - x : x);
+                        }
+                        __builtin_nontemporal_store(v, reinterpret_cast<Scores *>(reinterpret_cast<uint8_t *>(o) + (i * 32 + k * 8 + e) * up));
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < F; i++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    v4f part[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        part[j] = v4f{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+                    }
+                    store_scores<T, 4>(p, row + i * 32 + k * 8, col, part, b_sqr);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < F; i++) {
+#pragma unroll
+            for (int j = 0; j < F; j++) {
+                acc[i][j] = v16f{};
+            }
+        }
+        if (id >= end) {
+            return;
+        }
+    }
+}
+
+bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
 // Workgroups of a kernel that the GPU runs at a time.
 int64_t resident_workgroups(const void *kern, int threads, size_t lds)
 {
@@ -503,6 +806,21 @@ void launch_tiles(const ProductParams &p, hipStream_t s)
 }
 
 template <int FA, typename T>
+void launch_wide(const ProductParams &p, hipStream_t s)
+{
+    constexpr int R = FA == kE2M1 ? 4 : 3;
+    constexpr size_t lds = R * (256 * 64 * (FA == kE2M1 ? 2 : 3)) + 2 * 512 * 16;
+    const int64_t row_tiles = (p.m + 255) / 256, col_tiles = (p.n + 255) / 256;
+    const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
+    const void *kern = reinterpret_cast<const void *>(mx_wide_kernel<FA, R, T>);
+    require_dynamic_lds(kern, lds);
+    const int64_t grid = std::min(per_xcd * 8, resident_workgroups(kern, 256, lds));
+    hipLaunchKernelGGL((mx_wide_kernel<FA, R, T>), dim3((unsigned)grid), dim3(256), lds, s, p, (int)row_tiles, (int)col_tiles,
+                       per_xcd);
+    check_launch();
+}
+
+template <int FA, typename T>
 void launch_type(const ProductParams &p, hipStream_t s)
 {
     const int steps = (p.blocks + 3) / 4;
@@ -519,6 +837,10 @@ void launch_type(const ProductParams &p, hipStream_t s)
         return;
     }
     const int64_t tiles = ((p.m + 127) / 128) * ((p.n + 255) / 256);
+    if (p.blocks % 16 == 0 && p.m >= 256 && aligned(p.a_scales, 16) && aligned(p.b_scales, 16)) {
+        launch_wide<FA, T>(p, s);
+        return;
+    }
     if (tiles < 512) {
         launch_tiles<FA, 1, 4, 4, 1, T>(p, s);
     } else if (p.m <= 128 || p.blocks <= 64) {
@@ -539,8 +861,6 @@ void launch(const ProductParams &p, int out_type, hipStream_t s)
         launch_type<FA, __bf16>(p, s);
     }
 }
-
-bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 }  // namespace
 

@@ -394,7 +394,9 @@ def check_product(lib, m, n, d, a_fmt, metric, kind, wild, pad=0, seed=0):
 SHAPES = [(1, 1, 1), (1, 33, 32), (2, 31, 33), (31, 64, 64), (32, 32, 65), (33, 100, 96), (7, 1000, 128), (64, 257, 200),
           (65, 300, 256), (100, 129, 257), (127, 513, 288), (128, 256, 300), (129, 1025, 512), (200, 255, 520), (16, 4097, 768),
           (256, 512, 1000), (257, 700, 1030), (300, 1300, 64), (40, 600, 4096), (130, 300, 2080), (5, 70, 16384),
-          (520, 770, 16), (1000, 1024, 160)]
+          (520, 770, 16), (1000, 1024, 160),
+          # whole groups of 512 columns, tiles of 256 by 256 and their edges
+          (256, 256, 512), (256, 1, 500), (300, 700, 2048), (513, 260, 1024), (1030, 2100, 1536), (257, 515, 4096)]
 
 
 @pytest.mark.parametrize("m,n,d", SHAPES)
