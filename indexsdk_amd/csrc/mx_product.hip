@@ -483,7 +483,7 @@ __device__ __forceinline__ int wide_place(int r, int q) { return r * 64 + ((q ^ 
 // half-step of 64 columns reads the next one's fragments of stored rows while it multiplies its own, so that no wavefront
 // meets a barrier without products to do.  Whole groups of four steps and 16-byte aligned scales only.
 template <int FA, int R, typename T>
-__global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int row_tiles, int col_tiles, int64_t per_xcd)
+__global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
     constexpr int kHalves = FA == kE2M1 ? 1 : 2, kTile = 256, F = 4;
     constexpr int kABytes = kTile * 64 * kHalves, kBBytes = kTile * 64, kBuffer = kABytes + kBBytes;
@@ -497,8 +497,8 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
     const int a_row_bytes = p.blocks * 16 * kHalves, b_row_bytes = p.blocks * 16;
     // Workgroup b runs on XCD b mod 8: each gets a contiguous run of tiles, eight query tiles high, and its workgroups take
     // them in turn, so that those at work at a time lie next to each other.
-    const int64_t end = min((int64_t)(blockIdx.x & 7) * per_xcd + per_xcd, (int64_t)row_tiles * col_tiles);
-    int64_t id = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    const int end = min((int)(blockIdx.x & 7) * per_xcd + per_xcd, row_tiles * col_tiles);
+    int id = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
     if (id >= end) {
         return;
     }
@@ -507,15 +507,13 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
     // the piece that belongs at place l & 3 of row l >> 2.  Stored row 4 r + j of each 128 is row r of fragment j, so that
     // a lane ends up with four scores in a row; rows behind the last one repeat it.
     const int fr = lane >> 2, fq = (lane & 3) ^ ((fr >> 2) & 3);
-    int64_t row0, col0;
+    int64_t row0, col0;   // of the tile whose codes are loaded
     const uint8_t *a_base, *b_base, *a_scale_from, *b_scale_from;
     uint32_t a_from[4], b_from[4];
     auto set_tile = [&]() {
-        const int64_t band = id / (8 * (int64_t)col_tiles);
-        const int high = min(8, row_tiles - (int)band * 8);
-        const int64_t in = id - band * 8 * col_tiles;
-        row0 = (band * 8 + in % high) * kTile;
-        col0 = in / high * kTile;
+        const int band = id / (8 * col_tiles), in = id - band * 8 * col_tiles, high = min(8, row_tiles - band * 8);
+        row0 = (int64_t)(band * 8 + in % high) * kTile;
+        col0 = (int64_t)(in / high) * kTile;
         a_base = p.a_codes + row0 * a_row_bytes;
         b_base = p.b_codes + col0 * b_row_bytes;
         const int last_row = (int)min<int64_t>(kTile, p.m - row0) - 1, last_col = (int)min<int64_t>(kTile, p.n - col0) - 1;
@@ -534,13 +532,16 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
                                          (__attribute__((address_space(3))) void *)to, 16, 0, 0);
     };
-    auto issue = [&](int step, int k) {   // a quarter of a step's codes
+    int done = 0;   // steps of the tiles before: step `step` of this one lies at place (done + step) % R of the ring
+    auto slot = [&](int step) { return R == 4 ? step & 3 : (done + step) % R; };   // done is a multiple of 4
+    auto scales_of = [&](int step) { return scale_lds + ((done + step) >> 2 & 1) * kScaleBytes; };
+    auto issue = [&](int step, int place, int k) {   // a quarter of the codes of a step into the place of step `place`
         if (k == 0 && (step & 3) == 0) {
-            uint8_t *const to = scale_lds + (step >> 2 & 1) * kScaleBytes + wave * 1024;
+            uint8_t *const to = scales_of(place) + wave * 1024;
             load_lds(a_scale_from + step * 4, to);
             load_lds(b_scale_from + step * 4, to + kTile * 16);
         }
-        uint8_t *const to = smem + step % R * kBuffer + wave * 1024 + k * 4096;
+        uint8_t *const to = smem + slot(place) * kBuffer + wave * 1024 + k * 4096;
 #pragma unroll
         for (int half = 0; half < kHalves; half++) {
             load_lds(a_base + (step * kHalves + half) * 64 + a_from[k], to + half * (kTile * 64));
@@ -551,11 +552,11 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
     v16f acc[F][F] = {};
     u4 a[2][2][kHalves], b[2][F];   // of two blocks of two query fragments; of two half-steps
     auto read_b = [&](int step, int half, int j) {
-        return *reinterpret_cast<const u4 *>(smem + step % R * kBuffer + kABytes + (wn * 4 + j) * 2048 +
+        return *reinterpret_cast<const u4 *>(smem + slot(step) * kBuffer + kABytes + (wn * 4 + j) * 2048 +
                                              wide_place(r, half * 2 + h));
     };
     auto read_a = [&](int step, int half, int i, u4 (&v)[kHalves]) {
-        const uint8_t *const from = smem + step % R * kBuffer + (wm * 4 + i) * 2048;
+        const uint8_t *const from = smem + slot(step) * kBuffer + (wm * 4 + i) * 2048;
         if constexpr (FA == kE2M1) {
             v[0] = *reinterpret_cast<const u4 *>(from + wide_place(r, half * 2 + h));
         } else {
@@ -566,7 +567,7 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
     // blocks h of four half-steps in the bytes of one register, two registers for four steps, of row r of a fragment
     const uint32_t pick = 0x06040200u + 0x01010101u * h;
     auto read_scales = [&](int step, int row) {
-        return *reinterpret_cast<const u4 *>(scale_lds + (step >> 2 & 1) * kScaleBytes + (row + r) * 16);
+        return *reinterpret_cast<const u4 *>(scales_of(step) + (row + r) * 16);
     };
     auto block_scales = [&](u4 w, int (&sc)[2]) {
         sc[0] = (int)__builtin_amdgcn_perm(w[1], w[0], pick);
@@ -575,9 +576,19 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
     int a_scale[F][2], b_scale[F][2], a_scale_next[F][2], b_scale_next[F][2];
     const int a_row = wm * 128, b_row = kTile + wn * 128;
 
+    bool more = true, stores = false;
     auto one = [&](int step, auto which) {
         constexpr int u = decltype(which)::value;
-        const int after = u < 3 ? step + 1 : min(step + 1, steps - 1);
+        const int after = step + 1;   // behind the last step: the first one of the next tile
+        if (step + R - 1 == steps) {   // from here on the next tile's codes are loaded
+            id += gridDim.x >> 3;
+            more = id < end;
+            if (more) {
+                set_tile();
+            }
+        }
+        const bool loads = step + R - 1 < steps || more;
+        const int ahead = step + R - 1 < steps ? step + R - 1 : step + R - 1 - steps;
         // every wavefront is done with the step before: its place in the ring is free
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -594,8 +605,8 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
                 // others in flight, and have the time of the other seven
                 asm volatile("" : "+a"(acc[i][0]) : : "memory");
                 __builtin_amdgcn_sched_barrier(0);
-                if (step + R - 1 < steps) {
-                    issue(step + R - 1, half * 2 + (i >> 1));
+                if (loads) {
+                    issue(ahead, step + R - 1, half * 2 + (i >> 1));
                 }
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
@@ -640,8 +651,11 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
         half_step(std::integral_constant<int, 0>());
         // the other half reads ahead from the next step: its codes have to be there, what was issued later (half of a step's
         // loads and R - 3 steps' before) may be on its way
-        if (step + R - 1 < steps) {
-            constexpr int kLater = (R - 3) * kLoads + kLoads / 2;
+        constexpr int kLater = (R - 3) * kLoads + kLoads / 2;
+        if (loads && step < R - 2 && stores) {
+            // behind these loads 64 stores of the last tile's scores and kLater loads were issued: at most 63 are left
+            __builtin_amdgcn_s_waitcnt(0xcf7f);
+        } else if (loads) {
             __builtin_amdgcn_s_waitcnt(0x0f70 | (kLater & 15) | (kLater >> 4) << 14);
         } else {
             __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -661,47 +675,39 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
             }
         }
     };
-    auto begin = [&]() {
-        set_tile();
+    set_tile();
 #pragma unroll
-        for (int k = 0; k < R - 1; k++) {
+    for (int k = 0; k < R - 1; k++) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                issue(k, q);
-            }
+        for (int q = 0; q < 4; q++) {
+            issue(k, k, q);
         }
-    };
-    begin();
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < F; j++) {
+        b[0][j] = read_b(0, 0, j);
+        block_scales(read_scales(0, b_row + j * 32), b_scale[j]);
+        block_scales(read_scales(0, a_row + j * 32), a_scale[j]);
+    }
+    read_a(0, 0, 0, a[0][0]);
+    read_a(0, 0, 1, a[0][1]);
     for (;;) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int j = 0; j < F; j++) {
-            b[0][j] = read_b(0, 0, j);
-            block_scales(read_scales(0, b_row + j * 32), b_scale[j]);
-            block_scales(read_scales(0, a_row + j * 32), a_scale[j]);
-        }
-        read_a(0, 0, 0, a[0][0]);
-        read_a(0, 0, 1, a[0][1]);
+        const int64_t tile_row = row0, tile_col = col0;
         for (int step = 0; step < steps; step += 4) {
             one(step, std::integral_constant<int, 0>());
             one(step + 1, std::integral_constant<int, 1>());
             one(step + 2, std::integral_constant<int, 2>());
             one(step + 3, std::integral_constant<int, 3>());
         }
-        // the next tile's first codes are on their way while this one's scores leave, once nobody reads the last step's
-        __builtin_amdgcn_s_waitcnt(0x0070);
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        const int64_t row = row0 + wm * 128 + h * 4, col = col0 + wn * 128 + r * 4;
-        const bool inside = row0 + kTile <= p.m && col0 + kTile <= p.n && p.lines;
-        id += gridDim.x >> 3;
-        if (id < end) {
-            begin();
-        }
+        done += steps;
+        // the next tile's first codes are on their way while this one's scores leave
+        const int64_t row = tile_row + wm * 128 + h * 4, col = tile_col + wn * 128 + r * 4;
+        const bool inside = tile_row + kTile <= p.m && tile_col + kTile <= p.n && p.lines;
+        stores = inside;
         float b_sqr[4] = {};
         if (p.metric == kMetricL2 && col < p.n) {
             load_run(p.b_sqr, col, p.n, b_sqr);
@@ -752,7 +758,7 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
                 acc[i][j] = v16f{};
             }
         }
-        if (id >= end) {
+        if (!more) {
             return;
         }
     }
@@ -814,9 +820,10 @@ void launch_wide(const ProductParams &p, hipStream_t s)
     const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
     const void *kern = reinterpret_cast<const void *>(mx_wide_kernel<FA, R, T>);
     require_dynamic_lds(kern, lds);
+    IXA_REQUIRE(per_xcd <= 0x0fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m, (long)p.n);
     const int64_t grid = std::min(per_xcd * 8, resident_workgroups(kern, 256, lds));
     hipLaunchKernelGGL((mx_wide_kernel<FA, R, T>), dim3((unsigned)grid), dim3(256), lds, s, p, (int)row_tiles, (int)col_tiles,
-                       per_xcd);
+                       (int)per_xcd);
     check_launch();
 }
 
