@@ -114,8 +114,7 @@ __device__ __forceinline__ void store_scores(const ProductParams &p, int64_t row
             Scores v;
 #pragma unroll
             for (int j = 0; j < NF; j++) {
-                const float g = acc[j][i];
-                v[j] = (T)(l2 ? (a_sqr[i] + b_sqr[j]) - g - g : g);
+                v[j] = (T)(l2 ? fmaf(acc[j][i], -2.f, a_sqr[i] + b_sqr[j]) : acc[j][i]);
             }
             T *o = static_cast<T *>(p.out) + (row + i) * p.ld + col;
             if (col + NF <= p.n) {
@@ -481,8 +480,9 @@ __device__ __forceinline__ int wide_place(int r, int q) { return r * 64 + ((q ^ 
 // 32 rows), one to a SIMD with 512 registers: twice the products per byte read from LDS of the kernel above.  Codes go
 // from memory straight into a ring of R LDS buffers, one step of 128 columns each, scales into two buffers of four steps.  A
 // half-step of 64 columns reads the next one's fragments of stored rows while it multiplies its own, so that no wavefront
-// meets a barrier without products to do.  Whole groups of four steps and 16-byte aligned scales only.
-template <int FA, int R, typename T>
+// meets a barrier without products to do.  Whole groups of four steps, multiples of four stored rows, rows of scores that start
+// on 64 bytes and have at most 2^23 of them, and 16-byte aligned scales only.
+template <int FA, int R, bool L2, typename T>
 __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
     constexpr int kHalves = FA == kE2M1 ? 1 : 2, kTile = 256, F = 4;
@@ -705,49 +705,56 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
         }
         done += steps;
         // the next tile's first codes are on their way while this one's scores leave
-        const int64_t row = tile_row + wm * 128 + h * 4, col = tile_col + wn * 128 + r * 4;
-        const bool inside = tile_row + kTile <= p.m && tile_col + kTile <= p.n && p.lines;
-        stores = inside;
+        const int64_t col = tile_col + wn * 128 + r * 4;
+        stores = true;   // 64 of them, dropped ones among them
+        // The norms of the wavefront's 128 queries, one a lane: a load among the stores would wait for those before it.
         float b_sqr[4] = {};
-        if (p.metric == kMetricL2 && col < p.n) {
-            load_run(p.b_sqr, col, p.n, b_sqr);
-        }
-        if (inside) {
-            const bool l2 = p.metric == kMetricL2;
-            typedef T Scores __attribute__((ext_vector_type(4)));
-            T *o = static_cast<T *>(p.out) + row * p.ld + col;
-            const int64_t up = p.ld * (int64_t)sizeof(T);
-#pragma unroll
-            for (int i = 0; i < F; i++) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    float a_sqr[4] = {};
-                    if (l2) {
-                        load_run(p.a_sqr, row + i * 32 + k * 8, p.m, a_sqr);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        Scores v;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float x = acc[i][j][4 * k + e];
-                            v[j] = (T)(l2 ? (a_sqr[e] + b_sqr[j]) - x - x : x);
-                        }
-                        __builtin_nontemporal_store(v, reinterpret_cast<Scores *>(reinterpret_cast<uint8_t *>(o) + (i * 32 + k * 8 + e) * up));
-                    }
-                }
+        int norms[2] = {};
+        if constexpr (L2) {
+            if (col < p.n) {
+                load_run(p.b_sqr, col, p.n, b_sqr);
             }
-        } else {
+            norms[0] = __float_as_int(p.a_sqr[min(tile_row + wm * 128 + lane, p.m - 1)]);
+            norms[1] = __float_as_int(p.a_sqr[min(tile_row + wm * 128 + 64 + lane, p.m - 1)]);
+        }
+        // Stores with bounds of their own: what lies behind the last query or the last stored row is dropped, and no lane
+        // is masked out (v_readlane takes norms from all of them).  Rows of at most 2^23 bytes keep offsets in 32 bits.
+        const int64_t first = tile_row + wm * 128;
+        const uint32_t up = (uint32_t)p.ld * (uint32_t)sizeof(T), rows = (uint32_t)max((int64_t)0, min((int64_t)128, p.m - first));
+        const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
+            static_cast<uint8_t *>(p.out) + min(first, p.m - 1) * up, 0, (int)(rows * up), 0x00027000);
+        const uint32_t offset = col < p.n ? h * 4 * up + (uint32_t)col * (uint32_t)sizeof(T) : 0x80000000u;
+        typedef T Scores __attribute__((ext_vector_type(4)));
+        typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T))));
 #pragma unroll
-            for (int i = 0; i < F; i++) {
+        for (int i = 0; i < F; i++) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    v4f part[4];
+            for (int k = 0; k < 4; k++) {
+                // one group of stores after the other: all scores at a time would not fit the registers
+                asm volatile("" : "+v"(norms[0]), "+v"(norms[1]) : : "memory");
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int at = i % 2 * 32 + k * 8 + e;
+                    float a_sqr = 0.f;
+                    if constexpr (L2) {
+                        const int low = __builtin_amdgcn_readlane(norms[i / 2], at);
+                        const int high = __builtin_amdgcn_readlane(norms[i / 2], at + 4);
+                        a_sqr = __int_as_float(h ? high : low);
+                    }
+                    Scores v;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        part[j] = v4f{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+                        const float g = acc[i][j][4 * k + e];
+                        v[j] = (T)(L2 ? fmaf(g, -2.f, a_sqr + b_sqr[j]) : g);
                     }
-                    store_scores<T, 4>(p, row + i * 32 + k * 8, col, part, b_sqr);
+                    const uint32_t to = offset + (uint32_t)(i * 32 + k * 8 + e) * up;
+                    constexpr int kNonTemporal = 2;
+                    if constexpr (sizeof(T) == 4) {
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, v), out, to, 0, kNonTemporal);
+                    } else {
+                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(Words, v), out, to, 0, kNonTemporal);
+                    }
                 }
             }
         }
@@ -811,18 +818,18 @@ void launch_tiles(const ProductParams &p, hipStream_t s)
     check_launch();
 }
 
-template <int FA, typename T>
+template <int FA, bool L2, typename T>
 void launch_wide(const ProductParams &p, hipStream_t s)
 {
     constexpr int R = FA == kE2M1 ? 4 : 3;
     constexpr size_t lds = R * (256 * 64 * (FA == kE2M1 ? 2 : 3)) + 2 * 512 * 16;
     const int64_t row_tiles = (p.m + 255) / 256, col_tiles = (p.n + 255) / 256;
     const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
-    const void *kern = reinterpret_cast<const void *>(mx_wide_kernel<FA, R, T>);
+    const void *kern = reinterpret_cast<const void *>(mx_wide_kernel<FA, R, L2, T>);
     require_dynamic_lds(kern, lds);
     IXA_REQUIRE(per_xcd <= 0x0fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m, (long)p.n);
     const int64_t grid = std::min(per_xcd * 8, resident_workgroups(kern, 256, lds));
-    hipLaunchKernelGGL((mx_wide_kernel<FA, R, T>), dim3((unsigned)grid), dim3(256), lds, s, p, (int)row_tiles, (int)col_tiles,
+    hipLaunchKernelGGL((mx_wide_kernel<FA, R, L2, T>), dim3((unsigned)grid), dim3(256), lds, s, p, (int)row_tiles, (int)col_tiles,
                        (int)per_xcd);
     check_launch();
 }
@@ -844,8 +851,9 @@ void launch_type(const ProductParams &p, hipStream_t s)
         return;
     }
     const int64_t tiles = ((p.m + 127) / 128) * ((p.n + 255) / 256);
-    if (p.blocks % 16 == 0 && p.m >= 256 && aligned(p.a_scales, 16) && aligned(p.b_scales, 16)) {
-        launch_wide<FA, T>(p, s);
+    if (p.blocks % 16 == 0 && p.m >= 256 && p.n % 4 == 0 && p.lines && p.ld <= (1 << 23) / (int)sizeof(T) &&
+        aligned(p.a_scales, 16) && aligned(p.b_scales, 16)) {
+        p.metric == kMetricL2 ? launch_wide<FA, true, T>(p, s) : launch_wide<FA, false, T>(p, s);
         return;
     }
     if (tiles < 512) {
