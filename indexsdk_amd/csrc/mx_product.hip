@@ -850,12 +850,16 @@ void launch_type(const ProductParams &p, hipStream_t s)
         }
         return;
     }
-    const int64_t tiles = ((p.m + 127) / 128) * ((p.n + 255) / 256);
-    if (p.blocks % 16 == 0 && p.m >= 256 && p.n % 4 == 0 && p.lines && p.ld <= (1 << 23) / (int)sizeof(T) &&
-        aligned(p.a_scales, 16) && aligned(p.b_scales, 16)) {
+    // Wide tiles where at most a fifth of their queries do not exist and either every CU gets one (2048 x 131072 x 1024: 267 us,
+    // the tiles below 317) or there are many columns (2048 x 4096 x 4096: 39 us against 48; with few columns and 128 tiles the
+    // others are ahead, 1024 x 8192 x 1024: 20 against 18).
+    const int64_t wide_rows = (p.m + 255) / 256, wide_tiles = wide_rows * ((p.n + 255) / 256);
+    if (p.blocks % 16 == 0 && p.n % 4 == 0 && p.lines && p.ld <= (1 << 23) / (int)sizeof(T) && aligned(p.a_scales, 16) &&
+        aligned(p.b_scales, 16) && wide_rows * 256 * 4 <= p.m * 5 && wide_tiles >= (p.blocks >= 64 ? 128 : 256)) {
         p.metric == kMetricL2 ? launch_wide<FA, true, T>(p, s) : launch_wide<FA, false, T>(p, s);
         return;
     }
+    const int64_t tiles = ((p.m + 127) / 128) * ((p.n + 255) / 256);
     if (tiles < 512) {
         launch_tiles<FA, 1, 4, 4, 1, T>(p, s);
     } else if (p.m <= 128 || p.blocks <= 64) {

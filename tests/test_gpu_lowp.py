@@ -396,7 +396,8 @@ SHAPES = [(1, 1, 1), (1, 33, 32), (2, 31, 33), (31, 64, 64), (32, 32, 65), (33, 
           (256, 512, 1000), (257, 700, 1030), (300, 1300, 64), (40, 600, 4096), (130, 300, 2080), (5, 70, 16384),
           (520, 770, 16), (1000, 1024, 160),
           # whole groups of 512 columns, tiles of 256 by 256 and their edges
-          (256, 256, 512), (256, 1, 500), (300, 700, 2048), (513, 260, 1024), (1030, 2100, 1536), (257, 515, 4096)]
+          (256, 256, 512), (256, 1, 500), (300, 700, 2048), (513, 260, 1024), (1030, 2100, 1536), (257, 515, 4096),
+          (1000, 16400, 512), (1024, 16384, 500), (250, 65600, 510), (2000, 4096, 2048), (490, 16640, 4096)]
 
 
 @pytest.mark.parametrize("m,n,d", SHAPES)
