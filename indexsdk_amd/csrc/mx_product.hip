@@ -478,17 +478,17 @@ __device__ __forceinline__ int wide_place(int r, int q) { return r * 64 + ((q ^ 
 
 // Many queries and many columns: tiles of 256 queries by 256 stored rows, four wavefronts of 128 x 128 (4 x 4 fragments of
 // 32 rows), one to a SIMD with 512 registers: twice the products per byte read from LDS of the kernel above.  Codes go
-// from memory straight into a ring of R LDS buffers, one step of 128 columns each, scales into two buffers of four steps.  A
-// half-step of 64 columns reads the next one's fragments of stored rows while it multiplies its own, so that no wavefront
-// meets a barrier without products to do.  Whole groups of four steps, multiples of four stored rows, rows of scores that start
-// on 64 bytes and have at most 2^23 of them, and 16-byte aligned scales only.
+// from memory straight into a ring of R LDS buffers, one step of 128 columns each, scales four steps at a time (4 bytes of a
+// row at a time touch its line in every step: 4096 x 32768 x 4096 365 us instead of 325).  A half-step of 64 columns reads the next one's fragments of stored rows while it multiplies its own, so
+// that no wavefront meets a barrier without products to do.  Four steps and more, multiples of four stored rows, rows of scores
+// that start on 64 bytes and have at most 2^23 of them, and scales that start on 4 bytes only.
 template <int FA, int R, bool L2, typename T>
 __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
     constexpr int kHalves = FA == kE2M1 ? 1 : 2, kTile = 256, F = 4;
     constexpr int kABytes = kTile * 64 * kHalves, kBBytes = kTile * 64, kBuffer = kABytes + kBBytes;
     constexpr int kScaleBytes = 2 * kTile * 16;                       // of both sides, four steps
-    constexpr int kLoads = 4 * kHalves + 4;                           // 1 KB each, per wavefront and step
+    constexpr int kLoads = 4 * kHalves + 4;                           // of codes, 1 KB each, per wavefront and step
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t *const scale_lds = smem + R * kBuffer;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
@@ -506,11 +506,13 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
     // LDS holds 16 rows of 64 bytes in 1 KB (wide_place); a wavefront loads runs wave, wave + 4, ... of either side, lane l
     // the piece that belongs at place l & 3 of row l >> 2.  Stored row 4 r + j of each 128 is row r of fragment j, so that
     // a lane ends up with four scores in a row; rows behind the last one repeat it.
-    const int fr = lane >> 2, fq = (lane & 3) ^ ((fr >> 2) & 3);
     int64_t row0, col0;   // of the tile whose codes are loaded
     const uint8_t *a_base, *b_base, *a_scale_from, *b_scale_from;
     uint32_t a_from[4], b_from[4];
     auto set_tile = [&]() {
+        int l = lane;
+        asm volatile("" : "+v"(l));   // what follows from the lane alone is not kept in registers for the next tile
+        const int fr = l >> 2, fq = (l & 3) ^ ((fr >> 2) & 3);
         const int band = id / (8 * col_tiles), in = id - band * 8 * col_tiles, high = min(8, row_tiles - band * 8);
         row0 = (int64_t)(band * 8 + in % high) * kTile;
         col0 = (int64_t)(in / high) * kTile;
@@ -524,24 +526,25 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
             b_from[k] = (uint32_t)(min((run >> 3) * 128 + ((run & 1) * 16 + fr) * 4 + ((run >> 1) & 3), last_col) * b_row_bytes + fq * 16);
         }
         // rows of scales, 16 bytes each, in the order of the fragments' rows
-        const int scale_run = wave * 2 + (lane >> 5);   // 32 rows: of 128 rows scale_run >> 2, fragment scale_run & 3
-        a_scale_from = p.a_scales + (row0 + min(wave * 64 + lane, last_row)) * p.blocks;
-        b_scale_from = p.b_scales + (col0 + min((scale_run >> 2) * 128 + r * 4 + (scale_run & 3), last_col)) * p.blocks;
+        const int scale_run = wave * 2 + (l >> 5);   // 32 rows: of 128 rows scale_run >> 2, fragment scale_run & 3
+        a_scale_from = p.a_scales + (row0 + min(wave * 64 + l, last_row)) * p.blocks;
+        b_scale_from = p.b_scales + (col0 + min((scale_run >> 2) * 128 + (l & 31) * 4 + (scale_run & 3), last_col)) * p.blocks;
     };
     auto load_lds = [&](const uint8_t *from, uint8_t *to) {
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
                                          (__attribute__((address_space(3))) void *)to, 16, 0, 0);
     };
-    int done = 0;   // steps of the tiles before: step `step` of this one lies at place (done + step) % R of the ring
-    auto slot = [&](int step) { return R == 4 ? step & 3 : (done + step) % R; };   // done is a multiple of 4
-    auto scales_of = [&](int step) { return scale_lds + ((done + step) >> 2 & 1) * kScaleBytes; };
-    auto issue = [&](int step, int place, int k) {   // a quarter of the codes of a step into the place of step `place`
+    // The first of the four steps whose scales come together; the last four of a row may overlap those before.
+    auto first_of = [&](int step) { return min(step & ~3, steps - 4); };
+    int loaded = 0, used = 0;   // place of the scales among the R - 1 that R - 1 steps in a row may need
+    auto issue = [&](int step, uint8_t *ring, int k) {   // a quarter of the codes of a step, and four steps' scales
         if (k == 0 && (step & 3) == 0) {
-            uint8_t *const to = scales_of(place) + wave * 1024;
-            load_lds(a_scale_from + step * 4, to);
-            load_lds(b_scale_from + step * 4, to + kTile * 16);
+            uint8_t *const to = scale_lds + loaded * kScaleBytes + wave * 1024;
+            loaded = loaded == R - 2 ? 0 : loaded + 1;
+            load_lds(a_scale_from + first_of(step) * 4, to);
+            load_lds(b_scale_from + first_of(step) * 4, to + kTile * 16);
         }
-        uint8_t *const to = smem + slot(place) * kBuffer + wave * 1024 + k * 4096;
+        uint8_t *const to = ring + wave * 1024 + k * 4096;
 #pragma unroll
         for (int half = 0; half < kHalves; half++) {
             load_lds(a_base + (step * kHalves + half) * 64 + a_from[k], to + half * (kTile * 64));
@@ -551,12 +554,11 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
 
     v16f acc[F][F] = {};
     u4 a[2][2][kHalves], b[2][F];   // of two blocks of two query fragments; of two half-steps
-    auto read_b = [&](int step, int half, int j) {
-        return *reinterpret_cast<const u4 *>(smem + slot(step) * kBuffer + kABytes + (wn * 4 + j) * 2048 +
-                                             wide_place(r, half * 2 + h));
+    auto read_b = [&](const uint8_t *ring, int half, int j) {
+        return *reinterpret_cast<const u4 *>(ring + kABytes + (wn * 4 + j) * 2048 + wide_place(r, half * 2 + h));
     };
-    auto read_a = [&](int step, int half, int i, u4 (&v)[kHalves]) {
-        const uint8_t *const from = smem + slot(step) * kBuffer + (wm * 4 + i) * 2048;
+    auto read_a = [&](const uint8_t *ring, int half, int i, u4 (&v)[kHalves]) {
+        const uint8_t *const from = ring + (wm * 4 + i) * 2048;
         if constexpr (FA == kE2M1) {
             v[0] = *reinterpret_cast<const u4 *>(from + wide_place(r, half * 2 + h));
         } else {
@@ -564,22 +566,25 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
             v[1] = *reinterpret_cast<const u4 *>(from + half * (kTile * 64) + wide_place(r, 2 + h));
         }
     };
-    // blocks h of four half-steps in the bytes of one register, two registers for four steps, of row r of a fragment
-    const uint32_t pick = 0x06040200u + 0x01010101u * h;
-    auto read_scales = [&](int step, int row) {
-        return *reinterpret_cast<const u4 *>(scales_of(step) + (row + r) * 16);
+    // scales of row r of a fragment: those of blocks h and 2 + h in bytes 0 and 2
+    auto read_scales = [&](const uint8_t *of_step, int row) {
+        return *reinterpret_cast<const uint32_t *>(of_step + (row + r) * 16);
     };
-    auto block_scales = [&](u4 w, int (&sc)[2]) {
-        sc[0] = (int)__builtin_amdgcn_perm(w[1], w[0], pick);
-        sc[1] = (int)__builtin_amdgcn_perm(w[3], w[2], pick);
-    };
-    int a_scale[F][2], b_scale[F][2], a_scale_next[F][2], b_scale_next[F][2];
+    int a_scale[F], b_scale[F];
     const int a_row = wm * 128, b_row = kTile + wn * 128;
 
     bool more = true, stores = false;
-    auto one = [&](int step, auto which) {
-        constexpr int u = decltype(which)::value;
-        const int after = step + 1;   // behind the last step: the first one of the next tile
+    int place = 0;   // in the ring
+    auto one = [&](int step) {
+        const uint8_t *const here = smem + place * kBuffer;
+        uint8_t *const free = smem + (place == 0 ? R - 1 : place - 1) * kBuffer;
+        place = place == R - 1 ? 0 : place + 1;
+        const uint8_t *const after = smem + place * kBuffer;   // behind the last step: the first one of the next tile
+        const int step_after = step + 1 == steps ? 0 : step + 1;
+        if ((step_after & 3) == 0) {
+            used = used == R - 2 ? 0 : used + 1;
+        }
+        const uint8_t *const scales_after = scale_lds + used * kScaleBytes + (step_after - first_of(step_after)) * 4;
         if (step + R - 1 == steps) {   // from here on the next tile's codes are loaded
             id += gridDim.x >> 3;
             more = id < end;
@@ -595,30 +600,30 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
         asm volatile("" ::: "memory");
         auto half_step = [&](auto which_half) {
             constexpr int half = decltype(which_half)::value;
-            const int next_step = half == 0 ? step : after;
+            const uint8_t *const next = half == 0 ? here : after;
+            uint32_t w[2 * F];   // the next step's scales
 #pragma unroll
             for (int i = 0; i < F; i += 2) {   // eight products at a time
                 AFragment<FA> f;
                 f.set(a[i >> 1][0]);
-                acc[i][0] = multiply32<FA, (u & 1) * 2 + half>(f, a_scale[i][u >> 1], wide(b[half][0]), b_scale[0][u >> 1], acc[i][0]);
+                acc[i][0] = multiply32<FA, half * 2>(f, a_scale[i], wide(b[half][0]), b_scale[0], acc[i][0]);
                 // the reads for the next eight start behind the first of these, whose operands were waited for with all
                 // others in flight, and have the time of the other seven
                 asm volatile("" : "+a"(acc[i][0]) : : "memory");
                 __builtin_amdgcn_sched_barrier(0);
                 if (loads) {
-                    issue(ahead, step + R - 1, half * 2 + (i >> 1));
+                    issue(ahead, free, half * 2 + (i >> 1));
                 }
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    read_a(i == 0 ? step : next_step, i == 0 ? half : half ^ 1, i == 0 ? 2 + k : k, a[(i >> 1) ^ 1][k]);
-                    b[half ^ 1][i + k] = read_b(next_step, half ^ 1, i + k);
+                    read_a(i == 0 ? here : next, i == 0 ? half : half ^ 1, i == 0 ? 2 + k : k, a[(i >> 1) ^ 1][k]);
+                    b[half ^ 1][i + k] = read_b(next, half ^ 1, i + k);
                 }
-                u4 ws[2][2];
-                if constexpr (u == 3 && half == 1) {
+                if constexpr (half == 1) {
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        ws[k][0] = read_scales(after, a_row + (i + k) * 32);
-                        ws[k][1] = read_scales(after, b_row + (i + k) * 32);
+                        w[i + k] = read_scales(scales_after, a_row + (i + k) * 32);
+                        w[F + i + k] = read_scales(scales_after, b_row + (i + k) * 32);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -629,8 +634,7 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
                     }
 #pragma unroll
                     for (int j = 1 - k; j < F; j++) {
-                        acc[i + k][j] = multiply32<FA, (u & 1) * 2 + half>(f, a_scale[i + k][u >> 1], wide(b[half][j]),
-                                                                           b_scale[j][u >> 1], acc[i + k][j]);
+                        acc[i + k][j] = multiply32<FA, half * 2>(f, a_scale[i + k], wide(b[half][j]), b_scale[j], acc[i + k][j]);
                     }
                 }
                 asm volatile(""
@@ -638,14 +642,14 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
                                "+a"(acc[i + 1][2]), "+a"(acc[i + 1][3])
                              :
                              : "memory");
-                if constexpr (u == 3 && half == 1) {
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        block_scales(ws[k][0], a_scale_next[i + k]);
-                        block_scales(ws[k][1], b_scale_next[i + k]);
-                    }
-                }
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (half == 1) {
+#pragma unroll
+                for (int i = 0; i < F; i++) {
+                    a_scale[i] = (int)(w[i] >> (8 * h));
+                    b_scale[i] = (int)(w[F + i] >> (8 * h));
+                }
             }
         };
         half_step(std::integral_constant<int, 0>());
@@ -664,23 +668,13 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         half_step(std::integral_constant<int, 1>());
-        if constexpr (u == 3) {
-#pragma unroll
-            for (int i = 0; i < F; i++) {
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    a_scale[i][k] = a_scale_next[i][k];
-                    b_scale[i][k] = b_scale_next[i][k];
-                }
-            }
-        }
     };
     set_tile();
 #pragma unroll
     for (int k = 0; k < R - 1; k++) {
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            issue(k, k, q);
+            issue(k, smem + k * kBuffer, q);
         }
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -689,21 +683,18 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int j = 0; j < F; j++) {
-        b[0][j] = read_b(0, 0, j);
-        block_scales(read_scales(0, b_row + j * 32), b_scale[j]);
-        block_scales(read_scales(0, a_row + j * 32), a_scale[j]);
+        b[0][j] = read_b(smem, 0, j);
+        a_scale[j] = (int)(read_scales(scale_lds, a_row + j * 32) >> (8 * h));
+        b_scale[j] = (int)(read_scales(scale_lds, b_row + j * 32) >> (8 * h));
     }
-    read_a(0, 0, 0, a[0][0]);
-    read_a(0, 0, 1, a[0][1]);
+    read_a(smem, 0, 0, a[0][0]);
+    read_a(smem, 0, 1, a[0][1]);
     for (;;) {
         const int64_t tile_row = row0, tile_col = col0;
-        for (int step = 0; step < steps; step += 4) {
-            one(step, std::integral_constant<int, 0>());
-            one(step + 1, std::integral_constant<int, 1>());
-            one(step + 2, std::integral_constant<int, 2>());
-            one(step + 3, std::integral_constant<int, 3>());
+#pragma unroll 1
+        for (int step = 0; step < steps; step++) {
+            one(step);
         }
-        done += steps;
         // the next tile's first codes are on their way while this one's scores leave
         const int64_t col = tile_col + wn * 128 + r * 4;
         stores = true;   // 64 of them, dropped ones among them
@@ -730,8 +721,12 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
         for (int i = 0; i < F; i++) {
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                // one group of stores after the other: all scores at a time would not fit the registers
-                asm volatile("" : "+v"(norms[0]), "+v"(norms[1]) : : "memory");
+                // one group of stores after the other: all scores at a time would not fit the registers that take them from
+                // the accumulators, and what they displace would be waited for, with all codes on their way, in every step
+                asm volatile(""
+                             : "+a"(acc[i][0]), "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]), "+v"(norms[0]), "+v"(norms[1])
+                             :
+                             : "memory");
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -822,7 +817,7 @@ template <int FA, bool L2, typename T>
 void launch_wide(const ProductParams &p, hipStream_t s)
 {
     constexpr int R = FA == kE2M1 ? 4 : 3;
-    constexpr size_t lds = R * (256 * 64 * (FA == kE2M1 ? 2 : 3)) + 2 * 512 * 16;
+    constexpr size_t lds = R * (256 * 64 * (FA == kE2M1 ? 2 : 3)) + (R - 1) * 512 * 16;
     const int64_t row_tiles = (p.m + 255) / 256, col_tiles = (p.n + 255) / 256;
     const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
     const void *kern = reinterpret_cast<const void *>(mx_wide_kernel<FA, R, L2, T>);
@@ -850,12 +845,13 @@ void launch_type(const ProductParams &p, hipStream_t s)
         }
         return;
     }
-    // Wide tiles where at most a fifth of their queries do not exist and either every CU gets one (2048 x 131072 x 1024: 267 us,
-    // the tiles below 317) or there are many columns (2048 x 4096 x 4096: 39 us against 48; with few columns and 128 tiles the
-    // others are ahead, 1024 x 8192 x 1024: 20 against 18).
+    // Wide tiles where at most a fifth of their queries do not exist and either every CU gets one (2048 x 131072 x 768: 235 us,
+    // the tiles below 277; 1024 x 32768 x 768: 42 and 48; with 256 of them, 1024 x 16384 x 768, both 24) or there are many
+    // columns (2048 x 4096 x 4096: 39 us against 48; with few columns and 128 tiles the others are ahead, 1024 x 8192 x 1024: 20
+    // against 18).
     const int64_t wide_rows = (p.m + 255) / 256, wide_tiles = wide_rows * ((p.n + 255) / 256);
-    if (p.blocks % 16 == 0 && p.n % 4 == 0 && p.lines && p.ld <= (1 << 23) / (int)sizeof(T) && aligned(p.a_scales, 16) &&
-        aligned(p.b_scales, 16) && wide_rows * 256 * 4 <= p.m * 5 && wide_tiles >= (p.blocks >= 64 ? 128 : 256)) {
+    if (p.blocks % 4 == 0 && p.blocks >= 16 && p.n % 4 == 0 && p.lines && p.ld <= (1 << 23) / (int)sizeof(T) &&
+        aligned(p.a_scales, 4) && aligned(p.b_scales, 4) && wide_rows * 256 * 4 <= p.m * 5 && wide_tiles >= (p.blocks >= 64 ? 128 : 256)) {
         p.metric == kMetricL2 ? launch_wide<FA, true, T>(p, s) : launch_wide<FA, false, T>(p, s);
         return;
     }

@@ -409,6 +409,16 @@ def test_product(lib, m, n, d, a_fmt):
     check_product(lib, m, n, d, a_fmt, 1, "f16", wild=True)
 
 
+@pytest.mark.parametrize("m,n,d", [(1000, 16400, 384), (1024, 16384, 768), (760, 22016, 630), (512, 32832, 890), (2040, 4100, 2176)])
+@pytest.mark.parametrize("a_fmt", [MXFP4, MXFP8])
+def test_product_in_whole_steps_of_128_columns(lib, m, n, d, a_fmt):
+    check_product(lib, m, n, d, a_fmt, 1, "f32", wild=True)
+    check_product(lib, m, n, d, a_fmt, 0, "bf16", wild=False)
+    # rows of scores that are longer than their scores and still start on 64 bytes
+    check_product(lib, m, n - 12, d, a_fmt, 0, "f32", wild=False, pad=12 + 64 - n % 16)
+    check_product(lib, m, n - 12, d, a_fmt, 1, "f16", wild=True, pad=12 + 64 - n % 32)
+
+
 @pytest.mark.parametrize("a_fmt", [MXFP4, MXFP8])
 def test_product_of_one_large_and_many_small_numbers(lib, a_fmt):
     """What an instruction that aligns its products to the largest would drop: 448 * 6 next to 2^-9 * 0.5 in one block."""
