@@ -41,7 +41,7 @@ void op_rms_norm_quantise(const void *x, int64_t ld_x, const void *residual, int
                           int type, int64_t n, int d, float eps, void *sum, int64_t ld_sum, int format, float fixed_scale,
                           uint8_t *codes, void *scales, float *sqr_sum, hipStream_t s);
 
-// out[m][ld] = scores of rows a (MXFP4 or MXFP8) against rows b (MXFP4): inner products g, or (a_sqr + b_sqr) - g - g.
+// out[m][ld] = scores of rows a (MXFP4 or MXFP8) against rows b (MXFP4): inner products g, or (a_sqr + b_sqr) - 2 g.
 void op_mx_product(const uint8_t *a_codes, const uint8_t *a_scales, int a_format, int64_t m, const uint8_t *b_codes,
                    const uint8_t *b_scales, int64_t n, int d, int metric, const float *a_sqr, const float *b_sqr,
                    int out_type, void *out, int64_t ld, hipStream_t s);

@@ -1,5 +1,5 @@
 // Scores of query rows a against stored rows b in microscaled codes: g[i][j] = sum over k of a[i][k] b[j][k], or the squared
-// distance (|a_i|^2 + |b_j|^2) - g - g in the library's expanded form.
+// distance (|a_i|^2 + |b_j|^2) - 2 g, its last step one multiply-add.
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 codes and applies the power-of-two scale of each row's
 // block of 32 itself.  A lane (row r = l & 15, quarter g = l >> 4) gives it, in 4 bits, the 16 bytes of block g of its row;
@@ -167,42 +167,47 @@ __device__ __forceinline__ uint32_t take_scales(uint32_t w, const uint8_t *from,
     return blocks - b >= 4 ? w : w & ((1u << (8 * max(blocks - b, 0))) - 1u);
 }
 
-// Few queries: their codes stay in LDS (MF fragments of 16 rows, all columns) while every wavefront streams NF fragments of
-// stored rows past them, one step ahead.  The stored rows come in whole pieces of 64 bytes, four lanes each, and change lanes
-// in 1 KB of LDS per fragment that the wavefront has to itself: read the way the instruction wants them, 16 lanes
-// would touch 16 rows at a time.
-template <int FA, int MF, int NF, typename T>
+// Few queries (MF fragments of 16): their codes stay in LDS, all columns of them, while every wavefront streams NF fragments of
+// stored rows past them, U steps of 128 columns ahead.  Bound by the stored rows and the scores, both moved once: 64 x 1M x
+// 768 145 us, 4.6 TB/s; 1 x 1M x 1536 154 us, 5.3 TB/s; 1 x 1M x 128 15.5 us, 4.9 TB/s.  The stored rows come in whole pieces
+// of 64 bytes, four lanes each, and change lanes in 1 KB of LDS per fragment and step that the wavefront has to itself: read
+// the way the instruction wants them, 16 lanes would touch 16 rows at a time.  Only queries that exist take LDS, which is what
+// limits the wavefronts of a CU in long rows (1 x 50000 x 4096: 50 -> 27 us).
+template <int FA, int MF, int NF, int U, typename T>
 __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int steps, int64_t tiles)
 {
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int kHalves = FA == kE2M1 ? 1 : 2;           // 64-byte halves of a row's step
-    constexpr int kRows = MF * 16;
-    constexpr int kStepBytes = kRows * 64 * kHalves;
-    uint8_t *const scales = smem + (size_t)steps * kStepBytes;   // [step][row][block of the step]
+    // the rows of fragments behind the last query read its codes, and their scores are not stored
+    const int rows = (int)p.m, step_bytes = rows * 64 * kHalves;
+    uint8_t *const scales = smem + (size_t)steps * step_bytes;   // [step][row][block of the step]
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint8_t *const turn = scales + (size_t)steps * kRows * 4 + wave * (NF * (1024 + 64));
-    uint8_t *const turn_scales = turn + NF * 1024;
-    const int64_t row0 = (int64_t)blockIdx.y * kRows;
+    uint8_t *const turn = scales + (((size_t)steps * rows * 4 + 15) & ~(size_t)15) + wave * (NF * U * (1024 + 64));
+    uint8_t *const turn_scales = turn + NF * U * 1024;
+    static_assert(NF * U <= 4, "a lane brings the scales of one row and step");
     const int a_row_bytes = p.blocks * 16 * kHalves, b_row_bytes = p.blocks * 16;
-    // pieces behind the last block and rows behind the last query are zeros
-    for (int e = threadIdx.x; e < steps * kRows * 4 * kHalves; e += 256) {
-        const int q = e & 3, row = (e >> 2) % kRows, part = (e >> 2) / kRows;   // part: 64 bytes of the row
-        const int byte = part * 64 + q * 16;
-        u4 v = u4{};
-        if (byte < a_row_bytes && row0 + row < p.m) {
-            v = *reinterpret_cast<const u4 *>(p.a_codes + (row0 + row) * a_row_bytes + byte);
-        }
-        *reinterpret_cast<u4 *>(smem + (size_t)part * kRows * 64 + (row >> 4) * 1024 + fragment_place(row & 15, q)) = v;
-    }
-    for (int e = threadIdx.x; e < steps * kRows; e += 256) {
-        const int row = e % kRows;
-        const uint8_t *from = p.a_scales + min(row0 + row, p.m - 1) * p.blocks;
+    // 256, 128 ... 4 threads bring a row; pieces behind its last block are zeros
+    const int lg = rows > 1 ? 8 - (32 - __builtin_clz(rows - 1)) : 8, per_row = 1 << lg;
+    if (const int row = (int)threadIdx.x >> lg, e = (int)threadIdx.x & (per_row - 1); row < rows) {
         const int64_t total = p.m * p.blocks;
-        const uint8_t *last = p.a_scales + (total > 4 ? total - 4 : 0);
-        const int b = e / kRows * 4;
-        reinterpret_cast<uint32_t *>(scales)[e] =
-            take_scales(load_scales(from, last, total < 4 ? (int)total : 0, b), from, last, b, p.blocks);
+        const uint8_t *const from = p.a_scales + (int64_t)row * p.blocks, *const last = p.a_scales + (total > 4 ? total - 4 : 0);
+        for (int step = e; step < steps; step += per_row) {
+            reinterpret_cast<uint32_t *>(scales)[step * rows + row] = take_scales(
+                load_scales(from, last, total < 4 ? (int)total : 0, step * 4), from, last, step * 4, p.blocks);
+        }
+        for (int piece = e; piece < steps * 4 * kHalves; piece += per_row) {
+            u4 v = u4{};
+            if (piece * 16 < a_row_bytes) {
+                v = *reinterpret_cast<const u4 *>(p.a_codes + (int64_t)row * a_row_bytes + piece * 16);
+            }
+            *reinterpret_cast<u4 *>(smem + (size_t)(piece >> 2) * rows * 64 + fragment_place(row, piece & 3)) = v;
+        }
+    }
+    int a_row[MF];
+#pragma unroll
+    for (int i = 0; i < MF; i++) {
+        a_row[i] = min(i * 16 + r, rows - 1);
     }
     __syncthreads();
     const int64_t b_total = p.n * p.blocks;
@@ -218,59 +223,71 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
         for (int k = 0; k < NF; k++) {
             offset[k] = (uint32_t)(min(k * 16 + (lane >> 2), last) * b_row_bytes);
         }
-        const uint8_t *const scale_from = p.b_scales + (col0 + min(lane, last)) * p.blocks;
-        u4 next[NF];
+        const int scale_row = lane % (NF * 16), scale_step = lane / (NF * 16) % U;
+        const uint8_t *const scale_from = p.b_scales + (col0 + min(scale_row, last)) * p.blocks;
+        u4 next[U][NF];
         uint32_t next_scale = 0;
         // pieces behind the last block repeat it: the queries' codes are zeros there
         auto fetch = [&](int t) {
-            const uint32_t byte = (uint32_t)min(t * 64 + (lane & 3) * 16, b_row_bytes - 16);
 #pragma unroll
-            for (int k = 0; k < NF; k++) {
-                next[k] = *reinterpret_cast<const u4 *>(codes + (offset[k] + byte));
+            for (int u = 0; u < U; u++) {
+                const uint32_t byte = (uint32_t)min((t + u) * 64 + (lane & 3) * 16, b_row_bytes - 16);
+#pragma unroll
+                for (int k = 0; k < NF; k++) {
+                    next[u][k] = *reinterpret_cast<const u4 *>(codes + (offset[k] + byte));
+                }
             }
-            if (NF == 4 || lane < NF * 16) {
-                next_scale = load_scales(scale_from, scale_last, scale_few, t * 4);
-            }
+            next_scale = load_scales(scale_from, scale_last, scale_few, min(t + scale_step, steps - 1) * 4);
         };
         fetch(0);
         v4f acc[MF][NF] = {};
-        for (int t = 0; t < steps; t++) {
+        for (int t = 0; t < steps; t += U) {
 #pragma unroll
-            for (int k = 0; k < NF; k++) {
-                const int row = k * 16 + (lane >> 2);
-                *reinterpret_cast<u4 *>(turn + stored_place<NF>(row % NF, row / NF, lane & 3)) = next[k];
-            }
-            if (NF == 4 || lane < NF * 16) {
-                reinterpret_cast<uint32_t *>(turn_scales)[(lane % NF) * 16 + lane / NF] = take_scales(next_scale, scale_from, scale_last, t * 4, p.blocks);
-            }
-            if (t + 1 < steps) {
-                fetch(t + 1);
-            }
-            __builtin_amdgcn_wave_barrier();
-            v8i b[NF];
-            int b_scale[NF];
+            for (int u = 0; u < U; u++) {
 #pragma unroll
-            for (int j = 0; j < NF; j++) {
-                b[j] = wide(*reinterpret_cast<const u4 *>(turn + stored_place<NF>(j, r, g)));
-                b_scale[j] = turn_scales[(j * 16 + r) * 4 + g];
-            }
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int i = 0; i < MF; i++) {
-                u4 w[kHalves];
-#pragma unroll
-                for (int k = 0; k < kHalves; k++) {
-                    w[k] = *reinterpret_cast<const u4 *>(smem + (size_t)t * kStepBytes + k * kRows * 64 + i * 1024 +
-                                                            fragment_place(r, g));
+                for (int k = 0; k < NF; k++) {
+                    const int row = k * 16 + (lane >> 2);
+                    *reinterpret_cast<u4 *>(turn + u * (NF * 1024) + stored_place<NF>(row % NF, row / NF, lane & 3)) = next[u][k];
                 }
-                const int a_scale = scales[(t * kRows + i * 16 + r) * 4 + g];
-                AFragment<FA> a;
-                a.set(w);
+            }
+            if (NF * U == 4 || lane < NF * U * 16) {
+                reinterpret_cast<uint32_t *>(turn_scales)[scale_step * (NF * 16) + (scale_row % NF) * 16 + scale_row / NF] =
+                    take_scales(next_scale, scale_from, scale_last, min(t + scale_step, steps - 1) * 4, p.blocks);
+            }
+            if (t + U < steps) {
+                fetch(t + U);
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (u > 0 && t + u >= steps) {
+                    break;
+                }
+                v8i b[NF];
+                int b_scale[NF];
 #pragma unroll
                 for (int j = 0; j < NF; j++) {
-                    acc[i][j] = a.multiply(a_scale, b[j], b_scale[j], acc[i][j]);
+                    b[j] = wide(*reinterpret_cast<const u4 *>(turn + u * (NF * 1024) + stored_place<NF>(j, r, g)));
+                    b_scale[j] = turn_scales[((u * NF + j) * 16 + r) * 4 + g];
+                }
+#pragma unroll
+                for (int i = 0; i < MF; i++) {
+                    u4 w[kHalves];
+#pragma unroll
+                    for (int k = 0; k < kHalves; k++) {
+                        w[k] = *reinterpret_cast<const u4 *>(smem + (size_t)(t + u) * step_bytes + k * rows * 64 +
+                                                                fragment_place(a_row[i], g));
+                    }
+                    const int a_scale = scales[((t + u) * rows + a_row[i]) * 4 + g];
+                    AFragment<FA> a;
+                    a.set(w);
+#pragma unroll
+                    for (int j = 0; j < NF; j++) {
+                        acc[i][j] = a.multiply(a_scale, b[j], b_scale[j], acc[i][j]);
+                    }
                 }
             }
+            __builtin_amdgcn_wave_barrier();
         }
         const int64_t col = col0 + r * NF;
         float b_sqr[NF] = {};
@@ -279,7 +296,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
         }
 #pragma unroll
         for (int i = 0; i < MF; i++) {
-            store_scores<T, NF>(p, row0 + i * 16 + g * 4, col, acc[i], b_sqr);
+            store_scores<T, NF>(p, i * 16 + g * 4, col, acc[i], b_sqr);
         }
     }
 }
@@ -288,7 +305,8 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
 // and scales of both sides go through two LDS buffers of U steps (128 columns each); while one is multiplied, the next is
 // written from registers and the one after it is on its way from memory.
 template <int FA, int WM, int WN, int MF, int U, typename T>
-__global__ __launch_bounds__(WM * WN * 64, MF == 8 || FA == kE4M3 ? 2 : 3) void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
+__global__ __launch_bounds__(WM * WN * 64, MF == 8 || FA == kE4M3 ? 2 : 3)
+void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
     constexpr int kHalves = FA == kE2M1 ? 1 : 2, NF = 4, kThreads = WM * WN * 64;
     constexpr int kRows = WM * MF * 16, kCols = WN * 64;
@@ -479,9 +497,14 @@ __device__ __forceinline__ int wide_place(int r, int q) { return r * 64 + ((q ^ 
 // Many queries and many columns: tiles of 256 queries by 256 stored rows, four wavefronts of 128 x 128 (4 x 4 fragments of
 // 32 rows), one to a SIMD with 512 registers: twice the products per byte read from LDS of the kernel above.  Codes go
 // from memory straight into a ring of R LDS buffers, one step of 128 columns each, scales four steps at a time (4 bytes of a
-// row at a time touch its line in every step: 4096 x 32768 x 4096 365 us instead of 325).  A half-step of 64 columns reads the next one's fragments of stored rows while it multiplies its own, so
-// that no wavefront meets a barrier without products to do.  Four steps and more, multiples of four stored rows, rows of scores
-// that start on 64 bytes and have at most 2^23 of them, and scales that start on 4 bytes only.
+// row at a time touch its line in every step: 4096 x 32768 x 4096 365 us instead of 325).  A half-step of 64 columns reads the
+// next one's fragments of stored rows while it multiplies its own, so that no wavefront meets a barrier without products to
+// do; the last steps of a tile load the next one's first codes, which are on their way while scores leave.
+// Long rows are bound by the products (4096 x 32768 x 4096: 325 us, 3.4 PFLOP/s; the instruction alone reaches 7.5 at the clock
+// of a short loop, and the power of this one holds it near 1.7 GHz), short ones by the scores (2048 x 131072 x 768 to fp32:
+// 235 us, 4.8 TB/s); 8-bit queries take every product twice (748 us, 2.9 PFLOP/s of both halves).
+// Four steps and more, multiples of four stored rows, rows of scores that start on 64 bytes and have at most 2^23 of them, and
+// scales that start on 4 bytes only.
 template <int FA, int R, bool L2, typename T>
 __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
@@ -523,7 +546,8 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
         for (int k = 0; k < 4; k++) {
             a_from[k] = (uint32_t)(min((wave + 4 * k) * 16 + fr, last_row) * a_row_bytes + fq * 16);
             const int run = wave + 4 * k;   // of 128 rows run >> 3, fragment (run >> 1) & 3, rows 16 (run & 1) ...
-            b_from[k] = (uint32_t)(min((run >> 3) * 128 + ((run & 1) * 16 + fr) * 4 + ((run >> 1) & 3), last_col) * b_row_bytes + fq * 16);
+            const int row = (run >> 3) * 128 + ((run & 1) * 16 + fr) * 4 + ((run >> 1) & 3);
+            b_from[k] = (uint32_t)(min(row, last_col) * b_row_bytes + fq * 16);
         }
         // rows of scales, 16 bytes each, in the order of the fragments' rows
         const int scale_run = wave * 2 + (l >> 5);   // 32 rows: of 128 rows scale_run >> 2, fragment scale_run & 3
@@ -784,21 +808,21 @@ int64_t resident_workgroups(const void *kern, int threads, size_t lds)
 }
 
 template <int FA>
-size_t stream_lds(int mf, int nf, int steps)
+size_t stream_lds(int64_t m, int pieces, int steps)
 {
-    return (size_t)steps * mf * 16 * ((FA == kE2M1 ? 64 : 128) + 4) + 4 * nf * (1024 + 64);
+    return (size_t)steps * m * (FA == kE2M1 ? 64 : 128) + (((size_t)steps * m * 4 + 15) & ~(size_t)15) + 4 * pieces * (1024 + 64);
 }
 
-template <int FA, int MF, int NF, typename T>
+template <int FA, int MF, int NF, int U, typename T>
 void launch_stream(const ProductParams &p, hipStream_t s)
 {
     const int steps = (p.blocks + 3) / 4;
-    const size_t lds = stream_lds<FA>(MF, NF, steps);
+    const size_t lds = stream_lds<FA>(p.m, NF * U, steps);
     const int64_t tiles = (p.n + NF * 16 - 1) / (NF * 16);
-    const void *kern = reinterpret_cast<const void *>(mx_stream_kernel<FA, MF, NF, T>);
+    const void *kern = reinterpret_cast<const void *>(mx_stream_kernel<FA, MF, NF, U, T>);
     require_dynamic_lds(kern, lds);
-    const dim3 grid((unsigned)std::min((tiles + 3) / 4, resident_workgroups(kern, 256, lds)), (unsigned)((p.m + MF * 16 - 1) / (MF * 16)));
-    hipLaunchKernelGGL((mx_stream_kernel<FA, MF, NF, T>), grid, dim3(256), lds, s, p, steps, tiles);
+    const dim3 grid((unsigned)std::min((tiles + 3) / 4, resident_workgroups(kern, 256, lds)));
+    hipLaunchKernelGGL((mx_stream_kernel<FA, MF, NF, U, T>), grid, dim3(256), lds, s, p, steps, tiles);
     check_launch();
 }
 
@@ -834,14 +858,25 @@ void launch_type(const ProductParams &p, hipStream_t s)
 {
     const int steps = (p.blocks + 3) / 4;
     const int mf = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
-    if (p.m <= 64 && stream_lds<FA>(mf, 4, steps) <= 80 * 1024) {
-        const bool narrow = p.n <= 16 * 4096;   // too few tiles of 64 rows for every wavefront slot
+    if (p.m <= 64 && stream_lds<FA>(p.m, 4, steps) <= 80 * 1024) {
+        // Up to 2048 tiles of 16 stored rows (eight wavefronts per CU) such tiles, four steps at a time; else tiles of 64 rows,
+        // or, for up to 16 queries with more than one step, of 32 rows and 128 bytes of each at a time: with 64 bytes, and the
+        // many wavefronts that few queries leave room for, the two visits to a line of memory are too far apart.
+        // 1 x 20000 x 4096: 16 rows 9.9 us, 32 rows 12.5, 64 rows 20.6; 1 x 1M x 1536: 150, 154, 199; 64 x 1M x 768: 253, 171,
+        // 145; 32 x 1M x 512: 96, 76, 72; 1 x 1M x 128: 26.8, 17.8, 15.5.
+        const bool narrow = p.n <= 16 * 2048;
         if (mf == 1) {
-            narrow ? launch_stream<FA, 1, 1, T>(p, s) : launch_stream<FA, 1, 4, T>(p, s);
+            if (narrow) {
+                launch_stream<FA, 1, 1, 4, T>(p, s);
+            } else if (steps == 1) {
+                launch_stream<FA, 1, 4, 1, T>(p, s);
+            } else {
+                launch_stream<FA, 1, 2, 2, T>(p, s);
+            }
         } else if (mf == 2) {
-            narrow ? launch_stream<FA, 2, 1, T>(p, s) : launch_stream<FA, 2, 4, T>(p, s);
+            narrow ? launch_stream<FA, 2, 1, 4, T>(p, s) : launch_stream<FA, 2, 4, 1, T>(p, s);
         } else {
-            narrow ? launch_stream<FA, 4, 1, T>(p, s) : launch_stream<FA, 4, 4, T>(p, s);
+            narrow ? launch_stream<FA, 4, 1, 4, T>(p, s) : launch_stream<FA, 4, 4, 1, T>(p, s);
         }
         return;
     }
@@ -851,7 +886,8 @@ void launch_type(const ProductParams &p, hipStream_t s)
     // against 18).
     const int64_t wide_rows = (p.m + 255) / 256, wide_tiles = wide_rows * ((p.n + 255) / 256);
     if (p.blocks % 4 == 0 && p.blocks >= 16 && p.n % 4 == 0 && p.lines && p.ld <= (1 << 23) / (int)sizeof(T) &&
-        aligned(p.a_scales, 4) && aligned(p.b_scales, 4) && wide_rows * 256 * 4 <= p.m * 5 && wide_tiles >= (p.blocks >= 64 ? 128 : 256)) {
+        aligned(p.a_scales, 4) && aligned(p.b_scales, 4) && wide_rows * 256 * 4 <= p.m * 5 &&
+        wide_tiles >= (p.blocks >= 64 ? 128 : 256)) {
         p.metric == kMetricL2 ? launch_wide<FA, true, T>(p, s) : launch_wide<FA, false, T>(p, s);
         return;
     }
