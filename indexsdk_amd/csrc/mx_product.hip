@@ -147,25 +147,31 @@ __device__ __forceinline__ int stored_place(int j, int r, int q)
 }
 
 // The scales of one row, four blocks at a time and in two parts so that nothing waits for the load: load_scales brings four
-// bytes from block b on or, at the end of the array, from `last`, where its last four begin (`few`: the number of scales of
-// an array that has less); take_scales shifts and masks them.  Blocks behind the last get scale 0, the smallest power of two:
-// the queries' codes are zeros there.
-__device__ __forceinline__ uint32_t load_scales(const uint8_t *from, const uint8_t *last, int few, int b)
+// bytes at `at` or, where those would end `over` bytes behind the array, its last four (`few`: the number of scales of an array
+// that has less than four, else 0); take_scales shifts and masks them.  Blocks behind the last get scale 0, the smallest power
+// of two: the queries' codes are zeros there.
+__device__ __forceinline__ uint32_t load_scales(const uint8_t *base, int at, int over, int few)
 {
+    const uint8_t *from = base + (at - max(over, 0));
     uint32_t w = 0;
     if (few == 0) {
-        __builtin_memcpy(&w, from + b < last ? from + b : last, 4);
+        __builtin_memcpy(&w, from, 4);
     } else {   // no loop: around one the compiler waits for every load in flight
-        w = last[0] | (few > 1 ? (uint32_t)last[1] << 8 : 0u) | (few > 2 ? (uint32_t)last[2] << 16 : 0u);
+        w = from[0] | (few > 1 ? (uint32_t)from[1] << 8 : 0u) | (few > 2 ? (uint32_t)from[2] << 16 : 0u);
     }
     return w;
 }
-__device__ __forceinline__ uint32_t take_scales(uint32_t w, const uint8_t *from, const uint8_t *last, int b, int blocks)
+__device__ __forceinline__ uint32_t take_scales(uint32_t w, int b, int over, int blocks)
 {
-    const int64_t over = from + b - last;
-    w >>= 8 * (over < 0 ? 0 : over > 3 ? 3 : (int)over);
+    w >>= 8 * min(max(over, 0), 3);
     return blocks - b >= 4 ? w : w & ((1u << (8 * max(blocks - b, 0))) - 1u);
 }
+// `over` of a row's block 0 in an array of rows * blocks scales; of block b it is b more
+__device__ __forceinline__ int scales_over(int64_t row, int64_t rows, int blocks)
+{
+    return (int)max(row * blocks - max(rows * blocks - 4, (int64_t)0), (int64_t)-0x40000000);
+}
+__device__ __forceinline__ int few_scales(int64_t rows, int blocks) { return rows * blocks < 4 ? (int)rows * blocks : 0; }
 
 // Few queries (MF fragments of 16): their codes stay in LDS, all columns of them, while every wavefront streams NF fragments of
 // stored rows past them, U steps of 128 columns ahead.  Bound by the stored rows and the scores, both moved once: 64 x 1M x
@@ -190,11 +196,11 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
     // 256, 128 ... 4 threads bring a row; pieces behind its last block are zeros
     const int lg = rows > 1 ? 8 - (32 - __builtin_clz(rows - 1)) : 8, per_row = 1 << lg;
     if (const int row = (int)threadIdx.x >> lg, e = (int)threadIdx.x & (per_row - 1); row < rows) {
-        const int64_t total = p.m * p.blocks;
-        const uint8_t *const from = p.a_scales + (int64_t)row * p.blocks, *const last = p.a_scales + (total > 4 ? total - 4 : 0);
+        const uint8_t *const from = p.a_scales + (int64_t)row * p.blocks;
+        const int over = scales_over(row, p.m, p.blocks), few = few_scales(p.m, p.blocks);
         for (int step = e; step < steps; step += per_row) {
             reinterpret_cast<uint32_t *>(scales)[step * rows + row] = take_scales(
-                load_scales(from, last, total < 4 ? (int)total : 0, step * 4), from, last, step * 4, p.blocks);
+                load_scales(from, step * 4, over + step * 4, few), step * 4, over + step * 4, p.blocks);
         }
         for (int piece = e; piece < steps * 4 * kHalves; piece += per_row) {
             u4 v = u4{};
@@ -210,9 +216,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
         a_row[i] = min(i * 16 + r, rows - 1);
     }
     __syncthreads();
-    const int64_t b_total = p.n * p.blocks;
-    const uint8_t *const scale_last = p.b_scales + (b_total > 4 ? b_total - 4 : 0);
-    const int scale_few = b_total < 4 ? (int)b_total : 0;
+    const int few = few_scales(p.n, p.blocks);
     const int64_t stride = (int64_t)gridDim.x * 4;
     for (int64_t tile = (int64_t)blockIdx.x * 4 + wave; tile < tiles; tile += stride) {
         const int64_t col0 = tile * (NF * 16);
@@ -225,6 +229,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
         }
         const int scale_row = lane % (NF * 16), scale_step = lane / (NF * 16) % U;
         const uint8_t *const scale_from = p.b_scales + (col0 + min(scale_row, last)) * p.blocks;
+        const int over = scales_over(col0 + min(scale_row, last), p.n, p.blocks);
         u4 next[U][NF];
         uint32_t next_scale = 0;
         // pieces behind the last block repeat it: the queries' codes are zeros there
@@ -237,7 +242,8 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
                     next[u][k] = *reinterpret_cast<const u4 *>(codes + (offset[k] + byte));
                 }
             }
-            next_scale = load_scales(scale_from, scale_last, scale_few, min(t + scale_step, steps - 1) * 4);
+            const int b_from = min(t + scale_step, steps - 1) * 4;
+            next_scale = load_scales(scale_from, b_from, over + b_from, few);
         };
         fetch(0);
         v4f acc[MF][NF] = {};
@@ -251,8 +257,9 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
                 }
             }
             if (NF * U == 4 || lane < NF * U * 16) {
+                const int b_from = min(t + scale_step, steps - 1) * 4;
                 reinterpret_cast<uint32_t *>(turn_scales)[scale_step * (NF * 16) + (scale_row % NF) * 16 + scale_row / NF] =
-                    take_scales(next_scale, scale_from, scale_last, min(t + scale_step, steps - 1) * 4, p.blocks);
+                    take_scales(next_scale, b_from, over + b_from, p.blocks);
             }
             if (t + U < steps) {
                 fetch(t + U);
@@ -334,19 +341,30 @@ void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
     u4 a_piece[kAPieces], b_piece[kBPieces];
     uint32_t scale[kScaleRows][U];
     // the rows whose scales a thread brings
-    const uint8_t *scale_from[kScaleRows], *scale_last[kScaleRows];
-    int scale_few[kScaleRows];
+    static_assert(kRows % 64 == 0, "a wavefront's scales are all of one side");
+    const uint8_t *scale_base[kScaleRows];
+    int scale_offset[kScaleRows], over[kScaleRows];
+    const int few = few_scales(p.n, p.blocks);   // a tile's queries have more than four scales: they are many, or long
 #pragma unroll
     for (int k = 0; k < kScaleRows; k++) {
-        const int row = tid + k * kThreads;
-        const bool query = row < kRows;
-        const int64_t total = (query ? p.m : p.n) * p.blocks;
-        const uint8_t *const begin = query ? p.a_scales : p.b_scales;
-        scale_from[k] = begin + (query ? row0 + min(row, last_row) : col0 + min(row - kRows, last_col)) * p.blocks;
-        scale_last[k] = begin + (total > 4 ? total - 4 : 0);
-        scale_few[k] = total < 4 ? (int)total : 0;
+        const bool query = wave * 64 + k * kThreads < kRows;
+        const int row = tid + k * kThreads, in = query ? min(row, last_row) : min(row - kRows, last_col);
+        const int64_t first = query ? row0 : col0;
+        scale_base[k] = (query ? p.a_scales : p.b_scales) + first * p.blocks;
+        scale_offset[k] = in * p.blocks;
+        over[k] = scales_over(first + in, query ? p.m : p.n, p.blocks);
     }
     auto bring = [&](int stage) {   // from memory into registers
+#pragma unroll
+        for (int k = 0; k < kScaleRows; k++) {
+            if (const int row = wave * 64 + k * kThreads; row < kRows + kCols) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int b = (stage * U + u) * 4;
+                    scale[k][u] = load_scales(scale_base[k], scale_offset[k] + b, over[k] + b, row < kRows ? 0 : few);
+                }
+            }
+        }
 #pragma unroll
         for (int k = 0; k < kAPieces; k++) {
             const int e = tid + k * kThreads, row = min((e >> 2) % kRows, last_row);
@@ -358,16 +376,6 @@ void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
             const int e = tid + k * kThreads, row = min((e >> 2) % kCols, last_col);
             const int byte = (stage * U + (e >> 2) / kCols) * 64 + (e & 3) * 16;
             b_piece[k] = *reinterpret_cast<const u4 *>(b_base + (uint32_t)(row * b_row_bytes + min(byte, b_row_bytes - 16)));
-        }
-#pragma unroll
-        for (int k = 0; k < kScaleRows; k++) {
-            const int row = tid + k * kThreads;
-            if (row < kRows + kCols) {
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    scale[k][u] = load_scales(scale_from[k], scale_last[k], scale_few[k], (stage * U + u) * 4);
-                }
-            }
         }
     };
     auto put = [&](int stage) {     // from registers into LDS; queries' codes behind the last block are zeros
@@ -393,7 +401,8 @@ void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
                 uint8_t *const o = to + kABytes + kBBytes + place * 4 * U;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    scale[k][u] = take_scales(scale[k][u], scale_from[k], scale_last[k], (stage * U + u) * 4, p.blocks);
+                    const int b = (stage * U + u) * 4;
+                    scale[k][u] = take_scales(scale[k][u], b, over[k] + b, p.blocks);
                 }
                 if constexpr (U == 2) {   // block g of either step next to each other
                     *reinterpret_cast<uint2 *>(o) = make_uint2(__builtin_amdgcn_perm(scale[k][1], scale[k][0], 0x05010400u),
