@@ -308,9 +308,11 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
     }
 }
 
-// Many queries: tiles of WM * 128 queries by WN * 64 stored rows, one wavefront per 128 x 64 of them (8 x 4 fragments).  Codes
-// and scales of both sides go through two LDS buffers of U steps (128 columns each); while one is multiplied, the next is
-// written from registers and the one after it is on its way from memory.
+// Many queries: tiles of WM * MF * 16 queries by WN * 64 stored rows, one wavefront per MF * 16 x 64 of them (MF x 4 fragments).
+// Codes and scales of both sides go through two LDS buffers of U steps (128 columns each); while one is multiplied, the next is
+// written from registers and the one after it is on its way from memory.  Any sizes and strides.  Bound by the scores in short
+// rows (2048 x 131072 x 200 to fp32: 235 us, 4.6 TB/s), in long ones by what the wavefronts read from LDS between products: 2048 x
+// 100001 x 768 288 us, 1.1 PFLOP/s with 3 TB/s of scores; 1024 x 60001 x 2016 124 us, 2 PFLOP/s.
 template <int FA, int WM, int WN, int MF, int U, typename T>
 __global__ __launch_bounds__(WM * WN * 64, MF == 8 || FA == kE4M3 ? 2 : 3)
 void mx_tile_kernel(ProductParams p, int row_tiles, int col_tiles, int per_xcd)
@@ -901,13 +903,22 @@ void launch_type(const ProductParams &p, hipStream_t s)
         return;
     }
     const int64_t tiles = ((p.m + 127) / 128) * ((p.n + 255) / 256);
-    if (tiles < 512) {
+    // Tiles of 128 x 256, of 64 x 256 where that would be less than three for two CUs (300 x 20000 x 1030: 25 us, 128 x 256 31;
+    // 1024 x 8192 x 1024: 26 and 34; with 391 of them, 100 x 100003 x 200, 14.8 and 12.9), and of 256 x 256 and two steps at
+    // a time for 4-bit queries with two such tiles and more per CU in rows of 512 columns and more (1024 x 60001 x 2016: 124 us,
+    // 128 x 256 154; 2048 x 100001 x 768: 288 and 312; shorter rows 2048 x 131072 x 200: 282 and 234; fewer tiles
+    // 1000 x 20001 x 4096: 100 and 97; with 8-bit queries 4096 x 32768 x 2080: 513 and 498).
+    if (tiles < 384) {
         launch_tiles<FA, 1, 4, 4, 1, T>(p, s);
-    } else if (p.m <= 128 || p.blocks <= 64) {
-        launch_tiles<FA, 1, 4, 8, 1, T>(p, s);
-    } else {
-        launch_tiles<FA, 2, 4, 8, FA == kE2M1 ? 2 : 1, T>(p, s);
+        return;
     }
+    if constexpr (FA == kE2M1) {
+        if (p.blocks >= 16 && wide_rows * 256 * 4 <= p.m * 5 && wide_tiles >= 512) {
+            launch_tiles<FA, 2, 4, 8, 2, T>(p, s);
+            return;
+        }
+    }
+    launch_tiles<FA, 1, 4, 8, 1, T>(p, s);
 }
 
 template <int FA>

@@ -419,6 +419,13 @@ def test_product_in_whole_steps_of_128_columns(lib, m, n, d, a_fmt):
     check_product(lib, m, n - 12, d, a_fmt, 1, "f16", wild=True, pad=12 + 64 - n % 32)
 
 
+@pytest.mark.parametrize("m,n,d,kind", [(510, 65601, 520, "f32"), (1000, 33001, 700, "bf16")])
+@pytest.mark.parametrize("a_fmt", [MXFP4, MXFP8])
+def test_product_of_many_rows_of_any_length(lib, m, n, d, kind, a_fmt):
+    check_product(lib, m, n, d, a_fmt, 1, kind, wild=True)
+    check_product(lib, m, n, d, a_fmt, 0, kind, wild=False, pad=5)
+
+
 @pytest.mark.parametrize("a_fmt", [MXFP4, MXFP8])
 def test_product_of_one_large_and_many_small_numbers(lib, a_fmt):
     """What an instruction that aligns its products to the largest would drop: 448 * 6 next to 2^-9 * 0.5 in one block."""
