@@ -46,10 +46,9 @@ void op_mx_product(const uint8_t *a_codes, const uint8_t *a_scales, int a_format
                    const uint8_t *b_scales, int64_t n, int d, int metric, const float *a_sqr, const float *b_sqr,
                    int out_type, void *out, int64_t ld, hipStream_t s);
 
-// After a launch: an error the device (or its absence) answered with becomes this library's.
-inline void check_launch()
+// An error the device (or its absence) answered with becomes this library's.
+inline void check_answer(hipError_t e)
 {
-    const hipError_t e = hipGetLastError();
     if (e == hipSuccess) {
         return;
     }
@@ -58,5 +57,7 @@ inline void check_launch()
                 "no HIP device available: this library has no CPU path");
     IXA_HIP(e);
 }
+// after a launch
+inline void check_launch() { check_answer(hipGetLastError()); }
 
 }  // namespace ixa

@@ -957,6 +957,8 @@ void op_mx_product(const uint8_t *a_codes, const uint8_t *a_scales, int a_format
     if (m == 0 || n == 0) {
         return;
     }
+    int device;
+    check_answer(hipGetDevice(&device));   // what is asked of a kernel before its launch needs one
     const ProductParams p{a_codes, a_scales, b_codes, b_scales, a_sqr, b_sqr, m, n, ld, mx_blocks(d), metric, out,
                           aligned(out, 64) && ld * (out_type == kTypeF32 ? 4 : 2) % 64 == 0};
     if (a_format == kFormatMxFp4) {

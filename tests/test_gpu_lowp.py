@@ -576,3 +576,18 @@ def test_4_bit_rows_find_the_nearest(lib):
     go(None)
     torch.cuda.synchronize()
     assert (label[:, 0].cpu().numpy() == np.arange(64)).mean() > 0.95
+
+
+def test_the_example(lib, capsys):
+    """examples/low_precision_search.py: rows to 4 bits keep about a tenth of their norm as error, and the row that a query was
+    made from, far nearer than any other, comes first."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "low_precision_search.py")
+    spec = importlib.util.spec_from_file_location("low_precision_search", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.run(n=5003, m=300, d=200, k=10, page=128)
+    assert got["bytes"] == 5003 * (7 * 16 + 7 + 4)
+    assert got["itself"] == 1.0 and 0.05 < got["error"] < 0.2 and got["recall"] > 0.2
+    assert "nearest" in capsys.readouterr().out
