@@ -173,7 +173,7 @@ int ixa_op_dequantise(const uint8_t *codes_dev, const void *scales_dev, int form
 
 /* h = x + residual (residual may be NULL) is written to sum (may be NULL, may be x or residual themselves) rounded to `type`;
  * y = h / sqrt(mean(h^2) + eps) * weight (weight [d] may be NULL) becomes codes and scales as above.  x, residual, weight and
- * sum are all of `type`; the arithmetic is fp32 and y is made from the unrounded h.  eps > 0. */
+ * sum are all of `type`; y is made from the unrounded fp32 h, its sum and products are rounded to fp32 once.  eps > 0. */
 int ixa_op_rms_norm_quantise(const void *x_dev, int64_t ld_x, const void *residual_dev, int64_t ld_residual,
                              const void *weight_dev, int type, int64_t n, int d, float eps, void *sum_dev, int64_t ld_sum,
                              int format, float fixed_scale, uint8_t *codes_dev, void *scales_dev, float *sqr_sum_dev,

@@ -10,6 +10,8 @@
 // that holds an infinity or a NaN gets a NaN scale and zero codes.  With a fixed scale, codes are clamped to +-127, NaN to 0.
 #include "lowp.h"
 
+#include <type_traits>
+
 namespace ixa {
 
 namespace {
@@ -103,39 +105,69 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v)
     return umax(v, dpp<kQuadXor2>(v));
 }
 
-// Reductions over the L lanes of a row; with L = 256 over the workgroup, through `box` (4 words, a barrier on either side).
-template <int L, typename Op>
-__device__ __forceinline__ uint32_t row_reduce(uint32_t v, uint32_t *box, Op op)
+// v of another lane, 32 or 64 bits
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp_of(V v)
 {
-    v = op(v, dpp<kQuadXor1>(v));
-    v = op(v, dpp<kQuadXor2>(v));
-    v = op(v, dpp<kHalfMirror>(v));
-    v = op(v, dpp<kMirror>(v));
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, dpp<CTRL>(__builtin_bit_cast(uint32_t, v)));
+    } else {
+        const uint2 w = __builtin_bit_cast(uint2, v);
+        return __builtin_bit_cast(V, make_uint2(dpp<CTRL>(w.x), dpp<CTRL>(w.y)));
+    }
+}
+
+// v of a lane and of the one 16 or 32 (HALVES) lanes from it, joined: swapping odd rows of 16 lanes (the upper half) of one
+// register with even ones (the lower half) of its copy leaves one of the two in either register, without the LDS
+template <bool HALVES, typename V, typename Op>
+__device__ __forceinline__ V swapped(V v, Op op)
+{
+    struct Box {
+        uint32_t w[sizeof(V) / 4];
+    };
+    Box a = __builtin_bit_cast(Box, v), b;
+#pragma unroll
+    for (size_t i = 0; i < sizeof(V) / 4; i++) {
+        const auto t = HALVES ? __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false)
+                              : __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false);
+        a.w[i] = t[0];
+        b.w[i] = t[1];
+    }
+    return op(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b));
+}
+
+// Reductions over the L lanes of a row; with L = 256 over the workgroup, through `box` (a barrier on either side).
+template <int L, typename V, typename Op>
+__device__ __forceinline__ V row_reduce(V v, double *box, Op op)
+{
+    v = op(v, dpp_of<kQuadXor1>(v));
+    v = op(v, dpp_of<kQuadXor2>(v));
+    v = op(v, dpp_of<kHalfMirror>(v));
+    v = op(v, dpp_of<kMirror>(v));
     if constexpr (L >= 32) {
-        v = op(v, (uint32_t)__shfl_xor((int)v, 16));
+        v = swapped<false>(v, op);
     }
     if constexpr (L >= 64) {
-        v = op(v, (uint32_t)__shfl_xor((int)v, 32));
+        v = swapped<true>(v, op);
     }
     if constexpr (L == 256) {
+        V *const of = reinterpret_cast<V *>(box);
         __syncthreads();   // the readers of the last reduction are done with the box
         if ((threadIdx.x & 63) == 0) {
-            box[threadIdx.x >> 6] = v;
+            of[threadIdx.x >> 6] = v;
         }
         __syncthreads();
-        v = op(op(box[0], box[1]), op(box[2], box[3]));
+        v = op(op(of[0], of[1]), op(of[2], of[3]));
     }
     return v;
 }
-template <int L>
-__device__ __forceinline__ float row_sum(float v, uint32_t *box)
+template <int L, typename V>
+__device__ __forceinline__ V row_sum(V v, double *box)
 {
-    return __uint_as_float(row_reduce<L>(__float_as_uint(v), box, [](uint32_t a, uint32_t b) {
-        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-    }));
+    return row_reduce<L>(v, box, [](V a, V b) { return a + b; });
 }
 template <int L>
-__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *box)
+__device__ __forceinline__ uint32_t row_max(uint32_t v, double *box)
 {
     return row_reduce<L>(v, box, umax);
 }
@@ -145,6 +177,7 @@ struct RowParams {
     int64_t ld_x, ld_residual, ld_sum, n;
     int d, blocks;
     float eps, fixed_scale;
+    double inv_d;
     void *sum;
     uint8_t *codes;
     void *scales;
@@ -210,7 +243,7 @@ __device__ __forceinline__ float encode_fp8(const float (&y)[kVec], uint32_t bia
 template <typename T, int L, int C, bool NORM, bool PAST>
 __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
 {
-    __shared__ uint32_t box[4];
+    __shared__ double box[4];
     const int lane = threadIdx.x % L;
     const int64_t row = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
     if (L < 256 && row >= p.n) {
@@ -249,48 +282,69 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
                 store8<PAST>(o + (count ? at : 0), count, p.whole_sum, y[c]);
             }
         }
-        float ss = 0.f;
+        // Eight squares are added in 32 bits, all else up to the root's reciprocal r in 64; r and the products y r w are held in two
+        // parts of 32 and rounded once: codes are as far apart as 2^-3 of a value, and every rounding before them moves
+        // some to a neighbour.
+        auto sum_of_squares = [&]() {
+            double sum = 0.0;
 #pragma unroll
-        for (int c = 0; c < C; c++) {
+            for (int c = 0; c < C; c++) {
+                float ss = 0.f;
 #pragma unroll
-            for (int i = 0; i < kVec; i++) {
-                ss = fmaf(y[c][i], y[c][i], ss);
+                for (int i = 0; i < kVec; i++) {
+                    ss = fmaf(y[c][i], y[c][i], ss);
+                }
+                sum += (double)ss;
             }
-        }
-        ss = row_sum<L>(ss, box);
-        float r = 1.0f / sqrtf(ss / (float)p.d + p.eps);
-        if (ss == __builtin_inff()) {   // finite elements whose squares pass the largest number: once more, 2^-80 as large
-            ss = 0.f;
+            return row_sum<L>(sum, box);
+        };
+        double mean = sum_of_squares() * p.inv_d + p.eps;
+        if (mean == __builtin_inf()) {   // finite elements whose squares pass the largest number: once more, 2^-80 as large
 #pragma unroll
             for (int c = 0; c < C; c++) {
 #pragma unroll
                 for (int i = 0; i < kVec; i++) {
                     y[c][i] *= 0x1p-80f;
-                    ss = fmaf(y[c][i], y[c][i], ss);
                 }
             }
-            r = 1.0f / sqrtf(row_sum<L>(ss, box) / (float)p.d);
+            mean = sum_of_squares() * p.inv_d;
         }
+        double r = __builtin_amdgcn_rsq(mean);   // half of a double's bits at least, and a step of Newton's for the rest
+        r = mean == __builtin_inf() ? 0.0 : r * fma(-0.5 * mean * r, r, 1.5);
+        const float high = (float)r, low = (float)(r - (double)high);
         const T *w = static_cast<const T *>(p.weight);
+        auto multiply = [&](auto keep) {
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const int at = (c * L + lane) * kVec;
-            const int count = min(kVec, max(0, p.d - at));
-            float wv[kVec];
-            if (w) {
-                load8(w + (count ? at : 0), count, p.whole_weight, wv);
-            }
+            for (int c = 0; c < C; c++) {
+                const int at = (c * L + lane) * kVec;
+                const int count = min(kVec, max(0, p.d - at));
+                float wv[kVec];
+                if (w) {
+                    load8(w + (count ? at : 0), count, p.whole_weight, wv);
+                }
 #pragma unroll
-            for (int i = 0; i < kVec; i++) {
-                y[c][i] *= r;
-                y[c][i] = w ? y[c][i] * wv[i] : y[c][i];
+                for (int i = 0; i < kVec; i++) {
+                    float v = y[c][i] * high, rest = fmaf(y[c][i], low, fmaf(y[c][i], high, -v));
+                    if (w) {
+                        const float t = v * wv[i];
+                        rest = fmaf(rest, wv[i], fmaf(v, wv[i], -t));
+                        v = t;
+                    }
+                    y[c][i] = decltype(keep)::value && fabsf(v) == __builtin_inff() ? v : v + rest;
+                }
             }
+        };
+        // with a fixed scale an infinity ends at the last code; elsewhere it makes no difference whether a NaN takes its place
+        if (p.fixed_scale > 0.f) {
+            multiply(std::true_type());
+        } else {
+            multiply(std::false_type());
         }
     }
     const bool want_sqr = p.sqr_sum != nullptr;
     float ss = 0.f;
     if (p.format == kFormatInt8) {
-        float scale = p.fixed_scale, pre = 1.f, inv;
+        float scale = p.fixed_scale, inv;
         bool bad = false;
         if (scale > 0.f) {
             inv = 1.0f / scale;
@@ -305,35 +359,59 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
             }
             top = row_max<L>(top, box);
             bad = top >= kInfBits;
-            const float t = __uint_as_float(top);
-            pre = t < 0x1p-90f ? 0x1p64f : 1.f;   // 127 / t would not be finite
-            inv = t > 0.f && !bad ? 127.0f / (t * pre) : 0.f;
+            float t = __uint_as_float(top);
             scale = bad ? __builtin_nanf("") : t / 127.0f;
-        }
-        int sq = 0;
-        uint8_t *o = p.codes + row * p.d;
+            if (t < 0x1p-90f) {   // 127 / t would not be finite
+                t *= 0x1p64f;
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const int at = (c * L + lane) * kVec;
-            const int count = min(kVec, max(0, p.d - at));
-            uint32_t w[2] = {0, 0};
+                for (int c = 0; c < C; c++) {
 #pragma unroll
-            for (int i = 0; i < kVec; i++) {
-                const float v = y[c][i] * pre * inv;
-                const int q = bad || v != v ? 0 : (int)rintf(__builtin_amdgcn_fmed3f(v, -127.f, 127.f));
-                sq += q * q;
-                w[i / 4] |= (uint32_t)(q & 0xff) << (8 * (i % 4));
-            }
-            if (count == kVec && (p.d & 7) == 0) {
-                *reinterpret_cast<uint2 *>(o + at) = make_uint2(w[0], w[1]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kVec; i++) {
-                    if (i < count) {
-                        o[at + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+                    for (int i = 0; i < kVec; i++) {
+                        y[c][i] *= 0x1p64f;
                     }
                 }
             }
+            inv = t > 0.f && !bad ? 127.0f / t : 0.f;
+        }
+        int sq = 0;
+        uint8_t *o = p.codes + row * p.d;
+        auto encode = [&](auto fixed) {
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const int at = (c * L + lane) * kVec;
+                const int count = min(kVec, max(0, p.d - at));
+                uint32_t q[kVec], w[2];
+#pragma unroll
+                for (int i = 0; i < kVec; i++) {
+                    float v = y[c][i] * inv;
+                    if constexpr (decltype(fixed)::value) {
+                        v = v != v ? 0.f : __builtin_amdgcn_fmed3f(v, -127.f, 127.f);
+                    }
+                    q[i] = __float_as_uint(v + 0x1.8p23f);   // rounded to an integer, halfway to even: the lowest byte is the code
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    w[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[4 * k + 3], q[4 * k + 2], 0x0c0c0400u),
+                                                 __builtin_amdgcn_perm(q[4 * k + 1], q[4 * k], 0x0c0c0400u), 0x05040100u);
+                    w[k] = bad ? 0u : w[k];
+                    sq = __builtin_amdgcn_sdot4((int)w[k], (int)w[k], sq, false);
+                }
+                if (count == kVec && (p.d & 7) == 0) {
+                    *reinterpret_cast<uint2 *>(o + at) = make_uint2(w[0], w[1]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kVec; i++) {
+                        if (i < count) {
+                            o[at + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+                        }
+                    }
+                }
+            }
+        };
+        if (p.fixed_scale > 0.f) {
+            encode(std::true_type());
+        } else {
+            encode(std::false_type());
         }
         if (lane == 0 && p.scales) {
             static_cast<float *>(p.scales)[row] = scale;
@@ -651,6 +729,7 @@ void op_rms_norm_quantise(const void *x, int64_t ld_x, const void *residual, int
     p.d = d;
     p.blocks = mx_blocks(d);
     p.eps = eps;
+    p.inv_d = 1.0 / d;
     p.fixed_scale = fixed_scale;
     p.sum = sum;
     p.codes = codes;
