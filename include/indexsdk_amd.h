@@ -181,7 +181,8 @@ int ixa_op_rms_norm_quantise(const void *x_dev, int64_t ld_x, const void *residu
 
 /* Scores of m rows a (a_format IXA_FORMAT_MXFP8 or IXA_FORMAT_MXFP4) against n rows b (IXA_FORMAT_MXFP4), all of d dimensions:
  * out [m][ld] of out_type = inner products g, or for IXA_METRIC_L2 (a_sqr_sum + b_sqr_sum) - 2 g (both norms needed;
- * ignored for the inner product).  Sums are held in fp32.  A NaN scale makes every score of its row NaN.  fp32 scores are what
+ * ignored for the inner product).  Sums are held in fp32.  A NaN scale makes every score of its row NaN.  Columns behind d in a
+ * row's last block count as they are coded: zeros, as the operators above leave them.  fp32 scores are what
  * ixa_op_topk_flat_fp32 selects from. */
 int ixa_op_mx_product(const uint8_t *a_codes_dev, const uint8_t *a_scales_dev, int a_format, int64_t m,
                       const uint8_t *b_codes_dev, const uint8_t *b_scales_dev, int64_t n, int d, int metric,

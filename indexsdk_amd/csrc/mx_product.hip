@@ -842,7 +842,8 @@ void launch_tiles(const ProductParams &p, hipStream_t s)
 {
     const int64_t row_tiles = (p.m + WM * MF * 16 - 1) / (WM * MF * 16), col_tiles = (p.n + WN * 64 - 1) / (WN * 64);
     const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
-    IXA_REQUIRE(per_xcd <= 0x0fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m, (long)p.n);
+    IXA_REQUIRE(per_xcd * 8 * (WM * WN * 64) <= 0xffffffffll, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m,
+                (long)p.n);
     hipLaunchKernelGGL((mx_tile_kernel<FA, WM, WN, MF, U, T>), dim3((unsigned)per_xcd * 8), dim3(WM * WN * 64), 0, s, p,
                        (int)row_tiles, (int)col_tiles, (int)per_xcd);
     check_launch();

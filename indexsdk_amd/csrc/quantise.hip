@@ -10,6 +10,7 @@
 // that holds an infinity or a NaN gets a NaN scale and zero codes.  With a fixed scale, codes are clamped to +-127, NaN to 0.
 #include "lowp.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace ixa {
@@ -174,7 +175,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, double *box)
 
 struct RowParams {
     const void *x, *residual, *weight;
-    int64_t ld_x, ld_residual, ld_sum, n;
+    int64_t ld_x, ld_residual, ld_sum, n, row0;   // row0: the first row of this launch
     int d, blocks;
     float eps, fixed_scale;
     double inv_d;
@@ -245,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
 {
     __shared__ double box[4];
     const int lane = threadIdx.x % L;
-    const int64_t row = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+    const int64_t row = p.row0 + (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
     if (L < 256 && row >= p.n) {
         return;   // whole groups of lanes that share no data with others (with L = 256 the grid is the number of rows)
     }
@@ -461,17 +462,27 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
     }
 }
 
+// A launch has less than 2^32 threads: more rows than half a million workgroups take go in several.
+template <typename Params, typename Launch>
+void in_launches(Params p, int rows_per_group, Launch launch)
+{
+    constexpr int64_t kGroups = 1 << 19;
+    for (p.row0 = 0; p.row0 < p.n; p.row0 += kGroups * rows_per_group) {
+        launch(p, (unsigned)std::min(kGroups, (p.n - p.row0 + rows_per_group - 1) / rows_per_group));
+        check_launch();
+    }
+}
+
 template <typename T, int L, int C, bool NORM>
 void launch_rows_of(const RowParams &p, hipStream_t s)
 {
-    constexpr int kRows = kThreads / L;
-    const int64_t grid = (p.n + kRows - 1) / kRows;
-    if (NORM && p.past) {
-        hipLaunchKernelGGL((row_quantise_kernel<T, L, C, NORM, NORM>), dim3((unsigned)grid), dim3(kThreads), 0, s, p);
-    } else {
-        hipLaunchKernelGGL((row_quantise_kernel<T, L, C, NORM, false>), dim3((unsigned)grid), dim3(kThreads), 0, s, p);
-    }
-    check_launch();
+    in_launches(p, kThreads / L, [&](const RowParams &q, unsigned grid) {
+        if (NORM && p.past) {
+            hipLaunchKernelGGL((row_quantise_kernel<T, L, C, NORM, NORM>), dim3(grid), dim3(kThreads), 0, s, q);
+        } else {
+            hipLaunchKernelGGL((row_quantise_kernel<T, L, C, NORM, false>), dim3(grid), dim3(kThreads), 0, s, q);
+        }
+    });
 }
 
 // Few lanes with two to four times eight elements each: sums over lanes cost more than sums in a lane (norms of 500000 x 384: 32
@@ -517,7 +528,7 @@ bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(
 // Float rows that the last cache (256 MB) could not hold for whoever reads them next pass it by, which leaves it to what is
 // still to be read: the norm of 131072 x 4096 645 -> 627 us, and in turns with reading codes back the quantisation of
 // 1.2M x 200 243 -> 220.
-bool pass_caches(int64_t n, int64_t ld, int type) { return n * ld * (type == kTypeF32 ? 4 : 2) > (int64_t)1 << 27; }
+bool pass_caches(int64_t n, int64_t ld, int type) { return (double)n * (double)ld * (double)type_bytes(type) > 0x1p27; }
 // rows that all start on 16 bytes
 bool whole_rows(const void *p, int64_t ld, int type) { return aligned(p, 16) && (ld * (int64_t)type_bytes(type)) % 16 == 0; }
 
@@ -554,7 +565,7 @@ constexpr int kReadRows = 2;
 struct ReadParams {
     const uint8_t *codes;
     const void *scales;
-    int64_t n, ld;
+    int64_t n, ld, row0;           // row0: the first row of this launch
     int d, blocks, chunks, rows;   // chunks of 8 elements per row, rows that a workgroup reads at a time
     void *out;
     bool whole;
@@ -627,7 +638,7 @@ __global__ __launch_bounds__(kThreads) void read_codes_kernel(ReadParams p)
     if (in >= p.rows) {
         return;
     }
-    const int64_t first = (int64_t)blockIdx.x * (p.rows * kReadRows) + in;
+    const int64_t first = p.row0 + (int64_t)blockIdx.x * (p.rows * kReadRows) + in;
     for (int c = threadIdx.x - in * across; c < p.chunks; c += kThreads) {
         float v[kReadRows][kVec];
 #pragma unroll
@@ -647,14 +658,13 @@ __global__ __launch_bounds__(kThreads) void read_codes_kernel(ReadParams p)
 template <typename T, int FORMAT>
 void launch_read(const ReadParams &p, bool past, hipStream_t s)
 {
-    const int at_a_time = p.rows * kReadRows;
-    const dim3 grid((unsigned)((p.n + at_a_time - 1) / at_a_time));
-    if (past) {
-        hipLaunchKernelGGL((read_codes_kernel<T, FORMAT, true>), grid, dim3(kThreads), 0, s, p);
-    } else {
-        hipLaunchKernelGGL((read_codes_kernel<T, FORMAT, false>), grid, dim3(kThreads), 0, s, p);
-    }
-    check_launch();
+    in_launches(p, p.rows * kReadRows, [&](const ReadParams &q, unsigned grid) {
+        if (past) {
+            hipLaunchKernelGGL((read_codes_kernel<T, FORMAT, true>), dim3(grid), dim3(kThreads), 0, s, q);
+        } else {
+            hipLaunchKernelGGL((read_codes_kernel<T, FORMAT, false>), dim3(grid), dim3(kThreads), 0, s, q);
+        }
+    });
 }
 
 template <typename T>

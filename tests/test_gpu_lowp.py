@@ -506,6 +506,28 @@ def test_rows_at_large_offsets(lib):
     check_codes(want.astype(np.float64), want, MXFP4, out.get())
 
 
+def test_more_rows_than_one_launch_takes(lib):
+    """1.3 million rows of 2056 elements, 64 different ones over and over: the codes and values of the 64."""
+    d, n, some = 2056, 1_300_003, 64
+    few = rows(sample(some, d, 5), "bf16")
+    which = torch.arange(n, device="cuda") % some
+    x = few[which]
+    want, got = Codes(some, d, MXFP4), Codes(n, d, MXFP4)
+    for t, c in ((few, want), (x, got)):
+        lib[1](lib[0].ixa_op_rms_norm_quantise(at(t), d, None, 0, None, 2, c.n, d, 1e-6, None, 0, MXFP4, 0.0, at(c.codes),
+                                               at(c.scales), at(c.sqr), None))
+    values = [torch.full((c.n, d), 9.0, dtype=torch.bfloat16, device="cuda") for c in (want, got)]
+    for v, c in zip(values, (want, got)):
+        lib[1](lib[0].ixa_op_dequantise(at(c.codes), at(c.scales), MXFP4, c.n, d, 2, at(v), d, None))
+    torch.cuda.synchronize()
+    for name, size in (("codes", want.row), ("scales", want.per), ("sqr", 1)):
+        small, large = getattr(want, name)[:some * size].view(some, size), getattr(got, name)
+        assert all(torch.equal(large[i * size:j * size].view(-1, size), small[which[i:j]])
+                   for i in range(0, n, 200_000) for j in [min(n, i + 200_000)])
+        assert (large[n * size:] == (7 if name == "sqr" else GUARD)).all()
+    assert all(torch.equal(values[1][i:i + 200_000], values[0][which[i:i + 200_000]]) for i in range(0, n, 200_000))
+
+
 # ----- streams, graphs, the path as a whole ---------------------------------------------------------------------------------
 
 def chain(lib, x, q, w, stream):
