@@ -31,29 +31,40 @@ struct Vec8 {
     T v[kVec];
 };
 
+// Eight elements as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T *__restrict__ p, int count, bool whole, float (&v)[kVec])
-{
-    if (whole && count == kVec) {
-        constexpr int kWords = kVec * sizeof(T) / 16;
-        struct Words {
-            u4 w[kWords];
-        } w;
-#pragma unroll
-        for (int i = 0; i < kWords; i++) {
-            w.w[i] = reinterpret_cast<const u4 *>(p)[i];
-        }
-        const Vec8<T> t = __builtin_bit_cast(Vec8<T>, w);
+struct Raw8 {
+    u4 w[kVec * sizeof(T) / 16];
+    __device__ __forceinline__ void values(float (&v)[kVec]) const
+    {
+        const Vec8<T> t = __builtin_bit_cast(Vec8<T>, *this);
 #pragma unroll
         for (int i = 0; i < kVec; i++) {
             v[i] = (float)t.v[i];
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kVec; i++) {
-            v[i] = i < count ? (float)p[i] : 0.f;
-        }
     }
+};
+
+// `count` elements, zeros behind them.  FILL: none of them are loaded like eight, which p then points at, so that nothing
+// diverges.
+template <bool FILL, typename T>
+__device__ __forceinline__ Raw8<T> load8(const T *__restrict__ p, int count, bool whole)
+{
+    if (whole && (count == kVec || (FILL && count == 0))) {
+        Raw8<T> w;
+#pragma unroll
+        for (size_t i = 0; i < kVec * sizeof(T) / 16; i++) {
+            w.w[i] = reinterpret_cast<const u4 *>(p)[i];
+            w.w[i] = FILL && count == 0 ? u4{} : w.w[i];
+        }
+        return w;
+    }
+    Vec8<T> t;
+#pragma unroll
+    for (int i = 0; i < kVec; i++) {
+        t.v[i] = i < count ? p[i] : (T)0.f;
+    }
+    return __builtin_bit_cast(Raw8<T>, t);
 }
 
 // PAST: past the caches (two kinds of store in one kernel would be merged into the ordinary one)
@@ -79,7 +90,7 @@ __device__ __forceinline__ void store8(T *__restrict__ p, int count, bool whole,
                 reinterpret_cast<u4 *>(p)[i] = w.w[i];
             }
         }
-    } else {
+    } else if (count > 0) {
 #pragma unroll
         for (int i = 0; i < kVec; i++) {
             if (i < count) {
@@ -250,26 +261,49 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
     if (L < 256 && row >= p.n) {
         return;   // whole groups of lanes that share no data with others (with L = 256 the grid is the number of rows)
     }
-    float y[C][kVec];
-    const T *x = static_cast<const T *>(p.x) + row * p.ld_x;
-#pragma unroll
-    for (int c = 0; c < C; c++) {
+    // Up to 16 elements of a lane: the row, its residual and the weight are all on their way before the first is needed.
+    constexpr bool kTogether = NORM && C <= 2;
+    auto part = [&](const T *row_of, int c, bool whole) {
         const int at = (c * L + lane) * kVec;
         const int count = min(kVec, max(0, p.d - at));
-        load8(x + (count ? at : 0), count, p.whole_x, y[c]);
+        return load8<kTogether>(row_of + (count ? at : 0), count, whole);
+    };
+    const T *const w = NORM ? static_cast<const T *>(p.weight) : nullptr;
+    float y[C][kVec];
+    Raw8<T> xv[kTogether ? C : 1], wv[kTogether ? C : 1], rv[kTogether ? C : 1];
+    const T *x = static_cast<const T *>(p.x) + row * p.ld_x;
+    const T *r = static_cast<const T *>(p.residual) + row * p.ld_residual;
+    if constexpr (kTogether) {
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            xv[c] = part(x, c, p.whole_x);
+        }
+        if (p.residual) {
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                rv[c] = part(r, c, p.whole_residual);
+            }
+        }
+        if (w) {
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                wv[c] = part(w, c, p.whole_weight);
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        (kTogether ? xv[kTogether ? c : 0] : part(x, c, p.whole_x)).values(y[c]);
     }
     if constexpr (NORM) {
         if (p.residual) {
-            const T *r = static_cast<const T *>(p.residual) + row * p.ld_residual;
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const int at = (c * L + lane) * kVec;
-                const int count = min(kVec, max(0, p.d - at));
-                float rv[kVec];
-                load8(r + (count ? at : 0), count, p.whole_residual, rv);
+                float v[kVec];
+                (kTogether ? rv[kTogether ? c : 0] : part(r, c, p.whole_residual)).values(v);
 #pragma unroll
                 for (int i = 0; i < kVec; i++) {
-                    y[c][i] += rv[i];
+                    y[c][i] += v[i];
                 }
             }
         }
@@ -310,25 +344,22 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
             }
             mean = sum_of_squares() * p.inv_d;
         }
-        double r = __builtin_amdgcn_rsq(mean);   // half of a double's bits at least, and a step of Newton's for the rest
-        r = mean == __builtin_inf() ? 0.0 : r * fma(-0.5 * mean * r, r, 1.5);
-        const float high = (float)r, low = (float)(r - (double)high);
-        const T *w = static_cast<const T *>(p.weight);
+        double root = __builtin_amdgcn_rsq(mean);   // half of a double's bits at least, and a step of Newton's for the rest
+        root = mean == __builtin_inf() ? 0.0 : root * fma(-0.5 * mean * root, root, 1.5);
+        const float high = (float)root, low = (float)(root - (double)high);
         auto multiply = [&](auto keep) {
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const int at = (c * L + lane) * kVec;
-                const int count = min(kVec, max(0, p.d - at));
-                float wv[kVec];
+                float f[kVec];
                 if (w) {
-                    load8(w + (count ? at : 0), count, p.whole_weight, wv);
+                    (kTogether ? wv[kTogether ? c : 0] : part(w, c, p.whole_weight)).values(f);
                 }
 #pragma unroll
                 for (int i = 0; i < kVec; i++) {
                     float v = y[c][i] * high, rest = fmaf(y[c][i], low, fmaf(y[c][i], high, -v));
                     if (w) {
-                        const float t = v * wv[i];
-                        rest = fmaf(rest, wv[i], fmaf(v, wv[i], -t));
+                        const float t = v * f[i];
+                        rest = fmaf(rest, f[i], fmaf(v, f[i], -t));
                         v = t;
                     }
                     y[c][i] = decltype(keep)::value && fabsf(v) == __builtin_inff() ? v : v + rest;
@@ -529,8 +560,11 @@ bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(
 // still to be read: the norm of 131072 x 4096 645 -> 627 us, and in turns with reading codes back the quantisation of
 // 1.2M x 200 243 -> 220.
 bool pass_caches(int64_t n, int64_t ld, int type) { return (double)n * (double)ld * (double)type_bytes(type) > 0x1p27; }
-// rows that all start on 16 bytes
-bool whole_rows(const void *p, int64_t ld, int type) { return aligned(p, 16) && (ld * (int64_t)type_bytes(type)) % 16 == 0; }
+// rows of eight elements at least that all start on 16 bytes
+bool whole_rows(const void *p, int64_t ld, int type, int d)
+{
+    return d >= kVec && aligned(p, 16) && (ld * (int64_t)type_bytes(type)) % 16 == 0;
+}
 
 void check_rows(const char *op, const void *p, int64_t ld, int type, int64_t n, int d)
 {
@@ -702,7 +736,7 @@ void op_quantise(const void *x, int64_t ld, int type, int64_t n, int d, int form
     p.scales = scales;
     p.sqr_sum = sqr_sum;
     p.format = format;
-    p.whole_x = whole_rows(x, ld, type);
+    p.whole_x = whole_rows(x, ld, type, d);
     launch_rows<false>(p, type, s);
 }
 
@@ -746,10 +780,10 @@ void op_rms_norm_quantise(const void *x, int64_t ld_x, const void *residual, int
     p.scales = scales;
     p.sqr_sum = sqr_sum;
     p.format = format;
-    p.whole_x = whole_rows(x, ld_x, type);
-    p.whole_residual = whole_rows(residual, ld_residual, type);
-    p.whole_weight = aligned(weight, 16);
-    p.whole_sum = whole_rows(sum, ld_sum, type);
+    p.whole_x = whole_rows(x, ld_x, type, d);
+    p.whole_residual = whole_rows(residual, ld_residual, type, d);
+    p.whole_weight = whole_rows(weight, 0, type, d);
+    p.whole_sum = whole_rows(sum, ld_sum, type, d);
     p.past = sum && pass_caches(n, ld_sum, type);
     launch_rows<true>(p, type, s);
 }
@@ -772,7 +806,7 @@ void op_dequantise(const uint8_t *codes, const void *scales, int format, int64_t
     p.chunks = (d + kVec - 1) / kVec;
     p.rows = p.chunks >= kThreads ? 1 : kThreads / p.chunks;
     p.out = out;
-    p.whole = whole_rows(out, ld, type);
+    p.whole = whole_rows(out, ld, type, d);
     const bool past = pass_caches(n, ld, type);
     if (type == kTypeF32) {
         launch_read<float>(p, format, past, s);
