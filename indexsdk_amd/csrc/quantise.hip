@@ -251,7 +251,7 @@ __device__ __forceinline__ float encode_fp8(const float (&y)[kVec], uint32_t bia
 // One row per L lanes (16, 32, 64 or the workgroup's 256), held in registers: C times eight elements per lane, so that a
 // row is read once whatever is computed from it: its largest values, its sum of squares, and with a residual its sum, which is
 // written in between.  Bound by memory: 1.2M x 200 from fp32 to 4 bits 207 us, 5.5 TB/s; the norm of 131072 x 4096 bfloat16 with a
-// residual to int8 616 us, 6.1 TB/s; one row by the latency of its load and its sums, 4 to 5 us from call to call.
+// residual to int8 611 us, 6.2 TB/s; one row by the latency of its load and its sums, 4 to 5 us from call to call.
 template <typename T, int L, int C, bool NORM, bool PAST>
 __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
 {
@@ -261,7 +261,8 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
     if (L < 256 && row >= p.n) {
         return;   // whole groups of lanes that share no data with others (with L = 256 the grid is the number of rows)
     }
-    // Up to 16 elements of a lane: the row, its residual and the weight are all on their way before the first is needed.
+    // Up to 16 elements of a lane: the row, its residual and the weight are all on their way before the first is needed (1.2M x
+    // 200 with a residual 357 -> 342 us); with more they would take the registers of other wavefronts.
     constexpr bool kTogether = NORM && C <= 2;
     auto part = [&](const T *row_of, int c, bool whole) {
         const int at = (c * L + lane) * kVec;
@@ -516,9 +517,10 @@ void launch_rows_of(const RowParams &p, hipStream_t s)
     });
 }
 
-// Few lanes with two to four times eight elements each: sums over lanes cost more than sums in a lane (norms of 500000 x 384: 32
-// lanes 267 us, 64 lanes 317, the workgroup 940; of 1.2M x 200: 16 lanes 354, 32 lanes 393), up to what a wavefront's registers
-// keep in flight (131072 x 4096: 64 lanes with eight times eight elements 952 us, the workgroup with two times 615).
+// Few lanes with two to four times eight elements each: sums over lanes cost more than sums in a lane (norms with a residual to
+// int8 of 1M x 128: 16 lanes 184 us, 32 lanes 298; of 1.2M x 200: 16 lanes 351, 32 lanes 389; of 500000 x 384: 32 lanes 264, 64
+// lanes 309; of 150000 x 1536: 64 lanes 299, the workgroup 338), up to what a wavefront's registers keep in flight (131072 x
+// 4096: 64 lanes with eight times eight elements 954 us, the workgroup with two times 611).
 template <typename T, bool NORM>
 void launch_rows(const RowParams &p, hipStream_t s)
 {
