@@ -248,6 +248,19 @@ __device__ __forceinline__ float encode_fp8(const float (&y)[kVec], uint32_t bia
     return ss;
 }
 
+// Roundings of a value in two parts: to the nearest, the same with infinities kept, or to odd.
+constexpr int kNear = 0, kEnd = 1, kOdd = 2;
+
+// v + rest toward zero, its last bit set if anything was lost: rounding that once more, to a number of a few bits, gives what
+// rounding the sum itself would, also next to a halfway point and to a power of two (4096 x 768 to 8 bits: one to four codes
+// fall to the wrong side if a sum is rounded to nearest first).
+__device__ __forceinline__ float round_to_odd(float v, float rest)
+{
+    const float sum = v + rest, lost = rest - (sum - v);
+    const uint32_t bits = __float_as_uint(sum);
+    return lost == 0.f ? sum : __uint_as_float((bits - ((__float_as_uint(lost) ^ bits) >> 31)) | 1u);
+}
+
 // One row per L lanes (16, 32, 64 or the workgroup's 256), held in registers: C times eight elements per lane, so that a
 // row is read once whatever is computed from it: its largest values, its sum of squares, and with a residual its sum, which is
 // written in between.  Bound by memory: 1.2M x 200 from fp32 to 4 bits 207 us, 5.5 TB/s; the norm of 131072 x 4096 bfloat16 with a
@@ -318,9 +331,9 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
                 store8<PAST>(o + (count ? at : 0), count, p.whole_sum, y[c]);
             }
         }
-        // Eight squares are added in 32 bits, all else up to the root's reciprocal r in 64; r and the products y r w are held in two
-        // parts of 32 and rounded once: codes are as far apart as 2^-3 of a value, and every rounding before them moves
-        // some to a neighbour.
+        // Eight squares are added in 32 bits, all else up to the root's reciprocal in 64; that and the products with it and the
+        // weight are held in two parts of 32 and rounded once: codes are as far apart as 2^-3 of a value, and every
+        // rounding before them moves some to a neighbour.
         auto sum_of_squares = [&]() {
             double sum = 0.0;
 #pragma unroll
@@ -348,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
         double root = __builtin_amdgcn_rsq(mean);   // half of a double's bits at least, and a step of Newton's for the rest
         root = mean == __builtin_inf() ? 0.0 : root * fma(-0.5 * mean * root, root, 1.5);
         const float high = (float)root, low = (float)(root - (double)high);
-        auto multiply = [&](auto keep) {
+        auto multiply = [&](auto round) {
 #pragma unroll
             for (int c = 0; c < C; c++) {
                 float f[kVec];
@@ -363,15 +376,18 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
                         rest = fmaf(rest, f[i], fmaf(v, f[i], -t));
                         v = t;
                     }
-                    y[c][i] = decltype(keep)::value && fabsf(v) == __builtin_inff() ? v : v + rest;
+                    y[c][i] = decltype(round)::value == kOdd ? round_to_odd(v, rest)
+                              : decltype(round)::value == kEnd && fabsf(v) == __builtin_inff() ? v : v + rest;
                 }
             }
         };
         // with a fixed scale an infinity ends at the last code; elsewhere it makes no difference whether a NaN takes its place
-        if (p.fixed_scale > 0.f) {
-            multiply(std::true_type());
+        if (p.format != kFormatInt8) {
+            multiply(std::integral_constant<int, kOdd>());
+        } else if (p.fixed_scale > 0.f) {
+            multiply(std::integral_constant<int, kEnd>());
         } else {
-            multiply(std::false_type());
+            multiply(std::integral_constant<int, kNear>());
         }
     }
     const bool want_sqr = p.sqr_sum != nullptr;
