@@ -265,6 +265,19 @@ def test_rms_norm(lib, d, fmt):
         check_norm(ref.rms_norm(as64(h), None, None if w is None else as64(w), np.float32(1e-6)), got, fmt)
 
 
+@pytest.mark.parametrize("fmt", [MXFP8, MXFP4])
+def test_rms_norm_gives_the_codes_of_the_result_in_64_bits(lib, fmt):
+    """1.5 million values whose only error before the last rounding is that of eight squares added in 32 bits, 2^-29 of a value
+    over a row's 96 sums: with halfway points 2^-3 of a value apart, one in 2^25 may fall to the other side, here none or one."""
+    n, d = 2000, 768
+    x, res = rows(sample(n, d, 1) * np.float32(3), "bf16"), rows(sample(n, d, 2), "bf16")
+    w = rows(np.abs(sample(1, d, 3)) + np.float32(0.5), "bf16")[0]
+    (codes, scales, _), _ = norm(lib, x, res, w, "bf16", fmt)
+    want, s = ref.mx_codes(ref.rms_norm(as64(x), as64(res), as64(w), 1e-6), fmt)
+    got = ref.mx_values(codes, scales, fmt)[:, :d]
+    assert (got != ref.mx_values(ref.pack(want, fmt), s, fmt)[:, :d]).sum() <= 1
+
+
 @pytest.mark.parametrize("fmt", [INT8, MXFP8, MXFP4])
 def test_rms_norm_of_rows_at_the_ends(lib, fmt):
     """A row of zeros, rows whose squares overflow or vanish in 32 bits, one element that dwarfs the others."""
