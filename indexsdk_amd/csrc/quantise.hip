@@ -248,9 +248,6 @@ __device__ __forceinline__ float encode_fp8(const float (&y)[kVec], uint32_t bia
     return ss;
 }
 
-// Roundings of a value in two parts: to the nearest, the same with infinities kept, or to odd.
-constexpr int kNear = 0, kEnd = 1, kOdd = 2;
-
 // v + rest toward zero, its last bit set if anything was lost: rounding that once more, to a number of a few bits, gives what
 // rounding the sum itself would, also next to a halfway point and to a power of two (4096 x 768 to 8 bits: one to four codes
 // fall to the wrong side if a sum is rounded to nearest first).
@@ -264,9 +261,10 @@ __device__ __forceinline__ float round_to_odd(float v, float rest)
 // One row per L lanes (16, 32, 64 or the workgroup's 256), held in registers: C times eight elements per lane, so that a
 // row is read once whatever is computed from it: its largest values, its sum of squares, and with a residual its sum, which is
 // written in between.  Bound by memory: 1.2M x 200 from fp32 to 4 bits 207 us, 5.5 TB/s; the norm of 131072 x 4096 bfloat16 with a
-// residual to int8 611 us, 6.2 TB/s; one row by the latency of its load and its sums, 4 to 5 us from call to call.
+// residual to int8 620 us, 6.1 TB/s, with the vector units busy nearly all of it; one row by the latency of its load and its sums, 4 to 5 us from call to call.
 template <typename T, int L, int C, bool NORM, bool PAST>
-__global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
+__global__ __launch_bounds__(kThreads, C >= 8 ? 2 : C >= 4 ? 4 : 1)   // 30000 x 16384: one workgroup per CU 835 us, two 628
+void row_quantise_kernel(RowParams p)
 {
     __shared__ double box[4];
     const int lane = threadIdx.x % L;
@@ -331,9 +329,10 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
                 store8<PAST>(o + (count ? at : 0), count, p.whole_sum, y[c]);
             }
         }
-        // Eight squares are added in 32 bits, all else up to the root's reciprocal in 64; that and the products with it and the
-        // weight are held in two parts of 32 and rounded once: codes are as far apart as 2^-3 of a value, and every
-        // rounding before them moves some to a neighbour.
+        // Eight squares are added in 32 bits, all else up to the root's reciprocal in 64.  Before microscaled codes that and the
+        // products with it and the weight are held in two parts of 32 and rounded once: codes are as far apart as 2^-3 of a value,
+        // and every rounding before them moves some to a neighbour.  int8 codes come of two more products in 32 bits by their
+        // definition, and here of two before these (in two parts 500000 x 384 took 264 us instead of 253).
         auto sum_of_squares = [&]() {
             double sum = 0.0;
 #pragma unroll
@@ -361,7 +360,7 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
         double root = __builtin_amdgcn_rsq(mean);   // half of a double's bits at least, and a step of Newton's for the rest
         root = mean == __builtin_inf() ? 0.0 : root * fma(-0.5 * mean * root, root, 1.5);
         const float high = (float)root, low = (float)(root - (double)high);
-        auto multiply = [&](auto round) {
+        auto multiply = [&](auto in_parts) {
 #pragma unroll
             for (int c = 0; c < C; c++) {
                 float f[kVec];
@@ -370,24 +369,25 @@ __global__ __launch_bounds__(kThreads) void row_quantise_kernel(RowParams p)
                 }
 #pragma unroll
                 for (int i = 0; i < kVec; i++) {
-                    float v = y[c][i] * high, rest = fmaf(y[c][i], low, fmaf(y[c][i], high, -v));
-                    if (w) {
-                        const float t = v * f[i];
-                        rest = fmaf(rest, f[i], fmaf(v, f[i], -t));
-                        v = t;
+                    float v = y[c][i] * high;
+                    if constexpr (decltype(in_parts)::value) {
+                        float rest = fmaf(y[c][i], low, fmaf(y[c][i], high, -v));
+                        if (w) {
+                            const float t = v * f[i];
+                            rest = fmaf(rest, f[i], fmaf(v, f[i], -t));
+                            v = t;
+                        }
+                        y[c][i] = round_to_odd(v, rest);
+                    } else {
+                        y[c][i] = w ? v * f[i] : v;
                     }
-                    y[c][i] = decltype(round)::value == kOdd ? round_to_odd(v, rest)
-                              : decltype(round)::value == kEnd && fabsf(v) == __builtin_inff() ? v : v + rest;
                 }
             }
         };
-        // with a fixed scale an infinity ends at the last code; elsewhere it makes no difference whether a NaN takes its place
-        if (p.format != kFormatInt8) {
-            multiply(std::integral_constant<int, kOdd>());
-        } else if (p.fixed_scale > 0.f) {
-            multiply(std::integral_constant<int, kEnd>());
+        if (p.format == kFormatInt8) {
+            multiply(std::false_type());
         } else {
-            multiply(std::integral_constant<int, kNear>());
+            multiply(std::true_type());
         }
     }
     const bool want_sqr = p.sqr_sum != nullptr;
