@@ -260,11 +260,12 @@ __device__ __forceinline__ float round_to_odd(float v, float rest)
 
 // One row per L lanes (16, 32, 64 or the workgroup's 256), held in registers: C times eight elements per lane, so that a
 // row is read once whatever is computed from it: its largest values, its sum of squares, and with a residual its sum, which is
-// written in between.  Bound by memory: 1.2M x 200 from fp32 to 4 bits 207 us, 5.5 TB/s; the norm of 131072 x 4096 bfloat16 with a
-// residual to int8 620 us, 6.1 TB/s, with the vector units busy nearly all of it; one row by the latency of its load and its sums, 4 to 5 us from call to call.
+// written in between.  Bound by memory: 1.2M x 200 from fp32 to 4 bits 207 us, 5.5 TB/s; the norm of 131072 x 4096 bfloat16 with
+// a residual to int8 620 us, 6.1 TB/s, with the vector units busy nearly all of it; one row by the latency of its load and
+// its sums, 4 to 5 us from call to call.  The longest rows take a bound on registers (norm of 30000 x 16384: one workgroup per
+// CU 835 us, two 628).
 template <typename T, int L, int C, bool NORM, bool PAST>
-__global__ __launch_bounds__(kThreads, C >= 8 ? 2 : C >= 4 ? 4 : 1)   // 30000 x 16384: one workgroup per CU 835 us, two 628
-void row_quantise_kernel(RowParams p)
+__global__ __launch_bounds__(kThreads, C >= 8 ? 2 : C >= 4 ? 4 : 1) void row_quantise_kernel(RowParams p)
 {
     __shared__ double box[4];
     const int lane = threadIdx.x % L;
