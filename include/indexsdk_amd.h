@@ -134,9 +134,9 @@ int ixa_op_topk_ivfpq_l3(const int64_t *in_labels_dev, const float *in_values_de
  * or as the model's last step behind a residual addition and a root-mean-square norm), is read back, and is scored
  * against a 4-bit store on the matrix cores.  No counterpart in the reference, whose int8 indexes take vectors that
  * somebody else has quantised.  As the stage operators above: plain DEVICE pointers, nothing allocated, work only
- * queued on `stream`.  n = 0 (m = 0) is allowed and queues nothing.  Dimensions 1 ... 16384, rows < 2^31; `ld` is the
- * distance of two rows in elements (>= the row's length); rows of any alignment are accepted, rows that all start on
- * 16 bytes are read in wide loads.  Codes start on 16 bytes and rows of codes follow each other without gaps.
+ * queued on `stream`.  n = 0 (m = 0) is allowed, queues nothing and needs no buffers (the address of an empty array is
+ * null).  Dimensions 1 ... 16384, rows < 2^31; `ld` is the distance of two rows in elements (>= the row's length); rows of
+ * any alignment are accepted, rows that all start on 16 bytes are read in wide loads.  Codes start on 16 bytes and rows of codes follow each other without gaps.
  * ------------------------------------------------------------------------------------------- */
 
 /* element types of float rows, weights and results */

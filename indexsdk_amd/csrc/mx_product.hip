@@ -940,7 +940,9 @@ void op_mx_product(const uint8_t *a_codes, const uint8_t *a_scales, int a_format
                    const uint8_t *b_scales, int64_t n, int d, int metric, const float *a_sqr, const float *b_sqr,
                    int out_type, void *out, int64_t ld, hipStream_t s)
 {
-    IXA_REQUIRE(a_codes && a_scales && b_codes && b_scales && out, kErrInvalidParam, "operator buffers can not be nullptr.");
+    const bool none = m == 0 || n == 0;   // needs no buffers: the address of an empty array is null
+    IXA_REQUIRE((a_codes && a_scales && b_codes && b_scales && out) || none, kErrInvalidParam,
+                "operator buffers can not be nullptr.");
     IXA_REQUIRE(a_format == kFormatMxFp8 || a_format == kFormatMxFp4, kErrInvalidParam,
                 "mx_product: unsupported code format %d", a_format);
     IXA_REQUIRE(out_type >= kTypeF32 && out_type <= kTypeBF16, kErrInvalidParam, "mx_product: unsupported element type %d",
@@ -950,12 +952,12 @@ void op_mx_product(const uint8_t *a_codes, const uint8_t *a_scales, int a_format
     IXA_REQUIRE(ld >= n && ld <= (int64_t)1 << 40, kErrInvalidParam, "mx_product: rows of %ld scores in steps of %ld", (long)n,
                 (long)ld);
     IXA_REQUIRE(metric == kMetricL2 || metric == kMetricInnerProduct, kErrInvalidParam, "Unsupported metric type");
-    IXA_REQUIRE(metric != kMetricL2 || (a_sqr && b_sqr), kErrInvalidParam,
+    IXA_REQUIRE(metric != kMetricL2 || (a_sqr && b_sqr) || none, kErrInvalidParam,
                 "mx_product: squared distances need the squared norms of both sides");
     IXA_REQUIRE(aligned(a_codes, 16) && aligned(b_codes, 16) && aligned(out, out_type == kTypeF32 ? 4 : 2) &&
                     aligned(a_sqr, 4) && aligned(b_sqr, 4),
                 kErrInvalidParam, "mx_product: codes have to start on 16 bytes, norms and scores on their elements");
-    if (m == 0 || n == 0) {
+    if (none) {
         return;
     }
     int device;

@@ -585,12 +585,12 @@ bool whole_rows(const void *p, int64_t ld, int type, int d)
     return d >= kVec && aligned(p, 16) && (ld * (int64_t)type_bytes(type)) % 16 == 0;
 }
 
+// No rows need no buffers: the address of an empty array is null.
 void check_rows(const char *op, const void *p, int64_t ld, int type, int64_t n, int d)
 {
-    IXA_REQUIRE(p, kErrInvalidParam, "operator buffers can not be nullptr.");
+    IXA_REQUIRE(p || n == 0, kErrInvalidParam, "operator buffers can not be nullptr.");
     IXA_REQUIRE(aligned(p, type_bytes(type)), kErrInvalidParam, "%s: rows are not aligned to their elements", op);
     IXA_REQUIRE(ld >= d && ld <= (int64_t)1 << 40, kErrInvalidParam, "%s: rows of %d elements in steps of %ld", op, d, (long)ld);
-    (void)n;
 }
 
 void check_codes(const char *op, int type, int64_t n, int d, int format, const uint8_t *codes, const void *scales, bool fixed)
@@ -599,7 +599,7 @@ void check_codes(const char *op, int type, int64_t n, int d, int format, const u
     IXA_REQUIRE(format >= kFormatInt8 && format <= kFormatMxFp4, kErrInvalidParam, "%s: unsupported code format %d", op, format);
     IXA_REQUIRE(n >= 0 && n <= 0x7fffffff && d >= 1 && d <= kMaxCodeDim, kErrInvalidParam,
                 "%s: rows %ld (< 2^31), dims %d (1 ... %d)", op, (long)n, d, kMaxCodeDim);
-    IXA_REQUIRE(codes && (scales || fixed), kErrInvalidParam, "operator buffers can not be nullptr.");
+    IXA_REQUIRE((codes && (scales || fixed)) || n == 0, kErrInvalidParam, "operator buffers can not be nullptr.");
     IXA_REQUIRE(aligned(codes, 16) && (format != kFormatInt8 || aligned(scales, 4)), kErrInvalidParam,
                 "%s: codes have to start on 16 bytes and fp32 scales on 4", op);
 }

@@ -123,6 +123,28 @@ def test_no_rows_queue_nothing(capi, call):
     assert getattr(capi.load(), name)(*args) == 0
 
 
+# an empty array's address is null
+@pytest.mark.parametrize("call", [
+    _quantise(n=0, x=None, codes=None, scales=None), _quantise(n=0, x=None, codes=None, scales=None, format=0),
+    _dequantise(n=0, codes=None, scales=None, out=None), _norm(n=0, x=None, res=None, sum=None, codes=None, scales=None),
+    _product(m=0, ac=None, asc=None, asq=None, out=None), _product(n=0, ld=0, bc=None, bs=None, bsq=None, out=None),
+    _product(m=0, n=0, ac=None, asc=None, asq=None, bc=None, bs=None, bsq=None, out=None),
+])
+def test_no_rows_need_no_buffers(capi, call):
+    name, args = call
+    assert getattr(capi.load(), name)(*args) == 0, capi.load().ixa_last_error().decode()
+
+
+@pytest.mark.parametrize("call,needle", [
+    (_quantise(n=0, x=None, type=3), "element type"), (_dequantise(n=0, out=None, d=0), "dims"),
+    (_norm(n=0, x=None, eps=0.0), "eps"), (_product(m=0, ac=None, metric=2), "metric"), (_product(n=0, bc=None, ld=-1), "steps of"),
+])
+def test_no_rows_are_still_checked(capi, call, needle):
+    name, args = call
+    assert getattr(capi.load(), name)(*args) == 2001
+    assert needle in capi.load().ixa_last_error().decode()
+
+
 def test_no_device_is_an_error(capi):
     import torch
     if torch.cuda.is_available():
