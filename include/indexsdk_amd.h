@@ -171,7 +171,8 @@ int ixa_op_quantise(const void *x_dev, int64_t ld, int type, int64_t n, int d, i
 int ixa_op_dequantise(const uint8_t *codes_dev, const void *scales_dev, int format, int64_t n, int d, int type,
                       void *out_dev, int64_t ld, void *stream);
 
-/* h = x + residual (residual may be NULL) is written to sum (may be NULL, may be x or residual themselves) rounded to `type`;
+/* h = x + residual (residual may be NULL) is written to sum (may be NULL) rounded to `type`; sum may be x or residual
+ * themselves, with their address and stride, and otherwise shares no element with an input (other overlaps are refused);
  * y = h / sqrt(mean(h^2) + eps) * weight (weight [d] may be NULL) becomes codes and scales as above.  x, residual, weight and
  * sum are all of `type`; y is made from the unrounded fp32 h, its sum and products are rounded to fp32 once.  eps > 0. */
 int ixa_op_rms_norm_quantise(const void *x_dev, int64_t ld_x, const void *residual_dev, int64_t ld_residual,

@@ -593,6 +593,24 @@ void check_rows(const char *op, const void *p, int64_t ld, int type, int64_t n, 
     IXA_REQUIRE(ld >= d && ld <= (int64_t)1 << 40, kErrInvalidParam, "%s: rows of %d elements in steps of %ld", op, d, (long)ld);
 }
 
+// Rows are worked on side by side, in no order: a sum written over a row of an input that another workgroup (or another
+// wavefront of the same row) has still to read would change what that one reads.  Each row of the sum lies on its own input
+// row as a whole, where it is written behind its reads, or on none; the latter with the same stride (two column ranges of
+// one buffer) or outright.
+bool sum_collides(const void *sum, int64_t ld_sum, const void *in, int64_t ld_in, int type, int64_t n, int d)
+{
+    const __int128 size = (__int128)type_bytes(type), a = (__int128)reinterpret_cast<uintptr_t>(sum),
+                   b = (__int128)reinterpret_cast<uintptr_t>(in), row = size * d;
+    if (a + ((n - 1) * size * ld_sum + row) <= b || b + ((n - 1) * size * ld_in + row) <= a) {
+        return false;
+    }
+    if (n == 1 || ld_sum != ld_in) {
+        return n > 1 || a != b;
+    }
+    const __int128 step = size * ld_in, apart = (a > b ? a - b : b - a) % step;
+    return a != b && (apart < row || apart > step - row);
+}
+
 void check_codes(const char *op, int type, int64_t n, int d, int format, const uint8_t *codes, const void *scales, bool fixed)
 {
     IXA_REQUIRE(type >= kTypeF32 && type <= kTypeBF16, kErrInvalidParam, "%s: unsupported element type %d", op, type);
@@ -770,6 +788,10 @@ void op_rms_norm_quantise(const void *x, int64_t ld_x, const void *residual, int
     }
     if (sum) {
         check_rows("rms_norm_quantise", sum, ld_sum, type, n, d);
+        IXA_REQUIRE(n == 0 || (!sum_collides(sum, ld_sum, x, ld_x, type, n, d) &&
+                               !(residual && sum_collides(sum, ld_sum, residual, ld_residual, type, n, d))),
+                    kErrInvalidParam, "rms_norm_quantise: rows of the sum have to be an input's own rows (same address and "
+                    "stride) or share no element with it");
     }
     if (weight) {
         check_rows("rms_norm_quantise", weight, d, type, 1, d);

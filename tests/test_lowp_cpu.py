@@ -117,6 +117,36 @@ def test_entry_points_refuse(capi, call, needle):
     assert needle in lib.ixa_last_error().decode()
 
 
+# 4 rows of 64 bfloat16 in steps of 64 are 512 bytes
+NEXT = 512
+
+
+@pytest.mark.parametrize("call", [
+    _norm(res=None, ld_sum=65), _norm(x=2 * P, ld_sum=65), _norm(res=2 * P, ld_x=65), _norm(res=None, sum=P + 2),
+    _norm(res=None, sum=P - 2), _norm(res=None, n=1, sum=P + 2), _norm(res=None, sum=P + NEXT - 128),
+    _norm(x=2 * P, sum=P - NEXT + 128), _norm(res=None, ld_x=128, ld_sum=128, sum=P + 126),
+    _norm(res=None, ld_x=128, ld_sum=128, sum=P + 130), _norm(res=None, ld_x=128, ld_sum=256, sum=P + 128),
+])
+def test_a_sum_over_rows_that_are_still_to_be_read_is_refused(capi, call):
+    """Rows are worked on side by side: a row of the sum may lie on its own input row and on no other."""
+    name, args = call
+    assert getattr(capi.load(), name)(*args) == 2001
+    assert "sum" in capi.load().ixa_last_error().decode()
+
+
+@pytest.mark.parametrize("call", [
+    _norm(), _norm(res=None), _norm(x=2 * P), _norm(n=1, ld_sum=65), _norm(res=None, sum=P + NEXT), _norm(res=None, sum=P - NEXT),
+    _norm(res=None, ld_x=128, ld_sum=128, sum=P + 128), _norm(res=None, ld_x=1 << 40, ld_sum=1 << 40, n=0x7fffffff),
+    _norm(res=None, sum=None, ld_sum=0),
+])
+def test_sums_that_are_allowed(capi, call):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present: these would be launched")
+    name, args = call
+    assert getattr(capi.load(), name)(*args) == 2016        # as far as the missing device
+
+
 @pytest.mark.parametrize("call", [_quantise(n=0), _dequantise(n=0), _norm(n=0), _product(m=0), _product(n=0, ld=0)])
 def test_no_rows_queue_nothing(capi, call):
     name, args = call
