@@ -348,15 +348,18 @@ __global__ __launch_bounds__(kThreads, C >= 8 ? 2 : C >= 4 ? 4 : 1) void row_qua
             return row_sum<L>(sum, box);
         };
         double mean = sum_of_squares() * p.inv_d + p.eps;
-        if (mean == __builtin_inf()) {   // finite elements whose squares pass the largest number: once more, 2^-80 as large
+        // finite elements whose squares pass the largest number of 32 bits, or lose bits below the smallest that count next to eps:
+        // once more with elements 2^-80 or 2^80 times as large
+        if (mean == __builtin_inf() || mean < 0x1p-100) {
+            const float unit = mean < 0x1p-100 ? 0x1p80f : 0x1p-80f;
 #pragma unroll
             for (int c = 0; c < C; c++) {
 #pragma unroll
                 for (int i = 0; i < kVec; i++) {
-                    y[c][i] *= 0x1p-80f;
+                    y[c][i] *= unit;
                 }
             }
-            mean = sum_of_squares() * p.inv_d;
+            mean = sum_of_squares() * p.inv_d + (double)p.eps * unit * unit;
         }
         double root = __builtin_amdgcn_rsq(mean);   // half of a double's bits at least, and a step of Newton's for the rest
         root = mean == __builtin_inf() ? 0.0 : root * fma(-0.5 * mean * root, root, 1.5);

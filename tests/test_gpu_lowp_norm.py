@@ -80,6 +80,22 @@ def test_a_mean_without_its_last_columns_would_be_seen(left_out, fmt):
         check(y, got(z), fmt)
 
 
+@pytest.mark.parametrize("d", [40, 768, 5000])
+@pytest.mark.parametrize("fmt", [INT8, MXFP8, MXFP4])
+@pytest.mark.parametrize("size,eps", [(2e-20, 1e-40), (3e-23, 1e-45), (1e-30, 1e-45), (1e-16, 1e-36), (5e-24, 1e-38)])
+def test_squares_that_are_too_small_for_32_bits(lib, d, fmt, size, eps):  # noqa: F811
+    """Rows and an epsilon whose squares are subnormal or nothing in 32 bits."""
+    x = rows(sample(9, d, d) * np.float32(size), "f32")
+    got, _ = norm(lib, x, None, None, "f32", fmt, eps=eps, keep_sum=False)
+    y = ref.rms_norm(as64(x), None, None, float(np.float32(eps)))
+    keep = np.abs(y).max() > 1e-6       # smaller results are still squared right, but their codes' squares may be nothing
+    if keep:
+        check(y, got, fmt)
+    else:
+        assert np.allclose(got[1] if fmt == INT8 else got[1].astype(float),
+                           np.abs(y).max(-1) / 127 if fmt == INT8 else ref.mx_codes(y, fmt)[1], rtol=1e-6)
+
+
 @pytest.mark.parametrize("d", [100, 768, 5000])
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("over", ["x", "residual"])
