@@ -803,17 +803,20 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
 
 bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// Workgroups of a kernel that the GPU runs at a time.
+// Workgroups of a kernel that the current device runs at a time: devices and partitions differ in their CUs.
 int64_t resident_workgroups(const void *kern, int threads, size_t lds)
 {
     static std::mutex mu;
-    static std::map<std::tuple<const void *, int, size_t>, int64_t> known;
+    static std::map<std::tuple<int, const void *, int, size_t>, int64_t> known;
+    int device;
+    IXA_HIP(hipGetDevice(&device));
     std::lock_guard<std::mutex> lock(mu);
-    int64_t &count = known[std::make_tuple(kern, threads, lds)];
+    int64_t &count = known[std::make_tuple(device, kern, threads, lds)];
     if (count == 0) {
-        int per_cu = 0;
+        int per_cu = 0, cus = 0;
         IXA_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, threads, lds));
-        count = std::max(1, per_cu) * 256;
+        IXA_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
+        count = (int64_t)std::max(1, per_cu) * std::max(1, cus);
     }
     return count;
 }
@@ -859,7 +862,8 @@ void launch_wide(const ProductParams &p, hipStream_t s)
     const void *kern = reinterpret_cast<const void *>(mx_wide_kernel<FA, R, L2, T>);
     require_dynamic_lds(kern, lds);
     IXA_REQUIRE(per_xcd <= 0x0fffffff, kErrInvalidParam, "mx_product: %ld x %ld scores in one call", (long)p.m, (long)p.n);
-    const int64_t grid = std::min(per_xcd * 8, resident_workgroups(kern, 256, lds));
+    // a multiple of 8: the workgroups of an XCD share its run of tiles
+    const int64_t grid = std::min(per_xcd, std::max<int64_t>(1, resident_workgroups(kern, 256, lds) / 8)) * 8;
     hipLaunchKernelGGL((mx_wide_kernel<FA, R, L2, T>), dim3((unsigned)grid), dim3(256), lds, s, p, (int)row_tiles, (int)col_tiles,
                        (int)per_xcd);
     check_launch();
