@@ -348,10 +348,10 @@ __global__ __launch_bounds__(kThreads, C >= 8 ? 2 : C >= 4 ? 4 : 1) void row_qua
             return row_sum<L>(sum, box);
         };
         double mean = sum_of_squares() * p.inv_d + p.eps;
-        // finite elements whose squares pass the largest number of 32 bits, or lose bits below the smallest that count next to eps:
-        // once more with elements 2^-80 or 2^80 times as large
-        if (mean == __builtin_inf() || mean < 0x1p-100) {
-            const float unit = mean < 0x1p-100 ? 0x1p80f : 0x1p-80f;
+        // Finite elements whose squares pass the largest number of 32 bits, or lose bits below the smallest that count next to eps:
+        // once more with elements 2^-80 or 2^80 times as large.  (Two branches: with the factor chosen ahead of one, rows that need
+        // neither took 5 % longer, 1.2M x 200 with a residual to 4 bits 361 us instead of 345.)
+        auto again = [&](float unit) {
 #pragma unroll
             for (int c = 0; c < C; c++) {
 #pragma unroll
@@ -360,6 +360,11 @@ __global__ __launch_bounds__(kThreads, C >= 8 ? 2 : C >= 4 ? 4 : 1) void row_qua
                 }
             }
             mean = sum_of_squares() * p.inv_d + (double)p.eps * unit * unit;
+        };
+        if (mean == __builtin_inf()) {
+            again(0x1p-80f);
+        } else if (mean < 0x1p-100) {
+            again(0x1p80f);
         }
         double root = __builtin_amdgcn_rsq(mean);   // half of a double's bits at least, and a step of Newton's for the rest
         root = mean == __builtin_inf() ? 0.0 : root * fma(-0.5 * mean * root, root, 1.5);
