@@ -167,14 +167,17 @@ int ixa_code_bytes(int format, int d, int64_t *bytes_per_row, int64_t *scales_pe
 int ixa_op_quantise(const void *x_dev, int64_t ld, int type, int64_t n, int d, int format, float fixed_scale,
                     uint8_t *codes_dev, void *scales_dev, float *sqr_sum_dev, void *stream);
 
-/* The values that codes and scales stand for, rounded to `type`, in rows out [n][ld]; a NaN scale gives NaN. */
+/* The values that codes and scales stand for (int8: their fp32 product), rounded to `type`, in rows out [n][ld]; a NaN scale
+ * gives NaN. */
 int ixa_op_dequantise(const uint8_t *codes_dev, const void *scales_dev, int format, int64_t n, int d, int type,
                       void *out_dev, int64_t ld, void *stream);
 
 /* h = x + residual (residual may be NULL) is written to sum (may be NULL) rounded to `type`; sum may be x or residual
  * themselves, with their address and stride, and otherwise shares no element with an input (other overlaps are refused);
  * y = h / sqrt(mean(h^2) + eps) * weight (weight [d] may be NULL) becomes codes and scales as above.  x, residual, weight and
- * sum are all of `type`; y is made from the unrounded fp32 h, its sum and products are rounded to fp32 once.  eps > 0. */
+ * sum are all of `type`; y is made from the fp32 h, before it is rounded to `type`.  The mean and its root are held in 64 bits
+ * (eight squares at a time in fp32).  For the microscaled formats y is rounded only once before the numbers are; for int8 the
+ * root's reciprocal, its product with h and the product with the weight are each rounded to fp32.  eps > 0. */
 int ixa_op_rms_norm_quantise(const void *x_dev, int64_t ld_x, const void *residual_dev, int64_t ld_residual,
                              const void *weight_dev, int type, int64_t n, int d, float eps, void *sum_dev, int64_t ld_sum,
                              int format, float fixed_scale, uint8_t *codes_dev, void *scales_dev, float *sqr_sum_dev,

@@ -90,9 +90,10 @@ __device__ __forceinline__ void load_run(const float *from, int64_t at, int64_t 
     }
 }
 
-// Scores are not read again here: where a wavefront's runs are whole lines of 64 bytes they pass the caches by, which leaves
-// these to the codes (2048 x 131072 x 768 to fp32: 360 -> 290 us); rows that start anywhere share lines, which the L2 has
-// to join (1024 x 199999 x 128: 210 us, past the caches 330).
+// Scores are not read again here: where rows of scores start on 64 bytes they pass the caches by, which leaves these to the
+// codes (2048 x 131072 x 768 to fp32: 360 -> 290 us); rows that start anywhere share lines, which the L2 has to join (1024 x
+// 199999 x 128: 210 us, past the caches 330).  A wavefront's run is a line or more, but for 32 bytes where NF = 1 has 16-bit
+// scores: few rows, whose scores are small.
 // The scores of a lane: queries row ... row + 3 (element i of the accumulators) and columns col ... col + NF - 1 (fragment j).
 template <typename T, int NF>
 __device__ __forceinline__ void store_scores(const ProductParams &p, int64_t row, int64_t col, const v4f (&acc)[NF],
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint8_t *const turn = scales + (((size_t)steps * rows * 4 + 15) & ~(size_t)15) + wave * (NF * U * (1024 + 64));
     uint8_t *const turn_scales = turn + NF * U * 1024;
-    static_assert(NF * U <= 4, "a lane brings the scales of one row and step");
+    static_assert(NF * U == 4, "a lane brings the scales of one row and step");
     const int a_row_bytes = p.blocks * 16 * kHalves, b_row_bytes = p.blocks * 16;
     // 256, 128 ... 4 threads bring a row; pieces behind its last block are zeros
     const int lg = rows > 1 ? 8 - (32 - __builtin_clz(rows - 1)) : 8, per_row = 1 << lg;
@@ -256,11 +257,9 @@ __global__ __launch_bounds__(256) void mx_stream_kernel(ProductParams p, int ste
                     *reinterpret_cast<u4 *>(turn + u * (NF * 1024) + stored_place<NF>(row % NF, row / NF, lane & 3)) = next[u][k];
                 }
             }
-            if (NF * U == 4 || lane < NF * U * 16) {
-                const int b_from = min(t + scale_step, steps - 1) * 4;
-                reinterpret_cast<uint32_t *>(turn_scales)[scale_step * (NF * 16) + (scale_row % NF) * 16 + scale_row / NF] =
-                    take_scales(next_scale, b_from, over + b_from, p.blocks);
-            }
+            const int b_from = min(t + scale_step, steps - 1) * 4;
+            reinterpret_cast<uint32_t *>(turn_scales)[scale_step * (NF * 16) + (scale_row % NF) * 16 + scale_row / NF] =
+                take_scales(next_scale, b_from, over + b_from, p.blocks);
             if (t + U < steps) {
                 fetch(t + U);
             }
@@ -874,12 +873,18 @@ void launch_type(const ProductParams &p, hipStream_t s)
 {
     const int steps = (p.blocks + 3) / 4;
     const int mf = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
+    // Half a CU's LDS, so that two workgroups share it, is the line; it is right for 33 ... 64 queries in part only and for fewer
+    // not at all.  8-bit queries, the whole LDS and the tiles below: 64 x 20000 x 1024 18.5 us and 15.7, 64 x 500000 x 1024 121 and 143,
+    // 16 x 30000 x 4096 23.5 and 46, 16 x 200000 x 4096 111 and 226, 8 x 100000 x 8192 128 and 230; in 4 bits 64 x 200000 x 4096 163
+    // and 155.
     if (p.m <= 64 && stream_lds<FA>(p.m, 4, steps) <= 80 * 1024) {
         // Up to 2048 tiles of 16 stored rows (eight wavefronts per CU) such tiles, four steps at a time; else tiles of 64 rows,
         // or, for up to 16 queries with more than one step, of 32 rows and 128 bytes of each at a time: with 64 bytes, and the
         // many wavefronts that few queries leave room for, the two visits to a line of memory are too far apart.
         // 1 x 20000 x 4096: 16 rows 9.9 us, 32 rows 12.5, 64 rows 20.6; 1 x 1M x 1536: 150, 154, 199; 64 x 1M x 768: 253, 171,
-        // 145; 32 x 1M x 512: 96, 76, 72; 1 x 1M x 128: 26.8, 17.8, 15.5.
+        // 145; 32 x 1M x 512: 96, 76, 72; 1 x 1M x 128: 26.8, 17.8, 15.5.  Around the line, 16 rows and the other: 32 x 30000 x 512
+        // 6.9 and 7.7, 60000 10.3 and 8.5; 64 x 30000 x 768 14.0 and 13.9, 60000 22.0 and 15.4; 64 x 30000 x 128 6.6 and 7.1, 100000
+        // 13.5 and 8.6; 1 x 30000 x 1536 8.3 and 8.0, 60000 12.6 and 10.9, 100000 17.3 and 18.2.
         const bool narrow = p.n <= 16 * 2048;
         if (mf == 1) {
             if (narrow) {
@@ -912,7 +917,9 @@ void launch_type(const ProductParams &p, hipStream_t s)
     // 1024 x 8192 x 1024: 26 and 34; with 391 of them, 100 x 100003 x 200, 14.8 and 12.9), and of 256 x 256 and two steps at
     // a time for 4-bit queries with two such tiles and more per CU in rows of 512 columns and more (1024 x 60001 x 2016: 124 us,
     // 128 x 256 154; 2048 x 100001 x 768: 288 and 312; shorter rows 2048 x 131072 x 200: 282 and 234; fewer tiles
-    // 1000 x 20001 x 4096: 100 and 97; with 8-bit queries 4096 x 32768 x 2080: 513 and 498).
+    // 1000 x 20001 x 4096: 100 and 97; with 8-bit queries 4096 x 32768 x 2080: 513 and 498).  Half of a tile of 128 and more has
+    // no queries where there are 64: with 8-bit ones 64 x 256 would be ahead (64 x 500000 x 1024 100 us against 143, 16 x 200000 x
+    // 4096 151 and 226, 32 x 100000 x 16384 295 and 451), with 4-bit ones not (64 x 200000 x 4096 200 and 155).
     if (tiles < 384) {
         launch_tiles<FA, 1, 4, 4, 1, T>(p, s);
         return;

@@ -261,7 +261,7 @@ __device__ __forceinline__ float round_to_odd(float v, float rest)
 // One row per L lanes (16, 32, 64 or the workgroup's 256), held in registers: C times eight elements per lane, so that a
 // row is read once whatever is computed from it: its largest values, its sum of squares, and with a residual its sum, which is
 // written in between.  Bound by memory: 1.2M x 200 from fp32 to 4 bits 207 us, 5.5 TB/s; the norm of 131072 x 4096 bfloat16 with
-// a residual to int8 620 us, 6.1 TB/s, with the vector units busy nearly all of it; one row by the latency of its load and
+// a residual to int8 620 us, 6.1 TB/s, with the vector units busy for three quarters of it; one row by the latency of its load and
 // its sums, 4 to 5 us from call to call.  The longest rows take a bound on registers (norm of 30000 x 16384: one workgroup per
 // CU 835 us, two 628).
 template <typename T, int L, int C, bool NORM, bool PAST>
@@ -333,7 +333,8 @@ __global__ __launch_bounds__(kThreads, C >= 8 ? 2 : C >= 4 ? 4 : 1) void row_qua
         // Eight squares are added in 32 bits, all else up to the root's reciprocal in 64.  Before microscaled codes that and the
         // products with it and the weight are held in two parts of 32 and rounded once: codes are as far apart as 2^-3 of a value,
         // and every rounding before them moves some to a neighbour.  int8 codes come of two more products in 32 bits by their
-        // definition, and here of two before these (in two parts 500000 x 384 took 264 us instead of 253).
+        // definition, and here of two before these, with a root rounded to 32 bits (in two parts 500000 x 384 takes 288 us
+        // instead of 256, 131072 x 4096 642 instead of 623).
         auto sum_of_squares = [&]() {
             double sum = 0.0;
 #pragma unroll
@@ -543,9 +544,9 @@ void launch_rows_of(const RowParams &p, hipStream_t s)
 }
 
 // Few lanes with two to four times eight elements each: sums over lanes cost more than sums in a lane (norms with a residual to
-// int8 of 1M x 128: 16 lanes 184 us, 32 lanes 298; of 1.2M x 200: 16 lanes 351, 32 lanes 389; of 500000 x 384: 32 lanes 264, 64
-// lanes 309; of 150000 x 1536: 64 lanes 299, the workgroup 338), up to what a wavefront's registers keep in flight (131072 x
-// 4096: 64 lanes with eight times eight elements 954 us, the workgroup with two times 611).
+// int8 of 1M x 128: 16 lanes 162 us, 32 lanes 289; of 1.2M x 200: 16 lanes 327, 32 lanes 360; of 500000 x 384: 32 lanes 254, 64
+// lanes 297; of 150000 x 1536: 64 lanes 278, the workgroup 322), up to what a wavefront's registers keep in flight (131072 x
+// 4096: 64 lanes with eight times eight elements 665 us, the workgroup with two times 618).
 template <typename T, bool NORM>
 void launch_rows(const RowParams &p, hipStream_t s)
 {
@@ -584,8 +585,10 @@ void launch_rows(const RowParams &p, int type, hipStream_t s)
 size_t type_bytes(int type) { return type == kTypeF32 ? 4 : 2; }
 bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 // Float rows that the last cache (256 MB) could not hold for whoever reads them next pass it by, which leaves it to what is
-// still to be read: the norm of 131072 x 4096 645 -> 627 us, and in turns with reading codes back the quantisation of
-// 1.2M x 200 243 -> 220.
+// still to be read: the norm of 131072 x 4096 650 -> 624 us, and in turns with reading codes back the quantisation of
+// 1.2M x 200 243 -> 220.  Of fp32 rows a lane stores two pieces of 16 bytes 32 apart, which leave gaps past the caches: whole
+// pages do not mind (131072 x 4096 read back from int8 630 -> 580 us), other rows do (1.2M x 200 from 4 bits 244 -> 370; the norm
+// with its fp32 sum 588 -> 612, of 131072 x 4096 1230 -> 1243).
 bool pass_caches(int64_t n, int64_t ld, int type) { return (double)n * (double)ld * (double)type_bytes(type) > 0x1p27; }
 // rows of eight elements at least that all start on 16 bytes
 bool whole_rows(const void *p, int64_t ld, int type, int d)
