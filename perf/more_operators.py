@@ -167,6 +167,8 @@ def prepare(case, seed):
         s["x"] = _rows(m, d, gen).to(_TYPES[case["type"]][1])
         s["bias"] = torch.randn(n, device="cuda", generator=gen).mul_(0.1)
         s["out"] = torch.empty(m, n, device="cuda", dtype=_TYPES[case["out"]][1])
+        if own:
+            s["work"] = _workspace("ixa_group_product_workspace", _TYPES[case["type"]][0], m, d)
         return s
     rows, n, dtype = case["rows"], case["n"], _TYPES[case["type"]][1]
     if kind == "sample":
@@ -332,10 +334,10 @@ def _at(t):
     return ctypes.c_void_p(t.data_ptr() if t is not None else None)
 
 
-def _workspace(what, rows, n):
+def _workspace(what, *shape):
     lib, check = _lib()
     size = ctypes.c_int64()
-    check(getattr(lib, what)(rows, n, ctypes.byref(size)))
+    check(getattr(lib, what)(*shape, ctypes.byref(size)))
     return torch.empty(size.value, device="cuda", dtype=torch.uint8)
 
 
@@ -362,7 +364,8 @@ def _own_product(s):
     case = s["case"]
     check(lib.ixa_op_group_product(_at(s["x"]), case["d"], _TYPES[case["type"]][0], case["m"], _at(s["codes"]), _at(s["scales"]),
                                    _at(s["zeros"]), case["group"], _TYPES[case["scale"]][0], case["n"], case["d"], 1.0,
-                                   _at(s["bias"]), _TYPES[case["out"]][0], _at(s["out"]), case["n"], _stream()))
+                                   _at(s["bias"]), _TYPES[case["out"]][0], _at(s["out"]), case["n"], _at(s["work"]),
+                                   s["work"].numel(), _stream()))
     return s["out"]
 
 
