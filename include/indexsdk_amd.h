@@ -194,6 +194,47 @@ int ixa_op_mx_product(const uint8_t *a_codes_dev, const uint8_t *a_scales_dev, i
                       void *stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Scores and what is done with them: rows kept in 4 bits with a scale per group and scored against unrounded rows (a
+ * store against queries, or a model's output table against its last hidden states), columns drawn from rows of scores, and
+ * the loss of rows of scores against a teacher's top entries with its gradient.  No counterpart in the reference.  As the
+ * operators above: plain DEVICE pointers, nothing allocated, work only queued on `stream`, calls may be captured into a graph;
+ * no rows queue nothing and need no buffers; `ld` is the distance of two rows in elements, rows of any alignment.  Where an operator needs a
+ * workspace, a function beside it says how many bytes; its contents mean nothing between calls, it starts on 16 bytes, and
+ * calls that may run at the same time (two streams, two captured graphs) need workspaces of their own.  Outputs share no
+ * element with inputs, unless said.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Rows in 4 bits: groups of `group` (32, 64 or 128) consecutive elements of a row of d (1 ... 16384), ceil(d / group) of them,
+ * take group / 2 bytes of codes each (element 2 i in the lower half of byte i), a scale of `scale_type` (IXA_TYPE_*) and,
+ * unless `zeros` is NULL (all 8), one byte of zero point: value = (code - zero) * scale.  Codes start on 16 bytes; rows of
+ * codes, scales [n][groups] and zeros [n][groups] follow each other without gaps. */
+int ixa_group_bytes(int group, int d, int64_t *bytes_per_row, int64_t *groups_per_row);
+
+/* Rows x [n][ld] of `type` become codes, scales and (zeros not NULL) zero points.  Without zero points scale = max|x| / 7; with
+ * them scale = (high - low) / 15 and zero = -low / scale, rounded to nearest, for low = min(0, min x) and high = max(0, max x).  The
+ * quotient is rounded to fp32 and then to scale_type, and ends at its largest number.  code = x / scale (as it is stored), rounded
+ * to nearest, halfway to even, + zero, clamped to 0 ... 15; with scale 0 all values are 0 (code = zero).  Elements behind the
+ * last column are coded as 0 and count as 0.  A group with an infinity or a NaN: scale NaN. */
+int ixa_op_group_quantise(const void *x_dev, int64_t ld, int type, int64_t n, int d, int group, int scale_type,
+                          uint8_t *codes_dev, void *scales_dev, uint8_t *zeros_dev, void *stream);
+
+/* The values of rows of codes (fp32 products), rounded to `type`, in rows out [n][ld]. */
+int ixa_op_group_dequantise(const uint8_t *codes_dev, const void *scales_dev, const uint8_t *zeros_dev, int group,
+                            int scale_type, int64_t n, int d, int type, void *out_dev, int64_t ld, void *stream);
+
+/* out [m][ld] of out_type = alpha * (x . values) + bias for m rows x [m][ld_x] of `type` and n rows of codes; bias [n] fp32 or
+ * NULL.  alpha = -1, or -2 with squared norms as bias, gives scores that ixa_op_topk_flat_fp32 selects the best of.  Sums are
+ * held in fp32.  Products are those of fp16 numbers and integers: fp16 rows go in exactly; bfloat16 and fp32 rows are multiplied by a
+ * power of two each, which is taken back in fp32, and lose what lies 2^-39 below their largest finite element, fp32 also 2^-22 of
+ * each element.  Scales beyond 2^+-80 may lose more.  An infinity or a NaN in x, or a NaN scale, reaches the scores of its row.  m <= 2^23,
+ * n < 2^31.  The workspace is needed for more than 64 rows and for few long ones (the function says 0 where it is not). */
+int ixa_group_product_workspace(int type, int64_t m, int d, int64_t *bytes);
+int ixa_op_group_product(const void *x_dev, int64_t ld_x, int type, int64_t m, const uint8_t *codes_dev,
+                         const void *scales_dev, const uint8_t *zeros_dev, int group, int scale_type, int64_t n, int d,
+                         float alpha, const float *bias_dev, int out_type, void *out_dev, int64_t ld, void *workspace_dev,
+                         int64_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
  * IVFPQ
  * ------------------------------------------------------------------------------------------- */
 

@@ -707,6 +707,52 @@ IXA_EXPORT int ixa_op_mx_product(const uint8_t *a_codes_dev, const uint8_t *a_sc
                            b_sqr_sum_dev, out_type, out_dev, ld, static_cast<hipStream_t>(stream));
     });
 }
+IXA_EXPORT int ixa_group_bytes(int group, int d, int64_t *bytes_per_row, int64_t *groups_per_row)
+{
+    return guarded([&] {
+        IXA_REQUIRE((group == 32 || group == 64 || group == 128) && d >= 1 && d <= ixa::kMaxCodeDim, ixa::kErrInvalidParam,
+                    "group_bytes: groups of %d elements (32, 64 or 128), dims %d (1 ... %d)", group, d, ixa::kMaxCodeDim);
+        if (bytes_per_row) {
+            *bytes_per_row = ixa::group_row_bytes(group, d);
+        }
+        if (groups_per_row) {
+            *groups_per_row = ixa::group_count(group, d);
+        }
+    }, false);
+}
+IXA_EXPORT int ixa_op_group_quantise(const void *x_dev, int64_t ld, int type, int64_t n, int d, int group, int scale_type,
+                                     uint8_t *codes_dev, void *scales_dev, uint8_t *zeros_dev, void *stream)
+{
+    return guarded([&] {
+        ixa::op_group_quantise(x_dev, ld, type, n, d, group, scale_type, codes_dev, scales_dev, zeros_dev,
+                               static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_op_group_dequantise(const uint8_t *codes_dev, const void *scales_dev, const uint8_t *zeros_dev, int group,
+                                       int scale_type, int64_t n, int d, int type, void *out_dev, int64_t ld, void *stream)
+{
+    return guarded([&] {
+        ixa::op_group_dequantise(codes_dev, scales_dev, zeros_dev, group, scale_type, n, d, type, out_dev, ld,
+                                 static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_group_product_workspace(int type, int64_t m, int d, int64_t *bytes)
+{
+    return guarded([&] {
+        IXA_REQUIRE(bytes != nullptr, ixa::kErrInvalidParam, "bytes can not be nullptr.");
+        *bytes = ixa::group_product_workspace(type, m, d);
+    }, false);
+}
+IXA_EXPORT int ixa_op_group_product(const void *x_dev, int64_t ld_x, int type, int64_t m, const uint8_t *codes_dev,
+                                    const void *scales_dev, const uint8_t *zeros_dev, int group, int scale_type, int64_t n,
+                                    int d, float alpha, const float *bias_dev, int out_type, void *out_dev, int64_t ld,
+                                    void *workspace_dev, int64_t workspace_bytes, void *stream)
+{
+    return guarded([&] {
+        ixa::op_group_product(x_dev, ld_x, type, m, codes_dev, scales_dev, zeros_dev, group, scale_type, n, d, alpha, bias_dev,
+                              out_type, out_dev, ld, workspace_dev, workspace_bytes, static_cast<hipStream_t>(stream));
+    });
+}
 IXA_EXPORT int ivfpq_search_probes_device(ivfpq_index_t *h, int64_t n, const float *x_dev, const int32_t *probes_dev,
                                           int nprobe, int64_t k, float *distances_dev, int64_t *labels_dev)
 {

@@ -46,6 +46,28 @@ void op_mx_product(const uint8_t *a_codes, const uint8_t *a_scales, int a_format
                    const uint8_t *b_scales, int64_t n, int d, int metric, const float *a_sqr, const float *b_sqr,
                    int out_type, void *out, int64_t ld, hipStream_t s);
 
+// Rows of 4-bit codes with a scale, and where `zeros` is given a zero point, for each group of `group` (32, 64 or 128) elements:
+// value = (code - zero) * scale.  The lower half of a byte comes first; rows take whole groups.
+inline int group_count(int group, int d) { return (d + group - 1) / group; }
+inline int64_t group_row_bytes(int group, int d) { return (int64_t)group_count(group, d) * (group / 2); }
+void check_groups(const char *op, int group, int scale_type, int64_t n, int d, const uint8_t *codes, const void *scales);
+
+// Rows x[n][ld] become codes, scales of scale_type [n][groups] and, unless null, zeros [n][groups].
+void op_group_quantise(const void *x, int64_t ld, int type, int64_t n, int d, int group, int scale_type, uint8_t *codes,
+                       void *scales, uint8_t *zeros, hipStream_t s);
+
+// Their values, rounded to `type`, in rows out[n][ld].
+void op_group_dequantise(const uint8_t *codes, const void *scales, const uint8_t *zeros, int group, int scale_type, int64_t n,
+                         int d, int type, void *out, int64_t ld, hipStream_t s);
+
+// out[m][ld] = alpha * (rows x . the values of rows of codes) + bias (may be null), rounded to out_type.  The workspace takes
+// group_product_workspace bytes and holds x as the matrix cores want it where there are many rows or long ones.
+constexpr int64_t kMaxProductRows = 1 << 23;
+int64_t group_product_workspace(int type, int64_t m, int d);
+void op_group_product(const void *x, int64_t ld_x, int type, int64_t m, const uint8_t *codes, const void *scales,
+                      const uint8_t *zeros, int group, int scale_type, int64_t n, int d, float alpha, const float *bias,
+                      int out_type, void *out, int64_t ld, void *workspace, int64_t workspace_bytes, hipStream_t s);
+
 // An error the device (or its absence) answered with becomes this library's.
 inline void check_answer(hipError_t e)
 {

@@ -1,0 +1,103 @@
+// Eight elements of a row at a time, at any alignment, and exchanges between neighbouring lanes.
+#pragma once
+#include "lowp.h"
+
+namespace ixa {
+
+constexpr int kEight = 8;
+
+// Eight elements as they lie in memory.  Global memory takes wide loads and stores at any address: one instruction for 16-bit
+// elements and two for fp32, also where a row starts on an element only.
+template <typename T>
+struct Eight {
+    typedef T Lane __attribute__((ext_vector_type(kEight)));
+    typedef T Anywhere __attribute__((ext_vector_type(kEight), aligned(sizeof(T))));
+    Lane v;
+    // `count` elements, `fill` behind them
+    __device__ __forceinline__ void load(const T *__restrict__ p, int count, T fill)
+    {
+        if (count >= kEight) {
+            v = *reinterpret_cast<const Anywhere *>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEight; i++) {
+                v[i] = i < count ? p[i] : fill;
+            }
+        }
+    }
+    // PAST: past the caches
+    template <bool PAST = false>
+    __device__ __forceinline__ void store(T *__restrict__ p, int count) const
+    {
+        if (count >= kEight) {
+            if constexpr (PAST) {
+                __builtin_nontemporal_store(v, reinterpret_cast<Anywhere *>(p));
+            } else {
+                *reinterpret_cast<Anywhere *>(p) = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEight; i++) {
+                if (i < count) {
+                    p[i] = v[i];
+                }
+            }
+        }
+    }
+};
+
+// the value of the lane that CTRL names, within 16 lanes
+template <int CTRL>
+__device__ __forceinline__ int lane_of(int v)
+{
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+
+// Op over groups of LANES (4, 8 or 16) lanes; every one of them has the result.
+template <int LANES, typename Op>
+__device__ __forceinline__ int over_lanes(int v, Op op)
+{
+    v = op(v, lane_of<kXor1>(v));
+    v = op(v, lane_of<kXor2>(v));
+    if constexpr (LANES >= 8) {
+        v = op(v, lane_of<kMirror8>(v));
+    }
+    if constexpr (LANES >= 16) {
+        v = op(v, lane_of<kMirror16>(v));
+    }
+    return v;
+}
+
+// ----- host -------------------------------------------------------------------------------------------------------------
+
+inline size_t element_bytes(int type) { return type == kTypeF32 ? 4 : 2; }
+inline bool on_bytes(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+inline void check_type(const char *op, int type)
+{
+    IXA_REQUIRE(type >= kTypeF32 && type <= kTypeBF16, kErrInvalidParam, "%s: unsupported element type %d", op, type);
+}
+// Rows of an operator: no rows need no buffer.
+inline void check_row_buffer(const char *op, const void *p, int64_t ld, int type, int64_t n, int64_t d)
+{
+    IXA_REQUIRE(p || n == 0 || d == 0, kErrInvalidParam, "operator buffers can not be nullptr.");
+    IXA_REQUIRE(on_bytes(p, element_bytes(type)), kErrInvalidParam, "%s: rows are not aligned to their elements", op);
+    IXA_REQUIRE(ld >= d && ld <= (int64_t)1 << 40, kErrInvalidParam, "%s: rows of %ld elements in steps of %ld", op, (long)d,
+                (long)ld);
+}
+
+// A kernel for each element type.
+template <typename F>
+void with_type(int type, F f)
+{
+    if (type == kTypeF32) {
+        f(float());
+    } else if (type == kTypeF16) {
+        f((_Float16)0.f);
+    } else {
+        f((__bf16)0.f);
+    }
+}
+
+}  // namespace ixa
