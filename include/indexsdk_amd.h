@@ -234,6 +234,21 @@ int ixa_op_group_product(const void *x_dev, int64_t ld_x, int type, int64_t m, c
                          float alpha, const float *bias_dev, int out_type, void *out_dev, int64_t ld, void *workspace_dev,
                          int64_t workspace_bytes, void *stream);
 
+/* Columns drawn from rows of scores [rows][ld], n columns each (larger is better; -infinity and NaN: a column that is not
+ * there), `draws` of each row from the given random numbers uniform [rows][draws] in [0, 1), with replacement.  Settings per row
+ * [rows], each array may be NULL: temperature T (NULL: 1; 0 and less: the best column), top_k k (NULL, 0 and less: all), top_p p (NULL, 1
+ * and more: all; 0 and less: the best one), min_p m (NULL, 0 and less: all; 1 and more: those equal to the best).
+ * With weights w = exp((score - best) / T), the columns in the order of falling scores, equal ones in that of columns, are cut to
+ * the first k, then to the fewest whose weights reach p of the sum of those that are left, then to those with w >= m.  The
+ * draw's label is the first column, in the order of columns, at which the running sum of the weights that are left passes
+ * uniform * their total; its probability w / total goes to probs [rows][draws] (may be NULL).  Weights and sums are held in 64 bits.  Beside a
+ * score of +infinity only such columns count.  A row without a column: label -1, probability 0.
+ * rows <= 2^22, n < 2^31, draws <= 2^20. */
+int ixa_sample_workspace(int64_t rows, int64_t n, int64_t *bytes);
+int ixa_op_sample(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n, const float *temperature_dev,
+                  const int32_t *top_k_dev, const float *top_p_dev, const float *min_p_dev, const float *uniform_dev, int draws,
+                  int64_t *labels_dev, float *probs_dev, void *workspace_dev, int64_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------------------------------------
  * IVFPQ
  * ------------------------------------------------------------------------------------------- */

@@ -15,6 +15,7 @@
 #include "flat_index.h"
 #include "ivfpq_index.h"
 #include "lowp.h"
+#include "scores.h"
 #include "ops.h"
 #include "scan.h"
 
@@ -751,6 +752,23 @@ IXA_EXPORT int ixa_op_group_product(const void *x_dev, int64_t ld_x, int type, i
     return guarded([&] {
         ixa::op_group_product(x_dev, ld_x, type, m, codes_dev, scales_dev, zeros_dev, group, scale_type, n, d, alpha, bias_dev,
                               out_type, out_dev, ld, workspace_dev, workspace_bytes, static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_sample_workspace(int64_t rows, int64_t n, int64_t *bytes)
+{
+    return guarded([&] {
+        IXA_REQUIRE(bytes != nullptr, ixa::kErrInvalidParam, "bytes can not be nullptr.");
+        *bytes = ixa::sample_workspace(rows, n);
+    }, false);
+}
+IXA_EXPORT int ixa_op_sample(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n, const float *temperature_dev,
+                             const int32_t *top_k_dev, const float *top_p_dev, const float *min_p_dev, const float *uniform_dev,
+                             int draws, int64_t *labels_dev, float *probs_dev, void *workspace_dev, int64_t workspace_bytes,
+                             void *stream)
+{
+    return guarded([&] {
+        ixa::op_sample(scores_dev, ld, type, rows, n, temperature_dev, top_k_dev, top_p_dev, min_p_dev, uniform_dev, draws,
+                       labels_dev, probs_dev, workspace_dev, workspace_bytes, static_cast<hipStream_t>(stream));
     });
 }
 IXA_EXPORT int ivfpq_search_probes_device(ivfpq_index_t *h, int64_t n, const float *x_dev, const int32_t *probes_dev,
