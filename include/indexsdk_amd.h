@@ -249,6 +249,32 @@ int ixa_op_sample(const void *scores_dev, int64_t ld, int type, int64_t rows, in
                   const int32_t *top_k_dev, const float *top_p_dev, const float *min_p_dev, const float *uniform_dev, int draws,
                   int64_t *labels_dev, float *probs_dev, void *workspace_dev, int64_t workspace_bytes, void *stream);
 
+/* The loss of rows of scores [rows][ld], n columns each, against a teacher's top entries: `labels` (columns) and `teacher`
+ * (their scores, fp32; larger is better) [rows][k], in any order, as a search or a top-k selection leaves them: an entry with a
+ * label outside 0 ... n - 1 (-1: the list ran out) is not there.  With one temperature T (1e-6 ... 1e6) for both sides
+ *   p_j = exp(teacher_j / T - L),  L = whole [rows] (the log of the teacher's sum of exponentials over all its columns), or with
+ *         whole = NULL that of the entries that are there;  P = sum p_j
+ *   q = softmax(scores / T),  loss = T^2 sum_j p_j (log p_j - log q[label_j]),  gradient_i = weight T (P q_i - sum of p_j with
+ *         label_j = i)
+ * for the weight of the row, row_weight [rows] (NULL: 1; the upstream gradient of its loss).  A label may come more than once.  Scores
+ * of -infinity are columns that are masked out: gradient 0, unless a label asks for them (loss +infinity).  Rows without an entry or
+ * without a score have loss and gradient 0; a NaN or a score of +infinity makes its row's NaN.
+ * ixa_op_distil_loss writes loss [rows] and, if not NULL, stats [rows][2], the largest score and the sum of exponentials relative
+ * to it, from which ixa_op_distil_gradient writes gradient [rows][ld_gradient], of the scores' type, rounded once.
+ * ixa_op_distil_step does both.  The gradient may take the scores' place (same address and stride), or shares no element with
+ * them.  Sums over columns are held in 64 bits, 32 exponentials at a time in fp32.  rows <= 2^22, n < 2^31, k <= 2048. */
+int ixa_distil_workspace(int64_t rows, int64_t n, int64_t *bytes);
+int ixa_op_distil_loss(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n, const int64_t *labels_dev,
+                       const float *teacher_dev, int k, const float *whole_dev, float temperature, float *loss_dev,
+                       float *stats_dev, void *workspace_dev, int64_t workspace_bytes, void *stream);
+int ixa_op_distil_gradient(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n, const int64_t *labels_dev,
+                           const float *teacher_dev, int k, const float *whole_dev, float temperature, const float *stats_dev,
+                           const float *row_weight_dev, void *gradient_dev, int64_t ld_gradient, void *stream);
+int ixa_op_distil_step(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n, const int64_t *labels_dev,
+                       const float *teacher_dev, int k, const float *whole_dev, float temperature, const float *row_weight_dev,
+                       float *loss_dev, void *gradient_dev, int64_t ld_gradient, void *workspace_dev, int64_t workspace_bytes,
+                       void *stream);
+
 /* ---------------------------------------------------------------------------------------------
  * IVFPQ
  * ------------------------------------------------------------------------------------------- */

@@ -58,6 +58,9 @@ class FlatSearchStats(ctypes.Structure):
 
 # every exported symbol of include/indexsdk_amd.h: name -> (restype, argtypes)
 _H = ctypes.c_void_p
+# rows of scores and what a teacher says about them
+_DISTIL = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+           ctypes.c_int, ctypes.c_void_p, ctypes.c_float]
 _SIGNATURES = {
     "ixa_last_error": (ctypes.c_char_p, []),
     "ivfpq_last_error": (ctypes.c_char_p, []),
@@ -111,6 +114,13 @@ _SIGNATURES = {
                                      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                      ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                      ctypes.c_void_p]),
+    "ixa_distil_workspace": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, c_i64p]),
+    "ixa_op_distil_loss": (ctypes.c_int, _DISTIL + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                    ctypes.c_void_p]),
+    "ixa_op_distil_gradient": (ctypes.c_int, _DISTIL + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                        ctypes.c_void_p]),
+    "ixa_op_distil_step": (ctypes.c_int, _DISTIL + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                    ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
     "ivfpq_search_probes_device": (ctypes.c_int, [_H, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
                                                   ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
     "ivfpq_search_probes_device_noalloc": (ctypes.c_int, [_H, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,

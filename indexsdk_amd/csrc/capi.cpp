@@ -771,6 +771,42 @@ IXA_EXPORT int ixa_op_sample(const void *scores_dev, int64_t ld, int type, int64
                        labels_dev, probs_dev, workspace_dev, workspace_bytes, static_cast<hipStream_t>(stream));
     });
 }
+IXA_EXPORT int ixa_distil_workspace(int64_t rows, int64_t n, int64_t *bytes)
+{
+    return guarded([&] {
+        IXA_REQUIRE(bytes != nullptr, ixa::kErrInvalidParam, "bytes can not be nullptr.");
+        *bytes = ixa::distil_workspace(rows, n);
+    }, false);
+}
+IXA_EXPORT int ixa_op_distil_loss(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n, const int64_t *labels_dev,
+                                  const float *teacher_dev, int k, const float *whole_dev, float temperature, float *loss_dev,
+                                  float *stats_dev, void *workspace_dev, int64_t workspace_bytes, void *stream)
+{
+    return guarded([&] {
+        ixa::op_distil_loss({scores_dev, ld, type, rows, n, labels_dev, teacher_dev, k, whole_dev, temperature}, loss_dev, stats_dev,
+                            workspace_dev, workspace_bytes, static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_op_distil_gradient(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n,
+                                      const int64_t *labels_dev, const float *teacher_dev, int k, const float *whole_dev,
+                                      float temperature, const float *stats_dev, const float *row_weight_dev, void *gradient_dev,
+                                      int64_t ld_gradient, void *stream)
+{
+    return guarded([&] {
+        ixa::op_distil_gradient({scores_dev, ld, type, rows, n, labels_dev, teacher_dev, k, whole_dev, temperature}, stats_dev,
+                                row_weight_dev, gradient_dev, ld_gradient, static_cast<hipStream_t>(stream));
+    });
+}
+IXA_EXPORT int ixa_op_distil_step(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n, const int64_t *labels_dev,
+                                  const float *teacher_dev, int k, const float *whole_dev, float temperature,
+                                  const float *row_weight_dev, float *loss_dev, void *gradient_dev, int64_t ld_gradient,
+                                  void *workspace_dev, int64_t workspace_bytes, void *stream)
+{
+    return guarded([&] {
+        ixa::op_distil_step({scores_dev, ld, type, rows, n, labels_dev, teacher_dev, k, whole_dev, temperature}, row_weight_dev,
+                            loss_dev, gradient_dev, ld_gradient, workspace_dev, workspace_bytes, static_cast<hipStream_t>(stream));
+    });
+}
 IXA_EXPORT int ivfpq_search_probes_device(ivfpq_index_t *h, int64_t n, const float *x_dev, const int32_t *probes_dev,
                                           int nprobe, int64_t k, float *distances_dev, int64_t *labels_dev)
 {

@@ -87,6 +87,22 @@ inline void check_row_buffer(const char *op, const void *p, int64_t ld, int type
                 (long)ld);
 }
 
+// Whether rows of a result lie on rows of an input that others have still to read: each row has to be its own input row as a
+// whole, or to share no element with any (two column ranges of one buffer, or apart outright).
+inline bool rows_collide(const void *out, int64_t ld_out, const void *in, int64_t ld_in, int type, int64_t n, int64_t d)
+{
+    const __int128 size = (__int128)element_bytes(type), a = (__int128)reinterpret_cast<uintptr_t>(out),
+                   b = (__int128)reinterpret_cast<uintptr_t>(in), row = size * d;
+    if (a + ((n - 1) * size * ld_out + row) <= b || b + ((n - 1) * size * ld_in + row) <= a) {
+        return false;
+    }
+    if (n == 1 || ld_out != ld_in) {
+        return n > 1 || a != b;
+    }
+    const __int128 step = size * ld_in, apart = (a > b ? a - b : b - a) % step;
+    return a != b && (apart < row || apart > step - row);
+}
+
 // A kernel for each element type.
 template <typename F>
 void with_type(int type, F f)

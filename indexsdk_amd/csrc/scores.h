@@ -25,4 +25,23 @@ void op_sample(const void *scores, int64_t ld, int type, int64_t rows, int64_t n
                const float *top_p, const float *min_p, const float *uniform, int draws, int64_t *labels, float *probs,
                void *workspace, int64_t workspace_bytes, hipStream_t s);
 
+// What a teacher says about rows of scores, and the loss against it, see distil.hip.
+struct DistilTask {
+    const void *scores;
+    int64_t ld;
+    int type;
+    int64_t rows, n;
+    const int64_t *labels;     // [rows][k]
+    const float *teacher;      // [rows][k]
+    int k;
+    const float *whole;        // [rows] or null
+    float temperature;
+};
+int64_t distil_workspace(int64_t rows, int64_t n);
+void op_distil_loss(const DistilTask &task, float *loss, float *stats, void *workspace, int64_t workspace_bytes, hipStream_t s);
+void op_distil_gradient(const DistilTask &task, const float *stats, const float *row_weight, void *gradient, int64_t ld_gradient,
+                        hipStream_t s);
+void op_distil_step(const DistilTask &task, const float *row_weight, float *loss, void *gradient, int64_t ld_gradient,
+                    void *workspace, int64_t workspace_bytes, hipStream_t s);
+
 }  // namespace ixa

@@ -41,3 +41,33 @@ def drawn(w, u, label, prob, slack):
     near = slack * total
     return bool(run[label] > target - near and run[label] - w[label] <= target + near and
                 abs(prob - w[label] / total) <= 2.0 ** -23 * w[label] / total + 2.0 ** -149)
+
+
+def distil(x, labels, teacher, temperature, whole=None):
+    """(loss, gradient per unit of weight) of one row."""
+    x, teacher, T = np.asarray(x, dtype=np.float64), np.asarray(teacher, dtype=np.float64), float(temperature)
+    n = len(x)
+    there = (labels >= 0) & (labels < n)
+    l, t = labels[there], teacher[there] / T
+    gradient = np.zeros(n)
+    if np.isnan(x).any() or (x == np.inf).any():
+        return np.nan, np.full(n, np.nan)
+    if len(l) == 0 or not (x > -np.inf).any():
+        return 0.0, gradient
+    if whole is None:
+        top = t.max()
+        if top == -np.inf:
+            return 0.0, gradient
+        lse = top + np.log(np.exp(t - top).sum())
+    else:
+        lse = float(whole)
+    log_p = t - lse
+    p = np.exp(log_p)
+    e = np.exp((x - x.max()) / T)
+    with np.errstate(divide="ignore"):
+        log_q = (x - x.max()) / T - np.log(e.sum())
+    use = p > 0
+    loss = T * T * float((p[use] * (log_p[use] - log_q[l[use]])).sum())
+    gradient = T * p.sum() * e / e.sum()
+    np.subtract.at(gradient, l, T * p)
+    return loss, gradient
