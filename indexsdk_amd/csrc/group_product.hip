@@ -28,7 +28,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 128;         // columns of a step: 64 bytes of codes
 constexpr int kLoaded = 0x0f70;    // s_waitcnt: all loads are there, also those into LDS
-constexpr size_t kStreamLds = 80 * 1024;
+constexpr size_t kHalfLds = 72 * 1024;   // two workgroups share a CU's
 
 struct GroupProductParams {
     const void *x;
@@ -130,83 +130,54 @@ __device__ __forceinline__ u4 transpose(u4 d)
     return u4{lo[0], lo[1], hi[0], hi[1]};
 }
 
-// The scales and zero points of SG groups from `g` on of one row, in two parts so that nothing waits for the load.  The load
-// ends with the array at the latest.
+// The scales and zero points of SG groups from `g` on of one row, in two parts so that nothing waits for the load, which ends with
+// the array at the latest (the array has SG scales at least).
 template <int SG>
 struct GroupScales {
-    uint32_t raw[SG];
+    static_assert(SG == 1 || SG == 2 || SG == 4, "");
+    uint32_t raw[SG];       // fp32 scales; 16-bit ones fill the first half
     uint32_t zero_raw;
-    int over;
+    int over;               // scales of the run that lie before `g`
     __device__ __forceinline__ void load(const GroupProductParams &p, int64_t row, int g)
     {
-        const int64_t at = row * p.groups + g, from = min(at, max(p.scale_count - SG, (int64_t)0));
+        const int64_t at = row * p.groups + g, from = min(at, p.scale_count - SG);
         over = (int)(at - from);
-        zero_raw = 0x08080808u;
-        if (p.scale_count < SG) {
-#pragma unroll
-            for (int t = 0; t < SG; t++) {
-                const int64_t i = min(from + t, p.scale_count - 1);
-                raw[t] = p.scale_type == kTypeF32 ? static_cast<const uint32_t *>(p.scales)[i]
-                                                  : static_cast<const uint16_t *>(p.scales)[i];
-            }
-            if (p.zeros) {
-                zero_raw = 0;
-#pragma unroll
-                for (int t = 0; t < SG; t++) {
-                    zero_raw |= (uint32_t)p.zeros[min(from + t, p.scale_count - 1)] << (8 * t);
-                }
-            }
-            return;
-        }
         if (p.scale_type == kTypeF32) {
-            struct Wide {
-                uint32_t v[SG];
-            } w;
-            __builtin_memcpy(&w, static_cast<const uint32_t *>(p.scales) + from, sizeof(w));
-#pragma unroll
-            for (int t = 0; t < SG; t++) {
-                raw[t] = w.v[t];
-            }
+            __builtin_memcpy(raw, static_cast<const uint32_t *>(p.scales) + from, SG * 4);
         } else {
-            struct Narrow {
-                uint16_t v[SG];
-            } w;
-            __builtin_memcpy(&w, static_cast<const uint16_t *>(p.scales) + from, sizeof(w));
-#pragma unroll
-            for (int t = 0; t < SG; t++) {
-                raw[t] = w.v[t];
-            }
+            __builtin_memcpy(raw, static_cast<const uint16_t *>(p.scales) + from, SG * 2);
         }
+        zero_raw = 0x08080808u;
         if (p.zeros) {
-            uint32_t z = 0;
-            __builtin_memcpy(&z, p.zeros + from, SG);
-            zero_raw = z;
+            __builtin_memcpy(&zero_raw, p.zeros + from, SG);
         }
     }
     // groups behind the row's last one get scale 0: x has zeros there
-    __device__ __forceinline__ void take(const GroupProductParams &p, int g, float (&scale)[SG], h2 (&minus)[SG])
+    __device__ __forceinline__ void take(const GroupProductParams &p, int g, bool there, float (&scale)[SG], h2 (&minus)[SG])
     {
-        if constexpr (SG > 1) {
-            if (__builtin_expect(over != 0, 0)) {
-#pragma unroll
-                for (int k = 0; k < SG - 1; k++) {
-                    if (k < over) {
-#pragma unroll
-                        for (int t = 0; t < SG - 1; t++) {
-                            raw[t] = raw[t + 1];
-                        }
-                        zero_raw >>= 8;
-                    }
-                }
-            }
+        const bool wide = p.scale_type == kTypeF32, half = p.scale_type == kTypeF16;
+        uint32_t of[SG];
+        if constexpr (SG == 1) {
+            of[0] = wide ? raw[0] : raw[0] & 0xffffu;
+        } else if constexpr (SG == 2) {
+            const uint32_t narrow = raw[0] >> (16 * over);
+            of[0] = wide ? over ? raw[1] : raw[0] : narrow & 0xffffu;
+            of[1] = wide ? raw[1] : narrow >> 16;
+        } else {
+            const uint64_t narrow = ((uint64_t)raw[1] << 32 | raw[0]) >> (16 * over);
+            const uint32_t a = over & 2 ? raw[2] : raw[0], b = over & 2 ? raw[3] : raw[1], c = raw[2], d = raw[3];
+            of[0] = wide ? over & 1 ? b : a : (uint32_t)narrow & 0xffffu;
+            of[1] = wide ? over & 1 ? c : b : (uint32_t)(narrow >> 16) & 0xffffu;
+            of[2] = wide ? over & 1 ? d : c : (uint32_t)(narrow >> 32) & 0xffffu;
+            of[3] = wide ? d : (uint32_t)(narrow >> 48);
         }
+        const uint32_t zero = zero_raw >> (8 * over);
 #pragma unroll
         for (int t = 0; t < SG; t++) {
-            const float s = p.scale_type == kTypeF32   ? __uint_as_float(raw[t])
-                            : p.scale_type == kTypeF16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)raw[t])
-                                                       : __uint_as_float(raw[t] << 16);
-            scale[t] = g + t < p.groups ? s : 0.f;
-            minus[t] = minus_zero_point((float)(zero_raw >> (8 * t) & 255u));
+            const float f16 = (float)__builtin_bit_cast(_Float16, (uint16_t)of[t]);
+            const float s = half ? f16 : __uint_as_float(wide ? of[t] : of[t] << 16);
+            scale[t] = there && g + t < p.groups ? s : 0.f;
+            minus[t] = minus_zero_point((float)(zero >> (8 * t) & 255u));
         }
     }
 };
@@ -269,8 +240,8 @@ __device__ __forceinline__ int piece_place(int r, int q) { return r * 64 + ((q ^
 // them, U steps of 128 columns ahead.  KS wavefronts of the workgroup share a tile, a part of its steps each, where there are few
 // tiles.  Row j of 16 is row 4 (j & 3) + (j >> 2) of its fragment, so that RI = 1, 2 or 4 registers of a lane's four hold all
 // rows of up to 4, 8 or 16.
-template <int P, int MF, int RI, int NF, int U, int KS, int SG>
-__global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p, int64_t tiles)
+template <int P, int MF, int RI, int NF, int U, int KS, int SG, int W>
+__global__ __launch_bounds__(W * 64) void group_stream_kernel(GroupProductParams p, int64_t tiles)
 {
     static_assert(NF * U == 4 && (MF == 1 || RI == 4), "a lane brings the scales of one row and step");
     extern __shared__ __align__(16) uint8_t smem[];
@@ -281,8 +252,9 @@ __global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p,
     constexpr int kTurn = 64 * SG * 8;                       // scales and zero points of NF * 16 rows and U steps
     constexpr int kShare = KS > 1 ? MF * NF * RI * 256 : 0;   // a wavefront's sums, for the one that adds them up
     uint8_t *const turn = reinterpret_cast<uint8_t *>(power + 64) + wave * std::max(kTurn, kShare);
-    // 256, 128 ... 4 threads bring a row
-    const int lg = rows > 1 ? 8 - (32 - __builtin_clz(rows - 1)) : 8, per_row = 1 << lg;
+    // all threads, a half, a quarter ... of them bring a row
+    constexpr int kLog = W == 4 ? 8 : 9;
+    const int lg = rows > 1 ? kLog - (32 - __builtin_clz(rows - 1)) : kLog, per_row = 1 << lg;
     const int my_row = tid >> lg, e = tid & (per_row - 1);
     const size_t x_bytes = (size_t)(p.type == kTypeF32 ? 4 : 2) * (size_t)p.ld_x;
     const uint8_t *const x_row = static_cast<const uint8_t *>(p.x) + (size_t)min(my_row, rows - 1) * x_bytes;
@@ -326,15 +298,19 @@ __global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p,
         a_row[i] = min(i * 16 + (r >> 2) + (r & 3) * 4, rows - 1);
     }
     __syncthreads();
-    const int part = KS > 1 ? wave : 0;
+    const int part = wave % KS;
     // whole batches of U steps each
     const int share = KS > 1 ? ((p.steps + U * KS - 1) / (U * KS)) * U : p.steps;
     const int t0 = min(part * share, p.steps), t1 = min(t0 + share, p.steps);
-    const int64_t stride = (int64_t)gridDim.x * (4 / KS);
-    for (int64_t tile = (int64_t)blockIdx.x * (4 / KS) + (KS > 1 ? 0 : wave); tile < tiles; tile += stride) {
+    for (int64_t first = (int64_t)blockIdx.x * (W / KS); first < tiles; first += (int64_t)gridDim.x * (W / KS)) {
+        const int64_t tile = first + wave / KS;
+        if (KS == 1 && tile >= tiles) {
+            break;
+        }
+        const bool mine = KS == 1 || tile < tiles;     // wavefronts that share tiles meet at barriers
         const int64_t col0 = tile * (NF * 16);
-        const int last = (int)min<int64_t>(NF * 16, p.n - col0) - 1;   // rows behind the last one repeat it
-        const uint8_t *const codes = p.codes + col0 * p.row_bytes;
+        const int last = mine ? (int)min<int64_t>(NF * 16, p.n - col0) - 1 : 0;   // rows behind the last one repeat it
+        const uint8_t *const codes = p.codes + (mine ? col0 : 0) * p.row_bytes;
         uint32_t offset[NF];
 #pragma unroll
         for (int j = 0; j < NF; j++) {
@@ -352,7 +328,7 @@ __global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p,
                     next[u][j] = *reinterpret_cast<const u4 *>(codes + (offset[j] + byte));
                 }
             }
-            next_scales.load(p, col0 + min(scale_row, last), min((t + scale_step) * SG, p.groups - 1));
+            next_scales.load(p, (mine ? col0 : 0) + min(scale_row, last), min((t + scale_step) * SG, p.groups - 1));
         };
         v4f acc[MF][NF] = {};
         if (t0 < t1) {
@@ -362,12 +338,11 @@ __global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p,
             {
                 float scale[SG];
                 h2 minus[SG];
-                next_scales.take(p, min((t + scale_step) * SG, p.groups - 1), scale, minus);
+                next_scales.take(p, min((t + scale_step) * SG, p.groups - 1), t + scale_step < p.steps, scale, minus);
                 const int slot = (scale_step * NF + scale_row % NF) * 16 + scale_row / NF;
-                const bool there = t + scale_step < p.steps;
 #pragma unroll
                 for (int g = 0; g < SG; g++) {
-                    reinterpret_cast<float *>(turn)[slot * SG + g] = there ? scale[g] : 0.f;
+                    reinterpret_cast<float *>(turn)[slot * SG + g] = scale[g];
                     reinterpret_cast<h2 *>(turn + kTurn / 2)[slot * SG + g] = minus[g];
                 }
             }
@@ -431,6 +406,7 @@ __global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p,
                             for (int k = 0; k < RI; k++) {
                                 acc[i][j][k] = fmaf(scale[j][g], sum[i][j][k], acc[i][j][k]);
                             }
+                            asm volatile("" : "+v"(acc[i][j]));   // not left for later, which would keep the sums
                         }
                     }
                 }
@@ -438,11 +414,9 @@ __global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p,
             __builtin_amdgcn_wave_barrier();
         }
         if constexpr (KS > 1) {
-            // the first wavefront adds the others' sums to its own, in their order
-            v4f *const mine = reinterpret_cast<v4f *>(turn);
-            static_assert(RI == 4 || MF * NF == 1, "");
-            float *const box = reinterpret_cast<float *>(mine);
-            if (wave > 0) {
+            // the first of a tile's wavefronts adds the others' sums to its own, in their order
+            float *const box = reinterpret_cast<float *>(turn);
+            if (part > 0) {
 #pragma unroll
                 for (int i = 0; i < MF; i++) {
 #pragma unroll
@@ -455,7 +429,7 @@ __global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p,
                 }
             }
             __syncthreads();
-            if (wave == 0) {
+            if (part == 0) {
                 for (int w = 1; w < KS; w++) {
                     const float *const other = reinterpret_cast<const float *>(turn + w * std::max(kTurn, kShare));
 #pragma unroll
@@ -471,7 +445,7 @@ __global__ __launch_bounds__(256) void group_stream_kernel(GroupProductParams p,
                 }
             }
             __syncthreads();
-            if (wave > 0) {
+            if (part > 0 || !mine) {
                 continue;
             }
         }
@@ -586,13 +560,13 @@ __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p
         for (int j = 0; j < 4; j++) {
             next[j] = *reinterpret_cast<const u4 *>(codes + (b_from[j] + byte));
         }
-        next_scales.load(p, col0 + min(scale_col, last_col), min(step * SG, p.groups - 1));
+        next_scales.load(p, col0 + min(scale_col, last_col), step * SG);
     };
     auto put_scales = [&](int step, uint8_t *buffer) {
         if (tid < kCols) {
             float scale[SG];
             h2 minus[SG];
-            next_scales.take(p, min(step * SG, p.groups - 1), scale, minus);
+            next_scales.take(p, step * SG, true, scale, minus);
 #pragma unroll
             for (int g = 0; g < SG; g++) {
                 reinterpret_cast<float *>(buffer + kABytes)[scale_col * SG + g] = scale[g];
@@ -617,9 +591,13 @@ __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p
             fetch(step + 1, other);
         }
         constexpr int kBlocks = 4 / SG;
+        auto rows_of = [&](int k, int block, int i) {
+            const int row = wm * 64 + i * 16 + r;
+            return *reinterpret_cast<const h8 *>(here + k * kPiece + (block >> 1) * kHalf + row * 128 +
+                                                 ((((block & 1) * 4 + q) ^ ((row >> 1) & 7)) * 16));
+        };
 #pragma unroll
         for (int g = 0; g < SG; g++) {
-            v4f sum[4][4] = {};
             h2 minus[4];
             float scale[4];
 #pragma unroll
@@ -627,36 +605,71 @@ __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p
                 scale[j] = reinterpret_cast<const float *>(here + kABytes)[(wn * 64 + r * 4 + j) * SG + g];
                 minus[j] = reinterpret_cast<const h2 *>(here + kABytes + kScales)[(wn * 64 + r * 4 + j) * SG + g];
             }
+            if constexpr (SG == 1) {
+                // sums of all fragments, block by block
+                v4f sum[4][4] = {};
 #pragma unroll
-            for (int b = 0; b < kBlocks; b++) {
-                const int block = g * kBlocks + b;
-                h8 w[4];
+                for (int b = 0; b < kBlocks; b++) {
+                    h8 w[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    w[j] = integers(now[j][block], minus[j]);
-                }
+                    for (int j = 0; j < 4; j++) {
+                        w[j] = integers(now[j][b], minus[j]);
+                    }
 #pragma unroll
-                for (int k = 0; k < P; k++) {
+                    for (int k = 0; k < P; k++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int row = wm * 64 + i * 16 + r;
-                        const h8 a = *reinterpret_cast<const h8 *>(here + k * kPiece + (block >> 1) * kHalf + row * 128 +
-                                                                   ((((block & 1) * 4 + q) ^ ((row >> 1) & 7)) * 16));
+                        for (int i = 0; i < 4; i++) {
+                            const h8 a = rows_of(k, b, i);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[j], sum[i][j], 0, 0, 0);
+                            for (int j = 0; j < 4; j++) {
+                                sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[j], sum[i][j], 0, 0, 0);
+                            }
                         }
                     }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < 4; i++) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                    for (int j = 0; j < 4; j++) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        acc[i][j][k] = fmaf(scale[j], sum[i][j][k], acc[i][j][k]);
+                        for (int k = 0; k < 4; k++) {
+                            acc[i][j][k] = fmaf(scale[j], sum[i][j][k], acc[i][j][k]);
+                        }
                     }
+                }
+            } else {
+                // a group's few blocks at a time, so that only one row of fragments has sums of its own
+                h8 w[kBlocks][4];
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        w[b][j] = integers(now[j][g * kBlocks + b], minus[j]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v4f sum[4] = {};
+#pragma unroll
+                    for (int b = 0; b < kBlocks; b++) {
+#pragma unroll
+                        for (int k = 0; k < P; k++) {
+                            const h8 a = rows_of(k, g * kBlocks + b, i);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[b][j], sum[j], 0, 0, 0);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            acc[i][j][k] = fmaf(scale[j], sum[j][k], acc[i][j][k]);
+                        }
+                    }
+                    // multiply-adds left for later would keep all their sums in registers
+                    asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
                 }
             }
         }
@@ -680,41 +693,80 @@ __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p
     }
 }
 
+// Fewer than four scales in all (up to three short rows of codes): a thread per score.
+__global__ __launch_bounds__(256) void group_tiny_kernel(GroupProductParams p, int group)
+{
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / p.n, col = id - row * p.n;
+    if (row >= p.m) {
+        return;
+    }
+    const uint8_t *const x_row = static_cast<const uint8_t *>(p.x) + (size_t)row * (size_t)p.ld_x * (p.type == kTypeF32 ? 4 : 2);
+    float sum = 0.f, of_group = 0.f;
+    for (int at = 0; at < p.d; at += kEight) {
+        const int64_t slot = col * p.groups + at / group;
+        const float zero = p.zeros ? (float)p.zeros[slot] : 8.f;
+        const uint32_t code = *reinterpret_cast<const uint32_t *>(p.codes + col * p.row_bytes + at / 2);
+        float v[kEight];
+        load_eight(x_row, p.type, at, p.d, v);
+#pragma unroll
+        for (int i = 0; i < kEight; i++) {
+            of_group += at + i < p.d ? v[i] * ((float)(code >> (4 * i) & 15u) - zero) : 0.f;
+        }
+        if ((at + kEight) % group == 0 || at + kEight >= p.d) {
+            const float scale = p.scale_type == kTypeF32   ? static_cast<const float *>(p.scales)[slot]
+                                : p.scale_type == kTypeF16 ? (float)static_cast<const _Float16 *>(p.scales)[slot]
+                                                           : (float)static_cast<const __bf16 *>(p.scales)[slot];
+            sum = fmaf(scale, of_group, sum);
+            of_group = 0.f;
+        }
+    }
+    const float sums[1] = {sum};
+    float bias[1];
+    load_bias(p, col, bias);
+    store_scores(p, row, 0, col, sums, bias);
+}
+
 int pieces_of(int type) { return type == kTypeF32 ? 2 : 1; }
 int steps_of(int d) { return (d + kStep - 1) / kStep; }
 size_t row_lds(int type, int64_t m, int d) { return (size_t)steps_of(d) * 4 * pieces_of(type) * (size_t)m * 64; }
-// Few rows whose pieces fit half a CU's LDS stay there.
-bool stays(int type, int64_t m, int d) { return m <= 64 && row_lds(type, m, d) <= kStreamLds - 8192; }
+// Few rows whose pieces fit a CU's LDS stay there.
+constexpr size_t kTurnLds = 8 * 64 * 4 * 8;
+bool stays(int type, int64_t m, int d) { return m <= 64 && row_lds(type, m, d) + 256 + kTurnLds <= 160 * 1024; }
 
-template <int P, int MF, int RI, int NF, int U, int KS, int SG>
+template <int P, int MF, int RI, int NF, int U, int KS, int SG, int W>
 void launch_stream(const GroupProductParams &p, hipStream_t s)
 {
-    constexpr size_t turn = 4 * std::max(64 * SG * 8, KS > 1 ? MF * NF * RI * 256 : 0);
+    constexpr size_t turn = W * std::max(64 * SG * 8, KS > 1 ? MF * NF * RI * 256 : 0);
+    static_assert(turn <= kTurnLds, "");
     const size_t lds = row_lds(p.type, p.m, p.d) + 256 + turn;
     const int64_t tiles = (p.n + NF * 16 - 1) / (NF * 16);
-    const auto kern = group_stream_kernel<P, MF, RI, NF, U, KS, SG>;
+    const auto kern = group_stream_kernel<P, MF, RI, NF, U, KS, SG, W>;
     require_dynamic_lds(reinterpret_cast<const void *>(kern), lds);
-    int device, cus;
-    IXA_HIP(hipGetDevice(&device));
-    IXA_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
-    const int64_t per_cu = std::min<int64_t>(8, 160 * 1024 / (int64_t)lds);
-    const int64_t want = (tiles * KS + 3) / 4;
-    hipLaunchKernelGGL(kern, dim3((unsigned)std::min(want, per_cu * cus)), dim3(256), lds, s, p, tiles);
+    const int64_t most = resident_workgroups(reinterpret_cast<const void *>(kern), W * 64, lds);
+    hipLaunchKernelGGL(kern, dim3((unsigned)std::min((tiles * KS + W - 1) / W, most)), dim3(W * 64), lds, s, p, tiles);
     check_launch();
 }
 
-template <int P, int SG>
+template <int P, int SG, int W>
 void launch_stream(const GroupProductParams &p, hipStream_t s)
 {
     const bool narrow = p.n <= 32768, deep = narrow && p.steps >= 8;
     if (p.m <= 4) {
-        deep ? launch_stream<P, 1, 1, 1, 4, 4, SG>(p, s) : narrow ? launch_stream<P, 1, 1, 1, 4, 1, SG>(p, s) : launch_stream<P, 1, 1, 2, 2, 1, SG>(p, s);
+        if (deep) {
+            launch_stream<P, 1, 1, 1, 4, 4, SG, W>(p, s);
+        } else {
+            narrow ? launch_stream<P, 1, 1, 1, 4, 1, SG, W>(p, s) : launch_stream<P, 1, 1, 2, 2, 1, SG, W>(p, s);
+        }
     } else if (p.m <= 16) {
-        deep ? launch_stream<P, 1, 4, 1, 4, 4, SG>(p, s) : narrow ? launch_stream<P, 1, 4, 1, 4, 1, SG>(p, s) : launch_stream<P, 1, 4, 2, 2, 1, SG>(p, s);
+        if (deep) {
+            launch_stream<P, 1, 4, 1, 4, 4, SG, W>(p, s);
+        } else {
+            narrow ? launch_stream<P, 1, 4, 1, 4, 1, SG, W>(p, s) : launch_stream<P, 1, 4, 2, 2, 1, SG, W>(p, s);
+        }
     } else if (p.m <= 32) {
-        narrow ? launch_stream<P, 2, 4, 1, 4, 1, SG>(p, s) : launch_stream<P, 2, 4, 4, 1, 1, SG>(p, s);
+        narrow ? launch_stream<P, 2, 4, 1, 4, 1, SG, W>(p, s) : launch_stream<P, 2, 4, 4, 1, 1, SG, W>(p, s);
     } else {
-        narrow ? launch_stream<P, 4, 4, 1, 4, 1, SG>(p, s) : launch_stream<P, 4, 4, 4, 1, 1, SG>(p, s);
+        narrow ? launch_stream<P, 4, 4, 1, 4, 1, SG, W>(p, s) : launch_stream<P, 4, 4, 4, 1, 1, SG, W>(p, s);
     }
 }
 
@@ -736,7 +788,7 @@ template <int P, int SG>
 void launch(GroupProductParams &p, uint8_t *workspace, hipStream_t s)
 {
     if (stays(p.type, p.m, p.d)) {
-        launch_stream<P, SG>(p, s);
+        row_lds(p.type, p.m, p.d) <= kHalfLds ? launch_stream<P, SG, 4>(p, s) : launch_stream<P, SG, 8>(p, s);
         return;
     }
     int *const exponents = reinterpret_cast<int *>(workspace);
@@ -802,6 +854,11 @@ void op_group_product(const void *x, int64_t ld_x, int type, int64_t m, const ui
     p.steps = steps_of(d);
     p.scale_count = n * p.groups;
     p.alpha = alpha;
+    if (p.scale_count < 4) {
+        hipLaunchKernelGGL(group_tiny_kernel, dim3((unsigned)((m * n + 255) / 256)), dim3(256), 0, s, p, group);
+        check_launch();
+        return;
+    }
     uint8_t *const work = static_cast<uint8_t *>(workspace);
     const auto of_group = [&](auto pieces) {
         constexpr int P = decltype(pieces)::value;
