@@ -40,6 +40,7 @@ struct GroupProductParams {
     const int *exponents;
     int64_t m, n, ld_x, ld, scale_count;
     int type, scale_type, out_type, d, groups, row_bytes, steps;
+    bool has_zeros;
     float alpha;
 };
 
@@ -130,52 +131,55 @@ __device__ __forceinline__ u4 transpose(u4 d)
     return u4{lo[0], lo[1], hi[0], hi[1]};
 }
 
-// The scales and zero points of SG groups from `g` on of one row, in two parts so that nothing waits for the load, which ends with
-// the array at the latest (the array has SG scales at least).
-template <int SG>
+// The scales (WIDE: fp32) and zero points of SG groups from `g` on of one row, in two parts so that nothing waits for the load, which
+// ends with the array at the latest (the array has SG scales at least).  No branch is around a load: behind one the compiler
+// waits for it, and with it for all that is in flight.
+template <int SG, bool WIDE>
 struct GroupScales {
     static_assert(SG == 1 || SG == 2 || SG == 4, "");
-    uint32_t raw[SG];       // fp32 scales; 16-bit ones fill the first half
+    typedef std::conditional_t<WIDE, uint32_t, uint16_t> Raw;
+    Raw raw[SG];
     uint32_t zero_raw;
     int over;               // scales of the run that lie before `g`
     __device__ __forceinline__ void load(const GroupProductParams &p, int64_t row, int g)
     {
         const int64_t at = row * p.groups + g, from = min(at, p.scale_count - SG);
         over = (int)(at - from);
-        if (p.scale_type == kTypeF32) {
-            __builtin_memcpy(raw, static_cast<const uint32_t *>(p.scales) + from, SG * 4);
-        } else {
-            __builtin_memcpy(raw, static_cast<const uint16_t *>(p.scales) + from, SG * 2);
-        }
-        zero_raw = 0x08080808u;
-        if (p.zeros) {
-            __builtin_memcpy(&zero_raw, p.zeros + from, SG);
-        }
+        __builtin_memcpy(raw, static_cast<const Raw *>(p.scales) + from, sizeof(raw));
+        zero_raw = 0;
+        __builtin_memcpy(&zero_raw, p.zeros + from, SG);      // any bytes where there are no zero points
     }
     // groups behind the row's last one get scale 0: x has zeros there
     __device__ __forceinline__ void take(const GroupProductParams &p, int g, bool there, float (&scale)[SG], h2 (&minus)[SG])
     {
-        const bool wide = p.scale_type == kTypeF32, half = p.scale_type == kTypeF16;
         uint32_t of[SG];
         if constexpr (SG == 1) {
-            of[0] = wide ? raw[0] : raw[0] & 0xffffu;
+            of[0] = raw[0];
+        } else if constexpr (!WIDE) {
+            typedef std::conditional_t<SG == 2, uint32_t, uint64_t> All;
+            const All all = __builtin_bit_cast(All, raw) >> (16 * over);
+#pragma unroll
+            for (int t = 0; t < SG; t++) {
+                of[t] = (uint32_t)(all >> (16 * t)) & 0xffffu;
+            }
         } else if constexpr (SG == 2) {
-            const uint32_t narrow = raw[0] >> (16 * over);
-            of[0] = wide ? over ? raw[1] : raw[0] : narrow & 0xffffu;
-            of[1] = wide ? raw[1] : narrow >> 16;
+            of[0] = over ? raw[1] : raw[0];
+            of[1] = raw[1];
         } else {
-            const uint64_t narrow = ((uint64_t)raw[1] << 32 | raw[0]) >> (16 * over);
-            const uint32_t a = over & 2 ? raw[2] : raw[0], b = over & 2 ? raw[3] : raw[1], c = raw[2], d = raw[3];
-            of[0] = wide ? over & 1 ? b : a : (uint32_t)narrow & 0xffffu;
-            of[1] = wide ? over & 1 ? c : b : (uint32_t)(narrow >> 16) & 0xffffu;
-            of[2] = wide ? over & 1 ? d : c : (uint32_t)(narrow >> 32) & 0xffffu;
-            of[3] = wide ? d : (uint32_t)(narrow >> 48);
+            const uint32_t a = over & 2 ? raw[2] : raw[0], b = over & 2 ? raw[3] : raw[1];
+            of[0] = over & 1 ? b : a;
+            of[1] = over & 1 ? raw[2] : b;
+            of[2] = over & 1 ? raw[3] : raw[2];
+            of[3] = raw[3];
         }
-        const uint32_t zero = zero_raw >> (8 * over);
+        const uint32_t zero = p.has_zeros ? zero_raw >> (8 * over) : 0x08080808u;
+        const bool half = p.scale_type == kTypeF16;
 #pragma unroll
         for (int t = 0; t < SG; t++) {
-            const float f16 = (float)__builtin_bit_cast(_Float16, (uint16_t)of[t]);
-            const float s = half ? f16 : __uint_as_float(wide ? of[t] : of[t] << 16);
+            float s = __uint_as_float(WIDE ? of[t] : of[t] << 16);
+            if constexpr (!WIDE) {
+                s = half ? (float)__builtin_bit_cast(_Float16, (uint16_t)of[t]) : s;
+            }
             scale[t] = there && g + t < p.groups ? s : 0.f;
             minus[t] = minus_zero_point((float)(zero >> (8 * t) & 255u));
         }
@@ -240,7 +244,7 @@ __device__ __forceinline__ int piece_place(int r, int q) { return r * 64 + ((q ^
 // them, U steps of 128 columns ahead.  KS wavefronts of the workgroup share a tile, a part of its steps each, where there are few
 // tiles.  Row j of 16 is row 4 (j & 3) + (j >> 2) of its fragment, so that RI = 1, 2 or 4 registers of a lane's four hold all
 // rows of up to 4, 8 or 16.
-template <int P, int MF, int RI, int NF, int U, int KS, int SG, int W>
+template <int P, int MF, int RI, int NF, int U, int KS, int SG, bool WIDE, int W>
 __global__ __launch_bounds__(W * 64) void group_stream_kernel(GroupProductParams p, int64_t tiles)
 {
     static_assert(NF * U == 4 && (MF == 1 || RI == 4), "a lane brings the scales of one row and step");
@@ -318,7 +322,7 @@ __global__ __launch_bounds__(W * 64) void group_stream_kernel(GroupProductParams
         }
         const int scale_row = lane % (NF * 16), scale_step = lane / (NF * 16);
         u4 next[U][NF];
-        GroupScales<SG> next_scales;
+        GroupScales<SG, WIDE> next_scales;
         auto fetch = [&](int t) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
@@ -510,7 +514,7 @@ __global__ __launch_bounds__(256) void group_pieces_kernel(GroupProductParams p,
 // Many rows: tiles of WM * 64 rows by WN * 64 coded rows, 64 x 64 per wavefront.  A step's 128 columns of x's pieces go straight
 // into one of two LDS buffers while the other is multiplied; codes come to the registers of the wavefront that multiplies
 // them, scales and zero points through LDS, all a step ahead.
-template <int P, int WM, int WN, int SG>
+template <int P, int WM, int WN, int SG, bool WIDE>
 __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p, int row_tiles, int col_tiles, int per_xcd)
 {
     static_assert(WM * WN == 4, "");
@@ -535,7 +539,7 @@ __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p
         b_from[j] = (uint32_t)(min(wn * 64 + r * 4 + j, last_col) * p.row_bytes);
     }
     u4 next[4];
-    GroupScales<SG> next_scales;
+    GroupScales<SG, WIDE> next_scales;
     const int scale_col = tid % kCols;
     auto fetch = [&](int step, uint8_t *buffer) {
         // 8 rows of 128 bytes at a time; lane l brings the 16 bytes that belong at place l & 7 of row l >> 3
@@ -605,72 +609,38 @@ __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p
                 scale[j] = reinterpret_cast<const float *>(here + kABytes)[(wn * 64 + r * 4 + j) * SG + g];
                 minus[j] = reinterpret_cast<const h2 *>(here + kABytes + kScales)[(wn * 64 + r * 4 + j) * SG + g];
             }
-            if constexpr (SG == 1) {
-                // sums of all fragments, block by block
-                v4f sum[4][4] = {};
+            // one row of fragments at a time: no more sums than that at a time beside the results
+            h8 w[kBlocks][4];
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    w[b][j] = integers(now[j][g * kBlocks + b], minus[j]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v4f sum[4] = {};
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++) {
-                    h8 w[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        w[j] = integers(now[j][b], minus[j]);
-                    }
 #pragma unroll
                     for (int k = 0; k < P; k++) {
+                        const h8 a = rows_of(k, g * kBlocks + b, i);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const h8 a = rows_of(k, b, i);
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[j], sum[i][j], 0, 0, 0);
-                            }
+                        for (int j = 0; j < 4; j++) {
+                            sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[b][j], sum[j], 0, 0, 0);
                         }
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int j = 0; j < 4; j++) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            acc[i][j][k] = fmaf(scale[j], sum[i][j][k], acc[i][j][k]);
-                        }
+                    for (int k = 0; k < 4; k++) {
+                        acc[i][j][k] = fmaf(scale[j], sum[j][k], acc[i][j][k]);
                     }
                 }
-            } else {
-                // a group's few blocks at a time, so that only one row of fragments has sums of its own
-                h8 w[kBlocks][4];
-#pragma unroll
-                for (int b = 0; b < kBlocks; b++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        w[b][j] = integers(now[j][g * kBlocks + b], minus[j]);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    v4f sum[4] = {};
-#pragma unroll
-                    for (int b = 0; b < kBlocks; b++) {
-#pragma unroll
-                        for (int k = 0; k < P; k++) {
-                            const h8 a = rows_of(k, g * kBlocks + b, i);
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w[b][j], sum[j], 0, 0, 0);
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            acc[i][j][k] = fmaf(scale[j], sum[j][k], acc[i][j][k]);
-                        }
-                    }
-                    // multiply-adds left for later would keep all their sums in registers
-                    asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
-                }
+                // multiply-adds left for later would keep all their sums in registers
+                asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]));
             }
         }
         if (step + 1 < p.steps) {
@@ -704,7 +674,7 @@ __global__ __launch_bounds__(256) void group_tiny_kernel(GroupProductParams p, i
     float sum = 0.f, of_group = 0.f;
     for (int at = 0; at < p.d; at += kEight) {
         const int64_t slot = col * p.groups + at / group;
-        const float zero = p.zeros ? (float)p.zeros[slot] : 8.f;
+        const float zero = p.has_zeros ? (float)p.zeros[slot] : 8.f;
         const uint32_t code = *reinterpret_cast<const uint32_t *>(p.codes + col * p.row_bytes + at / 2);
         float v[kEight];
         load_eight(x_row, p.type, at, p.d, v);
@@ -733,44 +703,45 @@ size_t row_lds(int type, int64_t m, int d) { return (size_t)steps_of(d) * 4 * pi
 constexpr size_t kTurnLds = 8 * 64 * 4 * 8;
 bool stays(int type, int64_t m, int d) { return m <= 64 && row_lds(type, m, d) + 256 + kTurnLds <= 160 * 1024; }
 
-template <int P, int MF, int RI, int NF, int U, int KS, int SG, int W>
+template <int P, int MF, int RI, int NF, int U, int KS, int SG, bool WIDE, int W>
 void launch_stream(const GroupProductParams &p, hipStream_t s)
 {
     constexpr size_t turn = W * std::max(64 * SG * 8, KS > 1 ? MF * NF * RI * 256 : 0);
     static_assert(turn <= kTurnLds, "");
     const size_t lds = row_lds(p.type, p.m, p.d) + 256 + turn;
     const int64_t tiles = (p.n + NF * 16 - 1) / (NF * 16);
-    const auto kern = group_stream_kernel<P, MF, RI, NF, U, KS, SG, W>;
+    const auto kern = group_stream_kernel<P, MF, RI, NF, U, KS, SG, WIDE, W>;
     require_dynamic_lds(reinterpret_cast<const void *>(kern), lds);
     const int64_t most = resident_workgroups(reinterpret_cast<const void *>(kern), W * 64, lds);
     hipLaunchKernelGGL(kern, dim3((unsigned)std::min((tiles * KS + W - 1) / W, most)), dim3(W * 64), lds, s, p, tiles);
     check_launch();
 }
 
-template <int P, int SG, int W>
+template <int P, int SG, bool WIDE, int W>
 void launch_stream(const GroupProductParams &p, hipStream_t s)
 {
     const bool narrow = p.n <= 32768, deep = narrow && p.steps >= 8;
     if (p.m <= 4) {
         if (deep) {
-            launch_stream<P, 1, 1, 1, 4, 4, SG, W>(p, s);
+            launch_stream<P, 1, 1, 1, 4, 4, SG, WIDE, W>(p, s);
         } else {
-            narrow ? launch_stream<P, 1, 1, 1, 4, 1, SG, W>(p, s) : launch_stream<P, 1, 1, 2, 2, 1, SG, W>(p, s);
+            narrow ? launch_stream<P, 1, 1, 1, 4, 1, SG, WIDE, W>(p, s) : launch_stream<P, 1, 1, 2, 2, 1, SG, WIDE, W>(p, s);
         }
     } else if (p.m <= 16) {
         if (deep) {
-            launch_stream<P, 1, 4, 1, 4, 4, SG, W>(p, s);
+            launch_stream<P, 1, 4, 1, 4, 4, SG, WIDE, W>(p, s);
         } else {
-            narrow ? launch_stream<P, 1, 4, 1, 4, 1, SG, W>(p, s) : launch_stream<P, 1, 4, 2, 2, 1, SG, W>(p, s);
+            narrow ? launch_stream<P, 1, 4, 1, 4, 1, SG, WIDE, W>(p, s) : launch_stream<P, 1, 4, 2, 2, 1, SG, WIDE, W>(p, s);
         }
     } else if (p.m <= 32) {
-        narrow ? launch_stream<P, 2, 4, 1, 4, 1, SG, W>(p, s) : launch_stream<P, 2, 4, 4, 1, 1, SG, W>(p, s);
+        narrow ? launch_stream<P, 2, 4, 1, 4, 1, SG, WIDE, W>(p, s) : launch_stream<P, 2, 4, 4, 1, 1, SG, WIDE, W>(p, s);
     } else {
-        narrow ? launch_stream<P, 4, 4, 1, 4, 1, SG, W>(p, s) : launch_stream<P, 4, 4, 4, 1, 1, SG, W>(p, s);
+        // with eight wavefronts, 256 registers each, four columns' worth of fragments would spill
+        narrow ? launch_stream<P, 4, 4, 1, 4, 1, SG, WIDE, W>(p, s) : launch_stream<P, 4, 4, W == 8 ? 2 : 4, W == 8 ? 2 : 1, 1, SG, WIDE, W>(p, s);
     }
 }
 
-template <int P, int WM, int WN, int SG>
+template <int P, int WM, int WN, int SG, bool WIDE>
 void launch_tiles(const GroupProductParams &p, hipStream_t s)
 {
     const int64_t row_tiles = (p.m + WM * 64 - 1) / (WM * 64), col_tiles = (p.n + WN * 64 - 1) / (WN * 64);
@@ -778,17 +749,17 @@ void launch_tiles(const GroupProductParams &p, hipStream_t s)
     IXA_REQUIRE(per_xcd * 8 * 256 <= 0xffffffffll, kErrInvalidParam, "group_product: %ld x %ld scores in one call", (long)p.m,
                 (long)p.n);
     constexpr size_t lds = 2 * ((size_t)P * WM * 64 * 256 + 2 * WN * 64 * SG * 4);
-    const auto kern = group_tile_kernel<P, WM, WN, SG>;
+    const auto kern = group_tile_kernel<P, WM, WN, SG, WIDE>;
     require_dynamic_lds(reinterpret_cast<const void *>(kern), lds);
     hipLaunchKernelGGL(kern, dim3((unsigned)per_xcd * 8), dim3(256), lds, s, p, (int)row_tiles, (int)col_tiles, (int)per_xcd);
     check_launch();
 }
 
-template <int P, int SG>
+template <int P, int SG, bool WIDE>
 void launch(GroupProductParams &p, uint8_t *workspace, hipStream_t s)
 {
     if (stays(p.type, p.m, p.d)) {
-        row_lds(p.type, p.m, p.d) <= kHalfLds ? launch_stream<P, SG, 4>(p, s) : launch_stream<P, SG, 8>(p, s);
+        row_lds(p.type, p.m, p.d) <= kHalfLds ? launch_stream<P, SG, WIDE, 4>(p, s) : launch_stream<P, SG, WIDE, 8>(p, s);
         return;
     }
     int *const exponents = reinterpret_cast<int *>(workspace);
@@ -798,9 +769,9 @@ void launch(GroupProductParams &p, uint8_t *workspace, hipStream_t s)
     p.pieces = pieces;
     p.exponents = exponents;
     if (p.m <= 64) {
-        launch_tiles<P, 1, 4, SG>(p, s);
+        launch_tiles<P, 1, 4, SG, WIDE>(p, s);
     } else {
-        launch_tiles<P, 2, 2, SG>(p, s);
+        launch_tiles<P, 2, 2, SG, WIDE>(p, s);
     }
 }
 
@@ -837,7 +808,8 @@ void op_group_product(const void *x, int64_t ld_x, int type, int64_t m, const ui
     GroupProductParams p{};
     p.x = x;
     p.codes = codes;
-    p.zeros = zeros;
+    p.has_zeros = zeros != nullptr;
+    p.zeros = zeros ? zeros : codes;     // loads without use stay in an array
     p.scales = scales;
     p.bias = bias;
     p.out = out;
@@ -860,20 +832,28 @@ void op_group_product(const void *x, int64_t ld_x, int type, int64_t m, const ui
         return;
     }
     uint8_t *const work = static_cast<uint8_t *>(workspace);
-    const auto of_group = [&](auto pieces) {
+    const auto of_group = [&](auto pieces, auto wide) {
         constexpr int P = decltype(pieces)::value;
+        constexpr bool kWide = decltype(wide)::value;
         if (group == 32) {
-            launch<P, 4>(p, work, s);
+            launch<P, 4, kWide>(p, work, s);
         } else if (group == 64) {
-            launch<P, 2>(p, work, s);
+            launch<P, 2, kWide>(p, work, s);
         } else {
-            launch<P, 1>(p, work, s);
+            launch<P, 1, kWide>(p, work, s);
+        }
+    };
+    const auto of_type = [&](auto pieces) {
+        if (scale_type == kTypeF32) {
+            of_group(pieces, std::true_type());
+        } else {
+            of_group(pieces, std::false_type());
         }
     };
     if (type == kTypeF32) {
-        of_group(std::integral_constant<int, 2>());
+        of_type(std::integral_constant<int, 2>());
     } else {
-        of_group(std::integral_constant<int, 1>());
+        of_type(std::integral_constant<int, 1>());
     }
 }
 
