@@ -74,6 +74,45 @@ __device__ __forceinline__ int over_lanes(int v, Op op)
     return v;
 }
 
+// Op over the 64 lanes of a wavefront, 32 or 64 bits; every lane has the result.
+template <int CTRL, typename V>
+__device__ __forceinline__ V value_of_lane(V v)
+{
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, lane_of<CTRL>(__builtin_bit_cast(int, v)));
+    } else {
+        const int2 w = __builtin_bit_cast(int2, v);
+        return __builtin_bit_cast(V, make_int2(lane_of<CTRL>(w.x), lane_of<CTRL>(w.y)));
+    }
+}
+template <typename V, typename Op>
+__device__ __forceinline__ V over_wave(V v, Op op)
+{
+    v = op(v, value_of_lane<kXor1>(v));
+    v = op(v, value_of_lane<kXor2>(v));
+    v = op(v, value_of_lane<kMirror8>(v));
+    v = op(v, value_of_lane<kMirror16>(v));
+    struct Box {
+        uint32_t w[sizeof(V) / 4];
+    };
+    Box a = __builtin_bit_cast(Box, v), b;
+#pragma unroll
+    for (size_t i = 0; i < sizeof(V) / 4; i++) {
+        const auto t = __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false);
+        a.w[i] = t[0];
+        b.w[i] = t[1];
+    }
+    v = op(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b));
+    a = __builtin_bit_cast(Box, v);
+#pragma unroll
+    for (size_t i = 0; i < sizeof(V) / 4; i++) {
+        const auto t = __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false);
+        a.w[i] = t[0];
+        b.w[i] = t[1];
+    }
+    return op(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b));
+}
+
 // ----- host -------------------------------------------------------------------------------------------------------------
 
 inline size_t element_bytes(int type) { return type == kTypeF32 ? 4 : 2; }
