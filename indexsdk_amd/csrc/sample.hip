@@ -31,14 +31,14 @@ constexpr int kSegments = 512;      // at most: parts of a row whose sums are ke
 constexpr int kBlock = 512;         // columns that a wavefront reads at a time
 constexpr int kTurns = 4;           // such blocks in flight
 constexpr int kSample = 2;          // blocks of each wavefront that the bound comes from
-constexpr int kFew = 128;           // entries that are drawn from without being sorted by column
+constexpr int kFew = 256;           // candidates that every wavefront holds in registers, four per lane
 constexpr int kMaxParts = 16, kPartThreads = 512;
 constexpr double kNothing = -1100.0;   // logarithms of weights that are 0 in 64 bits
 
 // What a workgroup finds out about its part of a row.
 struct PartHead {
-    uint32_t top, reference, bound, listed;
-    uint32_t fine, unused[3];
+    uint32_t top, low, reference, bound;     // low: the lowest of the columns that the bound comes from
+    uint32_t listed, fine, unused[2];
 };
 
 struct SampleParams {
@@ -82,15 +82,23 @@ __device__ __forceinline__ double power_of_two(double t)
     return __builtin_ldexp(v, (int)whole);
 }
 
-template <typename V>
-__device__ __forceinline__ V wave_scan(V v)   // inclusive
+// The lane's that CTRL names within the rows of ROWS, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double shifted(double v)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const V up = __shfl_up(v, o);
-        v += lane >= o ? up : (V)0;
-    }
+    const int2 w = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_update_dpp(0, w.x, CTRL, ROWS, 0xf, false),
+                                                __builtin_amdgcn_update_dpp(0, w.y, CTRL, ROWS, 0xf, false)));
+}
+// Running sums over the wavefront, inclusive: within 16 lanes, then the last of a row to the next, and of two to the next two.
+__device__ __forceinline__ double wave_scan(double v)
+{
+    v += shifted<0x111, 0xf>(v);
+    v += shifted<0x112, 0xf>(v);
+    v += shifted<0x114, 0xf>(v);
+    v += shifted<0x118, 0xf>(v);
+    v += shifted<0x142, 0xa>(v);
+    v += shifted<0x143, 0xc>(v);
     return v;
 }
 
@@ -100,20 +108,21 @@ struct SampleShared {
     uint64_t list[kList];           // score's key above the column's complement
     union {
         double sum[kList];          // of the list's weights; a histogram is of no more use by then
+        unsigned long long tally[kBins];
+        float mass[kBins];
+        uint32_t count[kBins];
         struct {
-            unsigned long long mass[kBins];
-            uint32_t count[kBins];
+            uint64_t sorted[kFew];
+            uint32_t rank[2][kFew];
         };
     };
-    union {
-        double segment[kSegments];
-        double few[2][kFew];        // running sums by column, and weights
-    };
-    double box[16];
+    double segment[kSegments];
+    uint16_t segment_of[kList];
+    double box[2][16];
     uint32_t tops[64];
-    uint32_t ubox[16];
+    uint32_t ubox[16], lows[16];
     uint32_t listed, found;
-    uint64_t cut, before;
+    double before;
 };
 
 // What is drawn from: columns of at least `least` (an order of score and column as in the list) with weights of at least min_p.
@@ -194,12 +203,12 @@ struct Sampler {
         v = over_wave(v, [](double a, double b) { return a + b; });
         __syncthreads();
         if (lane == 0) {
-            s.box[wave] = v;
+            s.box[0][wave] = v;
         }
         __syncthreads();
         v = 0.0;
         for (int w = 0; w < kWaves; w++) {
-            v += s.box[w];
+            v += s.box[0][w];
         }
         return v;
     }
@@ -229,13 +238,13 @@ struct Sampler {
         const double upto = wave_scan(sum);
         __syncthreads();
         if (lane == 63) {
-            s.box[wave] = upto;
+            s.box[1][wave] = upto;
         }
         __syncthreads();
         const double before_me = __shfl_up(upto, 1);
         double run = lane == 0 ? 0.0 : before_me;
         for (int w = 0; w < wave; w++) {
-            run += s.box[w];
+            run += s.box[1][w];
         }
         for (int i = from; i < min(from + per, m); i++) {
             run += a[i];
@@ -355,13 +364,15 @@ struct Sampler {
         run = before;
         at = -1;
         what = 0.0;
-        const int64_t end = min(blocks(), (g + 1) * per);
-        for (int64_t b = g * per; b < end; b++) {
-            const Eight<T> e = load(b);
+        bool done = false;
+        this->run(g * per, min(blocks(), (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
+            if (done) {
+                return;
+            }
             double v[kEight], sum = 0.0;
 #pragma unroll
             for (int i = 0; i < kEight; i++) {
-                v[i] = value((float)e.v[i], column(b, i));
+                v[i] = value(x[i], column(b, i));
                 sum += v[i];
             }
             const double upto = wave_scan(sum), before_me = __shfl_up(upto, 1);
@@ -385,192 +396,219 @@ struct Sampler {
                 const int l = __builtin_ctzll(hits);
                 at = b * kBlock + l * kEight + __shfl(hit, l);
                 what = __shfl(hit_v, l);
-                return;
-            }
-            if (lasts) {
+                done = true;
+            } else if (lasts) {
                 const int l = 63 - __builtin_clzll(lasts);
                 at = b * kBlock + l * kEight + __shfl(last, l);
                 what = __shfl(last_v, l);
             }
             run += __shfl(upto, 63);
-        }
+        });
     }
 
-    // Columns for which pick(x, key, column) go to the list; false if they are too many.
-    template <typename F>
-    __device__ bool collect(F pick) const
+    // Columns for which pick(x, key) go to the list, and the sums of `value` over the others to the segments; returns their total.
+    template <typename P, typename F>
+    __device__ double collect(int64_t per, P pick, F value) const
     {
         if (tid == 0) {
             s.listed = 0;
         }
         __syncthreads();
-        each([&](int64_t b, const float(&x)[kEight]) {
-#pragma unroll
-            for (int i = 0; i < kEight; i++) {
-                const uint32_t key = key_of(x[i]), c = column(b, i);
-                if (key && pick(x[i], key, c)) {
-                    const uint32_t at = atomicAdd(&s.listed, 1u);
-                    if (at < kList) {
-                        s.list[at] = (uint64_t)key << 32 | ~c;
-                    }
+        return segment_sums(per, [&](float x, uint32_t c) {
+            const uint32_t key = key_of(x);
+            const bool listed = key && pick(x, key);
+            if (listed) {
+                const uint32_t at = atomicAdd(&s.listed, 1u);
+                if (at < kList) {
+                    s.list[at] = (uint64_t)key << 32 | ~c;
                 }
             }
+            return listed ? 0.0 : value(x, key);
         });
-        __syncthreads();
-        return s.listed <= kList;
     }
 
-    struct Limits {
-        int64_t count;     // columns that may be kept
-        double mass;       // and the sum that they have to reach (HUGE_VAL: none)
-    };
-
-    // The place (score and column) of the last column kept under either limit, among all columns that are there; the sum of the
-    // weights up to and with it goes to `sum`.
-    __device__ uint64_t find_cut(const Row &r, Limits limit, double &sum)
+    // The first of m bins at which what has been tallied, with `before` in front of the first, reaches `goal`, or the last that holds
+    // anything; `before` becomes what is in front of it.
+    template <typename V>
+    __device__ int cross(const V *bins, int m, double goal, double &before)
     {
-        // bins of equal width in the scores, down to weights of 2^-64 for sums, and to the lowest score for counts
-        float range = (float)(64.0 / r.scale);
-        if (limit.mass == __builtin_huge_val()) {
-            float lowest = __builtin_inff();
-            each([&](int64_t, const float(&x)[kEight]) {
-#pragma unroll
-                for (int i = 0; i < kEight; i++) {
-                    lowest = key_of(x[i]) ? fminf(lowest, x[i]) : lowest;
+        __syncthreads();
+        if (wave == 0) {
+            const int per = (m + 63) / 64, from = lane * per, to = min(from + per, m);
+            double sum = 0.0;
+            for (int i = from; i < to; i++) {
+                sum += (double)bins[i];
+            }
+            const double upto = before + wave_scan(sum);
+            const uint64_t over = __ballot(upto >= goal && sum > 0.0), some = __ballot(sum > 0.0);
+            const int l = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
+            if (lane == l) {
+                double run = upto - sum, found = run;
+                int at = from;
+                for (int i = from; i < to; i++) {
+                    const double v = (double)bins[i];
+                    if (v > 0.0) {
+                        at = i;
+                        found = run;
+                        if (run + v >= goal) {
+                            break;
+                        }
+                    }
+                    run += v;
                 }
-            });
-            range = r.top + score_of(block_max(key_of(-lowest)));
+                s.found = (uint32_t)at;
+                s.before = found;
+            }
         }
+        __syncthreads();
+        const int at = (int)s.found;
+        before = s.before;
+        __syncthreads();
+        return at;
+    }
+
+    // The place (score and column) of the last column kept: the count or (by_mass) the sum of weights up to it reaches `goal`.  Where
+    // `summed`, the sums of segments of what is kept, min_p apart, are in s.segment afterwards, their total in `total`.
+    __device__ uint64_t find_cut(const Row &r, float low, double goal, bool by_mass, bool &summed, double &total)
+    {
+        // Bins of equal width in the scores, for sums down to weights of 2^-64.  What is tallied there in 32 bits only says where
+        // to look.
+        const float width = r.top - low, range = by_mass ? fminf(width, (float)(64.0 / r.scale)) : width;
         const float unit = range > 0.f && range < __builtin_inff() ? (float)kBins / range : 0.f;
         auto bin_of = [&](float x) {
             const float d = (r.top - x) * unit;
             return d < (float)(kBins - 1) ? (int)d : kBins - 1;     // also where 0 meets infinity
         };
-        const double fixed = __builtin_ldexp(1.0, 62 - (64 - __builtin_clzll((unsigned long long)n)));
-        auto add = [&](int b, float x) {
-            atomicAdd(&s.count[b], 1u);
-            if (limit.mass < __builtin_huge_val()) {
-                atomicAdd(&s.mass[b], (unsigned long long)__builtin_rint(r.weight(x) * fixed));    // in any order
-            }
-        };
-        uint64_t before_count = 0, before_mass = 0;
-        // the first of m bins within a limit's reach
-        auto cross = [&](int m) {
-            __syncthreads();
-            if (wave == 0) {
-                const int per = (m + 63) / 64, from = lane * per, to = min(from + per, m);
-                uint64_t c = 0, w = 0;
-                for (int i = from; i < to; i++) {
-                    c += s.count[i];
-                    w += s.mass[i];
-                }
-                const uint64_t c_upto = before_count + wave_scan(c), w_upto = before_mass + wave_scan(w);
-                auto over = [&](uint64_t a, uint64_t b) { return a >= (uint64_t)limit.count || (double)b / fixed >= limit.mass; };
-                const uint64_t overs = __ballot(over(c_upto, w_upto) && c > 0), some = __ballot(c > 0);
-                const int l = overs ? __builtin_ctzll(overs) : some ? 63 - __builtin_clzll(some) : 0;
-                if (lane == l) {
-                    uint64_t c_run = c_upto - c, w_run = w_upto - w;
-                    int at = from;
-                    s.cut = c_run;
-                    s.before = w_run;
-                    for (int i = from; i < to; i++) {
-                        if (s.count[i]) {
-                            at = i;
-                            s.cut = c_run;
-                            s.before = w_run;
-                            if (over(c_run + s.count[i], w_run + s.mass[i])) {
-                                break;
-                            }
-                        }
-                        c_run += s.count[i];
-                        w_run += s.mass[i];
-                    }
-                    s.found = (uint32_t)at;
-                }
-            }
-            __syncthreads();
-            const int at = (int)s.found;
-            before_count = s.cut;
-            before_mass = s.before;
-            __syncthreads();
-            return at;
-        };
-        auto clear = [&]() {
-            __syncthreads();
-            for (int i = tid; i < kBins; i += NT) {
-                s.count[i] = 0;
-                s.mass[i] = 0;
-            }
-            __syncthreads();
-        };
-        clear();
+        const int64_t per = segment_size();
+        const float scale = (float)r.scale;
+        __syncthreads();
+        for (int i = tid; i < kBins; i += NT) {
+            s.count[i] = 0;      // 0 in either type
+        }
+        __syncthreads();
         each([&](int64_t, const float(&x)[kEight]) {
 #pragma unroll
             for (int i = 0; i < kEight; i++) {
                 if (key_of(x[i])) {
-                    add(bin_of(x[i]), x[i]);
+                    const int b = bin_of(x[i]);
+                    if (by_mass) {
+                        // up to a factor that all have in common, so that no sum is lost
+                        atomicAdd(&s.mass[b], x[i] == r.top ? 0x1p60f : __builtin_amdgcn_exp2f(fmaf(x[i] - r.top, scale, 60.f)));
+                    } else {
+                        atomicAdd(&s.count[b], 1u);
+                    }
                 }
             }
         });
-        const int bin = cross(kBins);
-        // a bin with too many for the list: by the bits of their keys, ten at a time
-        uint32_t prefix = 0, known = 0;
-        for (int shift = 32;;) {
-            if (collect([&](float x, uint32_t key, uint32_t) { return bin_of(x) == bin && (key & known) == prefix; }) || shift == 0) {
+        double before = 0.0;
+        int bin = by_mass ? cross(s.mass, kBins, goal * 0x1p60, before) : cross(s.count, kBins, goal, before);
+        int m, step = 0;
+        for (;;) {
+            // the bin's columns, and the sums of what lies above it
+            total = collect(per, [&](float x, uint32_t) { return bin_of(x) == bin; },
+                            [&](float x, uint32_t key) { return key && bin_of(x) < bin ? r.weight(x) : 0.0; });
+            m = (int)min(s.listed, (uint32_t)kList + 1u);
+            if (!by_mass) {
                 break;
             }
+            before = total;
+            if (m > kList) {
+                break;
+            }
+            sort(m);
+            for (int i = tid; i < m; i += NT) {
+                s.sum[i] = r.weight(score_of((uint32_t)(s.list[i] >> 32)));
+            }
+            __syncthreads();
+            scan(s.sum, m);
+            // 32 bits were wrong by a bin, which happens at its edge
+            const bool under = before >= goal && bin > 0 && step <= 0;
+            const bool over = (m == 0 || before + s.sum[m - 1] < goal) && bin < kBins - 1 && step >= 0;
+            __syncthreads();
+            if (!under && !over) {
+                break;
+            }
+            step = under ? -1 : 1;
+            bin += step;
+        }
+        if (m > kList) {
+            summed = false;
+            return find_tie(r, [&](float x) { return bin_of(x) == bin; }, before, goal, by_mass);
+        }
+        if (!by_mass) {
+            sort(m);
+            for (int i = tid; i < m; i += NT) {
+                s.sum[i] = r.weight(score_of((uint32_t)(s.list[i] >> 32)));
+            }
+            __syncthreads();
+        }
+        const double left = goal - before;
+        int take = by_mass ? reach(left, m) : left < (double)m ? (int)left : m;
+        take = min(take, m);
+        // Nothing of the bin is needed (rounding at its edge), or the bin is empty: the cut is the last place above it.
+        if (take < 1) {
+            take = min(1, m);
+        }
+        // to the segments, by each of them in the list's order
+        const uint64_t place = m > 0 ? s.list[take - 1] : 0;
+        const int64_t columns = per * kBlock;
+        for (int i = tid; i < take; i += NT) {
+            s.segment_of[i] = (uint16_t)((int64_t)(~(uint32_t)s.list[i]) / columns);
+        }
+        __syncthreads();
+        const int segments = (int)((blocks() + per - 1) / per);
+        for (int g = tid; g < segments; g += NT) {
+            double v = s.segment[g];
+            for (int i = 0; i < take; i++) {
+                const double prior = by_mass && i > 0 ? s.sum[i - 1] : 0.0, own = s.sum[i] - prior;
+                v += s.segment_of[i] == g ? own : 0.0;
+            }
+            s.segment[g] = v;
+        }
+        total = segment_total(segments);
+        summed = true;
+        return place;
+    }
+
+    // The same where a bin holds too many for the list: by the bits of their keys, ten at a time, and among equal scores by column.
+    template <typename B>
+    __device__ uint64_t find_tie(const Row &r, B in_bin, double before, double goal, bool by_mass)
+    {
+        const double fixed = by_mass ? __builtin_ldexp(1.0, 62 - (64 - __builtin_clzll((unsigned long long)n))) : 1.0;
+        double run = before * fixed;
+        uint32_t prefix = 0, known = 0;
+        const int64_t per = segment_size();
+        for (int shift = 32; shift > 0;) {
             const int bits = min(10, shift), to = shift - bits;
             const uint32_t mask = (1u << bits) - 1u;
-            clear();
+            __syncthreads();
+            for (int i = tid; i < kBins; i += NT) {
+                s.tally[i] = 0;
+            }
+            __syncthreads();
             each([&](int64_t, const float(&x)[kEight]) {
 #pragma unroll
                 for (int i = 0; i < kEight; i++) {
                     const uint32_t key = key_of(x[i]);
-                    if (key && bin_of(x[i]) == bin && (key & known) == prefix) {
-                        add(~(key >> to) & mask, x[i]);      // the largest first
+                    if (key && in_bin(x[i]) && (key & known) == prefix) {
+                        // integers: in any order; the largest scores first
+                        atomicAdd(&s.tally[~(key >> to) & mask], by_mass ? (unsigned long long)__builtin_rint(r.weight(x[i]) * fixed) : 1ull);
                     }
                 }
             });
-            prefix |= (~(uint32_t)cross(1 << bits) & mask) << to;
+            prefix |= (~(uint32_t)cross(s.tally, 1 << bits, goal * fixed, run) & mask) << to;
             known |= mask << to;
             shift = to;
         }
-        const double before = (double)before_mass / fixed;
-        if (s.listed > kList) {
-            // equal scores: as many of them as the limits allow, by their columns
-            const float x = score_of(prefix);
-            const double w = r.weight(x), ties = (double)s.listed;
-            double take = (double)(limit.count - (int64_t)before_count);
-            if (limit.mass < __builtin_huge_val()) {
-                take = fmin(take, w > 0.0 ? ceil((limit.mass - before) / w) : ties);
-            }
-            take = fmax(1.0, fmin(take, ties));
-            const int64_t per = segment_size();
-            auto tie = [&](float v, uint32_t) { return key_of(v) == prefix ? 1.0 : 0.0; };
-            segment_sums(per, tie);
-            int64_t at;
-            double one;
-            locate(per, take - 0.5, tie, at, one);
-            sum = before + take * w;
-            __syncthreads();
-            return r.place(prefix, (uint32_t)at);
-        }
-        const int m = (int)s.listed;
-        sort(m);
-        for (int i = tid; i < m; i += NT) {
-            s.sum[i] = r.weight(score_of((uint32_t)(s.list[i] >> 32)));
-        }
+        const double w = by_mass ? r.weight(score_of(prefix)) : 1.0;
+        auto tie = [&](float v, uint32_t) { return key_of(v) == prefix ? 1.0 : 0.0; };
+        const double ties = segment_sums(per, tie);
+        const double take = fmax(1.0, fmin(ties, w > 0.0 ? ceil((goal - run / fixed) / w) : ties));
+        int64_t at;
+        double one;
+        locate(per, take - 0.5, tie, at, one);
         __syncthreads();
-        scan(s.sum, m);
-        int take = (int)min((int64_t)m, limit.count - (int64_t)before_count);
-        if (limit.mass < __builtin_huge_val()) {
-            take = min(take, reach(limit.mass - before, m));
-        }
-        take = max(1, min(take, m));
-        sum = before + s.sum[take - 1];
-        const uint64_t place = s.list[take - 1];
-        __syncthreads();
-        return place;
+        return r.place(prefix, (uint32_t)at);
     }
 
     __device__ __forceinline__ int64_t segment_size() const
@@ -605,35 +643,51 @@ struct Settings {
     }
 };
 
-// A part of a row, once: its largest score, the sums of weights relative to a reference, segment by segment, and the list.
+// A part of a row, once: its largest score, the sums of weights relative to a reference (`total`, and segment by segment), and the
+// list.
 template <typename T, int NT>
-__device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Settings &set, int part, int parts)
+__device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Settings &set, int part, int parts, double &total)
 {
-    constexpr int kWaves = NT / 64;
+    constexpr int kWaves = NT / 64, kOwn = kEight * kSample;
     SampleShared &s = k.s;
     const int lane = k.lane, wave = k.wave;
     const int64_t per = k.segment_size(), all = (k.blocks() + per - 1) / per;
     const int g0 = (int)(all * part / parts), g1 = (int)(all * (part + 1) / parts);
-    const int64_t b0 = g0 * per, b1 = min(k.blocks(), g1 * per), mine = b1 - b0;
+    const int64_t b0 = g0 * per, b1 = min(k.blocks(), g1 * per), mine = b1 - b0, columns = min(k.n - b0 * kBlock, mine * kBlock);
+    const float inf = __builtin_inff();
 
-    // The largest of 64 groups of lanes in some of the columns.
+    // The largest of 64 groups of lanes in some of the columns: sixteen per lane, or all there are.
     constexpr int kLanes = kWaves;
-    const int64_t first = b0 + mine * wave / kWaves, end = b0 + mine * (wave + 1) / kWaves;
-    float lane_top = -__builtin_inff();
+    float lane_top = -inf, lane_low = inf;
+    auto see = [&](float x) {
+        lane_top = fmaxf(lane_top, x);
+        lane_low = x > -inf ? fminf(lane_low, x) : lane_low;
+    };
+    if (columns > NT * kOwn) {
+        const int64_t first = b0 + mine * wave / kWaves;
 #pragma unroll
-    for (int u = 0; u < kSample; u++) {
-        if (first + u < end) {
+        for (int u = 0; u < kSample; u++) {
             const Eight<T> e = k.load(first + u);
 #pragma unroll
             for (int i = 0; i < kEight; i++) {
-                lane_top = fmaxf(lane_top, (float)e.v[i]);
+                see((float)e.v[i]);
             }
+        }
+    } else if (columns > 0) {
+        const int each = (int)((columns + NT - 1) / NT);
+#pragma unroll
+        for (int i = 0; i < kOwn; i++) {
+            see((float)k.row[b0 * kBlock + min((int64_t)k.tid * each + min(i, each - 1), columns - 1)]);
         }
     }
     const int flip = (int)0x80000000;
     const int group_top = over_lanes<kLanes>((int)key_of(lane_top) ^ flip, [](int a, int b) { return max(a, b); });
     if (lane % kLanes == 0) {
         s.tops[wave * (64 / kLanes) + lane / kLanes] = (uint32_t)(group_top ^ flip);
+    }
+    if (k.tid < kFew) {
+        s.rank[0][k.tid] = 0;
+        s.rank[1][k.tid] = 0;
     }
     if (k.tid == 0) {
         s.listed = 0;
@@ -644,20 +698,19 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
     const float reference = score_of(sample_top);
     // A bound that so many of the sampled columns reach that all of them have what is kept, but for one time in thousands: as
     // many more than expected as three deviations.
-    PartHead h{0, sample_top, 0xffffffffu, 0, 1, {}};
-    const int64_t columns = min(k.n - b0 * kBlock, mine * kBlock);
-    if (set.filtered && sample_top && columns > 0) {
-        const float share = (float)min(columns, (int64_t)NT * kEight * kSample) / (float)columns;
-        // what is wanted of all parts: k, or for sums a few hundred
-        const float wanted = (set.by_count ? (float)min(set.count, (int64_t)kList) : 256.f) / (float)parts * share;
-        const float reach = wanted + 3.f * __builtin_amdgcn_sqrtf(wanted) + 4.f;
-        if (columns <= 4 * kFew) {
+    PartHead h{0, 0, sample_top, 0xffffffffu, 0, 1, {}};
+    if (set.filtered && sample_top) {
+        const float share = columns > NT * kOwn ? (float)(NT * kOwn) / (float)columns : 1.f;
+        // what is wanted of all parts: k, or for sums a hundred and more
+        const float wanted = (set.by_count ? (float)min(set.count, (int64_t)kList) : 128.f) / (float)parts * share;
+        const float reach = share < 1.f ? wanted + 3.f * __builtin_amdgcn_sqrtf(wanted) + 4.f : wanted;
+        if (columns <= kFew) {
             h.bound = 1;      // everything that is there
-        } else if (reach <= 130.f || !set.by_count) {
+        } else if (reach <= 130.f) {
             // of 64 groups those that hold one of `reach` columns at least
-            const int groups = (int)fminf(56.f, 64.f * (1.f - __expf(-reach / 64.f)) + 0.5f);
+            const int groups = (int)fminf(60.f, 64.f * (1.f - __expf(-reach / 64.f)) + 1.5f);
             uint32_t b = 0;
-#pragma unroll
+#pragma unroll 1
             for (int bit = 31; bit >= 16; bit--) {
                 const uint32_t at = b | 1u << bit;
                 b = __popcll(__ballot(tops >= at)) >= groups ? at : b;
@@ -667,8 +720,9 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
     }
     const float bound = h.bound == 0xffffffffu ? __builtin_nanf("") : h.bound == 1 ? -3.402823466e+38f : score_of(h.bound);
     const bool sums = set.need_mass;
-    float top = -__builtin_inff();
-    const int limit = parts > 1 ? kPartList : kList;
+    const uint32_t limit = parts > 1 ? kPartList : kList;
+    float top = -inf;
+    double sum = 0.0;
     for (int g = g0 + wave; g < g1; g += kWaves) {
         double v = 0.0;
         k.run(g * per, min(b1, (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
@@ -689,7 +743,7 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
                 for (int i = 0; i < kEight; i++) {
                     if (x[i] >= bound) {
                         const uint32_t at = atomicAdd(&s.listed, 1u);
-                        if (at < (uint32_t)limit) {
+                        if (at < limit) {
                             s.list[at] = (uint64_t)key_of(x[i]) << 32 | ~k.column(b, i);
                         }
                     }
@@ -698,17 +752,159 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
         });
         if (sums) {
             v = over_wave(v, [](double a, double b) { return a + b; });
+            sum += v;
             if (lane == 0) {
                 s.segment[g] = v;
             }
         }
     }
-    h.top = k.block_max(key_of(top));
+    const uint32_t wave_top = over_wave(key_of(top), [](uint32_t a, uint32_t b) { return max(a, b); });
+    const uint32_t wave_low = over_wave(key_of(-lane_low), [](uint32_t a, uint32_t b) { return max(a, b); });
+    if (lane == 0) {
+        s.box[0][wave] = sum;
+        s.ubox[wave] = wave_top;
+        s.lows[wave] = wave_low;
+    }
+    __syncthreads();
+    total = 0.0;
+#pragma unroll 4
+    for (int w = 0; w < kWaves; w++) {
+        total += s.box[0][w];
+        h.top = max(h.top, s.ubox[w]);
+        h.low = max(h.low, s.lows[w]);
+    }
     h.listed = h.bound == 0xffffffffu ? 0xffffffffu : s.listed;
     return h;
 }
 
-// The draws from a row whose list and sums are in LDS.
+// The draws from a row whose candidates, at most kFew, are in the list, if these hold all that is kept: they are put in the order of
+// their scores and, those that are kept, in that of their columns, by how many come before each; cuts and draws are ballots over what
+// every wavefront holds in registers.
+template <typename T, int NT, typename U>
+__device__ __forceinline__ bool finish_few(const Sampler<T, NT> &k, const SampleParams &p, const Settings &set, const Row &r, int m,
+                                           bool complete, double total, int64_t *labels, float *probs, U draw_number)
+{
+    constexpr int kWaves = NT / 64, kParts = NT / kFew, kOf = kFew / 64;
+    SampleShared &s = k.s;
+    const int tid = k.tid, lane = k.lane, wave = k.wave, own = tid % kFew, part = tid / kFew;
+    auto count_before = [&](const uint64_t *of, int size, uint32_t *rank, auto before) {
+        if (own < size) {
+            const uint64_t mine = of[own];
+            int c = 0;
+#pragma unroll 4
+            for (int i = part; i < size; i += kParts) {
+                c += before(of[i], mine) ? 1 : 0;
+            }
+            if (kParts > 1) {
+                atomicAdd(&rank[own], (uint32_t)c);
+            } else {
+                rank[own] = (uint32_t)c;
+            }
+        }
+        __syncthreads();
+    };
+    count_before(s.list, m, s.rank[0], [](uint64_t a, uint64_t b) { return a > b; });
+    if (tid < m) {
+        s.sorted[s.rank[0][tid]] = s.list[tid];
+    }
+    __syncthreads();
+    double w[kOf], upto[kOf], run = 0.0;
+#pragma unroll
+    for (int c = 0; c < kOf; c++) {
+        const int e = c * 64 + lane;
+        w[c] = upto[c] = 0.0;
+        if (c * 64 < m) {
+            w[c] = e < m ? r.weight(score_of((uint32_t)(s.sorted[e] >> 32))) : 0.0;
+            upto[c] = run + wave_scan(w[c]);
+            run = __shfl(upto[c], 63);
+        }
+    }
+    auto how_many = [&](int size, auto is) {
+        int count = 0;
+#pragma unroll
+        for (int c = 0; c < kOf; c++) {
+            count += __popcll(__ballot(c * 64 + lane < size && is(c)));
+        }
+        return count;
+    };
+    auto sum_upto = [&](int size) {     // of the first `size` entries
+        double v = 0.0;
+#pragma unroll
+        for (int c = 0; c < kOf; c++) {
+            v = (size - 1) / 64 == c ? __shfl(upto[c], (size - 1) % 64) : v;
+        }
+        return v;
+    };
+    bool cut = complete;               // whether the list holds all that is kept
+    int take = m;
+    if (set.by_count) {
+        cut = cut || m >= set.count;
+        take = (int)min((int64_t)m, set.count);
+    }
+    if (set.by_mass && (cut || !set.by_count)) {
+        // of the sum of all that is left, which the list has or the whole row
+        const double goal = set.top_p * (cut ? sum_upto(take) : total);
+        const int need = how_many(take, [&](int c) { return upto[c] < goal; }) + 1;
+        cut = cut || need <= take;
+        take = min(take, need);
+    }
+    if (set.min_p > 0.0 && !(set.by_count && !cut)) {
+        const int above = how_many(m, [&](int c) { return w[c] >= set.min_p; });
+        cut = cut || above < m;
+        take = min(take, above);
+    }
+    if (!cut) {
+        return false;
+    }
+    take = max(take, 1);
+    const double all = sum_upto(take);
+    count_before(s.sorted, take, s.rank[1], [](uint64_t a, uint64_t b) { return (uint32_t)a > (uint32_t)b; });
+    if (tid < take) {
+        double mine = w[0];
+#pragma unroll
+        for (int c = 1; c < kOf; c++) {
+            mine = wave == c ? w[c] : mine;
+        }
+        s.list[s.rank[1][tid]] = s.sorted[tid];
+        s.segment[s.rank[1][tid]] = mine;
+    }
+    __syncthreads();
+    run = 0.0;
+#pragma unroll
+    for (int c = 0; c < kOf; c++) {
+        const int e = c * 64 + lane;
+        w[c] = upto[c] = 0.0;
+        if (c * 64 < take) {
+            w[c] = e < take ? s.segment[e] : 0.0;
+            upto[c] = run + wave_scan(w[c]);
+            run = __shfl(upto[c], 63);
+        }
+    }
+    for (int d = wave; d < p.draws; d += kWaves) {
+        const double target = draw_number(d) * all;
+        int at = 0;       // the first that passes it, or the last with a weight if rounding hides that
+#pragma unroll
+        for (int c = kOf - 1; c >= 0; c--) {
+            const uint64_t some = __ballot(w[c] > 0.0);
+            at = at == 0 && some ? c * 64 + 63 - __builtin_clzll(some) : at;
+        }
+#pragma unroll
+        for (int c = kOf - 1; c >= 0; c--) {
+            const uint64_t passes = __ballot(w[c] > 0.0 && upto[c] > target);
+            at = passes ? c * 64 + __builtin_ctzll(passes) : at;
+        }
+        if (lane == 0) {
+            labels[d] = (int64_t)(~(uint32_t)s.list[at]);
+            if (probs) {
+                probs[d] = (float)(s.segment[at] / all);
+            }
+        }
+    }
+    return true;
+}
+
+// The draws from a row whose list and sums are in LDS; `total`: of the row's weights relative to its largest score, or without filters
+// to the reference.
 template <typename T, int NT>
 __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams &p, const Settings &set, int64_t row,
                                            const PartHead &h, double total)
@@ -729,7 +925,7 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
         return;
     }
     const int64_t per = k.segment_size(), count = set.count;
-    Row r{set.scale, score_of(h.top), set.min_p, 0};
+    Row r{set.scale, score_of(set.filtered || !h.fine ? h.top : h.reference), set.min_p, 0};
     if (set.need_mass && !h.fine) {
         total = k.segment_sums(per, [&](float x, uint32_t) { return key_of(x) ? r.weight(x) : 0.0; });
     }
@@ -739,21 +935,25 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
     };
     if (set.filtered) {
         const bool complete = h.bound == 1;      // every column that is there is in the list
-        int m = h.listed <= kList ? (int)h.listed : 0, take = m;
-        if (m > 0) {
+        const int m = h.listed <= kList ? (int)h.listed : 0;
+        if (m > 0 && m <= kFew) {
+            if (finish_few(k, p, set, r, m, complete, total, labels, probs, draw_number)) {
+                return;
+            }
+        } else if (m > 0) {
+            int take = m;
             k.sort(m);
             for (int i = tid; i < m; i += NT) {
                 s.sum[i] = r.weight(score_of((uint32_t)(s.list[i] >> 32)));
             }
             __syncthreads();
             k.scan(s.sum, m);
-            bool cut = complete;               // whether the list holds all that is kept
+            bool cut = complete;
             if (set.by_count) {
                 cut = cut || m >= count;
                 take = (int)min((int64_t)m, count);
             }
             if (set.by_mass && (cut || !set.by_count)) {
-                // of the sum of all that is left, which the list has or the whole row
                 const int need = k.reach(set.top_p * (cut ? s.sum[take - 1] : total), take);
                 cut = cut || need <= take;
                 take = min(take, need);
@@ -772,47 +972,7 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
                 take = min(take, above);
             }
             take = max(take, 1);
-            const double all = s.sum[take - 1];
             __syncthreads();
-            if (cut && take <= kFew) {
-                // each entry's running sum by column, from all others in the order of the list
-                if (tid < take) {
-                    s.few[1][tid] = r.weight(score_of((uint32_t)(s.list[tid] >> 32)));
-                }
-                __syncthreads();
-                if (tid < take) {
-                    const uint32_t mine = (uint32_t)s.list[tid];       // the complement of the column
-                    double v = 0.0;
-                    for (int i = 0; i < take; i++) {
-                        v += (uint32_t)s.list[i] >= mine ? s.few[1][i] : 0.0;
-                    }
-                    s.few[0][tid] = v;
-                }
-                __syncthreads();
-                for (int d = wave; d < p.draws; d += kWaves) {
-                    const double target = draw_number(d) * all;
-                    // the lowest column that passes it, or the last with a weight if rounding hides that
-                    uint64_t best = 0;
-#pragma unroll
-                    for (int c = 0; c < kFew / 64; c++) {
-                        const int i = c * 64 + lane;
-                        if (i < take && s.few[1][i] > 0.0) {
-                            const uint32_t place = (uint32_t)s.list[i];
-                            best = larger(best, s.few[0][i] > target ? 1ull << 63 | (uint64_t)place << 8 | (uint64_t)i
-                                                                     : (uint64_t)(uint32_t)~place << 8 | (uint64_t)i);
-                        }
-                    }
-                    best = over_wave(best, larger);
-                    if (lane == 0) {
-                        const int i = (int)(best & 127u);
-                        labels[d] = (int64_t)(~(uint32_t)s.list[i]);
-                        if (probs) {
-                            probs[d] = (float)(s.few[1][i] / all);
-                        }
-                    }
-                }
-                return;
-            }
             if (cut) {
                 // by columns: the complement falls as they rise
                 for (int i = tid; i < take; i += NT) {
@@ -848,19 +1008,27 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
         }
         __syncthreads();
         // the row again
+        const float low = -score_of(h.low);
         double sum = total;
+        bool summed = false;
         if (set.by_count) {
-            r.least = k.find_cut(r, {count, __builtin_huge_val()}, sum);
-            if (set.by_mass) {
+            r.least = k.find_cut(r, low, (double)count, false, summed, sum);
+            if (set.by_mass && !summed) {
                 // the sum up to the cut by its columns
-                auto value = [&](float x, uint32_t c) { return key_of(x) && r.place(key_of(x), c) >= r.least ? r.weight(x) : 0.0; };
-                sum = k.segment_sums(per, value);
+                sum = k.segment_sums(per, [&](float x, uint32_t c) { return key_of(x) && r.place(key_of(x), c) >= r.least ? r.weight(x) : 0.0; });
             }
         }
         if (set.by_mass) {
-            r.least = larger(r.least, k.find_cut(r, {k.n + 1, set.top_p * sum}, sum));
+            const uint64_t least = k.find_cut(r, low, set.top_p * sum, true, summed, sum);
+            summed = summed && least >= r.least;
+            r.least = larger(r.least, least);
         }
-        total = k.segment_sums(per, [&](float x, uint32_t c) { return r.kept(x, c); });
+        // where min_p cuts more than the others the sums are not those of what is kept
+        if (summed && (set.min_p == 0.0 || (r.least >> 32 && r.weight(score_of((uint32_t)(r.least >> 32))) >= set.min_p))) {
+            total = sum;
+        } else {
+            total = k.segment_sums(per, [&](float x, uint32_t c) { return r.kept(x, c); });
+        }
     }
     // by the sums of segments
     auto value = [&](float x, uint32_t c) { return r.kept(x, c); };
@@ -892,41 +1060,33 @@ __device__ __forceinline__ double unit_of(float reference, float top, double sca
 }
 
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void sample_kernel(SampleParams p)
+__global__ __launch_bounds__(NT, NT == 256 ? 3 : 4) void sample_kernel(SampleParams p)
 {
     __shared__ SampleShared s;
     const int64_t row = blockIdx.x;
     Sampler<T, NT> k = sampler<T, NT>(s, p, row);
     const Settings set(p, row);
-    PartHead h = scan_part(k, set, 0, 1);
-    double total = 0.0;
-    if (set.need_mass && h.top && h.fine) {
-        const int64_t per = k.segment_size();
-        const int segments = (int)((k.blocks() + per - 1) / per);
-        const double unit = unit_of(score_of(h.reference), score_of(h.top), set.scale);
-        total = k.segment_total(segments);
-        h.fine = total < 0x1p1000 && unit > 0.0;
+    double total;
+    PartHead h = scan_part(k, set, 0, 1, total);
+    if (set.need_mass) {
+        const double unit = set.filtered ? unit_of(score_of(h.reference), score_of(h.top), set.scale) : 1.0;
+        h.fine = total > 0.0 && total < 0x1p1000 && unit > 0.0;
         total *= unit;
-        if (!set.filtered) {
-            for (int g = k.tid; g < segments; g += NT) {
-                s.segment[g] *= unit;
-            }
-            __syncthreads();
-        }
     }
     finish_row(k, p, set, row, h, total);
 }
 
 // A part of a row per workgroup, and what it found out.
 template <typename T>
-__global__ __launch_bounds__(kPartThreads) void sample_part_kernel(SampleParams p)
+__global__ __launch_bounds__(kPartThreads, 4) void sample_part_kernel(SampleParams p)
 {
     __shared__ SampleShared s;
     const int64_t row = blockIdx.x / p.parts;
     const int part = (int)(blockIdx.x - row * p.parts);
     const Sampler<T, kPartThreads> k = sampler<T, kPartThreads>(s, p, row);
     const Settings set(p, row);
-    const PartHead h = scan_part(k, set, part, p.parts);
+    double total;
+    const PartHead h = scan_part(k, set, part, p.parts, total);
     if (k.tid == 0) {
         p.heads[blockIdx.x] = h;
     }
@@ -935,7 +1095,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_part_kernel(SampleParams 
             p.lists[(int64_t)blockIdx.x * kPartList + i] = s.list[i];
         }
     }
-    if (set.need_mass && h.fine) {
+    if (set.need_mass) {
         const int64_t per = k.segment_size(), all = (k.blocks() + per - 1) / per;
         for (int g = (int)(all * part / p.parts) + k.tid; g < (int)(all * (part + 1) / p.parts); g += kPartThreads) {
             p.segments[row * kSegments + g] = s.segment[g];
@@ -945,24 +1105,29 @@ __global__ __launch_bounds__(kPartThreads) void sample_part_kernel(SampleParams 
 
 // The parts of a row, joined: the highest of their bounds is one that all lists go down to.
 template <typename T>
-__global__ __launch_bounds__(kPartThreads) void sample_join_kernel(SampleParams p)
+__global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SampleParams p)
 {
     __shared__ SampleShared s;
     const int64_t row = blockIdx.x;
     Sampler<T, kPartThreads> k = sampler<T, kPartThreads>(s, p, row);
     const Settings set(p, row);
-    PartHead all{0, 0, 0, 0, 1, {}};
+    PartHead all{0, 0, 0, 0, 0, 1, {}};
     bool listed = true;
     for (int i = 0; i < p.parts; i++) {
         const PartHead h = p.heads[row * p.parts + i];
         if (h.top) {
             all.top = max(all.top, h.top);
+            all.low = max(all.low, h.low);
             all.bound = max(all.bound, h.bound);
             listed = listed && h.listed <= kPartList;
-            all.fine &= h.fine;
         }
     }
     all.bound = max(all.bound, 1u);
+    all.reference = all.top;
+    if (k.tid < kFew) {
+        s.rank[0][k.tid] = 0;
+        s.rank[1][k.tid] = 0;
+    }
     if (k.tid == 0) {
         s.listed = 0;
     }
@@ -982,21 +1147,21 @@ __global__ __launch_bounds__(kPartThreads) void sample_join_kernel(SampleParams 
                 }
             }
         }
-        if (set.need_mass && all.fine) {
-            const double unit = h.top ? unit_of(score_of(h.reference), top, set.scale) : 0.0;
+        if (set.need_mass) {
+            const double unit = h.top ? unit_of(score_of(h.reference), top, set.scale) : 1.0;
             for (int g = (int)(segments * i / p.parts) + k.tid; g < (int)(segments * (i + 1) / p.parts); g += kPartThreads) {
                 const double v = h.top ? p.segments[row * kSegments + g] : 0.0;
                 // what does not come out as a sum is found out again
-                s.segment[g] = h.top && !(unit > 0.0) ? __builtin_nan("") : v * unit;
+                s.segment[g] = unit > 0.0 ? v * unit : __builtin_nan("");
             }
         }
     }
     __syncthreads();
     all.listed = listed ? s.listed : 0xffffffffu;
     double total = 0.0;
-    if (set.need_mass && all.top && all.fine) {
+    if (set.need_mass && all.top) {
         total = k.segment_total((int)segments);
-        all.fine = total < 0x1p1000;      // also not of what is no number
+        all.fine = total > 0.0 && total < 0x1p1000;      // also not of what is no number
     }
     finish_row(k, p, set, row, all, total);
 }
