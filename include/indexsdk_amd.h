@@ -241,7 +241,7 @@ int ixa_op_group_product(const void *x_dev, int64_t ld_x, int type, int64_t m, c
  * With weights w = exp((score - best) / T), the columns in the order of falling scores, equal ones in that of columns, are cut to
  * the first k, then to the fewest whose weights reach p of the sum of those that are left, then to those with w >= m.  The
  * draw's label is the first column, in the order of columns, at which the running sum of the weights that are left passes
- * uniform * their total; its probability w / total goes to probs [rows][draws] (may be NULL).  Weights and sums are held in 64 bits.  Beside a
+ * uniform * their total; its probability w / total goes to probs [rows][draws] (may be NULL).  Weights and sums are held in 64 bits; weights below 2^-960 count as 0.  Beside a
  * score of +infinity only such columns count.  A row without a column: label -1, probability 0.
  * rows <= 2^22, n < 2^31, draws <= 2^20. */
 int ixa_sample_workspace(int64_t rows, int64_t n, int64_t *bytes);

@@ -6,8 +6,8 @@
 //   left passes u times their total
 // Scores of -infinity and NaN are columns that are not there; beside +infinity everything else is.
 //
-// Every decision is one about sums of weights next to a border, so weights and sums are held in 64 bits: an exponential is 17
-// instructions of the same rate as in 32.
+// Weights below 2^-960 count as 0.  Every decision is one about sums of weights next to a border, so weights and sums are held in 64
+// bits: an exponential is 13 instructions of the same rate as in 32.
 //
 // One workgroup per row reads it once (a few, each a part, where there are few rows).  The largest scores of some of its columns
 // give a bound that about a hundred scores of the row reach; these go to a list in LDS, and while k or p or m keep no more than what
@@ -32,8 +32,9 @@ constexpr int kBlock = 512;         // columns that a wavefront reads at a time
 constexpr int kTurns = 4;           // such blocks in flight
 constexpr int kSample = 2;          // blocks of each wavefront that the bound comes from
 constexpr int kFew = 256;           // candidates that every wavefront holds in registers, four per lane
+constexpr int kOneWave = 32;        // draws up to which one wavefront makes them all
 constexpr int kMaxParts = 16, kPartThreads = 512;
-constexpr double kNothing = -1100.0;   // logarithms of weights that are 0 in 64 bits
+constexpr double kNothing = -960.0;    // logarithms of weights that count as 0; in sums over whole rows as 2^-960
 
 // What a workgroup finds out about its part of a row.
 struct PartHead {
@@ -63,23 +64,25 @@ __device__ __forceinline__ uint32_t key_of(float x)
 }
 __device__ __forceinline__ float score_of(uint32_t k) { return __uint_as_float((int)k < 0 ? k & 0x7fffffffu : ~k); }
 
-// 2^t for t <= 0 (and a little above): the polynomial of exp to the eleventh power, 6e-15
+// 2^t for t in [-1022, 1000]: the nearest integer by adding 1.5 * 2^52, whose low bits then are the exponent, and the polynomial of
+// degree 9 through 2^r at Chebyshev's points of [-1/2, 1/2], its constant set to 1 (2^0 is 1): 3.2e-14 of the value at most.
 __device__ __forceinline__ double power_of_two(double t)
 {
-    const double whole = __builtin_rint(t), r = (t - whole) * 0.693147180559945309417232;
-    double v = 1.0 / 39916800;
-    v = fma(v, r, 1.0 / 3628800);
-    v = fma(v, r, 1.0 / 362880);
-    v = fma(v, r, 1.0 / 40320);
-    v = fma(v, r, 1.0 / 5040);
-    v = fma(v, r, 1.0 / 720);
-    v = fma(v, r, 1.0 / 120);
-    v = fma(v, r, 1.0 / 24);
-    v = fma(v, r, 1.0 / 6);
-    v = fma(v, r, 0.5);
+    constexpr double kRound = 6755399441055744.0;
+    const double u = t + kRound, r = t - (u - kRound);
+    double v = 1.0205905413765595e-07;
+    v = fma(v, r, 1.325964524488711e-06);
+    v = fma(v, r, 1.5252672924850737e-05);
+    v = fma(v, r, 0.0001540343375125101);
+    v = fma(v, r, 0.0013333558200794592);
+    v = fma(v, r, 0.009618129193934313);
+    v = fma(v, r, 0.05550410866465167);
+    v = fma(v, r, 0.2402265069564034);
+    v = fma(v, r, 0.6931471805599462);
     v = fma(v, r, 1.0);
-    v = fma(v, r, 1.0);
-    return __builtin_ldexp(v, (int)whole);
+    int2 bits = __builtin_bit_cast(int2, v);
+    bits.y += __builtin_bit_cast(int2, u).x << 20;
+    return __builtin_bit_cast(double, bits);
 }
 
 // The lane's that CTRL names within the rows of ROWS, 0 where there is none.
@@ -113,7 +116,7 @@ struct SampleShared {
         uint32_t count[kBins];
         struct {
             uint64_t sorted[kFew];
-            uint32_t rank[2][kFew];
+            uint32_t rank[kFew];
         };
     };
     double segment[kSegments];
@@ -125,6 +128,9 @@ struct SampleShared {
     double before;
 };
 
+// The workgroup's; by this name everywhere, so that the compiler sees LDS in every access.
+__shared__ SampleShared lds;
+
 // What is drawn from: columns of at least `least` (an order of score and column as in the list) with weights of at least min_p.
 struct Row {
     double scale;      // log2(e) / T
@@ -134,7 +140,7 @@ struct Row {
     __device__ __forceinline__ double weight(float x) const
     {
         const double t = ((double)x - (double)top) * scale;
-        return x == top ? 1.0 : t > kNothing ? power_of_two(t) : 0.0;
+        return x == top ? 1.0 : t > kNothing ? power_of_two(fmin(t, 1000.0)) : 0.0;
     }
     __device__ __forceinline__ uint64_t place(uint32_t key, uint32_t column) const { return (uint64_t)key << 32 | ~column; }
     // of a column: 0 where it is cut off
@@ -152,7 +158,6 @@ struct Row {
 template <typename T, int NT>
 struct Sampler {
     static constexpr int kWaves = NT / 64;
-    SampleShared &s;
     const T *row;
     const int64_t n;
     const int tid, lane, wave;
@@ -168,18 +173,18 @@ struct Sampler {
     __device__ __forceinline__ int64_t blocks() const { return (n + kBlock - 1) / kBlock; }
     __device__ __forceinline__ uint32_t column(int64_t block, int i) const { return (uint32_t)(block * kBlock + lane * kEight + i); }
 
-    // f(block, scores) over blocks from ... to - 1, kTurns of them in flight
-    template <typename F>
+    // f(block, scores) over blocks from ... to - 1, TURNS of them in flight
+    template <int TURNS, typename F>
     __device__ __forceinline__ void run(int64_t from, int64_t to, F f) const
     {
-        for (int64_t b = from; b < to; b += kTurns) {
-            Eight<T> e[kTurns];
+        for (int64_t b = from; b < to; b += TURNS) {
+            Eight<T> e[TURNS];
 #pragma unroll
-            for (int u = 0; u < kTurns; u++) {
+            for (int u = 0; u < TURNS; u++) {
                 e[u] = load(min(b + u, to - 1));
             }
 #pragma unroll
-            for (int u = 0; u < kTurns; u++) {
+            for (int u = 0; u < TURNS; u++) {
                 if (u == 0 || b + u < to) {
                     float x[kEight];
 #pragma unroll
@@ -195,7 +200,7 @@ struct Sampler {
     template <typename F>
     __device__ __forceinline__ void each(F f) const
     {
-        run(blocks() * wave / kWaves, blocks() * (wave + 1) / kWaves, f);
+        run<2>(blocks() * wave / kWaves, blocks() * (wave + 1) / kWaves, f);
     }
 
     __device__ __forceinline__ double block_sum(double v) const
@@ -203,12 +208,12 @@ struct Sampler {
         v = over_wave(v, [](double a, double b) { return a + b; });
         __syncthreads();
         if (lane == 0) {
-            s.box[0][wave] = v;
+            lds.box[0][wave] = v;
         }
         __syncthreads();
         v = 0.0;
         for (int w = 0; w < kWaves; w++) {
-            v += s.box[0][w];
+            v += lds.box[0][w];
         }
         return v;
     }
@@ -217,18 +222,18 @@ struct Sampler {
         v = over_wave(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
         __syncthreads();
         if (lane == 0) {
-            s.ubox[wave] = v;
+            lds.ubox[wave] = v;
         }
         __syncthreads();
         v = 0;
         for (int w = 0; w < kWaves; w++) {
-            v = max(v, s.ubox[w]);
+            v = max(v, lds.ubox[w]);
         }
         return v;
     }
 
     // Running sums (inclusive) of a[0 ... m), in place.
-    __device__ void scan(double *a, int m) const
+    __device__ __forceinline__ void scan(double *a, int m) const
     {
         const int per = (m + NT - 1) / NT, from = tid * per;
         double sum = 0.0;
@@ -238,13 +243,13 @@ struct Sampler {
         const double upto = wave_scan(sum);
         __syncthreads();
         if (lane == 63) {
-            s.box[1][wave] = upto;
+            lds.box[1][wave] = upto;
         }
         __syncthreads();
         const double before_me = __shfl_up(upto, 1);
         double run = lane == 0 ? 0.0 : before_me;
         for (int w = 0; w < wave; w++) {
-            run += s.box[1][w];
+            run += lds.box[1][w];
         }
         for (int i = from; i < min(from + per, m); i++) {
             run += a[i];
@@ -254,14 +259,14 @@ struct Sampler {
     }
 
     // list[0 ... m) in falling order (m <= kList)
-    __device__ void sort(int m) const
+    __device__ __forceinline__ void sort(int m) const
     {
         int size = 2;
         while (size < m) {
             size <<= 1;
         }
         for (int i = m + tid; i < size; i += NT) {
-            s.list[i] = 0;
+            lds.list[i] = 0;
         }
         // Exchanges over up to 64 entries stay among the 128 that one wavefront has, whose accesses to LDS happen in their order.
         __syncthreads();
@@ -269,10 +274,10 @@ struct Sampler {
             for (int j = k >> 1; j > 0; j >>= 1) {
                 for (int t = tid; t < size / 2; t += NT) {
                     const int a = (t & ~(j - 1)) * 2 + (t & (j - 1)), b = a + j;
-                    const uint64_t x = s.list[a], y = s.list[b];
+                    const uint64_t x = lds.list[a], y = lds.list[b];
                     if ((x < y) == ((a & k) == 0)) {
-                        s.list[a] = y;
-                        s.list[b] = x;
+                        lds.list[a] = y;
+                        lds.list[b] = x;
                     }
                 }
                 if (j >= 128 || (j == 1 && k >= 128)) {
@@ -293,7 +298,7 @@ struct Sampler {
         int lo = 0, hi = m;    // the first that is not less
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (s.sum[mid] < target) {
+            if (lds.sum[mid] < target) {
                 lo = mid + 1;
             } else {
                 hi = mid;
@@ -304,12 +309,12 @@ struct Sampler {
 
     // sums of `value(x, column)` over segments of `per` blocks
     template <typename F>
-    __device__ double segment_sums(int64_t per, F value) const
+    __device__ __forceinline__ double segment_sums(int64_t per, F value) const
     {
         const int segments = (int)((blocks() + per - 1) / per);
         for (int g = wave; g < segments; g += kWaves) {
             double v = 0.0;
-            run(g * per, min(blocks(), (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
+            run<2>(g * per, min(blocks(), (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
 #pragma unroll
                 for (int i = 0; i < kEight; i++) {
                     v += value(x[i], column(b, i));
@@ -317,24 +322,24 @@ struct Sampler {
             });
             v = over_wave(v, [](double a, double b) { return a + b; });
             if (lane == 0) {
-                s.segment[g] = v;
+                lds.segment[g] = v;
             }
         }
         return segment_total(segments);
     }
-    __device__ double segment_total(int segments) const
+    __device__ __forceinline__ double segment_total(int segments) const
     {
         __syncthreads();
         double v = 0.0;
         for (int g = tid; g < segments; g += NT) {
-            v += s.segment[g];
+            v += lds.segment[g];
         }
         return block_sum(v);
     }
     // A wavefront's search: the first column at which the running sum of `value` passes `target`, and its value; the last one with
     // a value if rounding hides it.
     template <typename F>
-    __device__ void locate(int64_t per, double target, F value, int64_t &at, double &what) const
+    __device__ __forceinline__ void locate(int64_t per, double target, F value, int64_t &at, double &what) const
     {
         const int segments = (int)((blocks() + per - 1) / per);
         double before = 0.0;
@@ -342,7 +347,7 @@ struct Sampler {
         double sum = 0.0, run = 0.0;
         const int each_lane = (segments + 63) / 64, from = lane * each_lane, to = min(from + each_lane, segments);
         for (int i = from; i < to; i++) {
-            sum += s.segment[i];
+            sum += lds.segment[i];
         }
         const double upto_lane = wave_scan(sum);
         const uint64_t passes = __ballot(upto_lane > target && sum > 0.0), some = __ballot(sum > 0.0);
@@ -351,7 +356,7 @@ struct Sampler {
         run = l == 0 ? 0.0 : __shfl(before_lane, l);
         int g = l * each_lane;
         for (int i = g; i < min((l + 1) * each_lane, segments); i++) {      // the same in every lane
-            const double v = s.segment[i];
+            const double v = lds.segment[i];
             if (v > 0.0) {
                 g = i;
                 before = run;
@@ -365,62 +370,66 @@ struct Sampler {
         at = -1;
         what = 0.0;
         bool done = false;
-        this->run(g * per, min(blocks(), (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
-            if (done) {
-                return;
-            }
-            double v[kEight], sum = 0.0;
-#pragma unroll
-            for (int i = 0; i < kEight; i++) {
-                v[i] = value(x[i], column(b, i));
-                sum += v[i];
-            }
-            const double upto = wave_scan(sum), before_me = __shfl_up(upto, 1);
-            double mine = run + (lane == 0 ? 0.0 : before_me);
-            int hit = -1, last = -1;
-            double hit_v = 0.0, last_v = 0.0;
-#pragma unroll
-            for (int i = 0; i < kEight; i++) {
-                mine += v[i];
-                if (v[i] > 0.0) {
-                    if (hit < 0 && mine > target) {
-                        hit = i;
-                        hit_v = v[i];
-                    }
-                    last = i;
-                    last_v = v[i];
+        // a segment whose sum is of nothing but weights that count as 0 is passed over
+#pragma unroll 1
+        for (; at < 0 && g < segments; g++) {
+            this->template run<1>(g * per, min(blocks(), (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
+                if (done) {
+                    return;
                 }
-            }
-            const uint64_t hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
-            if (hits) {
-                const int l = __builtin_ctzll(hits);
-                at = b * kBlock + l * kEight + __shfl(hit, l);
-                what = __shfl(hit_v, l);
-                done = true;
-            } else if (lasts) {
-                const int l = 63 - __builtin_clzll(lasts);
-                at = b * kBlock + l * kEight + __shfl(last, l);
-                what = __shfl(last_v, l);
-            }
-            run += __shfl(upto, 63);
-        });
+                double v[kEight], sum = 0.0;
+#pragma unroll
+                for (int i = 0; i < kEight; i++) {
+                    v[i] = value(x[i], column(b, i));
+                    sum += v[i];
+                }
+                const double upto = wave_scan(sum), before_me = __shfl_up(upto, 1);
+                double mine = run + (lane == 0 ? 0.0 : before_me);
+                int hit = -1, last = -1;
+                double hit_v = 0.0, last_v = 0.0;
+#pragma unroll
+                for (int i = 0; i < kEight; i++) {
+                    mine += v[i];
+                    if (v[i] > 0.0) {
+                        if (hit < 0 && mine > target) {
+                            hit = i;
+                            hit_v = v[i];
+                        }
+                        last = i;
+                        last_v = v[i];
+                    }
+                }
+                const uint64_t hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
+                if (hits) {
+                    const int l = __builtin_ctzll(hits);
+                    at = b * kBlock + l * kEight + __shfl(hit, l);
+                    what = __shfl(hit_v, l);
+                    done = true;
+                } else if (lasts) {
+                    const int l = 63 - __builtin_clzll(lasts);
+                    at = b * kBlock + l * kEight + __shfl(last, l);
+                    what = __shfl(last_v, l);
+                }
+                run += __shfl(upto, 63);
+            });
+        }
     }
 
     // Columns for which pick(x, key) go to the list, and the sums of `value` over the others to the segments; returns their total.
     template <typename P, typename F>
-    __device__ double collect(int64_t per, P pick, F value) const
+    __device__ __forceinline__ double collect(int64_t per, P pick, F value) const
     {
         if (tid == 0) {
-            s.listed = 0;
+            lds.listed = 0;
         }
         __syncthreads();
         return segment_sums(per, [&](float x, uint32_t c) {
             const uint32_t key = key_of(x);
             const bool listed = key && pick(x, key);
             if (listed) {
-                const uint32_t at = atomicAdd(&s.listed, 1u);
+                const uint32_t at = atomicAdd(&lds.listed, 1u);
                 if (at < kList) {
-                    s.list[at] = (uint64_t)key << 32 | ~c;
+                    lds.list[at] = (uint64_t)key << 32 | ~c;
                 }
             }
             return listed ? 0.0 : value(x, key);
@@ -430,7 +439,7 @@ struct Sampler {
     // The first of m bins at which what has been tallied, with `before` in front of the first, reaches `goal`, or the last that holds
     // anything; `before` becomes what is in front of it.
     template <typename V>
-    __device__ int cross(const V *bins, int m, double goal, double &before)
+    __device__ __forceinline__ int cross(const V *bins, int m, double goal, double &before)
     {
         __syncthreads();
         if (wave == 0) {
@@ -456,20 +465,20 @@ struct Sampler {
                     }
                     run += v;
                 }
-                s.found = (uint32_t)at;
-                s.before = found;
+                lds.found = (uint32_t)at;
+                lds.before = found;
             }
         }
         __syncthreads();
-        const int at = (int)s.found;
-        before = s.before;
+        const int at = (int)lds.found;
+        before = lds.before;
         __syncthreads();
         return at;
     }
 
     // The place (score and column) of the last column kept: the count or (by_mass) the sum of weights up to it reaches `goal`.  Where
-    // `summed`, the sums of segments of what is kept, min_p apart, are in s.segment afterwards, their total in `total`.
-    __device__ uint64_t find_cut(const Row &r, float low, double goal, bool by_mass, bool &summed, double &total)
+    // `summed`, the sums of segments of what is kept, min_p apart, are in lds.segment afterwards, their total in `total`.
+    __device__ __forceinline__ uint64_t find_cut(const Row &r, float low, double goal, bool by_mass, bool &summed, double &total)
     {
         // Bins of equal width in the scores, for sums down to weights of 2^-64.  What is tallied there in 32 bits only says where
         // to look.
@@ -483,7 +492,7 @@ struct Sampler {
         const float scale = (float)r.scale;
         __syncthreads();
         for (int i = tid; i < kBins; i += NT) {
-            s.count[i] = 0;      // 0 in either type
+            lds.count[i] = 0;      // 0 in either type
         }
         __syncthreads();
         each([&](int64_t, const float(&x)[kEight]) {
@@ -493,21 +502,21 @@ struct Sampler {
                     const int b = bin_of(x[i]);
                     if (by_mass) {
                         // up to a factor that all have in common, so that no sum is lost
-                        atomicAdd(&s.mass[b], x[i] == r.top ? 0x1p60f : __builtin_amdgcn_exp2f(fmaf(x[i] - r.top, scale, 60.f)));
+                        atomicAdd(&lds.mass[b], x[i] == r.top ? 0x1p60f : __builtin_amdgcn_exp2f(fmaf(x[i] - r.top, scale, 60.f)));
                     } else {
-                        atomicAdd(&s.count[b], 1u);
+                        atomicAdd(&lds.count[b], 1u);
                     }
                 }
             }
         });
         double before = 0.0;
-        int bin = by_mass ? cross(s.mass, kBins, goal * 0x1p60, before) : cross(s.count, kBins, goal, before);
+        int bin = by_mass ? cross(lds.mass, kBins, goal * 0x1p60, before) : cross(lds.count, kBins, goal, before);
         int m, step = 0;
         for (;;) {
             // the bin's columns, and the sums of what lies above it
             total = collect(per, [&](float x, uint32_t) { return bin_of(x) == bin; },
                             [&](float x, uint32_t key) { return key && bin_of(x) < bin ? r.weight(x) : 0.0; });
-            m = (int)min(s.listed, (uint32_t)kList + 1u);
+            m = (int)min(lds.listed, (uint32_t)kList + 1u);
             if (!by_mass) {
                 break;
             }
@@ -517,13 +526,13 @@ struct Sampler {
             }
             sort(m);
             for (int i = tid; i < m; i += NT) {
-                s.sum[i] = r.weight(score_of((uint32_t)(s.list[i] >> 32)));
+                lds.sum[i] = r.weight(score_of((uint32_t)(lds.list[i] >> 32)));
             }
             __syncthreads();
-            scan(s.sum, m);
+            scan(lds.sum, m);
             // 32 bits were wrong by a bin, which happens at its edge
             const bool under = before >= goal && bin > 0 && step <= 0;
-            const bool over = (m == 0 || before + s.sum[m - 1] < goal) && bin < kBins - 1 && step >= 0;
+            const bool over = (m == 0 || before + lds.sum[m - 1] < goal) && bin < kBins - 1 && step >= 0;
             __syncthreads();
             if (!under && !over) {
                 break;
@@ -538,7 +547,7 @@ struct Sampler {
         if (!by_mass) {
             sort(m);
             for (int i = tid; i < m; i += NT) {
-                s.sum[i] = r.weight(score_of((uint32_t)(s.list[i] >> 32)));
+                lds.sum[i] = r.weight(score_of((uint32_t)(lds.list[i] >> 32)));
             }
             __syncthreads();
         }
@@ -550,20 +559,20 @@ struct Sampler {
             take = min(1, m);
         }
         // to the segments, by each of them in the list's order
-        const uint64_t place = m > 0 ? s.list[take - 1] : 0;
+        const uint64_t place = m > 0 ? lds.list[take - 1] : 0;
         const int64_t columns = per * kBlock;
         for (int i = tid; i < take; i += NT) {
-            s.segment_of[i] = (uint16_t)((int64_t)(~(uint32_t)s.list[i]) / columns);
+            lds.segment_of[i] = (uint16_t)((int64_t)(~(uint32_t)lds.list[i]) / columns);
         }
         __syncthreads();
         const int segments = (int)((blocks() + per - 1) / per);
         for (int g = tid; g < segments; g += NT) {
-            double v = s.segment[g];
+            double v = lds.segment[g];
             for (int i = 0; i < take; i++) {
-                const double prior = by_mass && i > 0 ? s.sum[i - 1] : 0.0, own = s.sum[i] - prior;
-                v += s.segment_of[i] == g ? own : 0.0;
+                const double prior = by_mass && i > 0 ? lds.sum[i - 1] : 0.0, own = lds.sum[i] - prior;
+                v += lds.segment_of[i] == g ? own : 0.0;
             }
-            s.segment[g] = v;
+            lds.segment[g] = v;
         }
         total = segment_total(segments);
         summed = true;
@@ -572,7 +581,7 @@ struct Sampler {
 
     // The same where a bin holds too many for the list: by the bits of their keys, ten at a time, and among equal scores by column.
     template <typename B>
-    __device__ uint64_t find_tie(const Row &r, B in_bin, double before, double goal, bool by_mass)
+    __device__ __forceinline__ uint64_t find_tie(const Row &r, B in_bin, double before, double goal, bool by_mass)
     {
         const double fixed = by_mass ? __builtin_ldexp(1.0, 62 - (64 - __builtin_clzll((unsigned long long)n))) : 1.0;
         double run = before * fixed;
@@ -583,7 +592,7 @@ struct Sampler {
             const uint32_t mask = (1u << bits) - 1u;
             __syncthreads();
             for (int i = tid; i < kBins; i += NT) {
-                s.tally[i] = 0;
+                lds.tally[i] = 0;
             }
             __syncthreads();
             each([&](int64_t, const float(&x)[kEight]) {
@@ -592,11 +601,11 @@ struct Sampler {
                     const uint32_t key = key_of(x[i]);
                     if (key && in_bin(x[i]) && (key & known) == prefix) {
                         // integers: in any order; the largest scores first
-                        atomicAdd(&s.tally[~(key >> to) & mask], by_mass ? (unsigned long long)__builtin_rint(r.weight(x[i]) * fixed) : 1ull);
+                        atomicAdd(&lds.tally[~(key >> to) & mask], by_mass ? (unsigned long long)__builtin_rint(r.weight(x[i]) * fixed) : 1ull);
                     }
                 }
             });
-            prefix |= (~(uint32_t)cross(s.tally, 1 << bits, goal * fixed, run) & mask) << to;
+            prefix |= (~(uint32_t)cross(lds.tally, 1 << bits, goal * fixed, run) & mask) << to;
             known |= mask << to;
             shift = to;
         }
@@ -649,7 +658,7 @@ template <typename T, int NT>
 __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Settings &set, int part, int parts, double &total)
 {
     constexpr int kWaves = NT / 64, kOwn = kEight * kSample;
-    SampleShared &s = k.s;
+    SampleShared &s = lds;
     const int lane = k.lane, wave = k.wave;
     const int64_t per = k.segment_size(), all = (k.blocks() + per - 1) / per;
     const int g0 = (int)(all * part / parts), g1 = (int)(all * (part + 1) / parts);
@@ -686,8 +695,7 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
         s.tops[wave * (64 / kLanes) + lane / kLanes] = (uint32_t)(group_top ^ flip);
     }
     if (k.tid < kFew) {
-        s.rank[0][k.tid] = 0;
-        s.rank[1][k.tid] = 0;
+        s.rank[k.tid] = 0;
     }
     if (k.tid == 0) {
         s.listed = 0;
@@ -702,8 +710,8 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
     if (set.filtered && sample_top) {
         const float share = columns > NT * kOwn ? (float)(NT * kOwn) / (float)columns : 1.f;
         // what is wanted of all parts: k, or for sums a hundred and more
-        const float wanted = (set.by_count ? (float)min(set.count, (int64_t)kList) : 128.f) / (float)parts * share;
-        const float reach = share < 1.f ? wanted + 3.f * __builtin_amdgcn_sqrtf(wanted) + 4.f : wanted;
+        const float wanted = (set.by_count ? (float)min(set.count, (int64_t)kList) : 160.f) / (float)parts * share;
+        const float reach = set.by_count ? wanted + 3.f * __builtin_amdgcn_sqrtf(wanted) + 4.f : wanted + 2.f;
         if (columns <= kFew) {
             h.bound = 1;      // everything that is there
         } else if (reach <= 130.f) {
@@ -725,7 +733,7 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
     double sum = 0.0;
     for (int g = g0 + wave; g < g1; g += kWaves) {
         double v = 0.0;
-        k.run(g * per, min(b1, (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
+        k.template run<kTurns>(g * per, min(b1, (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
             float most = x[0];
 #pragma unroll
             for (int i = 1; i < kEight; i++) {
@@ -735,7 +743,7 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
             if (sums) {
 #pragma unroll
                 for (int i = 0; i < kEight; i++) {
-                    v += power_of_two(fmax(((double)x[i] - (double)reference) * set.scale, kNothing));   // NaN and -infinity: 0
+                    v += power_of_two(fmin(fmax(((double)x[i] - (double)reference) * set.scale, kNothing), 1000.0));
                 }
             }
             if (most >= bound) {
@@ -785,90 +793,108 @@ __device__ __forceinline__ bool finish_few(const Sampler<T, NT> &k, const Sample
                                            bool complete, double total, int64_t *labels, float *probs, U draw_number)
 {
     constexpr int kWaves = NT / 64, kParts = NT / kFew, kOf = kFew / 64;
-    SampleShared &s = k.s;
+    SampleShared &s = lds;
     const int tid = k.tid, lane = k.lane, wave = k.wave, own = tid % kFew, part = tid / kFew;
-    auto count_before = [&](const uint64_t *of, int size, uint32_t *rank, auto before) {
-        if (own < size) {
-            const uint64_t mine = of[own];
-            int c = 0;
+    if (own < m) {
+        const uint64_t mine = s.list[own];
+        int before = 0;
 #pragma unroll 4
-            for (int i = part; i < size; i += kParts) {
-                c += before(of[i], mine) ? 1 : 0;
-            }
-            if (kParts > 1) {
-                atomicAdd(&rank[own], (uint32_t)c);
-            } else {
-                rank[own] = (uint32_t)c;
-            }
+        for (int i = part; i < m; i += kParts) {
+            before += s.list[i] > mine ? 1 : 0;
         }
-        __syncthreads();
-    };
-    count_before(s.list, m, s.rank[0], [](uint64_t a, uint64_t b) { return a > b; });
-    if (tid < m) {
-        s.sorted[s.rank[0][tid]] = s.list[tid];
+        if (kParts > 1) {
+            atomicAdd(&s.rank[own], (uint32_t)before);
+        } else {
+            s.rank[own] = (uint32_t)before;
+        }
     }
     __syncthreads();
-    double w[kOf], upto[kOf], run = 0.0;
-#pragma unroll
-    for (int c = 0; c < kOf; c++) {
-        const int e = c * 64 + lane;
-        w[c] = upto[c] = 0.0;
-        if (c * 64 < m) {
-            w[c] = e < m ? r.weight(score_of((uint32_t)(s.sorted[e] >> 32))) : 0.0;
-            upto[c] = run + wave_scan(w[c]);
-            run = __shfl(upto[c], 63);
-        }
+    if (tid < m) {
+        s.sorted[s.rank[tid]] = s.list[tid];
     }
-    auto how_many = [&](int size, auto is) {
-        int count = 0;
-#pragma unroll
-        for (int c = 0; c < kOf; c++) {
-            count += __popcll(__ballot(c * 64 + lane < size && is(c)));
-        }
-        return count;
-    };
-    auto sum_upto = [&](int size) {     // of the first `size` entries
-        double v = 0.0;
-#pragma unroll
-        for (int c = 0; c < kOf; c++) {
-            v = (size - 1) / 64 == c ? __shfl(upto[c], (size - 1) % 64) : v;
-        }
-        return v;
-    };
-    bool cut = complete;               // whether the list holds all that is kept
+    __syncthreads();
+    // One wavefront goes on (all of them at the same would take turns); the others wait for its word, and for many draws of theirs.
+    double w[kOf], upto[kOf], run = 0.0, all = 0.0;
     int take = m;
-    if (set.by_count) {
-        cut = cut || m >= set.count;
-        take = (int)min((int64_t)m, set.count);
+    if (wave == 0) {
+#pragma unroll
+        for (int c = 0; c < kOf; c++) {
+            const int e = c * 64 + lane;
+            w[c] = upto[c] = 0.0;
+            if (c * 64 < m) {
+                w[c] = e < m ? r.weight(score_of((uint32_t)(s.sorted[e] >> 32))) : 0.0;
+                upto[c] = run + wave_scan(w[c]);
+                run = __shfl(upto[c], 63);
+            }
+        }
+        auto how_many = [&](int size, auto is) {
+            int count = 0;
+#pragma unroll
+            for (int c = 0; c < kOf; c++) {
+                count += __popcll(__ballot(c * 64 + lane < size && is(c)));
+            }
+            return count;
+        };
+        auto sum_upto = [&](int size) {     // of the first `size` entries
+            double v = 0.0;
+#pragma unroll
+            for (int c = 0; c < kOf; c++) {
+                v = (size - 1) / 64 == c ? __shfl(upto[c], (size - 1) % 64) : v;
+            }
+            return v;
+        };
+        bool cut = complete;               // whether the list holds all that is kept
+        if (set.by_count) {
+            cut = cut || m >= set.count;
+            take = (int)min((int64_t)m, set.count);
+        }
+        if (set.by_mass && (cut || !set.by_count)) {
+            // of the sum of all that is left, which the list has or the whole row
+            const double goal = set.top_p * (cut ? sum_upto(take) : total);
+            const int need = how_many(take, [&](int c) { return upto[c] < goal; }) + 1;
+            cut = cut || need <= take;
+            take = min(take, need);
+        }
+        if (set.min_p > 0.0 && !(set.by_count && !cut)) {
+            const int above = how_many(m, [&](int c) { return w[c] >= set.min_p; });
+            cut = cut || above < m;
+            take = min(take, above);
+        }
+        take = max(take, 1);
+        if (cut) {
+            all = sum_upto(take);
+            // by column: how many of those that are kept come before each
+#pragma unroll
+            for (int c = 0; c < kOf; c++) {
+                const int e = c * 64 + lane;
+                if (c * 64 < take) {
+                    const uint64_t mine = s.sorted[min(e, kFew - 1)];
+                    int before = 0;
+#pragma unroll 4
+                    for (int i = 0; i < take; i++) {
+                        before += (uint32_t)s.sorted[i] > (uint32_t)mine ? 1 : 0;
+                    }
+                    if (e < take) {
+                        s.list[before] = mine;
+                        s.segment[before] = w[c];
+                    }
+                }
+            }
+        }
+        if (lane == 0) {
+            s.found = cut ? (uint32_t)take : 0u;
+            s.before = all;
+        }
     }
-    if (set.by_mass && (cut || !set.by_count)) {
-        // of the sum of all that is left, which the list has or the whole row
-        const double goal = set.top_p * (cut ? sum_upto(take) : total);
-        const int need = how_many(take, [&](int c) { return upto[c] < goal; }) + 1;
-        cut = cut || need <= take;
-        take = min(take, need);
-    }
-    if (set.min_p > 0.0 && !(set.by_count && !cut)) {
-        const int above = how_many(m, [&](int c) { return w[c] >= set.min_p; });
-        cut = cut || above < m;
-        take = min(take, above);
-    }
-    if (!cut) {
+    __syncthreads();
+    take = (int)s.found;
+    if (take == 0) {
         return false;
     }
-    take = max(take, 1);
-    const double all = sum_upto(take);
-    count_before(s.sorted, take, s.rank[1], [](uint64_t a, uint64_t b) { return (uint32_t)a > (uint32_t)b; });
-    if (tid < take) {
-        double mine = w[0];
-#pragma unroll
-        for (int c = 1; c < kOf; c++) {
-            mine = wave == c ? w[c] : mine;
-        }
-        s.list[s.rank[1][tid]] = s.sorted[tid];
-        s.segment[s.rank[1][tid]] = mine;
+    if (wave > 0 && p.draws <= kOneWave) {
+        return true;
     }
-    __syncthreads();
+    all = s.before;
     run = 0.0;
 #pragma unroll
     for (int c = 0; c < kOf; c++) {
@@ -880,7 +906,8 @@ __device__ __forceinline__ bool finish_few(const Sampler<T, NT> &k, const Sample
             run = __shfl(upto[c], 63);
         }
     }
-    for (int d = wave; d < p.draws; d += kWaves) {
+    const int step = p.draws <= kOneWave ? 1 : kWaves;
+    for (int d = wave; d < p.draws; d += step) {
         const double target = draw_number(d) * all;
         int at = 0;       // the first that passes it, or the last with a weight if rounding hides that
 #pragma unroll
@@ -910,7 +937,7 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
                                            const PartHead &h, double total)
 {
     constexpr int kWaves = NT / 64;
-    SampleShared &s = k.s;
+    SampleShared &s = lds;
     const int tid = k.tid, lane = k.lane, wave = k.wave;
     int64_t *const labels = p.labels + row * p.draws;
     float *const probs = p.probs ? p.probs + row * p.draws : nullptr;
@@ -1011,15 +1038,16 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
         const float low = -score_of(h.low);
         double sum = total;
         bool summed = false;
-        if (set.by_count) {
-            r.least = k.find_cut(r, low, (double)count, false, summed, sum);
-            if (set.by_mass && !summed) {
+#pragma unroll 1
+        for (int mass = 0; mass < 2; mass++) {
+            if (mass == 0 ? !set.by_count : !set.by_mass) {
+                continue;
+            }
+            if (mass && set.by_count && !summed) {
                 // the sum up to the cut by its columns
                 sum = k.segment_sums(per, [&](float x, uint32_t c) { return key_of(x) && r.place(key_of(x), c) >= r.least ? r.weight(x) : 0.0; });
             }
-        }
-        if (set.by_mass) {
-            const uint64_t least = k.find_cut(r, low, set.top_p * sum, true, summed, sum);
+            const uint64_t least = k.find_cut(r, low, mass ? set.top_p * sum : (double)count, mass, summed, sum);
             summed = summed && least >= r.least;
             r.least = larger(r.least, least);
         }
@@ -1046,9 +1074,9 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
 }
 
 template <typename T, int NT>
-__device__ __forceinline__ Sampler<T, NT> sampler(SampleShared &s, const SampleParams &p, int64_t row)
+__device__ __forceinline__ Sampler<T, NT> sampler(const SampleParams &p, int64_t row)
 {
-    return Sampler<T, NT>{s, static_cast<const T *>(p.scores) + row * p.ld, p.n, (int)threadIdx.x, (int)threadIdx.x & 63,
+    return Sampler<T, NT>{static_cast<const T *>(p.scores) + row * p.ld, p.n, (int)threadIdx.x, (int)threadIdx.x & 63,
                           __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
 }
 
@@ -1056,21 +1084,20 @@ __device__ __forceinline__ Sampler<T, NT> sampler(SampleShared &s, const SampleP
 __device__ __forceinline__ double unit_of(float reference, float top, double scale)
 {
     const double t = ((double)reference - (double)top) * scale;
-    return reference == top && top < __builtin_inff() ? 1.0 : t > -1000.0 ? power_of_two(t) : 0.0;
+    return reference == top && top < __builtin_inff() ? 1.0 : t > kNothing ? power_of_two(t) : 0.0;
 }
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT, NT == 256 ? 3 : 4) void sample_kernel(SampleParams p)
 {
-    __shared__ SampleShared s;
     const int64_t row = blockIdx.x;
-    Sampler<T, NT> k = sampler<T, NT>(s, p, row);
+    Sampler<T, NT> k = sampler<T, NT>(p, row);
     const Settings set(p, row);
     double total;
     PartHead h = scan_part(k, set, 0, 1, total);
     if (set.need_mass) {
         const double unit = set.filtered ? unit_of(score_of(h.reference), score_of(h.top), set.scale) : 1.0;
-        h.fine = total > 0.0 && total < 0x1p1000 && unit > 0.0;
+        h.fine = h.reference && score_of(h.reference) < __builtin_inff() && total < 0x1p990 && unit > 0.0;
         total *= unit;
     }
     finish_row(k, p, set, row, h, total);
@@ -1080,10 +1107,10 @@ __global__ __launch_bounds__(NT, NT == 256 ? 3 : 4) void sample_kernel(SamplePar
 template <typename T>
 __global__ __launch_bounds__(kPartThreads, 4) void sample_part_kernel(SampleParams p)
 {
-    __shared__ SampleShared s;
+    SampleShared &s = lds;
     const int64_t row = blockIdx.x / p.parts;
     const int part = (int)(blockIdx.x - row * p.parts);
-    const Sampler<T, kPartThreads> k = sampler<T, kPartThreads>(s, p, row);
+    const Sampler<T, kPartThreads> k = sampler<T, kPartThreads>(p, row);
     const Settings set(p, row);
     double total;
     const PartHead h = scan_part(k, set, part, p.parts, total);
@@ -1107,9 +1134,9 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_part_kernel(SamplePara
 template <typename T>
 __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SampleParams p)
 {
-    __shared__ SampleShared s;
+    SampleShared &s = lds;
     const int64_t row = blockIdx.x;
-    Sampler<T, kPartThreads> k = sampler<T, kPartThreads>(s, p, row);
+    Sampler<T, kPartThreads> k = sampler<T, kPartThreads>(p, row);
     const Settings set(p, row);
     PartHead all{0, 0, 0, 0, 0, 1, {}};
     bool listed = true;
@@ -1125,8 +1152,7 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
     all.bound = max(all.bound, 1u);
     all.reference = all.top;
     if (k.tid < kFew) {
-        s.rank[0][k.tid] = 0;
-        s.rank[1][k.tid] = 0;
+        s.rank[k.tid] = 0;
     }
     if (k.tid == 0) {
         s.listed = 0;
@@ -1148,7 +1174,7 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
             }
         }
         if (set.need_mass) {
-            const double unit = h.top ? unit_of(score_of(h.reference), top, set.scale) : 1.0;
+            const double unit = !h.top ? 1.0 : h.reference ? unit_of(score_of(h.reference), top, set.scale) : 0.0;
             for (int g = (int)(segments * i / p.parts) + k.tid; g < (int)(segments * (i + 1) / p.parts); g += kPartThreads) {
                 const double v = h.top ? p.segments[row * kSegments + g] : 0.0;
                 // what does not come out as a sum is found out again
@@ -1161,7 +1187,7 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
     double total = 0.0;
     if (set.need_mass && all.top) {
         total = k.segment_total((int)segments);
-        all.fine = total > 0.0 && total < 0x1p1000;      // also not of what is no number
+        all.fine = total < 0x1p990;      // also not of what is no number
     }
     finish_row(k, p, set, row, all, total);
 }

@@ -16,7 +16,7 @@ def kept_weights(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         temperature, top_k = 1.0, 1
     with np.errstate(invalid="ignore", over="ignore", under="ignore"):
         w = np.where(x[order] == best, 1.0, np.exp((x[order] - best) / np.float64(temperature)))
-    w = np.nan_to_num(w)
+    w = np.where(w > 2.0 ** -960, w, 0.0)        # what is below counts as nothing; so does no number
     if top_k > 0:
         order, w = order[:top_k], w[:top_k]
     if top_p < 1:
