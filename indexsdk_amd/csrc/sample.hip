@@ -26,7 +26,8 @@ namespace {
 
 constexpr int kList = 2048;         // candidates of a row
 constexpr int kPartList = 1024;     // and of a part of one
-constexpr int kBins = 1024;
+constexpr int kBins = 4096;         // of a histogram of counts
+constexpr int kDigits = 1024;
 constexpr int kSegments = 512;      // at most: parts of a row whose sums are kept
 constexpr int kBlock = 512;         // columns that a wavefront reads at a time
 constexpr int kTurns = 4;           // such blocks in flight
@@ -39,7 +40,8 @@ constexpr double kNothing = -960.0;    // logarithms of weights that count as 0;
 // What a workgroup finds out about its part of a row.
 struct PartHead {
     uint32_t top, low, reference, bound;     // low: the lowest of the columns that the bound comes from
-    uint32_t listed, fine, unused[2];
+    uint32_t listed, fine;
+    uint32_t high, unused;                   // high: a bound that about kFew / 2 scores reach
 };
 
 struct SampleParams {
@@ -111,8 +113,7 @@ struct SampleShared {
     uint64_t list[kList];           // score's key above the column's complement
     union {
         double sum[kList];          // of the list's weights; a histogram is of no more use by then
-        unsigned long long tally[kBins];
-        float mass[kBins];
+        unsigned long long tally[kDigits];
         uint32_t count[kBins];
         struct {
             uint64_t sorted[kFew];
@@ -120,11 +121,15 @@ struct SampleShared {
         };
     };
     double segment[kSegments];
-    uint16_t segment_of[kList];
+    union {
+        uint16_t segment_of[kList];
+        uint64_t best[kFew];        // the highest of a longer list
+    };
     double box[2][16];
     uint32_t tops[64];
     uint32_t ubox[16], lows[16];
-    uint32_t listed, found;
+    uint32_t lengths[16];           // of the wavefronts' lists
+    uint32_t listed, found, found_best;
     double before;
 };
 
@@ -373,7 +378,7 @@ struct Sampler {
         // a segment whose sum is of nothing but weights that count as 0 is passed over
 #pragma unroll 1
         for (; at < 0 && g < segments; g++) {
-            this->template run<1>(g * per, min(blocks(), (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
+            this->template run<2>(g * per, min(blocks(), (g + 1) * per), [&](int64_t b, const float(&x)[kEight]) {
                 if (done) {
                     return;
                 }
@@ -436,52 +441,68 @@ struct Sampler {
         });
     }
 
-    // The first of m bins at which what has been tallied, with `before` in front of the first, reaches `goal`, or the last that holds
-    // anything; `before` becomes what is in front of it.
-    template <typename V>
-    __device__ __forceinline__ int cross(const V *bins, int m, double goal, double &before)
+    // The first of BINS bins at which the running sum of value(bin), with `before` in front of the first, reaches `goal`, or the last
+    // with a value; `before` becomes the sum in front of it.
+    template <int BINS, typename F>
+    __device__ __forceinline__ int cross(F value, double goal, double &before)
     {
+        constexpr int kPer = (BINS + NT - 1) / NT;
         __syncthreads();
-        if (wave == 0) {
-            const int per = (m + 63) / 64, from = lane * per, to = min(from + per, m);
-            double sum = 0.0;
-            for (int i = from; i < to; i++) {
-                sum += (double)bins[i];
-            }
-            const double upto = before + wave_scan(sum);
-            const uint64_t over = __ballot(upto >= goal && sum > 0.0), some = __ballot(sum > 0.0);
-            const int l = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
-            if (lane == l) {
-                double run = upto - sum, found = run;
-                int at = from;
-                for (int i = from; i < to; i++) {
-                    const double v = (double)bins[i];
-                    if (v > 0.0) {
-                        at = i;
-                        found = run;
-                        if (run + v >= goal) {
-                            break;
-                        }
-                    }
-                    run += v;
-                }
-                lds.found = (uint32_t)at;
-                lds.before = found;
-            }
+        double v[kPer], sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            v[i] = tid * kPer + i < BINS ? value(tid * kPer + i) : 0.0;
+            sum += v[i];
+        }
+        const double upto = wave_scan(sum);
+        if (lane == 63) {
+            lds.box[1][wave] = upto;
+        }
+        if (tid == 0) {
+            lds.found = 0;
+            lds.before = before;
         }
         __syncthreads();
-        const int at = (int)lds.found;
-        before = lds.before;
+        double run = before;
+        for (int w = 0; w < wave; w++) {
+            run += lds.box[1][w];
+        }
+        const double before_me = __shfl_up(upto, 1);
+        run += lane == 0 ? 0.0 : before_me;
+        int at = -1, last = -1;
+        double in_front = 0.0, in_front_of_last = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            if (v[i] > 0.0) {
+                if (at < 0 && run + v[i] >= goal) {
+                    at = tid * kPer + i;
+                    in_front = run;
+                }
+                last = tid * kPer + i;
+                in_front_of_last = run;
+            }
+            run += v[i];
+        }
+        // the lowest bin that reaches it, else the highest with a value
+        const uint32_t mine = at >= 0 ? 0x80000000u | (uint32_t)(BINS - at) : last >= 0 ? (uint32_t)last + 1u : 0u;
+        const uint32_t best = block_max(mine);
+        if (best && mine == best) {
+            lds.found = (uint32_t)(at >= 0 ? at : last);
+            lds.before = at >= 0 ? in_front : in_front_of_last;
+        }
         __syncthreads();
-        return at;
+        before = lds.before;
+        const int found = (int)lds.found;
+        __syncthreads();
+        return found;
     }
 
     // The place (score and column) of the last column kept: the count or (by_mass) the sum of weights up to it reaches `goal`.  Where
     // `summed`, the sums of segments of what is kept, min_p apart, are in lds.segment afterwards, their total in `total`.
     __device__ __forceinline__ uint64_t find_cut(const Row &r, float low, double goal, bool by_mass, bool &summed, double &total)
     {
-        // Bins of equal width in the scores, for sums down to weights of 2^-64.  What is tallied there in 32 bits only says where
-        // to look.
+        // Counts in bins of equal width in the scores, for sums down to weights of 2^-64; a bin's weights are its count times that of
+        // its middle.  That is only where to look: sums in 64 bits decide.
         const float width = r.top - low, range = by_mass ? fminf(width, (float)(64.0 / r.scale)) : width;
         const float unit = range > 0.f && range < __builtin_inff() ? (float)kBins / range : 0.f;
         auto bin_of = [&](float x) {
@@ -489,28 +510,25 @@ struct Sampler {
             return d < (float)(kBins - 1) ? (int)d : kBins - 1;     // also where 0 meets infinity
         };
         const int64_t per = segment_size();
-        const float scale = (float)r.scale;
         __syncthreads();
         for (int i = tid; i < kBins; i += NT) {
-            lds.count[i] = 0;      // 0 in either type
+            lds.count[i] = 0;
         }
         __syncthreads();
         each([&](int64_t, const float(&x)[kEight]) {
 #pragma unroll
             for (int i = 0; i < kEight; i++) {
-                if (key_of(x[i])) {
-                    const int b = bin_of(x[i]);
-                    if (by_mass) {
-                        // up to a factor that all have in common, so that no sum is lost
-                        atomicAdd(&lds.mass[b], x[i] == r.top ? 0x1p60f : __builtin_amdgcn_exp2f(fmaf(x[i] - r.top, scale, 60.f)));
-                    } else {
-                        atomicAdd(&lds.count[b], 1u);
-                    }
+                if (x[i] > -__builtin_inff()) {
+                    atomicAdd(&lds.count[bin_of(x[i])], 1u);
                 }
             }
         });
         double before = 0.0;
-        int bin = by_mass ? cross(lds.mass, kBins, goal * 0x1p60, before) : cross(lds.count, kBins, goal, before);
+        const float step_down = unit > 0.f ? (float)r.scale / unit : 0.f;
+        int bin = cross<kBins>([&](int b) {
+            const double c = (double)lds.count[b];
+            return by_mass ? c * (double)__builtin_amdgcn_exp2f(((float)b + 0.5f) * -step_down) : c;
+        }, goal, before);
         int m, step = 0;
         for (;;) {
             // the bin's columns, and the sums of what lies above it
@@ -591,7 +609,7 @@ struct Sampler {
             const int bits = min(10, shift), to = shift - bits;
             const uint32_t mask = (1u << bits) - 1u;
             __syncthreads();
-            for (int i = tid; i < kBins; i += NT) {
+            for (int i = tid; i < kDigits; i += NT) {
                 lds.tally[i] = 0;
             }
             __syncthreads();
@@ -605,7 +623,7 @@ struct Sampler {
                     }
                 }
             });
-            prefix |= (~(uint32_t)cross(lds.tally, 1 << bits, goal * fixed, run) & mask) << to;
+            prefix |= (~(uint32_t)cross<kDigits>([&](int b) { return (double)lds.tally[b]; }, goal * fixed, run) & mask) << to;
             known |= mask << to;
             shift = to;
         }
@@ -694,28 +712,17 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
     if (lane % kLanes == 0) {
         s.tops[wave * (64 / kLanes) + lane / kLanes] = (uint32_t)(group_top ^ flip);
     }
-    if (k.tid < kFew) {
-        s.rank[k.tid] = 0;
-    }
-    if (k.tid == 0) {
-        s.listed = 0;
-    }
     __syncthreads();
     const uint32_t tops = s.tops[lane];
     const uint32_t sample_top = over_wave(tops, [](uint32_t a, uint32_t b) { return max(a, b); });
     const float reference = score_of(sample_top);
     // A bound that so many of the sampled columns reach that all of them have what is kept, but for one time in thousands: as
     // many more than expected as three deviations.
-    PartHead h{0, 0, sample_top, 0xffffffffu, 0, 1, {}};
+    PartHead h{0, 0, sample_top, 0xffffffffu, 0, 1, 0xffffffffu, 0};
     if (set.filtered && sample_top) {
         const float share = columns > NT * kOwn ? (float)(NT * kOwn) / (float)columns : 1.f;
-        // what is wanted of all parts: k, or for sums a hundred and more
-        const float wanted = (set.by_count ? (float)min(set.count, (int64_t)kList) : 160.f) / (float)parts * share;
-        const float reach = set.by_count ? wanted + 3.f * __builtin_amdgcn_sqrtf(wanted) + 4.f : wanted + 2.f;
-        if (columns <= kFew) {
-            h.bound = 1;      // everything that is there
-        } else if (reach <= 130.f) {
-            // of 64 groups those that hold one of `reach` columns at least
+        // the highest bound that one of so many of 64 groups of the sampled columns reaches as hold one of `reach` columns at least
+        auto bound_for = [&](float reach) {
             const int groups = (int)fminf(60.f, 64.f * (1.f - __expf(-reach / 64.f)) + 1.5f);
             uint32_t b = 0;
 #pragma unroll 1
@@ -723,12 +730,25 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
                 const uint32_t at = b | 1u << bit;
                 b = __popcll(__ballot(tops >= at)) >= groups ? at : b;
             }
-            h.bound = max(b, 1u);
+            return max(b, 1u);
+        };
+        if (columns <= kFew) {
+            h.bound = 1;      // everything that is there
+        } else if (set.by_count) {
+            const float wanted = (float)min(set.count, (int64_t)kList) / (float)parts * share;
+            const float reach = wanted + 3.f * __builtin_amdgcn_sqrtf(wanted) + 4.f;
+            h.bound = reach <= 130.f ? bound_for(reach) : h.bound;
+        } else {
+            // what a sum takes is not known ahead: a few hundred, and the highest of them first
+            h.bound = bound_for(fminf(640.f / (float)parts * share + 4.f, 130.f));
+            h.high = bound_for(fminf(140.f / (float)parts * share + 1.f, 100.f));
         }
     }
     const float bound = h.bound == 0xffffffffu ? __builtin_nanf("") : h.bound == 1 ? -3.402823466e+38f : score_of(h.bound);
     const bool sums = set.need_mass;
-    const uint32_t limit = parts > 1 ? kPartList : kList;
+    constexpr int kOwnList = kList / kWaves;      // every wavefront has a list of its own
+    uint64_t *const list = s.list + wave * kOwnList;
+    int listed = 0;
     float top = -inf;
     double sum = 0.0;
     for (int g = g0 + wave; g < g1; g += kWaves) {
@@ -746,14 +766,16 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
                     v += power_of_two(fmin(fmax(((double)x[i] - (double)reference) * set.scale, kNothing), 1000.0));
                 }
             }
-            if (most >= bound) {
+            if (__ballot(most >= bound)) {
 #pragma unroll
                 for (int i = 0; i < kEight; i++) {
-                    if (x[i] >= bound) {
-                        const uint32_t at = atomicAdd(&s.listed, 1u);
-                        if (at < limit) {
-                            s.list[at] = (uint64_t)key_of(x[i]) << 32 | ~k.column(b, i);
+                    const uint64_t hits = __ballot(x[i] >= bound);
+                    if (hits) {
+                        const int at = listed + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0));
+                        if (x[i] >= bound && at < kOwnList) {
+                            list[at] = (uint64_t)key_of(x[i]) << 32 | ~k.column(b, i);
                         }
+                        listed += __popcll(hits);
                     }
                 }
             }
@@ -772,16 +794,38 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
         s.box[0][wave] = sum;
         s.ubox[wave] = wave_top;
         s.lows[wave] = wave_low;
+        s.lengths[wave] = (uint32_t)listed;
     }
     __syncthreads();
     total = 0.0;
+    uint32_t together = 0, mine_from = 0;
+    bool fits = true;
 #pragma unroll 4
     for (int w = 0; w < kWaves; w++) {
         total += s.box[0][w];
         h.top = max(h.top, s.ubox[w]);
         h.low = max(h.low, s.lows[w]);
+        mine_from += w < wave ? s.lengths[w] : 0u;
+        together += s.lengths[w];
+        fits = fits && s.lengths[w] <= (uint32_t)kOwnList;
     }
-    h.listed = h.bound == 0xffffffffu ? 0xffffffffu : s.listed;
+    h.listed = h.bound == 0xffffffffu || !fits || (parts > 1 && together > (uint32_t)kPartList) ? 0xffffffffu : together;
+    if (h.listed != 0xffffffffu) {
+        // one list of all
+        uint64_t mine_of[(kOwnList + 63) / 64];
+#pragma unroll
+        for (int i = 0; i < (kOwnList + 63) / 64; i++) {
+            mine_of[i] = i * 64 + lane < listed ? list[i * 64 + lane] : 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < (kOwnList + 63) / 64; i++) {
+            if (i * 64 + lane < listed) {
+                s.list[mine_from + i * 64 + lane] = mine_of[i];
+            }
+        }
+    }
+    __syncthreads();
     return h;
 }
 
@@ -789,18 +833,22 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
 // their scores and, those that are kept, in that of their columns, by how many come before each; cuts and draws are ballots over what
 // every wavefront holds in registers.
 template <typename T, int NT, typename U>
-__device__ __forceinline__ bool finish_few(const Sampler<T, NT> &k, const SampleParams &p, const Settings &set, const Row &r, int m,
-                                           bool complete, double total, int64_t *labels, float *probs, U draw_number)
+__device__ __forceinline__ bool finish_few(const Sampler<T, NT> &k, const SampleParams &p, const Settings &set, const Row &r,
+                                           const uint64_t *list, int m, bool complete, double total, int64_t *labels, float *probs, U draw_number)
 {
     constexpr int kWaves = NT / 64, kParts = NT / kFew, kOf = kFew / 64;
     SampleShared &s = lds;
     const int tid = k.tid, lane = k.lane, wave = k.wave, own = tid % kFew, part = tid / kFew;
+    if (tid < kFew) {
+        s.rank[tid] = 0;
+    }
+    __syncthreads();
     if (own < m) {
-        const uint64_t mine = s.list[own];
+        const uint64_t mine = list[own];
         int before = 0;
 #pragma unroll 4
         for (int i = part; i < m; i += kParts) {
-            before += s.list[i] > mine ? 1 : 0;
+            before += list[i] > mine ? 1 : 0;
         }
         if (kParts > 1) {
             atomicAdd(&s.rank[own], (uint32_t)before);
@@ -810,7 +858,7 @@ __device__ __forceinline__ bool finish_few(const Sampler<T, NT> &k, const Sample
     }
     __syncthreads();
     if (tid < m) {
-        s.sorted[s.rank[tid]] = s.list[tid];
+        s.sorted[s.rank[tid]] = list[tid];
     }
     __syncthreads();
     // One wavefront goes on (all of them at the same would take turns); the others wait for its word, and for many draws of theirs.
@@ -963,11 +1011,29 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
     if (set.filtered) {
         const bool complete = h.bound == 1;      // every column that is there is in the list
         const int m = h.listed <= kList ? (int)h.listed : 0;
-        if (m > 0 && m <= kFew) {
-            if (finish_few(k, p, set, r, m, complete, total, labels, probs, draw_number)) {
-                return;
+        // All candidates, or the highest of them, if they are few.
+        int high = m;
+        if (m > kFew && h.high != 0xffffffffu) {
+            if (tid == 0) {
+                s.found_best = 0;
             }
-        } else if (m > 0) {
+            __syncthreads();
+            for (int i = tid; i < m; i += NT) {
+                if ((uint32_t)(s.list[i] >> 32) >= h.high) {
+                    const uint32_t at = atomicAdd(&s.found_best, 1u);      // in any order: they are put in theirs
+                    if (at < kFew) {
+                        s.best[at] = s.list[i];
+                    }
+                }
+            }
+            __syncthreads();
+            high = (int)s.found_best;
+        }
+        if (high > 0 && high <= kFew &&
+            finish_few(k, p, set, r, high < m ? s.best : s.list, high, complete && high == m, total, labels, probs, draw_number)) {
+            return;
+        }
+        if (m > kFew) {
             int take = m;
             k.sort(m);
             for (int i = tid; i < m; i += NT) {
@@ -1138,7 +1204,7 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
     const int64_t row = blockIdx.x;
     Sampler<T, kPartThreads> k = sampler<T, kPartThreads>(p, row);
     const Settings set(p, row);
-    PartHead all{0, 0, 0, 0, 0, 1, {}};
+    PartHead all{0, 0, 0, 0, 0, 1, 0, 0};
     bool listed = true;
     for (int i = 0; i < p.parts; i++) {
         const PartHead h = p.heads[row * p.parts + i];
@@ -1146,14 +1212,12 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
             all.top = max(all.top, h.top);
             all.low = max(all.low, h.low);
             all.bound = max(all.bound, h.bound);
+            all.high = max(all.high, h.high);
             listed = listed && h.listed <= kPartList;
         }
     }
     all.bound = max(all.bound, 1u);
     all.reference = all.top;
-    if (k.tid < kFew) {
-        s.rank[k.tid] = 0;
-    }
     if (k.tid == 0) {
         s.listed = 0;
     }
