@@ -27,7 +27,7 @@ namespace {
 constexpr int kList = 2048;         // candidates of a row
 constexpr int kPartList = 1024;     // and of a part of one
 constexpr int kBins = 4096;         // of a histogram of counts
-constexpr int kDigits = 1024;
+constexpr int kDigits = 1024, kAround = 32;
 constexpr int kSegments = 512;      // at most: parts of a row whose sums are kept
 constexpr int kBlock = 512;         // columns that a wavefront reads at a time
 constexpr int kTurns = 4;           // such blocks in flight
@@ -139,14 +139,25 @@ __shared__ SampleShared lds;
 // What is drawn from: columns of at least `least` (an order of score and column as in the list) with weights of at least min_p.
 struct Row {
     double scale;      // log2(e) / T
-    float top;         // the largest score
+    float top;         // the largest score, or another that weights are relative to
+    double from;       // the same in 64 bits, where infinity is a number that all others are far below
     double min_p;
     uint64_t least;
+    __device__ __forceinline__ Row(double s, float t, double m) : scale(s), top(t), from(t), min_p(m), least(0)
+    {
+        if (t == __builtin_inff()) {
+            from = 1e300;
+            scale = fmax(s, 1.0);
+        }
+    }
+    __device__ __forceinline__ double logarithm(float x) const { return (fmin((double)x, 1e300) - from) * scale; }
+    // of a score that is there; what counts as 0 is 0, or in a sum of many 2^-960
     __device__ __forceinline__ double weight(float x) const
     {
-        const double t = ((double)x - (double)top) * scale;
-        return x == top ? 1.0 : t > kNothing ? power_of_two(fmin(t, 1000.0)) : 0.0;
+        const double t = logarithm(x);
+        return t > kNothing ? power_of_two(t) : 0.0;
     }
+    __device__ __forceinline__ double addend(float x) const { return power_of_two(fmax(logarithm(x), kNothing)); }
     __device__ __forceinline__ uint64_t place(uint32_t key, uint32_t column) const { return (uint64_t)key << 32 | ~column; }
     // of a column: 0 where it is cut off
     __device__ __forceinline__ double kept(float x, uint32_t column) const
@@ -420,25 +431,28 @@ struct Sampler {
         }
     }
 
-    // Columns for which pick(x, key) go to the list, and the sums of `value` over the others to the segments; returns their total.
-    template <typename P, typename F>
-    __device__ __forceinline__ double collect(int64_t per, P pick, F value) const
+    // Columns with scores in [low, high] go to the list, the sums of the weights above to the segments; their total, and the
+    // number of columns above.
+    __device__ __forceinline__ double collect(int64_t per, const Row &r, float low, float high, double &above) const
     {
         if (tid == 0) {
             lds.listed = 0;
         }
         __syncthreads();
-        return segment_sums(per, [&](float x, uint32_t c) {
-            const uint32_t key = key_of(x);
-            const bool listed = key && pick(x, key);
-            if (listed) {
+        int mine = 0;
+        const double total = segment_sums(per, [&](float x, uint32_t c) {
+            const double w = r.addend(x);
+            if (x >= low && x <= high) {
                 const uint32_t at = atomicAdd(&lds.listed, 1u);
                 if (at < kList) {
-                    lds.list[at] = (uint64_t)key << 32 | ~c;
+                    lds.list[at] = (uint64_t)key_of(x) << 32 | ~c;
                 }
             }
-            return listed ? 0.0 : value(x, key);
+            mine += x > high ? 1 : 0;
+            return x > high ? w : 0.0;
         });
+        above = block_sum((double)mine);
+        return total;
     }
 
     // The first of BINS bins at which the running sum of value(bin), with `before` in front of the first, reaches `goal`, or the last
@@ -529,16 +543,29 @@ struct Sampler {
             const double c = (double)lds.count[b];
             return by_mass ? c * (double)__builtin_amdgcn_exp2f(((float)b + 0.5f) * -step_down) : c;
         }, goal, before);
-        int m, step = 0;
-        for (;;) {
-            // the bin's columns, and the sums of what lies above it
-            total = collect(per, [&](float x, uint32_t) { return bin_of(x) == bin; },
-                            [&](float x, uint32_t key) { return key && bin_of(x) < bin ? r.weight(x) : 0.0; });
-            m = (int)min(lds.listed, (uint32_t)kList + 1u);
-            if (!by_mass) {
+        // The bin and its neighbours, as long as the list is likely to hold them: where the counts were off by little, the cut still
+        // is among these.  That scores next to a threshold may fall to either side of the bins' edge does not matter.
+        int first = bin, last = bin;
+        uint32_t room = lds.count[bin] < kList / 2 ? kList / 2 - lds.count[bin] : 0u;
+        for (int i = 1; i <= kAround; i++) {
+            const uint32_t up = bin - i >= 0 ? lds.count[bin - i] : 0u, down = bin + i < kBins ? lds.count[bin + i] : 0u;
+            if (up + down > room) {
                 break;
             }
-            before = total;
+            room -= up + down;
+            first = max(bin - i, 0);
+            last = min(bin + i, kBins - 1);
+        }
+        __syncthreads();
+        const float inf = __builtin_inff(), least = -3.402823466e+38f, wide = unit > 0.f ? kAround / unit : inf;
+        float high = first == 0 || !(unit > 0.f) ? inf : r.top - (float)first / unit;
+        float bottom = last >= kBins - 1 || !(unit > 0.f) ? least : r.top - (float)(last + 1) / unit;
+        int m, way = 0;
+        for (;;) {
+            double above;
+            total = collect(per, r, bottom, high, above);
+            before = by_mass ? total : above;
+            m = (int)min(lds.listed, (uint32_t)kList + 1u);
             if (m > kList) {
                 break;
             }
@@ -547,37 +574,36 @@ struct Sampler {
                 lds.sum[i] = r.weight(score_of((uint32_t)(lds.list[i] >> 32)));
             }
             __syncthreads();
-            scan(lds.sum, m);
-            // 32 bits were wrong by a bin, which happens at its edge
-            const bool under = before >= goal && bin > 0 && step <= 0;
-            const bool over = (m == 0 || before + lds.sum[m - 1] < goal) && bin < kBins - 1 && step >= 0;
+            if (by_mass) {
+                scan(lds.sum, m);
+            }
+            const double upto = before + (m == 0 ? 0.0 : by_mass ? lds.sum[m - 1] : (double)m);
+            const bool under = before >= goal && high < inf && way <= 0, over = upto < goal && bottom > least && way >= 0;
             __syncthreads();
             if (!under && !over) {
                 break;
             }
-            step = under ? -1 : 1;
-            bin += step;
+            if (under) {
+                way = -1;
+                bottom = score_of(key_of(high) + 1);
+                high = fminf(high + wide, inf);
+            } else {
+                way = 1;
+                high = score_of(key_of(bottom) - 1);
+                bottom = fmaxf(bottom - wide, least);
+            }
         }
         if (m > kList) {
             summed = false;
-            return find_tie(r, [&](float x) { return bin_of(x) == bin; }, before, goal, by_mass);
-        }
-        if (!by_mass) {
-            sort(m);
-            for (int i = tid; i < m; i += NT) {
-                lds.sum[i] = r.weight(score_of((uint32_t)(lds.list[i] >> 32)));
-            }
-            __syncthreads();
+            return find_tie(r, [&](float x) { return x >= bottom && x <= high; }, before, goal, by_mass);
         }
         const double left = goal - before;
         int take = by_mass ? reach(left, m) : left < (double)m ? (int)left : m;
         take = min(take, m);
-        // Nothing of the bin is needed (rounding at its edge), or the bin is empty: the cut is the last place above it.
-        if (take < 1) {
-            take = min(1, m);
-        }
+        take = max(take, min(1, m));
+        // an empty list: everything above it is kept, or everything that is there
+        const uint64_t place = m > 0 ? lds.list[take - 1] : before >= goal ? (uint64_t)(key_of(high) + 1) << 32 : 0;
         // to the segments, by each of them in the list's order
-        const uint64_t place = m > 0 ? lds.list[take - 1] : 0;
         const int64_t columns = per * kBlock;
         for (int i = tid; i < take; i += NT) {
             lds.segment_of[i] = (uint16_t)((int64_t)(~(uint32_t)lds.list[i]) / columns);
@@ -603,9 +629,20 @@ struct Sampler {
     {
         const double fixed = by_mass ? __builtin_ldexp(1.0, 62 - (64 - __builtin_clzll((unsigned long long)n))) : 1.0;
         double run = before * fixed;
-        uint32_t prefix = 0, known = 0;
+        uint32_t prefix = 0, known = 0, top = 0, bottom = 0;
         const int64_t per = segment_size();
-        for (int shift = 32; shift > 0;) {
+        each([&](int64_t, const float(&x)[kEight]) {
+#pragma unroll
+            for (int i = 0; i < kEight; i++) {
+                const uint32_t key = in_bin(x[i]) ? key_of(x[i]) : 0u;
+                top = max(top, key);
+                bottom = max(bottom, key ? ~key : 0u);
+            }
+        });
+        top = block_max(top);
+        bottom = ~block_max(bottom);
+        prefix = top == bottom ? top : 0u;
+        for (int shift = top == bottom ? 0 : 32; shift > 0;) {
             const int bits = min(10, shift), to = shift - bits;
             const uint32_t mask = (1u << bits) - 1u;
             __syncthreads();
@@ -763,7 +800,7 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
             if (sums) {
 #pragma unroll
                 for (int i = 0; i < kEight; i++) {
-                    v += power_of_two(fmin(fmax(((double)x[i] - (double)reference) * set.scale, kNothing), 1000.0));
+                    v += power_of_two(fmax(((double)x[i] - (double)reference) * set.scale, kNothing));
                 }
             }
             if (__ballot(most >= bound)) {
@@ -1000,7 +1037,7 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
         return;
     }
     const int64_t per = k.segment_size(), count = set.count;
-    Row r{set.scale, score_of(set.filtered || !h.fine ? h.top : h.reference), set.min_p, 0};
+    Row r(set.scale, score_of(set.filtered || !h.fine ? h.top : h.reference), set.min_p);
     if (set.need_mass && !h.fine) {
         total = k.segment_sums(per, [&](float x, uint32_t) { return key_of(x) ? r.weight(x) : 0.0; });
     }
@@ -1033,7 +1070,15 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
             finish_few(k, p, set, r, high < m ? s.best : s.list, high, complete && high == m, total, labels, probs, draw_number)) {
             return;
         }
-        if (m > kFew) {
+        bool hopeless = false;      // the whole list is short of what p takes
+        if (m > kFew && set.by_mass && !set.by_count && !complete && set.min_p == 0.0) {
+            double sum = 0.0;
+            for (int i = tid; i < m; i += NT) {
+                sum += r.weight(score_of((uint32_t)(s.list[i] >> 32)));
+            }
+            hopeless = k.block_sum(sum) < 0.999 * set.top_p * total;
+        }
+        if (m > kFew && !hopeless) {
             int take = m;
             k.sort(m);
             for (int i = tid; i < m; i += NT) {
@@ -1146,7 +1191,7 @@ __device__ __forceinline__ Sampler<T, NT> sampler(const SampleParams &p, int64_t
                           __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)};
 }
 
-// What a sum relative to `reference` is multiplied by to be one relative to `top`; 0: it can not be.
+// What a sum relative to `reference` is multiplied by to be one relative to `top`; 0: it can not be, exponentials were out of range.
 __device__ __forceinline__ double unit_of(float reference, float top, double scale)
 {
     const double t = ((double)reference - (double)top) * scale;
@@ -1162,9 +1207,9 @@ __global__ __launch_bounds__(NT, NT == 256 ? 3 : 4) void sample_kernel(SamplePar
     double total;
     PartHead h = scan_part(k, set, 0, 1, total);
     if (set.need_mass) {
-        const double unit = set.filtered ? unit_of(score_of(h.reference), score_of(h.top), set.scale) : 1.0;
-        h.fine = h.reference && score_of(h.reference) < __builtin_inff() && total < 0x1p990 && unit > 0.0;
-        total *= unit;
+        const double unit = h.reference ? unit_of(score_of(h.reference), score_of(h.top), set.scale) : 0.0;
+        h.fine = unit > 0.0;
+        total *= set.filtered ? unit : 1.0;
     }
     finish_row(k, p, set, row, h, total);
 }
@@ -1251,7 +1296,7 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
     double total = 0.0;
     if (set.need_mass && all.top) {
         total = k.segment_total((int)segments);
-        all.fine = total < 0x1p990;      // also not of what is no number
+        all.fine = total == total;
     }
     finish_row(k, p, set, row, all, total);
 }
@@ -1260,10 +1305,10 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
 // 131072 under top-p: SAMPLE_PARTS).
 int parts_of(int64_t rows, int64_t n)
 {
-    if (rows == 0 || rows > 128 || n < 65536) {
+    if (rows == 0 || rows > 256 || n < 65536) {
         return 1;
     }
-    return (int)std::min<int64_t>({kMaxParts, 256 / rows, n / 16384});
+    return (int)std::min<int64_t>({kMaxParts, std::max<int64_t>(2, 512 / rows), n / 16384});
 }
 
 }  // namespace
