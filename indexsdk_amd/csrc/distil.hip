@@ -6,10 +6,14 @@
 // Entries with a label outside 0 ... n - 1 are not there.  Rows without an entry or without a score above -infinity have loss and
 // gradient 0.
 //
-// All of it is bound by memory: the scores are read once for their largest and their sum of exponentials, and once more to
-// write the gradient.  Exponentials of fp32 scores take 2^t of both parts of the product with log2(e) / T, those of 16-bit
-// scores the rounded product; 32 of them are added in 32 bits, all else in 64, also what the teacher's entries need: the loss
-// is a small difference of large logarithms.
+// All of it is bound by memory.  A row that fits into a workgroup's registers is read once, while the gradient of the row before it is
+// written: 4096 rows of 131072 bf16 take 435 us, 4.95 TB/s of the 5.2 at which memory is copied.  Longer rows are read twice, by a
+// kernel for the sums (5.4 TB/s) and one for the gradient (5.6), or where only one of the two is asked for.  Reading a row again
+// soon, from the cache behind the L2, is no faster than from memory: both come through the same 5.8 TB/s.
+//
+// Exponentials of fp32 scores take 2^t of both parts of the product with log2(e) / T, those of 16-bit scores the rounded product; 32 of
+// them are added in 32 bits, all else in 64, also what the teacher's entries need: the loss is a small difference of large logarithms.
+#include "power_of_two.h"
 #include "row_access.h"
 #include "scores.h"
 
@@ -22,8 +26,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTurns = 4;                         // times eight scores of a thread in flight
-constexpr int kPart = kThreads * kEight * kTurns;   // scores that a workgroup reads at a time
-constexpr int kEntries = kMaxTeacher / kThreads;  // a thread's
+constexpr int kPart = kThreads * kEight * kTurns;   // scores that such a workgroup reads at a time
+constexpr int kAlone = 256;                       // entries that one wavefront sees to
 constexpr double kLog2e = 1.44269504088896340735992468, kLn2 = 0.693147180559945309417232;
 
 struct DistilParams {
@@ -31,9 +35,9 @@ struct DistilParams {
     int64_t ld, n, rows;
     const int64_t *labels;
     const float *teacher, *whole;
-    int k, parts, slots;        // parts of a row; places of the table of labels
-    double temperature;
-    float high, low;            // log2(e) / T in two parts
+    int k, parts, slots, buffers;       // parts of a row; places of the table of labels; rows of entries in LDS
+    double temperature, scale;  // scale: log2(e) / T
+    float high, low;            // the same in two parts
     int64_t part;               // scores per part
     float *loss, *stats;
     double *partial;            // [rows][parts][2]
@@ -57,6 +61,37 @@ __device__ __forceinline__ float exponential(float x, float top, const DistilPar
     }
 }
 
+// exp((x - top) / T) where many scores share one `top`: 2^(h x - c) of 16-bit scores is one instruction less, and its product is
+// rounded once, together with the difference.  c is rounded too, by a factor that is the same for all of them.
+template <typename T>
+struct Exponent {
+    float reference, h, c;
+    __device__ __forceinline__ Exponent(float top, const DistilParams &p)
+    {
+        reference = top == -__builtin_inff() ? 0.f : top;
+        h = p.high;
+        if (fabsf(reference * h) > 0x1p21f && reference < __builtin_inff()) {
+            // scores that differ from the largest one, by a 2048th of it at least, are e^-700 of it and less: also with a smaller h,
+            // with which h x - c is exact for x = top
+            h = __builtin_ldexpf(1.f, 21 - __builtin_amdgcn_frexp_expf(reference));
+        }
+        c = reference * h;
+    }
+    __device__ __forceinline__ float operator()(float x, const DistilParams &p) const
+    {
+        if constexpr (sizeof(T) == 4) {
+            return exponential<T>(x, reference, p);
+        } else {
+            return __builtin_amdgcn_exp2f(fmaf(x, h, -c));
+        }
+    }
+    // what these are to be multiplied by
+    __device__ __forceinline__ double factor() const
+    {
+        return sizeof(T) == 4 || !(reference < __builtin_inff()) ? 1.0 : any_power_of_two((double)c - (double)reference * (double)h);
+    }
+};
+
 // A largest score and the sum of exponentials relative to it (to 0 where there is none).
 struct Sum {
     float top;
@@ -66,43 +101,63 @@ struct Sum {
     {
         const float both = fmaxf(top, other_top), r = both == -__builtin_inff() ? 0.f : both;
         // sums of nothing are 0 or no number
-        const double mine = top == -__builtin_inff() ? 1.0 : exp2(((double)top - r) * kLog2e / p.temperature);
-        const double others = other_top == -__builtin_inff() ? 1.0 : exp2(((double)other_top - r) * kLog2e / p.temperature);
+        const double mine = top == -__builtin_inff() ? 1.0 : any_power_of_two(((double)top - r) * p.scale);
+        const double others = other_top == -__builtin_inff() ? 1.0 : any_power_of_two(((double)other_top - r) * p.scale);
         sum = sum * mine + other_sum * others;
         top = both;
     }
 };
 
-template <typename V, typename Op>
-__device__ __forceinline__ V over_block(V v, V *box, Op op)
+// Op over groups of LANES (1, 2, 4, 8 or 16) lanes, of 32 or 64 bits
+template <int LANES, typename V, typename Op>
+__device__ __forceinline__ V over_lanes_of(V v, Op op)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        v = op(v, __shfl_xor(v, o));
+    if constexpr (LANES >= 2) {
+        v = op(v, value_of_lane<kXor1>(v));
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-        box[threadIdx.x >> 6] = v;
+    if constexpr (LANES >= 4) {
+        v = op(v, value_of_lane<kXor2>(v));
     }
-    __syncthreads();
-    v = box[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / 64; w++) {
-        v = op(v, box[w]);
+    if constexpr (LANES >= 8) {
+        v = op(v, value_of_lane<kMirror8>(v));
+    }
+    if constexpr (LANES >= 16) {
+        v = op(v, value_of_lane<kMirror16>(v));
     }
     return v;
 }
 
+// The threads' sums together.  box [NT / 64] is no other joint's until the workgroup's next barrier.
+template <int NT>
+__device__ __forceinline__ Sum joined(Sum mine, const DistilParams &p, Sum *box)
+{
+    auto both = [&](Sum a, float top) {
+        const float r = top == -__builtin_inff() ? 0.f : top;
+        return a.top == -__builtin_inff() ? a.sum : a.sum * any_power_of_two(((double)a.top - r) * p.scale);
+    };
+    auto larger = [](float a, float b) { return fmaxf(a, b); };
+    auto add = [](double a, double b) { return a + b; };
+    float top = over_wave(mine.top, larger);
+    const double sum = over_wave(both(mine, top), add);
+    if ((threadIdx.x & 63) == 0) {
+        box[threadIdx.x >> 6] = {top, sum};
+    }
+    __syncthreads();
+    Sum all = box[threadIdx.x & (NT / 64 - 1)];
+    top = over_lanes_of<NT / 64>(all.top, larger);
+    return {top, over_lanes_of<NT / 64>(both(all, top), add)};
+}
+
 // The sum over scores from ... to - 1 of a row, by the workgroup.
-template <typename T>
-__device__ Sum sum_of(const DistilParams &p, const T *row, int64_t from, int64_t to, double *box)
+template <typename T, int NT>
+__device__ Sum sum_of(const DistilParams &p, const T *row, int64_t from, int64_t to, Sum *box)
 {
     Sum mine{-__builtin_inff(), 0.0};
-    for (int64_t at = from; at < to; at += kPart) {
+    for (int64_t at = from; at < to; at += NT * kEight * kTurns) {
         Eight<T> v[kTurns];
 #pragma unroll
         for (int u = 0; u < kTurns; u++) {
-            const int64_t i = at + (u * kThreads + (int)threadIdx.x) * kEight;
+            const int64_t i = at + (u * NT + (int)threadIdx.x) * kEight;
             const int count = (int)min((int64_t)kEight, max((int64_t)0, to - i));
             v[u].load(row + (count ? i : from), count, (T)-__builtin_inff());
         }
@@ -127,122 +182,134 @@ __device__ Sum sum_of(const DistilParams &p, const T *row, int64_t from, int64_t
         mine.sum = mine.sum * (mine.top == -__builtin_inff() ? 1.0 : (double)exponential<float>(mine.top, r, p)) + (double)sum;
         mine.top = top;
     }
-    Sum all{over_block(mine.top, reinterpret_cast<float *>(box), [](float a, float b) { return fmaxf(a, b); }), 0.0};
-    const float r = all.reference();
-    const double part = mine.top == -__builtin_inff() ? mine.sum : mine.sum * exp2(((double)mine.top - r) * kLog2e / p.temperature);
-    all.sum = over_block(part, box, [](double a, double b) { return a + b; });
-    return all;
+    return joined<NT>(mine, p, box);
 }
 
-// A thread's entries of the teacher's: columns (-1: not there), log p and p; returns P, the same in every thread.
-__device__ double entries_of(const DistilParams &p, int64_t row, int (&column)[kEntries], double (&log_p)[kEntries], double *box)
-{
-    double top = -__builtin_inf();
-#pragma unroll
-    for (int e = 0; e < kEntries; e++) {
-        const int j = e * kThreads + (int)threadIdx.x;
-        column[e] = -1;
-        log_p[e] = -__builtin_inf();
-        if (e * kThreads < p.k && j < p.k) {
-            const int64_t l = p.labels[row * p.k + j];
-            const double t = (double)p.teacher[row * p.k + j] / p.temperature;
-            if (l >= 0 && l < p.n) {
-                column[e] = (int)l;
-                log_p[e] = t;
-                top = fmax(top, t);
+// The teacher's entries of rows, in LDS.  A crew works on them: the first wavefront, without a barrier, while the others go on; or
+// where there are many the whole workgroup.  Its thread j has entries j, j + threads() ...
+template <int NT>
+struct Entries {
+    struct Buffer {
+        double *log_p;      // to the base of 2; later p
+        int *column;        // -1: not there
+        float *value;       // the score at the column, later the gradient
+    };
+    uint8_t *buffers;
+    uint32_t *key, *first, *count;      // a table of the columns in the gradient's part
+    double *box;
+    int k, slots;
+    bool alone;
+
+    __device__ __forceinline__ Entries(const DistilParams &p, uint8_t *smem, double *box)
+        : buffers(smem), key(reinterpret_cast<uint32_t *>(smem + p.buffers * buffer_bytes(p.k))), first(key + p.slots),
+          count(first + p.slots), box(box), k(p.k), slots(p.slots), alone(p.k <= kAlone)
+    {
+    }
+    static __host__ __device__ __forceinline__ uint32_t buffer_bytes(int k) { return (uint32_t)(k + (k & 1)) * 16; }
+    __device__ __forceinline__ Buffer buffer(int which) const
+    {
+        double *const log_p = reinterpret_cast<double *>(buffers + which * buffer_bytes(k));
+        int *const column = reinterpret_cast<int *>(log_p + k);
+        return {log_p, column, reinterpret_cast<float *>(column + k)};
+    }
+    __device__ __forceinline__ bool crew() const { return !alone || __builtin_amdgcn_readfirstlane(threadIdx.x) < 64; }
+    __device__ __forceinline__ int threads() const { return alone ? 64 : NT; }
+    __device__ __forceinline__ int self() const
+    {
+        int j = threadIdx.x;
+        asm volatile("" : "+v"(j));      // addresses are computed for each row: kept for all, they would not fit into registers
+        return j;
+    }
+    __device__ __forceinline__ void sync() const
+    {
+        if (alone) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            __syncthreads();
+        }
+    }
+    template <typename Op>
+    __device__ __forceinline__ double over(double v, Op op) const
+    {
+        v = over_wave(v, op);
+        if (!alone) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) {
+                box[threadIdx.x >> 6] = v;
+            }
+            __syncthreads();
+            v = over_lanes_of<NT / 64>(box[threadIdx.x & (NT / 64 - 1)], op);
+        }
+        return v;
+    }
+    static __device__ __forceinline__ bool in_part(int column, int64_t from, int64_t to) { return column >= from && column < to; }
+
+    // A row's labels, log p, and the scores at those in from ... to - 1; returns P.
+    template <typename T>
+    __device__ __forceinline__ double load(const Buffer &b, const DistilParams &p, int64_t row, int64_t from, int64_t to) const
+    {
+        const T *const scores = static_cast<const T *>(p.scores) + row * p.ld;
+        const int64_t *const labels = p.labels + row * k;
+        const float *const teacher = p.teacher + row * k;
+        const int me = self();
+        double top = -__builtin_inf();
+#pragma unroll 2
+        for (int j = me; j < k; j += threads()) {
+            const int64_t l = labels[j];
+            const double t = (double)teacher[j] * p.scale;
+            const bool there = l >= 0 && l < p.n;
+            b.column[j] = there ? (int)l : -1;
+            b.log_p[j] = there ? t : -__builtin_inf();
+            b.value[j] = there && l >= from && l < to ? (float)scores[l] : 0.f;
+            top = there ? fmax(top, t) : top;
+        }
+        double lse;
+        if (p.whole) {
+            lse = (double)p.whole[row] * kLog2e;
+        } else {
+            top = over(top, [](double x, double y) { return fmax(x, y); });
+            const double r = top == -__builtin_inf() ? 0.0 : top;
+            double sum = 0.0;
+            for (int j = me; j < k; j += threads()) {
+                sum += b.column[j] >= 0 ? any_power_of_two(b.log_p[j] - r) : 0.0;
+            }
+            sum = over(sum, [](double x, double y) { return x + y; });
+            lse = sum == 0.0 ? 0.0 : r + log2_of(sum);      // no entry above -infinity: p is 0
+        }
+        double total = 0.0;
+        for (int j = me; j < k; j += threads()) {
+            if (b.column[j] >= 0) {
+                const double log_p = b.log_p[j] - lse;
+                b.log_p[j] = log_p;
+                total += any_power_of_two(log_p);
+            }
+        }
+        return over(total, [](double x, double y) { return x + y; });
+    }
+
+    __device__ __forceinline__ void write_loss(const Buffer &b, const DistilParams &p, int64_t row, const Sum &all) const
+    {
+        const double log_sum = log2_of(all.sum);
+        double loss = 0.0;
+        for (int j = self(); j < k; j += threads()) {
+            const double log_p = b.log_p[j], prob = any_power_of_two(log_p);      // 0 times infinity is nothing
+            if (b.column[j] >= 0 && prob != 0.0) {
+                loss += prob * (log_p - (((double)b.value[j] - (double)all.reference()) * p.scale - log_sum));
+            }
+        }
+        loss = over(loss, [](double x, double y) { return x + y; });
+        if (threadIdx.x == 0) {
+            if (p.loss) {
+                p.loss[row] = all.sum == 0.0 ? 0.f : (float)(loss * kLn2 * p.temperature * p.temperature);
+            }
+            if (p.stats) {
+                p.stats[row * 2] = all.top;
+                p.stats[row * 2 + 1] = (float)all.sum;
             }
         }
     }
-    double lse;
-    if (p.whole) {
-        lse = p.whole[row];
-    } else {
-        top = over_block(top, box, [](double a, double b) { return fmax(a, b); });
-        const double r = top == -__builtin_inf() ? 0.0 : top;
-        double sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < kEntries; e++) {
-            sum += e * kThreads < p.k && column[e] >= 0 ? exp(log_p[e] - r) : 0.0;
-        }
-        sum = over_block(sum, box, [](double a, double b) { return a + b; });
-        lse = sum == 0.0 ? 0.0 : r + log(sum);      // no entry above -infinity: p is 0
-    }
-    double total = 0.0;
-#pragma unroll
-    for (int e = 0; e < kEntries; e++) {
-        if (e * kThreads < p.k && column[e] >= 0) {
-            log_p[e] -= lse;
-            total += exp(log_p[e]);
-        }
-    }
-    return over_block(total, box, [](double a, double b) { return a + b; });
-}
 
-template <typename T>
-__device__ void finish_loss(const DistilParams &p, int64_t row, const Sum &all, double *box)
-{
-    int column[kEntries];
-    double log_p[kEntries];
-    entries_of(p, row, column, log_p, box);
-    const T *const scores = static_cast<const T *>(p.scores) + row * p.ld;
-    const double log_sum = log(all.sum);
-    double loss = 0.0;
-#pragma unroll
-    for (int e = 0; e < kEntries; e++) {
-        const double prob = exp(log_p[e]);      // 0 times infinity is nothing
-        if (e * kThreads < p.k && column[e] >= 0 && prob != 0.0) {
-            const double log_q = ((double)(float)scores[column[e]] - (double)all.reference()) / p.temperature - log_sum;
-            loss += prob * (log_p[e] - log_q);
-        }
-    }
-    loss = over_block(loss, box, [](double a, double b) { return a + b; });
-    if (threadIdx.x == 0) {
-        if (p.loss) {
-            p.loss[row] = all.sum == 0.0 ? 0.f : (float)(loss * p.temperature * p.temperature);
-        }
-        if (p.stats) {
-            p.stats[row * 2] = all.top;
-            p.stats[row * 2 + 1] = (float)all.sum;
-        }
-    }
-}
-
-// One workgroup per row or per part of a row.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distil_sum_kernel(DistilParams p)
-{
-    __shared__ double box[4];
-    const int64_t row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts;
-    const T *const scores = static_cast<const T *>(p.scores) + row * p.ld;
-    const Sum all = sum_of(p, scores, part * p.part, min(p.n, (part + 1) * p.part), box);
-    if (p.parts == 1) {
-        finish_loss<T>(p, row, all, box);
-    } else if (threadIdx.x == 0) {
-        p.partial[blockIdx.x * 2] = all.top;
-        p.partial[blockIdx.x * 2 + 1] = all.sum;
-    }
-}
-
-// The parts of a row, joined in their order.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distil_join_kernel(DistilParams p)
-{
-    __shared__ double box[4];
-    const int64_t row = blockIdx.x;
-    const double *const of = p.partial + row * p.parts * 2;
-    Sum all{-__builtin_inff(), 0.0};
-    for (int i = 0; i < p.parts; i++) {
-        all.join((float)of[i * 2], of[i * 2 + 1], p);
-    }
-    finish_loss<T>(p, row, all, box);
-}
-
-// The labels of a row that lie in one part of it, each once, in a table in LDS.
-struct Labels {
-    uint32_t *key, *first, *count;
-    int slots;
-    float *prob;
-    int *column;
     __device__ __forceinline__ int place(uint32_t of, bool insert) const
     {
         uint32_t at = (of * 2654435761u) & (uint32_t)(slots - 1);
@@ -254,95 +321,314 @@ struct Labels {
             at = (at + 1) & (uint32_t)(slots - 1);
         }
     }
+    __device__ __forceinline__ bool is_first(int j, int column) const { return first[place((uint32_t)column, false)] == (uint32_t)j; }
+
+    // The gradient at the labels in from ... to - 1: unit (P q - sum of p)
+    __device__ __forceinline__ void differentiate(const Buffer &b, const DistilParams &p, int64_t from, int64_t to, float reference,
+                                                  float sum, double whole, double unit) const
+    {
+        const int me = self();
+        for (int i = me; i < slots; i += threads()) {
+            key[i] = first[i] = 0xffffffffu;
+            count[i] = 0;
+        }
+        sync();
+        for (int j = me; j < k; j += threads()) {
+            const int column = b.column[j];
+            b.log_p[j] = any_power_of_two(b.log_p[j]);
+            if (in_part(column, from, to)) {
+                const int at = place((uint32_t)column, true);
+                atomicMin(&first[at], (uint32_t)j);
+                atomicAdd(&count[at], 1u);
+            }
+        }
+        sync();
+        const double share = whole / (double)sum;
+        for (int j = me; j < k; j += threads()) {
+            const int column = b.column[j];
+            if (in_part(column, from, to) && is_first(j, column)) {
+                double prob = b.log_p[j];
+                if (count[place((uint32_t)column, false)] > 1) {      // the same label again: added in the entries' order
+                    for (int i = j + 1; i < k; i++) {
+                        prob += b.column[i] == column ? b.log_p[i] : 0.0;
+                    }
+                }
+                const double q = any_power_of_two(((double)b.value[j] - (double)reference) * p.scale) * share;
+                b.value[j] = (float)(unit * (q - prob));
+            }
+        }
+    }
+    // Columns with labels, behind all others.
+    template <typename T>
+    __device__ __forceinline__ void write(const Buffer &b, T *gradient, int64_t from, int64_t to) const
+    {
+        for (int j = self(); j < k; j += threads()) {
+            const int column = b.column[j];
+            if (in_part(column, from, to) && is_first(j, column)) {
+                gradient[column] = (T)b.value[j];
+            }
+        }
+    }
 };
 
-// The gradient of one part of a row.  Columns with labels are written once more behind the others.
+// One workgroup per row or per part of a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void distil_sum_kernel(DistilParams p)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ double box[kThreads / 64];
+    __shared__ Sum sums[kThreads / 64];
+    const int64_t row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts;
+    const T *const scores = static_cast<const T *>(p.scores) + row * p.ld;
+    const Sum all = sum_of<T, kThreads>(p, scores, part * p.part, min(p.n, (part + 1) * p.part), sums);
+    if (p.parts == 1) {
+        const Entries<kThreads> entries(p, smem, box);
+        if (entries.crew()) {
+            entries.template load<T>(entries.buffer(0), p, row, 0, p.n);
+            entries.write_loss(entries.buffer(0), p, row, all);
+        }
+    } else if (threadIdx.x == 0) {
+        p.partial[blockIdx.x * 2] = all.top;
+        p.partial[blockIdx.x * 2 + 1] = all.sum;
+    }
+}
+
+// The parts of a row, joined in their order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void distil_join_kernel(DistilParams p)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ double box[kThreads / 64];
+    const int64_t row = blockIdx.x;
+    const Entries<kThreads> entries(p, smem, box);
+    if (entries.crew()) {
+        const double *const of = p.partial + row * p.parts * 2;
+        Sum all{-__builtin_inff(), 0.0};
+        for (int i = 0; i < p.parts; i++) {
+            all.join((float)of[i * 2], of[i * 2 + 1], p);
+        }
+        entries.template load<T>(entries.buffer(0), p, row, 0, p.n);
+        entries.write_loss(entries.buffer(0), p, row, all);
+    }
+}
+
+// What is computed from v is computed again behind this, rather than kept.
+template <typename T>
+__device__ __forceinline__ void forget(Eight<T> &v)
+{
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(v.v) / 4)));
+    Words w = __builtin_bit_cast(Words, v.v);
+    asm volatile("" : "+v"(w));
+    v.v = __builtin_bit_cast(typename Eight<T>::Lane, w);
+}
+
+// What a row's gradient is made of.
+template <typename T>
+struct Gradient {
+    Exponent<T> exponent;
+    double unit;
+    float sum, factor;
+    bool nothing;
+    __device__ __forceinline__ Gradient(const DistilParams &p, int64_t row, float top, float sum, double whole)
+        : exponent(top, p), unit((p.row_weight ? (double)p.row_weight[row] : 1.0) * p.temperature), sum(sum),
+          factor((float)(unit * whole * exponent.factor() / (double)sum)),
+          nothing(__builtin_amdgcn_readfirstlane(sum == 0.f || whole == 0.0))      // the same in all lanes
+    {
+    }
+    // eight scores
+    __device__ __forceinline__ void of(Eight<T> &v, const DistilParams &p) const
+    {
+        if (nothing) {
+            v.v = (T)0.f;
+            return;
+        }
+        typedef float Floats __attribute__((ext_vector_type(kEight)));
+        Floats g;
+#pragma unroll
+        for (int c = 0; c < kEight; c++) {
+            g[c] = exponent((float)v.v[c], p) * factor;
+        }
+        v.v = __builtin_convertvector(g, typename Eight<T>::Lane);
+    }
+};
+
+// One workgroup per part of a row.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void distil_gradient_kernel(DistilParams p)
 {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ double box[4];
+    __shared__ double box[kThreads / 64], whole;
     const int64_t row = blockIdx.x / p.parts, from = (blockIdx.x - row * p.parts) * p.part, to = min(p.n, from + p.part);
     const T *const scores = static_cast<const T *>(p.scores) + row * p.ld;
     T *const gradient = static_cast<T *>(p.gradient) + row * p.ld_gradient;
-    uint32_t *const table = reinterpret_cast<uint32_t *>(smem);
-    const Labels labels{table, table + p.slots, table + 2 * p.slots, p.slots, reinterpret_cast<float *>(table + 3 * p.slots),
-                        reinterpret_cast<int *>(table + 3 * p.slots) + p.k};
-    for (int i = threadIdx.x; i < p.slots; i += kThreads) {
-        labels.key[i] = 0xffffffffu;
-        labels.first[i] = 0xffffffffu;
-        labels.count[i] = 0;
-    }
-    int column[kEntries];
-    double log_p[kEntries];
-    const double whole = entries_of(p, row, column, log_p, box);
-    const float top = p.given_stats[row * 2], sum = p.given_stats[row * 2 + 1];
-    const float reference = top == -__builtin_inff() ? 0.f : top;
-    const double unit = (p.row_weight ? (double)p.row_weight[row] : 1.0) * p.temperature;
-    const bool nothing = sum == 0.f || whole == 0.0;
-    const float factor = nothing ? 0.f : (float)(unit * whole / (double)sum);
-    auto mine = [&](int e) { return e * kThreads < p.k && column[e] >= from && column[e] < to && !nothing; };
-#pragma unroll
-    for (int e = 0; e < kEntries; e++) {
-        const int j = e * kThreads + (int)threadIdx.x;
-        if (e * kThreads < p.k && j < p.k) {
-            labels.prob[j] = (float)exp(log_p[e]);
-            labels.column[j] = column[e];
-        }
-        if (mine(e)) {
-            const int at = labels.place((uint32_t)column[e], true);
-            atomicMin(&labels.first[at], (uint32_t)j);
-            atomicAdd(&labels.count[at], 1u);
-        }
-    }
-    __syncthreads();
-    T value[kEntries];
-#pragma unroll
-    for (int e = 0; e < kEntries; e++) {
-        const int j = e * kThreads + (int)threadIdx.x;
-        value[e] = (T)0.f;
-        if (mine(e)) {
-            const int at = labels.place((uint32_t)column[e], false);
-            if (labels.first[at] != (uint32_t)j) {
-                column[e] = -1;
-                continue;
-            }
-            double prob = exp(log_p[e]);
-            if (labels.count[at] > 1) {      // the same label again: added in the entries' order
-                for (int i = j + 1; i < p.k; i++) {
-                    prob += labels.column[i] == column[e] ? (double)labels.prob[i] : 0.0;
-                }
-            }
-            const double q = exp(((double)(float)scores[column[e]] - (double)reference) / p.temperature) / (double)sum;
-            value[e] = (T)(float)(unit * (whole * q - prob));
-        }
-    }
-    __syncthreads();       // the scores at labels have been read: the gradient may take their place
-    for (int64_t at = from; at < to; at += kPart) {
-        Eight<T> v[kTurns];
+    Eight<T> v[kTurns];
+    auto load = [&](int64_t at) {
 #pragma unroll
         for (int u = 0; u < kTurns; u++) {
             const int64_t i = at + (u * kThreads + (int)threadIdx.x) * kEight;
             const int count = (int)min((int64_t)kEight, max((int64_t)0, to - i));
             v[u].load(scores + (count ? i : from), count, (T)-__builtin_inff());
         }
+    };
+    load(from);
+    const Entries<kThreads> entries(p, smem, box);
+    if (entries.crew()) {
+        const double sum = entries.template load<T>(entries.buffer(0), p, row, from, to);
+        if (threadIdx.x == 0) {
+            whole = sum;
+        }
+    }
+    __syncthreads();       // the scores at labels have been read: the gradient may take their place
+    const Gradient<T> all(p, row, p.given_stats[row * 2], p.given_stats[row * 2 + 1], whole);
+    if (entries.crew() && !all.nothing) {
+        entries.differentiate(entries.buffer(0), p, from, to, all.exponent.reference, all.sum, whole, all.unit);
+    }
+    for (int64_t at = from; at < to; at += kPart) {
 #pragma unroll
         for (int u = 0; u < kTurns; u++) {
             const int64_t i = at + (u * kThreads + (int)threadIdx.x) * kEight;
-#pragma unroll
-            for (int c = 0; c < kEight; c++) {
-                const float g = exponential<T>((float)v[u].v[c], reference, p) * factor;
-                v[u].v[c] = (T)(nothing ? 0.f : g);
-            }
-            v[u].store(gradient + min(i, to), (int)min((int64_t)kEight, to - i));
+            all.of(v[u], p);
+            v[u].template store<true>(gradient + min(i, to), (int)min((int64_t)kEight, to - i));
+        }
+        if (at + kPart < to) {
+            load(at + kPart);
         }
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);     // vmcnt(0): a column's first value is in memory before its second is sent
     __syncthreads();
+    if (entries.crew() && !all.nothing) {
+        entries.write(entries.buffer(0), gradient, from, to);
+    }
+}
+
+// Workgroups with rows of their own, which stay in registers, EIGHTS times eight scores of a thread's: loss and gradient.  A row is
+// read while the gradient of the one before it is written.
+template <typename T, int NT, int EIGHTS>
+__global__ __launch_bounds__(NT, 4) void distil_row_kernel(DistilParams p)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ double box[NT / 64], whole_of[2];
+    __shared__ Sum sums[2][NT / 64];
+    const int whole = (int)p.n & ~(kEight - 1), left = (int)p.n - whole;     // the last scores are single ones
+    Eight<T> v[EIGHTS];
+    T last;
+    // Eight scores of a thread (a row has eight at least), the first of the row's in place of those past its end.  No branch around it, or the scores would be waited for
+    // where the branch ends.
+    auto load = [&](int u, const T *scores, int end, uint32_t at) {
+        const int from = u * NT * kEight;
+        at = from + (int)at < end ? at : 0u;
+        v[u].load(reinterpret_cast<const T *>(reinterpret_cast<const char *>(scores + (from < end ? from : 0)) + at * sizeof(T)),
+                  kEight, (T)0.f);
+    };
+    auto load_last = [&](const T *scores) {
+        last = (int)threadIdx.x < left ? scores[whole + (int)threadIdx.x] : (T)-__builtin_inff();
+    };
+    {
+        int end = whole;
+        uint32_t at = threadIdx.x * kEight;
+        asm volatile("" : "+s"(end), "+v"(at));
 #pragma unroll
-    for (int e = 0; e < kEntries; e++) {
-        if (mine(e)) {
-            gradient[column[e]] = value[e];
+        for (int u = 0; u < EIGHTS; u++) {
+            load(u, static_cast<const T *>(p.scores) + blockIdx.x * p.ld, end, at);
+        }
+    }
+    load_last(static_cast<const T *>(p.scores) + blockIdx.x * p.ld);
+    const Entries<NT> entries(p, smem, box);
+    auto load_entries = [&](int64_t row, int which) {
+        const double sum = entries.template load<T>(entries.buffer(which), p, row, 0, p.n);
+        if (threadIdx.x == 0) {
+            whole_of[which] = sum;
+        }
+    };
+    if (entries.crew()) {
+        load_entries(blockIdx.x, 0);
+    }
+    T *before = nullptr;       // a gradient whose columns with labels are not written yet
+    int which = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, which ^= 1) {
+        // what follows from these is computed for each row: kept for all of them it would not fit into the registers
+        int end = whole;
+        uint32_t at = threadIdx.x * kEight;
+        asm volatile("" : "+s"(end), "+v"(at));
+        float top = (float)last;
+#pragma unroll
+        for (int u = 0; u < EIGHTS; u++) {
+            if ((u + 1) * NT * kEight > end) {
+                if (u * NT * kEight + (int)at >= end) {
+                    v[u].v = (T)-__builtin_inff();
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < kEight; c++) {
+                top = fmaxf(top, (float)v[u].v[c]);
+            }
+        }
+        const Exponent<T> mine(top, p);
+        float part = 0.f;
+        double sum = (double)mine((float)last, p);
+        asm volatile("" : "+s"(end), "+v"(at));
+#pragma unroll
+        for (int u = 0; u < EIGHTS; u++) {
+            if (u * NT * kEight < end) {
+                forget(v[u]);
+#pragma unroll
+                for (int c = 0; c < kEight; c++) {
+                    part += mine((float)v[u].v[c], p);
+                }
+            }
+            if (u % 4 == 3) {
+                sum += (double)part;
+                part = 0.f;
+            }
+        }
+        const int64_t next = row + gridDim.x;
+        __builtin_amdgcn_s_waitcnt(0x0f70);     // vmcnt(0): what is before has been written
+        const Sum all = joined<NT>({top, sum * mine.factor()}, p, sums[which]);
+        const double mass = whole_of[which];
+        const Gradient<T> g(p, row, all.top, (float)all.sum, mass);
+        if (entries.crew()) {
+            if (before) {
+                entries.write(entries.buffer(which ^ 1), before, 0, p.n);
+            }
+            const auto buffer = entries.buffer(which);
+            entries.write_loss(buffer, p, row, all);
+            if (!g.nothing) {
+                entries.differentiate(buffer, p, 0, p.n, g.exponent.reference, g.sum, mass, g.unit);
+            }
+            if (next < p.rows) {
+                load_entries(next, which ^ 1);
+            }
+        }
+        T *const gradient = static_cast<T *>(p.gradient) + row * p.ld_gradient;
+        const T *const scores = static_cast<const T *>(p.scores) + (next < p.rows ? next : row) * p.ld;
+        asm volatile("" : "+s"(end), "+v"(at));
+#pragma unroll
+        for (int u = 0; u < EIGHTS; u++) {
+            const int from = u * NT * kEight;
+            if (from < end) {
+                forget(v[u]);
+                g.of(v[u], p);
+                if (from + (int)at < end) {
+                    v[u].template store<true>(
+                        reinterpret_cast<T *>(reinterpret_cast<char *>(gradient + from) + at * sizeof(T)), kEight);
+                }
+            }
+            load(u, scores, next < p.rows ? end : 0, at);
+        }
+        if ((int)threadIdx.x < left) {
+            Eight<T> one;
+            one.v = last;
+            g.of(one, p);
+            gradient[whole + (int)threadIdx.x] = one.v[0];
+        }
+        load_last(scores);
+        before = g.nothing ? nullptr : gradient;
+    }
+    if (before) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __syncthreads();
+        if (entries.crew()) {
+            entries.write(entries.buffer(which ^ 1), before, 0, p.n);
         }
     }
 }
@@ -366,10 +652,11 @@ DistilParams params_of(const DistilTask &t)
     p.teacher = t.teacher;
     p.whole = t.whole;
     p.k = t.k;
+    p.buffers = 1;
     p.temperature = t.temperature;
-    const double scale = kLog2e / (double)t.temperature;
-    p.high = (float)scale;
-    p.low = (float)(scale - (double)p.high);
+    p.scale = kLog2e / (double)t.temperature;
+    p.high = (float)p.scale;
+    p.low = (float)(p.scale - (double)p.high);
     return p;
 }
 void set_parts(DistilParams &p, int parts)
@@ -392,6 +679,19 @@ void check_task(const char *op, const DistilTask &t)
                 (double)t.temperature);
 }
 
+int slots_for(int k) { return std::max(64, pow2_ceil(2 * k)); }
+size_t entry_bytes(const DistilParams &p)
+{
+    return (size_t)p.buffers * Entries<kThreads>::buffer_bytes(p.k) + (size_t)p.slots * 12;
+}
+
+void launch(void (*kernel)(DistilParams), int64_t groups, int threads, size_t lds, const DistilParams &p, hipStream_t s)
+{
+    require_dynamic_lds(reinterpret_cast<const void *>(kernel), lds);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), lds, s, p);
+    check_launch();
+}
+
 void run_loss(const DistilTask &t, float *loss, float *stats, double *partial, hipStream_t s)
 {
     DistilParams p = params_of(t);
@@ -401,11 +701,9 @@ void run_loss(const DistilTask &t, float *loss, float *stats, double *partial, h
     set_parts(p, sum_parts(t.rows, t.n));
     with_type(t.type, [&](auto e) {
         typedef decltype(e) T;
-        hipLaunchKernelGGL((distil_sum_kernel<T>), dim3((unsigned)(t.rows * p.parts)), dim3(kThreads), 0, s, p);
-        check_launch();
+        launch(distil_sum_kernel<T>, t.rows * p.parts, kThreads, p.parts == 1 ? entry_bytes(p) : 0, p, s);
         if (p.parts > 1) {
-            hipLaunchKernelGGL((distil_join_kernel<T>), dim3((unsigned)t.rows), dim3(kThreads), 0, s, p);
-            check_launch();
+            launch(distil_join_kernel<T>, t.rows, kThreads, entry_bytes(p), p, s);
         }
     });
 }
@@ -418,15 +716,57 @@ void run_gradient(const DistilTask &t, const float *stats, const float *row_weig
     p.row_weight = row_weight;
     p.gradient = gradient;
     p.ld_gradient = ld_gradient;
-    p.slots = std::max(64, pow2_ceil(2 * t.k));
-    set_parts(p, std::max(parts_for(t.rows, t.n, 2048, kPart), parts_for(1, t.n, 1 << 20, 2 * kPart)));
-    const size_t lds = (size_t)p.slots * 12 + (size_t)t.k * 8;
+    p.slots = slots_for(t.k);
+    // parts of 32 KB of scores, or less where there are few (4096 rows of 131072 bf16: 381 us, 404 with 16 KB and 410 with 64 KB;
+    // 999 of 100003 fp32: 162 us, 175 with 64 KB)
+    set_parts(p, std::max(parts_for(t.rows, t.n, 2048, kPart), parts_for(1, t.n, 1 << 20, (t.type == kTypeF32 ? 1 : 2) * kPart)));
+    with_type(t.type, [&](auto e) { launch(distil_gradient_kernel<decltype(e)>, t.rows * p.parts, kThreads, entry_bytes(p), p, s); });
+}
+
+template <int NT, int EIGHTS>
+void run_rows(const DistilTask &t, const float *row_weight, float *loss, void *gradient, int64_t ld_gradient, hipStream_t s)
+{
+    DistilParams p = params_of(t);
+    p.row_weight = row_weight;
+    p.loss = loss;
+    p.gradient = gradient;
+    p.ld_gradient = ld_gradient;
+    p.slots = slots_for(t.k);
+    p.buffers = 2;
     with_type(t.type, [&](auto e) {
-        const auto kern = distil_gradient_kernel<decltype(e)>;
-        require_dynamic_lds(reinterpret_cast<const void *>(kern), lds);
-        hipLaunchKernelGGL(kern, dim3((unsigned)(t.rows * p.parts)), dim3(kThreads), lds, s, p);
-        check_launch();
+        typedef decltype(e) T;
+        // as many workgroups as are resident at once
+        const auto kernel = distil_row_kernel<T, NT, std::max(EIGHTS / (sizeof(T) == 4 ? 2 : 1), 4)>;
+        require_dynamic_lds(reinterpret_cast<const void *>(kernel), entry_bytes(p));
+        const int64_t groups = resident_workgroups(reinterpret_cast<const void *>(kernel), NT, entry_bytes(p));
+        launch(kernel, std::min(t.rows, groups), NT, entry_bytes(p), p, s);
     });
+}
+
+// Rows that fit into a workgroup's registers, 256 bytes of each thread's, are read once.  From 2048 rows on a wavefront or two of
+// them take a row (4096 rows of 8192 bf16: 38.5 us, 47.2 with 256 threads; 1024 rows: 20.0 and 17.6), but not where there is more to do
+// about the labels.  A few rows of more than 8192 go in parts, as longer ones do (64 rows of 131072 bf16: 21.1 us, 23.8 in registers).
+bool in_rows(const DistilTask &t, const float *row_weight, float *loss, void *gradient, int64_t ld_gradient, hipStream_t s)
+{
+    const int64_t threads = (t.n + 127) / 128 * (int64_t)(element_bytes(t.type) / 2);
+    if (t.n < kEight || threads > 1024) {
+        return false;
+    }
+    if (t.rows >= 2048 && t.k <= kAlone && threads <= (t.n <= 256 * 4 * kEight ? 64 : 128)) {
+        threads <= 64 ? run_rows<64, 16>(t, row_weight, loss, gradient, ld_gradient, s)
+                      : run_rows<128, 16>(t, row_weight, loss, gradient, ld_gradient, s);
+    } else if (t.n <= 256 * 4 * kEight) {
+        run_rows<256, 4>(t, row_weight, loss, gradient, ld_gradient, s);
+    } else if (t.rows < 128) {
+        return false;
+    } else if (threads <= 256) {
+        run_rows<256, 16>(t, row_weight, loss, gradient, ld_gradient, s);
+    } else if (threads <= 512) {
+        run_rows<512, 16>(t, row_weight, loss, gradient, ld_gradient, s);
+    } else {
+        run_rows<1024, 16>(t, row_weight, loss, gradient, ld_gradient, s);
+    }
+    return true;
 }
 
 void check_gradient(const char *op, const DistilTask &t, const float *row_weight, const void *gradient, int64_t ld_gradient)
@@ -488,6 +828,9 @@ void op_distil_step(const DistilTask &t, const float *row_weight, float *loss, v
     check_workspace("distil_step", workspace, workspace_bytes, distil_workspace(t.rows, t.n));
     int device;
     check_answer(hipGetDevice(&device));
+    if (in_rows(t, row_weight, loss, gradient, ld_gradient, s)) {
+        return;
+    }
     double *const partial = static_cast<double *>(workspace);
     float *const stats = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) +
                                                    round_up(t.rows * sum_parts(t.rows, t.n) * 16, 256));

@@ -14,6 +14,7 @@
 // is in the list, all else happens there: sorted by score, cut, and drawn from.  Rows without filters are drawn from by the sums
 // of their segments.  Everything else (flat rows whose p keeps thousands, large k) reads the row again: a histogram of counts and
 // weights finds the bin in which the cut lies, whose columns go through the list.
+#include "power_of_two.h"
 #include "row_access.h"
 #include "scores.h"
 
@@ -65,27 +66,6 @@ __device__ __forceinline__ uint32_t key_of(float x)
     return x > -__builtin_inff() ? k : 0u;
 }
 __device__ __forceinline__ float score_of(uint32_t k) { return __uint_as_float((int)k < 0 ? k & 0x7fffffffu : ~k); }
-
-// 2^t for t in [-1022, 1000]: the nearest integer by adding 1.5 * 2^52, whose low bits then are the exponent, and the polynomial of
-// degree 9 through 2^r at Chebyshev's points of [-1/2, 1/2], its constant set to 1 (2^0 is 1): 3.2e-14 of the value at most.
-__device__ __forceinline__ double power_of_two(double t)
-{
-    constexpr double kRound = 6755399441055744.0;
-    const double u = t + kRound, r = t - (u - kRound);
-    double v = 1.0205905413765595e-07;
-    v = fma(v, r, 1.325964524488711e-06);
-    v = fma(v, r, 1.5252672924850737e-05);
-    v = fma(v, r, 0.0001540343375125101);
-    v = fma(v, r, 0.0013333558200794592);
-    v = fma(v, r, 0.009618129193934313);
-    v = fma(v, r, 0.05550410866465167);
-    v = fma(v, r, 0.2402265069564034);
-    v = fma(v, r, 0.6931471805599462);
-    v = fma(v, r, 1.0);
-    int2 bits = __builtin_bit_cast(int2, v);
-    bits.y += __builtin_bit_cast(int2, u).x << 20;
-    return __builtin_bit_cast(double, bits);
-}
 
 // The lane's that CTRL names within the rows of ROWS, 0 where there is none.
 template <int CTRL, int ROWS>

@@ -250,7 +250,7 @@ def test_captured_steps_give_what_eager_ones_do(lib, rows, n):
     dev = rows_of(x, "bf16")
     dl, dt = torch.from_numpy(labels).cuda(), torch.from_numpy(teacher.astype(np.float32)).cuda()
     out, value, stats = torch.empty_like(dev), torch.zeros(rows + 1, device="cuda"), torch.zeros(rows + 1, 2, device="cuda")
-    out2 = torch.empty_like(dev)
+    out2, value2 = torch.empty_like(dev), torch.zeros(rows + 1, device="cuda")
     work = workspace(lib, rows, n)
     step(lib, dev, "bf16", dl, dt, None, 2.0, None, out, value, work=work)
     torch.cuda.synchronize()
@@ -258,14 +258,52 @@ def test_captured_steps_give_what_eager_ones_do(lib, rows, n):
     with torch.cuda.graph(graph):
         stream = torch.cuda.current_stream().cuda_stream
         step(lib, dev, "bf16", dl, dt, None, 2.0, None, out, value, stream=stream, work=work)
-        loss(lib, dev, "bf16", dl, dt, None, 2.0, stream=stream, out=(value, stats), work=work)
+        loss(lib, dev, "bf16", dl, dt, None, 2.0, stream=stream, out=(value2, stats), work=work)
         gradient(lib, dev, "bf16", dl, dt, None, 2.0, stats, None, out2, stream=stream)
     for _ in range(3):
         dev.copy_(dev.roll(1, 1))
         want = torch.empty_like(dev)
         one = step(lib, dev, "bf16", dl, dt, None, 2.0, None, want)
+        two, _ = loss(lib, dev, "bf16", dl, dt, None, 2.0)
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(out, want) and torch.equal(value[:rows], one[:rows])
+        assert torch.equal(out, want) and torch.equal(value[:rows], one[:rows]) and torch.equal(value2[:rows], two[:rows])
         assert (out2.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+
+
+# Rows that a workgroup keeps in its registers while it writes those before them: every size of a workgroup, and more rows than
+# workgroups are resident, in an order in which all kinds of rows follow each other.
+@pytest.mark.parametrize("T", [1.0, 1e-6])
+@pytest.mark.parametrize("kind,rows,n,k", [("f32", 4400, 13, 3), ("bf16", 4400, 1003, 20), ("bf16", 5000, 260, 256), ("f16", 4200, 8192, 9),
+                                           ("f32", 2200, 4100, 20), ("bf16", 2200, 16_384, 20), ("f16", 2300, 1000, 300),
+                                           ("bf16", 1100, 17_001, 20), ("f32", 1100, 16_384, 300), ("f16", 600, 60_000, 20),
+                                           ("bf16", 300, 131_072, 20), ("f32", 300, 65_533, 20), ("bf16", 300, 70_007, 300)])
+def test_rows_in_registers(lib, kind, rows, n, k, T):
+    x, labels, teacher = task(13, n, k, 21)
+    x[1] = -np.inf
+    x[3, n // 2] = np.nan
+    x[4, n - 1] = np.inf
+    x[5] = float(torch.finfo(TYPES[kind][1]).min)
+    x[6] = float(torch.finfo(TYPES[kind][1]).min)
+    x[6, n - 1] = 0.0
+    x[7, 1:] = -np.inf
+    x[8] = float(torch.finfo(TYPES[kind][1]).max)
+    labels[9] = -1
+    labels[10] = n // 3
+    teacher[11] = -np.inf
+    labels[7] = 0
+    T = float(np.float32(T))
+    first = rows_of(x, kind)
+    of = torch.arange(rows, device="cuda") % 13
+    dev = first[of]
+    dl, dt = torch.from_numpy(labels).cuda()[of].contiguous(), torch.from_numpy(teacher.astype(np.float32)).cuda()[of].contiguous()
+    out = torch.full((rows + 1, n), 5.0, dtype=dev.dtype, device="cuda")
+    value = step(lib, dev, kind, dl, dt, None, T, None, out)
+    as64 = lambda t: t.double().cpu().numpy()
+    compare(kind, T, as64(first), labels, as64(dt[:13]), None, None, as64(value[:13]), as64(out[:13]))
+    assert value[rows] == 9 and (out[rows] == 5).all()
+    assert torch.equal(value[:rows].nan_to_num(7.0), value[:13][of].nan_to_num(7.0))
+    assert torch.equal(out[:rows].nan_to_num(7.0), out[:13][of].nan_to_num(7.0))
+    both = step(lib, dev, kind, dl, dt, None, T, None, dev)
+    assert torch.equal(both.nan_to_num(7.0), value.nan_to_num(7.0)) and torch.equal(dev.nan_to_num(7.0), out[:rows].nan_to_num(7.0))
