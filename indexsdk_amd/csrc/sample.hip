@@ -101,10 +101,7 @@ struct SampleShared {
         };
     };
     double segment[kSegments];
-    union {
-        uint16_t segment_of[kList];
-        uint64_t best[kFew];        // the highest of a longer list
-    };
+    uint64_t best[kFew];            // the highest of a longer list
     double box[2][16];
     uint32_t tops[64];
     uint32_t ubox[16], lows[16];
@@ -435,6 +432,12 @@ struct Sampler {
         return total;
     }
 
+    // what weights of up to 1 are multiplied by to be integers of which n can be added up
+    __device__ __forceinline__ double fixed_point() const
+    {
+        return __builtin_ldexp(1.0, 62 - (64 - __builtin_clzll((unsigned long long)n)));
+    }
+
     // The first of BINS bins at which the running sum of value(bin), with `before` in front of the first, reaches `goal`, or the last
     // with a value; `before` becomes the sum in front of it.
     template <int BINS, typename F>
@@ -493,7 +496,7 @@ struct Sampler {
 
     // The place (score and column) of the last column kept: the count or (by_mass) the sum of weights up to it reaches `goal`.  Where
     // `summed`, the sums of segments of what is kept, min_p apart, are in lds.segment afterwards, their total in `total`.
-    __device__ __forceinline__ uint64_t find_cut(const Row &r, float low, double goal, bool by_mass, bool &summed, double &total)
+    __device__ __forceinline__ uint64_t find_cut(const Row &r, float low, double goal, bool by_mass, double whole, bool &summed, double &total)
     {
         // Counts in bins of equal width in the scores, for sums down to weights of 2^-64; a bin's weights are its count times that of
         // its middle.  That is only where to look: sums in 64 bits decide.
@@ -519,14 +522,25 @@ struct Sampler {
         });
         double before = 0.0;
         const float step_down = unit > 0.f ? (float)r.scale / unit : 0.f;
-        int bin = cross<kBins>([&](int b) {
+        auto about = [&](int b) {
             const double c = (double)lds.count[b];
             return by_mass ? c * (double)__builtin_amdgcn_exp2f(((float)b + 0.5f) * -step_down) : c;
-        }, goal, before);
+        };
+        __syncthreads();
+        // What these are off by comes from the few columns with large weights: as much is added to the goal as all are off by.
+        double off = 0.0;
+        if (whole > 0.0) {
+            for (int b = tid; b < kBins; b += NT) {
+                off += about(b);
+            }
+            off = block_sum(off) - whole;
+        }
+        int bin = cross<kBins>(about, goal + off, before);
         // The bin and its neighbours, as long as the list is likely to hold them: where the counts were off by little, the cut still
         // is among these.  That scores next to a threshold may fall to either side of the bins' edge does not matter.
         int first = bin, last = bin;
-        uint32_t room = lds.count[bin] < kList / 2 ? kList / 2 - lds.count[bin] : 0u;
+        const uint32_t likely = whole > 0.0 || !by_mass ? kFew : kList / 2;
+        uint32_t room = lds.count[bin] < likely ? likely - lds.count[bin] : 0u;
         for (int i = 1; i <= kAround; i++) {
             const uint32_t up = bin - i >= 0 ? lds.count[bin - i] : 0u, down = bin + i < kBins ? lds.count[bin + i] : 0u;
             if (up + down > room) {
@@ -546,18 +560,18 @@ struct Sampler {
             total = collect(per, r, bottom, high, above);
             before = by_mass ? total : above;
             m = (int)min(lds.listed, (uint32_t)kList + 1u);
-            if (m > kList) {
-                break;
+            double upto = __builtin_inf();     // of more than the list holds: not known, and not needed
+            if (m <= kList) {
+                sort(m);
+                for (int i = tid; i < m; i += NT) {
+                    lds.sum[i] = r.weight(score_of((uint32_t)(lds.list[i] >> 32)));
+                }
+                __syncthreads();
+                if (by_mass) {
+                    scan(lds.sum, m);
+                }
+                upto = before + (m == 0 ? 0.0 : by_mass ? lds.sum[m - 1] : (double)m);
             }
-            sort(m);
-            for (int i = tid; i < m; i += NT) {
-                lds.sum[i] = r.weight(score_of((uint32_t)(lds.list[i] >> 32)));
-            }
-            __syncthreads();
-            if (by_mass) {
-                scan(lds.sum, m);
-            }
-            const double upto = before + (m == 0 ? 0.0 : by_mass ? lds.sum[m - 1] : (double)m);
             const bool under = before >= goal && high < inf && way <= 0, over = upto < goal && bottom > least && way >= 0;
             __syncthreads();
             if (!under && !over) {
@@ -575,7 +589,7 @@ struct Sampler {
         }
         if (m > kList) {
             summed = false;
-            return find_tie(r, [&](float x) { return x >= bottom && x <= high; }, before, goal, by_mass);
+            return find_tie(r, bottom, high, before, goal, by_mass);
         }
         const double left = goal - before;
         int take = by_mass ? reach(left, m) : left < (double)m ? (int)left : m;
@@ -583,71 +597,86 @@ struct Sampler {
         take = max(take, min(1, m));
         // an empty list: everything above it is kept, or everything that is there
         const uint64_t place = m > 0 ? lds.list[take - 1] : before >= goal ? (uint64_t)(key_of(high) + 1) << 32 : 0;
-        // to the segments, by each of them in the list's order
+        // to the segments, as integers: their sums do not depend on an order
         const int64_t columns = per * kBlock;
-        for (int i = tid; i < take; i += NT) {
-            lds.segment_of[i] = (uint16_t)((int64_t)(~(uint32_t)lds.list[i]) / columns);
+        const int segments = (int)((blocks() + per - 1) / per);
+        const double fixed = fixed_point();
+        __syncthreads();       // the list's sums have been read: the tallies take their place
+        for (int g = tid; g < segments; g += NT) {
+            lds.tally[g] = 0;
         }
         __syncthreads();
-        const int segments = (int)((blocks() + per - 1) / per);
+        for (int i = tid; i < take; i += NT) {
+            const uint64_t e = lds.list[i];
+            atomicAdd(&lds.tally[(int64_t)(~(uint32_t)e) / columns],
+                      (unsigned long long)__builtin_rint(r.weight(score_of((uint32_t)(e >> 32))) * fixed));
+        }
+        __syncthreads();
         for (int g = tid; g < segments; g += NT) {
-            double v = lds.segment[g];
-            for (int i = 0; i < take; i++) {
-                const double prior = by_mass && i > 0 ? lds.sum[i - 1] : 0.0, own = lds.sum[i] - prior;
-                v += lds.segment_of[i] == g ? own : 0.0;
-            }
-            lds.segment[g] = v;
+            lds.segment[g] += (double)lds.tally[g] / fixed;
         }
         total = segment_total(segments);
         summed = true;
         return place;
     }
 
-    // The same where a bin holds too many for the list: by the bits of their keys, ten at a time, and among equal scores by column.
-    template <typename B>
-    __device__ __forceinline__ uint64_t find_tie(const Row &r, B in_bin, double before, double goal, bool by_mass)
+    // The same where [low, high] holds too many for the list, `before` above it: where they are equal, among these, else among all up
+    // to `high` by the bits of their keys, ten at a time; among equal scores by column.
+    __device__ __forceinline__ uint64_t find_tie(const Row &r, float low, float high, double before, double goal, bool by_mass)
     {
-        const double fixed = by_mass ? __builtin_ldexp(1.0, 62 - (64 - __builtin_clzll((unsigned long long)n))) : 1.0;
-        double run = before * fixed;
-        uint32_t prefix = 0, known = 0, top = 0, bottom = 0;
         const int64_t per = segment_size();
+        uint32_t prefix = 0, top = 0, bottom = 0;
         each([&](int64_t, const float(&x)[kEight]) {
 #pragma unroll
             for (int i = 0; i < kEight; i++) {
-                const uint32_t key = in_bin(x[i]) ? key_of(x[i]) : 0u;
+                const uint32_t key = x[i] >= low && x[i] <= high ? key_of(x[i]) : 0u;
                 top = max(top, key);
                 bottom = max(bottom, key ? ~key : 0u);
             }
         });
         top = block_max(top);
         bottom = ~block_max(bottom);
-        prefix = top == bottom ? top : 0u;
-        for (int shift = top == bottom ? 0 : 32; shift > 0;) {
-            const int bits = min(10, shift), to = shift - bits;
-            const uint32_t mask = (1u << bits) - 1u;
-            __syncthreads();
-            for (int i = tid; i < kDigits; i += NT) {
-                lds.tally[i] = 0;
-            }
-            __syncthreads();
-            each([&](int64_t, const float(&x)[kEight]) {
-#pragma unroll
-                for (int i = 0; i < kEight; i++) {
-                    const uint32_t key = key_of(x[i]);
-                    if (key && in_bin(x[i]) && (key & known) == prefix) {
-                        // integers: in any order; the largest scores first
-                        atomicAdd(&lds.tally[~(key >> to) & mask], by_mass ? (unsigned long long)__builtin_rint(r.weight(x[i]) * fixed) : 1ull);
-                    }
-                }
-            });
-            prefix |= (~(uint32_t)cross<kDigits>([&](int b) { return (double)lds.tally[b]; }, goal * fixed, run) & mask) << to;
-            known |= mask << to;
-            shift = to;
-        }
-        const double w = by_mass ? r.weight(score_of(prefix)) : 1.0;
         auto tie = [&](float v, uint32_t) { return key_of(v) == prefix ? 1.0 : 0.0; };
-        const double ties = segment_sums(per, tie);
-        const double take = fmax(1.0, fmin(ties, w > 0.0 ? ceil((goal - run / fixed) / w) : ties));
+        double ties = 0.0, w = 1.0;
+        if (top == bottom) {
+            prefix = top;
+            w = by_mass ? r.weight(score_of(prefix)) : 1.0;
+            ties = segment_sums(per, tie);
+        }
+        if (top != bottom || before + ties * w < goal) {
+            const double fixed = by_mass ? fixed_point() : 1.0;
+            double run = before * fixed;
+            uint32_t known = 0;
+            prefix = 0;
+#pragma unroll 1
+            for (int shift = 32; shift > 0;) {
+                const int bits = min(10, shift), to = shift - bits;
+                const uint32_t mask = (1u << bits) - 1u;
+                __syncthreads();
+                for (int i = tid; i < kDigits; i += NT) {
+                    lds.tally[i] = 0;
+                }
+                __syncthreads();
+                each([&](int64_t, const float(&x)[kEight]) {
+#pragma unroll
+                    for (int i = 0; i < kEight; i++) {
+                        const uint32_t key = key_of(x[i]);
+                        if (key && x[i] <= high && (key & known) == prefix) {
+                            // integers: in any order; the largest scores first
+                            atomicAdd(&lds.tally[~(key >> to) & mask],
+                                      by_mass ? (unsigned long long)__builtin_rint(r.weight(x[i]) * fixed) : 1ull);
+                        }
+                    }
+                });
+                prefix |= (~(uint32_t)cross<kDigits>([&](int b) { return (double)lds.tally[b]; }, goal * fixed, run) & mask) << to;
+                known |= mask << to;
+                shift = to;
+            }
+            before = run / fixed;
+            w = by_mass ? r.weight(score_of(prefix)) : 1.0;
+            ties = segment_sums(per, tie);
+        }
+        const double take = fmax(1.0, fmin(ties, w > 0.0 ? ceil((goal - before) / w) : ties));
         int64_t at;
         double one;
         locate(per, take - 0.5, tie, at, one);
@@ -1028,9 +1057,17 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
     if (set.filtered) {
         const bool complete = h.bound == 1;      // every column that is there is in the list
         const int m = h.listed <= kList ? (int)h.listed : 0;
+        bool hopeless = false;      // the whole list is short of what p takes
+        if (m > kFew && set.by_mass && !set.by_count && !complete && set.min_p == 0.0) {
+            double sum = 0.0;
+            for (int i = tid; i < m; i += NT) {
+                sum += r.weight(score_of((uint32_t)(s.list[i] >> 32)));
+            }
+            hopeless = k.block_sum(sum) < 0.999 * set.top_p * total;
+        }
         // All candidates, or the highest of them, if they are few.
         int high = m;
-        if (m > kFew && h.high != 0xffffffffu) {
+        if (m > kFew && !hopeless && h.high != 0xffffffffu) {
             if (tid == 0) {
                 s.found_best = 0;
             }
@@ -1046,17 +1083,9 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
             __syncthreads();
             high = (int)s.found_best;
         }
-        if (high > 0 && high <= kFew &&
+        if (!hopeless && high > 0 && high <= kFew &&
             finish_few(k, p, set, r, high < m ? s.best : s.list, high, complete && high == m, total, labels, probs, draw_number)) {
             return;
-        }
-        bool hopeless = false;      // the whole list is short of what p takes
-        if (m > kFew && set.by_mass && !set.by_count && !complete && set.min_p == 0.0) {
-            double sum = 0.0;
-            for (int i = tid; i < m; i += NT) {
-                sum += r.weight(score_of((uint32_t)(s.list[i] >> 32)));
-            }
-            hopeless = k.block_sum(sum) < 0.999 * set.top_p * total;
         }
         if (m > kFew && !hopeless) {
             int take = m;
@@ -1138,7 +1167,8 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
                 // the sum up to the cut by its columns
                 sum = k.segment_sums(per, [&](float x, uint32_t c) { return key_of(x) && r.place(key_of(x), c) >= r.least ? r.weight(x) : 0.0; });
             }
-            const uint64_t least = k.find_cut(r, low, mass ? set.top_p * sum : (double)count, mass, summed, sum);
+            const uint64_t least = k.find_cut(r, low, mass ? set.top_p * sum : (double)count, mass, mass && !set.by_count ? total : 0.0, summed,
+                                             sum);
             summed = summed && least >= r.least;
             r.least = larger(r.least, least);
         }

@@ -244,3 +244,30 @@ def test_the_same_draws_every_time(lib):
     for _ in range(5):
         again = call(lib, x, "bf16", u, **s)[:2]
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# More equal scores than a list holds on both sides of a cut, which lies a few columns off the border between them or on it.
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("off", [-40, -1, 0, 1, 40])
+@pytest.mark.parametrize("with_count", [False, True])
+def test_cuts_next_to_many_equal_scores(lib, kind, off, with_count):
+    n, many = 30_000, 5000
+    rng = np.random.default_rng(7)
+    x = np.full((4, n), -20.0) + rng.integers(0, 4, (4, n)) / 4
+    at = rng.permutation(n)
+    x[:, at[:many]] = 0.0
+    x[:, at[many:2 * many]] = -1.0
+    x[2:, at[2 * many:2 * many + 50]] = rng.integers(1, 9, 50) / 8      # a few larger ones
+    x[1, at[many:2 * many]] = -0.0078125
+    x[3, at[2 * many + 60:2 * many + 70]] = -0.25
+    w = np.exp(x - x.max(1, keepdims=True))
+    count = 2 * many + 1000
+    if with_count:
+        w = -np.sort(-w, 1)[:, :count]
+    # in the middle of a column's weight
+    weights = np.exp(x - x.max(1, keepdims=True))
+    goal = np.where(x >= 0, weights, 0).sum(1) + (off + 0.5) * np.exp((-1.0 if off >= 0 else 0.0) - x.max(1))
+    settings = {"top_p": np.float32(goal / w.sum(1))}
+    if with_count:
+        settings["top_k"] = count
+    check(lib, x, kind, draws=8, **settings)
