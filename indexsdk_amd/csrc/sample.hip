@@ -33,6 +33,7 @@ constexpr int kSegments = 512;      // at most: parts of a row whose sums are ke
 constexpr int kBlock = 512;         // columns that a wavefront reads at a time
 constexpr int kTurns = 4;           // such blocks in flight
 constexpr int kSample = 2;          // blocks of each wavefront that the bound comes from
+constexpr int kSmall = 64;          // entries that are sorted by exchanges, or by counting
 constexpr int kFew = 256;           // candidates that every wavefront holds in registers, four per lane
 constexpr int kOneWave = 32;        // draws up to which one wavefront makes them all
 constexpr int kMaxParts = 16, kPartThreads = 512;
@@ -102,6 +103,7 @@ struct SampleShared {
     };
     double segment[kSegments];
     uint64_t best[kFew];            // the highest of a longer list
+    uint32_t places[kDigits];       // of parts of the list
     double box[2][16];
     uint32_t tops[64];
     uint32_t ubox[16], lows[16];
@@ -251,8 +253,93 @@ struct Sampler {
         __syncthreads();
     }
 
-    // list[0 ... m) in falling order (m <= kList)
+    // list[0 ... m) in falling order (m <= kList): by 1024 parts of the range of the keys' upper halves, and in each part by counting
+    // the larger ones.
     __device__ __forceinline__ void sort(int m) const
+    {
+        constexpr int kOwn = (kList + NT - 1) / NT, kPer = kDigits / NT > 0 ? kDigits / NT : 1;
+        if (m <= kSmall) {
+            return sort_by_exchange(m);
+        }
+        uint64_t e[kOwn];
+        uint32_t top = 0, low = 0;
+#pragma unroll
+        for (int u = 0; u < kOwn; u++) {
+            const int i = u * NT + tid;
+            e[u] = i < m ? lds.list[i] : 0;
+            top = max(top, (uint32_t)(e[u] >> 32));
+            low = max(low, i < m ? ~(uint32_t)(e[u] >> 32) : 0u);
+        }
+        top = block_max(top);
+        low = ~block_max(low);
+        const int shift = max(0, 32 - __builtin_clz((top - low) | 1u) - 10);
+        auto part_of = [&](uint64_t v) { return (top - (uint32_t)(v >> 32)) >> shift; };
+        for (int i = tid; i < kDigits; i += NT) {
+            lds.places[i] = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kOwn; u++) {
+            if (u * NT + tid < m) {
+                atomicAdd(&lds.places[part_of(e[u])], 1u);
+            }
+        }
+        __syncthreads();
+        uint32_t n_of[kPer], sum = 0, most = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            n_of[i] = tid * kPer + i < kDigits ? lds.places[tid * kPer + i] : 0u;
+            sum += n_of[i];
+            most = max(most, n_of[i]);
+        }
+        if (block_max(most) > (uint32_t)kSmall) {
+            return sort_by_exchange(m);      // many equal ones, or few far from the others
+        }
+        const double upto = wave_scan((double)sum);
+        if (lane == 63) {
+            lds.box[1][wave] = upto;
+        }
+        __syncthreads();
+        uint32_t start = (uint32_t)upto - sum;
+        for (int w = 0; w < wave; w++) {
+            start += (uint32_t)lds.box[1][w];
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            if (tid * kPer + i < kDigits) {
+                lds.places[tid * kPer + i] = start;
+            }
+            start += n_of[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kOwn; u++) {
+            if (u * NT + tid < m) {
+                lds.list[atomicAdd(&lds.places[part_of(e[u])], 1u)] = e[u];     // now where the next part starts
+            }
+        }
+        __syncthreads();
+        uint32_t to[kOwn];
+#pragma unroll
+        for (int u = 0; u < kOwn; u++) {
+            const uint32_t part = part_of(e[u]);
+            const bool there = u * NT + tid < m;
+            const int from = there && part > 0 ? (int)lds.places[part - 1] : 0, end = there ? (int)lds.places[part] : 0;
+            to[u] = (uint32_t)from;
+            for (int i = from; i < end; i++) {
+                to[u] += lds.list[i] > e[u] ? 1u : 0u;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kOwn; u++) {
+            if (u * NT + tid < m) {
+                lds.list[to[u]] = e[u];
+            }
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void sort_by_exchange(int m) const
     {
         int size = 2;
         while (size < m) {
