@@ -10,10 +10,14 @@
 // bits: an exponential is 13 instructions of the same rate as in 32.
 //
 // One workgroup per row reads it once (a few, each a part, where there are few rows).  The largest scores of some of its columns
-// give a bound that about a hundred scores of the row reach; these go to a list in LDS, and while k or p or m keep no more than what
+// give a bound that a few hundred scores of the row reach; these go to a list in LDS, and while k or p or m keep no more than what
 // is in the list, all else happens there: sorted by score, cut, and drawn from.  Rows without filters are drawn from by the sums
-// of their segments.  Everything else (flat rows whose p keeps thousands, large k) reads the row again: a histogram of counts and
-// weights finds the bin in which the cut lies, whose columns go through the list.
+// of their segments.  Everything else (flat rows whose p keeps thousands, large k) reads the row twice again: a histogram of counts
+// finds the bins around the cut, whose columns go through the list while the weights above them are added up.
+//
+// What bounds it: one read of the scores where k cuts (1024 rows of 100003 bf16: 67 us, 3.1 TB/s), the exponentials in 64 bits where
+// all of a row's are needed (without filters 99 us, with top-p 134 us, with settings that leave every fifth row flat 190 us), and
+// for a few rows the steps of one workgroup that wait for each other (a row of 32768 fp32 under all filters: 13 us).
 #include "power_of_two.h"
 #include "row_access.h"
 #include "scores.h"
@@ -873,7 +877,7 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
             h.bound = reach <= 130.f ? bound_for(reach) : h.bound;
         } else {
             // what a sum takes is not known ahead: a few hundred, and the highest of them first
-            h.bound = bound_for(fminf(640.f / (float)parts * share + 4.f, 130.f));
+            h.bound = bound_for(fminf(350.f / (float)parts * share + 4.f, 130.f));
             h.high = bound_for(fminf(140.f / (float)parts * share + 1.f, 100.f));
         }
     }
@@ -1398,11 +1402,11 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
     finish_row(k, p, set, row, all, total);
 }
 
-// Parts of each row where there are few rows: as many as give every second CU a workgroup, of 16384 columns at least (64 rows of
-// 131072 under top-p: SAMPLE_PARTS).
+// Parts of each row where there are few rows: as many as give every CU two workgroups, of 16384 columns at least.  Rows of 131072 fp32
+// scores under top-p: one takes 26 us, 40 as a whole; 64 take 46 us, 60 as whole rows; 256 would take 67 us, 66 as whole rows.
 int parts_of(int64_t rows, int64_t n)
 {
-    if (rows == 0 || rows > 256 || n < 65536) {
+    if (rows == 0 || rows > 128 || n < 65536) {
         return 1;
     }
     return (int)std::min<int64_t>({kMaxParts, std::max<int64_t>(2, 512 / rows), n / 16384});
