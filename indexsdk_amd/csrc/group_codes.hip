@@ -6,7 +6,8 @@
 // The quotient is rounded to fp32 and then to the scale's type, and ends at that type's largest number; with the scale as it is
 // stored, code = x / scale rounded to the nearest integer (halfway to even), plus zero, clamped to 0 ... 15.  Where the scale is
 // 0 all values are.  A group with an infinity or a NaN gets a NaN scale and codes that stand for zeros.
-// Both directions move every byte once and are bound by memory.
+// Both directions move every byte once and are bound by memory: 1,000,003 x 200 fp32 rows in steps of 208 take 179 us into codes
+// (5.1 TB/s) and 207 back (4.5), 131072 x 4096 462 (5.2) and 544 (4.5).  Two rows in flight per thread; four are no faster.
 #include "row_access.h"
 
 #include <algorithm>
@@ -291,6 +292,9 @@ void op_group_dequantise(const uint8_t *codes, const void *scales, const uint8_t
     if (n == 0) {
         return;
     }
+    // Rows that do not fit into the last cache go past it: 1,000,003 x 200 fp32 222 -> 207 us, and a quantisation that follows has no lines to
+    // write back, 216 -> 179; 131072 x 4096 615 -> 544 and 506 -> 462.  16384 x 768, which fit, 13.8 -> 19.5.
+    const bool past = (double)n * (double)ld * (double)element_bytes(type) > 0x1p27;
     GroupParams p = params(n, d, group, scale_type);
     p.out = out;
     p.ld = ld;
@@ -300,7 +304,11 @@ void op_group_dequantise(const uint8_t *codes, const void *scales, const uint8_t
     with_type(type, [&](auto t) {
         with_group(group, [&](auto g) {
             in_launches(p, [&](const GroupParams &q, dim3 grid) {
-                hipLaunchKernelGGL((group_read_kernel<decltype(t), decltype(g)::value, false>), grid, dim3(kThreads), 0, s, q);
+                if (past) {
+                    hipLaunchKernelGGL((group_read_kernel<decltype(t), decltype(g)::value, true>), grid, dim3(kThreads), 0, s, q);
+                } else {
+                    hipLaunchKernelGGL((group_read_kernel<decltype(t), decltype(g)::value, false>), grid, dim3(kThreads), 0, s, q);
+                }
             });
         });
     });
