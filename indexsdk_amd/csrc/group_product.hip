@@ -209,7 +209,8 @@ __device__ __forceinline__ void store_scores(const GroupProductParams &p, int64_
             s[j] = (T)v[j];
         }
         if (col + N <= p.n) {
-            *reinterpret_cast<Scores *>(out + at) = s;
+            // past the caches, which keep what is read again: 2048 x 131072 scores 733 -> 635 us, 64 x 1M 163 -> 132, few ones as fast
+            __builtin_nontemporal_store(s, reinterpret_cast<Scores *>(out + at));
         } else {
 #pragma unroll
             for (int j = 0; j < N; j++) {

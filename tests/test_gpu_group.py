@@ -381,3 +381,17 @@ def test_quantised_rows_score_as_their_values(lib):
     lib[1](lib[0].ixa_op_topk_flat_fp32(at(scores), m, n, n, 3, 1, at(dist), at(label), None))
     exact = torch.cdist(x[:m].double(), back.double()).topk(3, largest=False).indices
     assert (label[:, 0] == torch.arange(m, device="cuda")).all() and (label == exact).float().mean() > 0.95
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_many_rows_read_back_are_those_of_few(lib, kind):
+    n, d, group = 400_000 if kind == "bf16" else 200_000, 201, 32
+    store = Store.random(n, d, group, "f16", True, np.random.default_rng(4))
+    read = lambda codes, scales, zeros, rows_, out: lib[1](lib[0].ixa_op_group_dequantise(
+        at(codes), at(scales), at(zeros), group, 1, rows_, d, TYPES[kind][0], at(out), d, None))
+    out, part = torch.empty(n, d, dtype=TYPES[kind][1], device="cuda"), torch.empty(50_000, d, dtype=TYPES[kind][1], device="cuda")
+    read(store.codes, store.scales, store.zeros, n, out)
+    for first in range(0, n, 50_000):
+        slot = first * store.ng
+        read(store.codes[slot * group // 2:], store.scales[slot:], store.zeros[slot:], 50_000, part)
+        assert torch.equal(out[first:first + 50_000], part)
