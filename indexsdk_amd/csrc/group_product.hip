@@ -387,6 +387,9 @@ __global__ __launch_bounds__(W * 64) void group_stream_kernel(GroupProductParams
                 constexpr int kBlocks = 4 / SG;   // of 32 columns per group, 4 of a step
 #pragma unroll
                 for (int g = 0; g < SG; g++) {
+                    if (g > 0 && (t + u) * SG + g >= p.groups) {
+                        break;      // x has zeros there
+                    }
                     v4f sum[MF][NF] = {};
 #pragma unroll
                     for (int b = 0; b < kBlocks; b++) {
@@ -609,6 +612,9 @@ __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p
         };
 #pragma unroll
         for (int g = 0; g < SG; g++) {
+            if (g > 0 && step * SG + g >= p.groups) {
+                break;      // x has zeros there
+            }
             h2 minus[4];
             float scale[4];
 #pragma unroll
@@ -773,7 +779,8 @@ void launch_tiles(const GroupProductParams &p, hipStream_t s)
     const int64_t per_xcd = (row_tiles * col_tiles + 7) / 8;
     IXA_REQUIRE(per_xcd * 8 * 256 <= 0xffffffffll, kErrInvalidParam, "group_product: %ld x %ld scores in one call", (long)p.m,
                 (long)p.n);
-    constexpr size_t lds = 2 * ((size_t)P * WM * 64 * 256 + 2 * WN * 64 * SG * 4);
+    // one buffer where there is one step: of two pieces two workgroups share a CU then
+    const size_t lds = std::min(p.steps, 2) * ((size_t)P * WM * 64 * 256 + 2 * WN * 64 * SG * 4);
     const auto kern = group_tile_kernel<P, WM, WN, SG, WIDE>;
     require_dynamic_lds(reinterpret_cast<const void *>(kern), lds);
     hipLaunchKernelGGL(kern, dim3((unsigned)per_xcd * 8), dim3(256), lds, s, p, (int)row_tiles, (int)col_tiles, (int)per_xcd);

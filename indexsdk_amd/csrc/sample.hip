@@ -38,6 +38,7 @@ constexpr int kBlock = 512;         // columns that a wavefront reads at a time
 constexpr int kTurns = 4;           // such blocks in flight
 constexpr int kSample = 2;          // blocks of each wavefront that the bound comes from
 constexpr int kSmall = 64;          // entries that are sorted by exchanges, or by counting
+constexpr int kReach = 350;         // candidates that p is hoped to be content with
 constexpr int kFew = 256;           // candidates that every wavefront holds in registers, four per lane
 constexpr int kOneWave = 32;        // draws up to which one wavefront makes them all
 constexpr int kMaxParts = 16, kPartThreads = 512;
@@ -823,8 +824,11 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
     // The largest of 64 groups of lanes in some of the columns: sixteen per lane, or all there are.
     constexpr int kLanes = kWaves;
     float lane_top = -inf, lane_low = inf;
-    auto see = [&](float x) {
-        lane_top = fmaxf(lane_top, x);
+    const int each = (int)min((int64_t)kOwn, (columns + NT - 1) / NT);
+    // of columns that many of the sampled ones of which are wanted fewer are sampled: every group would have one
+    const int seen = set.by_count ? kOwn : (int)min((int64_t)each, 1 + columns * 100 / ((int64_t)kReach / parts * NT));
+    auto see = [&](float x, bool counts) {
+        lane_top = counts ? fmaxf(lane_top, x) : lane_top;
         lane_low = x > -inf ? fminf(lane_low, x) : lane_low;
     };
     if (columns > NT * kOwn) {
@@ -834,14 +838,13 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
             const Eight<T> e = k.load(first + u);
 #pragma unroll
             for (int i = 0; i < kEight; i++) {
-                see((float)e.v[i]);
+                see((float)e.v[i], u * kEight + i < seen);
             }
         }
     } else if (columns > 0) {
-        const int each = (int)((columns + NT - 1) / NT);
 #pragma unroll
         for (int i = 0; i < kOwn; i++) {
-            see((float)k.row[b0 * kBlock + min((int64_t)k.tid * each + min(i, each - 1), columns - 1)]);
+            see((float)k.row[b0 * kBlock + min((int64_t)k.tid * each + min(i, each - 1), columns - 1)], i < seen);
         }
     }
     const int flip = (int)0x80000000;
@@ -857,7 +860,7 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
     // many more than expected as three deviations.
     PartHead h{0, 0, sample_top, 0xffffffffu, 0, 1, 0xffffffffu, 0};
     if (set.filtered && sample_top) {
-        const float share = columns > NT * kOwn ? (float)(NT * kOwn) / (float)columns : 1.f;
+        const float share = columns > NT * kOwn ? (float)(NT * min(seen, kOwn)) / (float)columns : fminf(1.f, (float)seen / (float)each);
         // the highest bound that one of so many of 64 groups of the sampled columns reaches as hold one of `reach` columns at least
         auto bound_for = [&](float reach) {
             const int groups = (int)fminf(60.f, 64.f * (1.f - __expf(-reach / 64.f)) + 1.5f);
@@ -877,7 +880,7 @@ __device__ __forceinline__ PartHead scan_part(const Sampler<T, NT> &k, const Set
             h.bound = reach <= 130.f ? bound_for(reach) : h.bound;
         } else {
             // what a sum takes is not known ahead: a few hundred, and the highest of them first
-            h.bound = bound_for(fminf(350.f / (float)parts * share + 4.f, 130.f));
+            h.bound = bound_for(fminf((float)kReach / (float)parts * share + 4.f, 130.f));
             h.high = bound_for(fminf(140.f / (float)parts * share + 1.f, 100.f));
         }
     }
