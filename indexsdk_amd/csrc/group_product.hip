@@ -387,8 +387,9 @@ __global__ __launch_bounds__(W * 64) void group_stream_kernel(GroupProductParams
                 constexpr int kBlocks = 4 / SG;   // of 32 columns per group, 4 of a step
 #pragma unroll
                 for (int g = 0; g < SG; g++) {
-                    if (g > 0 && (t + u) * SG + g >= p.groups) {
-                        break;      // x has zeros there
+                    // x has zeros there; where a branch would make registers spill they are multiplied
+                    if (g > 0 && !(P == 2 && MF == 4 && W == 8) && (t + u) * SG + g >= p.groups) {
+                        break;
                     }
                     v4f sum[MF][NF] = {};
 #pragma unroll
