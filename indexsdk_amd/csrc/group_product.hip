@@ -483,34 +483,32 @@ __global__ __launch_bounds__(W * 64) void group_stream_kernel(GroupProductParams
     }
 }
 
-// Rows of x as fp16 pieces for the kernel below, zeros up to whole steps, and the power of two each was multiplied by.
+// Rows of x as fp16 pieces for the kernel below, zeros up to whole steps, and the power of two each was multiplied by.  A wavefront
+// per row: 2048 rows of 768 take 6.8 us, 10.7 with a workgroup per row and its barriers.
 template <int P>
 __global__ __launch_bounds__(256) void group_pieces_kernel(GroupProductParams p, uint8_t *pieces, int *exponents)
 {
-    __shared__ int top_of;
-    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (row >= p.m) {
+        return;
+    }
     const uint8_t *const x_row = static_cast<const uint8_t *>(p.x) + (size_t)row * (size_t)p.ld_x * (p.type == kTypeF32 ? 4 : 2);
     int power = 0;
     if (p.type != kTypeF16) {
-        if (threadIdx.x == 0) {
-            top_of = 0;
-        }
-        __syncthreads();
         int top = 0;
-        for (int c = threadIdx.x; c * kEight < p.d; c += 256) {
+        for (int c = lane; c * kEight < p.d; c += 64) {
             float v[kEight];
             load_eight(x_row, p.type, c * kEight, p.d, v);
             top = max(top, finite_top(v));
         }
-        atomicMax(&top_of, top);
-        __syncthreads();
-        power = power_for(top_of);
+        power = power_for(over_wave(top, [](int a, int b) { return max(a, b); }));
     }
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         exponents[row] = power;
     }
     const int across = p.steps * (kStep / kEight);
-    for (int c = threadIdx.x; c < across; c += 256) {
+    for (int c = lane; c < across; c += 64) {
         float v[kEight];
         h8 piece[P];
         load_eight(x_row, p.type, c * kEight, p.d, v);
@@ -797,7 +795,7 @@ void launch(GroupProductParams &p, uint8_t *workspace, hipStream_t s)
     }
     int *const exponents = reinterpret_cast<int *>(workspace);
     uint8_t *const pieces = workspace + round_up(p.m * 4, 256);
-    hipLaunchKernelGGL((group_pieces_kernel<P>), dim3((unsigned)p.m), dim3(256), 0, s, p, pieces, exponents);
+    hipLaunchKernelGGL((group_pieces_kernel<P>), dim3((unsigned)((p.m + 3) / 4)), dim3(256), 0, s, p, pieces, exponents);
     check_launch();
     p.pieces = pieces;
     p.exponents = exponents;
