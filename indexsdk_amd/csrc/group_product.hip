@@ -16,8 +16,8 @@
 // What bounds it: for few rows the codes, which are read once (one bfloat16 row against 1,000,000 x 768 in groups of 64 with zero
 // points: 88 us, 4.9 TB/s; 64 rows against 1,000,000 x 200: 133 us, two thirds of them stores); for many the vector
 // instructions that make integers of codes, which share a SIMD's issue with the products (2048 x 131,072 x 768 bfloat16 in groups of 128 to
-// bfloat16: 618 us, 0.67 PFLOP/s, the vector unit busy for 57 % and the matrix cores for 28 % of the cycles; in groups of 32 with
-// four times as many multiply-adds to fp32 829 us; fp32 rows, two pieces, 1442 us).
+// bfloat16: 615 us, 0.67 PFLOP/s, the vector unit busy for 57 % and the matrix cores for 28 % of the cycles; in groups of 32 with
+// four times as many multiply-adds to fp32 818 us; fp32 rows, two pieces, 1442 us).
 #include "row_access.h"
 
 #include <algorithm>
