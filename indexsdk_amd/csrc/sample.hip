@@ -32,7 +32,7 @@ namespace {
 constexpr int kList = 2048;         // candidates of a row
 constexpr int kPartList = 1024;     // and of a part of one
 constexpr int kBins = 4096;         // of a histogram of counts
-constexpr int kDigits = 1024, kAround = 32;
+constexpr int kDigits = 1024, kAround = 32, kMoves = 3;
 constexpr int kSegments = 512;      // at most: parts of a row whose sums are kept
 constexpr int kBlock = 512;         // columns that a wavefront reads at a time
 constexpr int kTurns = 4;           // such blocks in flight
@@ -647,7 +647,7 @@ struct Sampler {
         float high = first == 0 || !(unit > 0.f) ? inf : r.top - (float)first / unit;
         float bottom = last >= kBins - 1 || !(unit > 0.f) ? least : r.top - (float)(last + 1) / unit;
         int m, way = 0;
-        for (;;) {
+        for (int moves = 0;; moves++) {
             double above;
             total = collect(per, r, bottom, high, above);
             before = by_mass ? total : above;
@@ -669,14 +669,18 @@ struct Sampler {
             if (!under && !over) {
                 break;
             }
+            if (moves == kMoves) {      // scores so far off, or so near to each other, that bins say little: bit by bit
+                summed = false;
+                return find_tie(r, least, inf, 0.0, goal, by_mass);
+            }
             if (under) {
                 way = -1;
                 bottom = score_of(key_of(high) + 1);
-                high = fminf(high + wide, inf);
+                high = fmaxf(fminf(high + wide, inf), bottom);
             } else {
                 way = 1;
                 high = score_of(key_of(bottom) - 1);
-                bottom = fmaxf(bottom - wide, least);
+                bottom = fminf(fmaxf(bottom - wide, least), high);
             }
         }
         if (m > kList) {

@@ -271,3 +271,19 @@ def test_cuts_next_to_many_equal_scores(lib, kind, off, with_count):
     if with_count:
         settings["top_k"] = count
     check(lib, x, kind, draws=8, **settings)
+
+
+@pytest.mark.parametrize("temperature", [0.5, 4.0, 40.0, 1e4])
+@pytest.mark.parametrize("filters", [{"top_p": 0.3}, {"top_p": 0.9}, {"top_p": 0.9999}, {"top_k": 7001}, {"top_k": 7001, "top_p": 0.7}])
+def test_scores_a_few_steps_of_their_type_apart(lib, temperature, filters):
+    """Bins of a histogram are finer than the scores here, or the scores finer than the type next to them."""
+    rng = np.random.default_rng(17)
+    n = 30_000
+    x = np.empty((5, n))
+    x[0] = 1e8 - 8.0 * rng.integers(0, 30, n)
+    x[1] = -1e8 - 8.0 * rng.integers(0, 30, n)
+    x[2] = 3e30 - 2.0 ** 78 * rng.integers(0, 5, n)
+    x[3] = rng.choice([1e8, 5.0, 4.0, -3e30], n)
+    x[4] = rng.standard_normal(n)
+    x[4, 7] = 1e8
+    check(lib, x, "f32", draws=8, temperature=temperature, **filters)
