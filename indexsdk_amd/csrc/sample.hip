@@ -782,8 +782,8 @@ struct Sampler {
 
     __device__ __forceinline__ int64_t segment_size() const
     {
-        // four blocks where every wavefront gets that many
-        return max(min((int64_t)kTurns, (blocks() + kWaves - 1) / kWaves), (blocks() + kSegments - 1) / kSegments);
+        // four blocks where every wavefront gets that many; a row of no columns has no segment, but what is divided by is not 0
+        return max(max((int64_t)1, min((int64_t)kTurns, (blocks() + kWaves - 1) / kWaves)), (blocks() + kSegments - 1) / kSegments);
     }
 };
 
