@@ -99,7 +99,7 @@ struct SampleShared {
     uint64_t list[kList];           // score's key above the column's complement
     union {
         double sum[kList];          // of the list's weights; a histogram is of no more use by then
-        unsigned long long tally[kDigits];
+        unsigned long long tally[2 * kDigits];
         uint32_t count[kBins];
         struct {
             uint64_t sorted[kFew];
@@ -647,6 +647,7 @@ struct Sampler {
         float high = first == 0 || !(unit > 0.f) ? inf : r.top - (float)first / unit;
         float bottom = last >= kBins - 1 || !(unit > 0.f) ? least : r.top - (float)(last + 1) / unit;
         int m, way = 0;
+        bool lost = false;
         for (int moves = 0;; moves++) {
             double above;
             total = collect(per, r, bottom, high, above);
@@ -669,9 +670,12 @@ struct Sampler {
             if (!under && !over) {
                 break;
             }
-            if (moves == kMoves) {      // scores so far off, or so near to each other, that bins say little: bit by bit
-                summed = false;
-                return find_tie(r, least, inf, 0.0, goal, by_mass);
+            if (moves == kMoves) {      // scores so far off, or so near to each other, that bins say little: all of them
+                lost = true;
+                bottom = least;
+                high = inf;
+                before = 0.0;
+                break;
             }
             if (under) {
                 way = -1;
@@ -683,7 +687,7 @@ struct Sampler {
                 bottom = fminf(fmaxf(bottom - wide, least), high);
             }
         }
-        if (m > kList) {
+        if (lost || m > kList) {
             summed = false;
             return find_tie(r, bottom, high, before, goal, by_mass);
         }
@@ -716,68 +720,110 @@ struct Sampler {
         return place;
     }
 
-    // The same where [low, high] holds too many for the list, `before` above it: where they are equal, among these, else among all up
-    // to `high` by the bits of their keys, ten at a time; among equal scores by column.
+    // The same where [low, high] holds too many for the list, `before` above it: in up to kDigits parts, of which the one with the cut is
+    // looked at again, until it is one key; among equal scores by column.  Where the cut is not among these, all up to `high` are gone through.
+    // Sums of parts are integers, which do not depend on an order: weights relative to the part's highest, in units of 2^-62 and two
+    // words.  So that none is small next to that, a range of weights wider than 2^8 goes by their logarithms first; then by keys.
     __device__ __forceinline__ uint64_t find_tie(const Row &r, float low, float high, double before, double goal, bool by_mass)
     {
         const int64_t per = segment_size();
-        uint32_t prefix = 0, top = 0, bottom = 0;
-        each([&](int64_t, const float(&x)[kEight]) {
-#pragma unroll
-            for (int i = 0; i < kEight; i++) {
-                const uint32_t key = x[i] >= low && x[i] <= high ? key_of(x[i]) : 0u;
-                top = max(top, key);
-                bottom = max(bottom, key ? ~key : 0u);
-            }
-        });
-        top = block_max(top);
-        bottom = ~block_max(bottom);
-        auto tie = [&](float v, uint32_t) { return key_of(v) == prefix ? 1.0 : 0.0; };
-        double ties = 0.0, w = 1.0;
-        if (top == bottom) {
-            prefix = top;
-            w = by_mass ? r.weight(score_of(prefix)) : 1.0;
-            ties = segment_sums(per, tie);
-        }
-        if (top != bottom || before + ties * w < goal) {
-            const double fixed = by_mass ? fixed_point() : 1.0;
-            double run = before * fixed;
-            uint32_t known = 0;
-            prefix = 0;
+        const float inf = __builtin_inff(), least = -3.402823466e+38f;
+        uint32_t *const ends = reinterpret_cast<uint32_t *>(lds.list);     // each part's highest key, and the complements of the lowest ones
+        uint32_t top, bottom;
+        double run, w, ties;
+        auto tie = [&](float v, uint32_t) { return key_of(v) == top ? 1.0 : 0.0; };
 #pragma unroll 1
-            for (int shift = 32; shift > 0;) {
-                const int bits = min(10, shift), to = shift - bits;
-                const uint32_t mask = (1u << bits) - 1u;
+        for (bool again = true; again;) {
+            again = false;
+            uint32_t most = 0, fewest = 0;
+            each([&](int64_t, const float(&x)[kEight]) {
+#pragma unroll
+                for (int i = 0; i < kEight; i++) {
+                    const uint32_t key = x[i] >= low && x[i] <= high ? key_of(x[i]) : 0u;
+                    most = max(most, key);
+                    fewest = max(fewest, key ? ~key : 0u);
+                }
+            });
+            top = block_max(most);
+            bottom = ~block_max(fewest);
+            run = before;
+            if (top == 0 || (by_mass && r.logarithm(score_of(top)) <= kNothing)) {      // nothing here, or of no weight
+                return high < inf ? (uint64_t)(key_of(high) + 1) << 32 : 0;
+            }
+            bool first = low > least;
+#pragma unroll 1
+            while (top > bottom) {
+                const double from = by_mass ? r.logarithm(score_of(top)) : 0.0;
+                const double range = by_mass ? from - fmax(r.logarithm(score_of(bottom)), kNothing) : 0.0;
+                const bool by_size = range > 8.0;      // once: a part of them is narrower than 1
+                const double width = range / kDigits, unit = by_size ? kDigits / range : 0.0;
+                const int shift = max(0, 32 - __builtin_clz(top - bottom) - 10);
+                auto highest = [&](int part) { return by_size ? from - part * width : from; };
                 __syncthreads();
                 for (int i = tid; i < kDigits; i += NT) {
-                    lds.tally[i] = 0;
+                    lds.tally[i] = lds.tally[kDigits + i] = 0;
+                    ends[i] = ends[kDigits + i] = 0;
                 }
                 __syncthreads();
                 each([&](int64_t, const float(&x)[kEight]) {
 #pragma unroll
                     for (int i = 0; i < kEight; i++) {
                         const uint32_t key = key_of(x[i]);
-                        if (key && x[i] <= high && (key & known) == prefix) {
-                            // integers: in any order; the largest scores first
-                            atomicAdd(&lds.tally[~(key >> to) & mask],
-                                      by_mass ? (unsigned long long)__builtin_rint(r.weight(x[i]) * fixed) : 1ull);
+                        if (key < bottom || key > top) {
+                            continue;
+                        }
+                        if (!by_mass) {
+                            atomicAdd(&lds.tally[(top - key) >> shift], 1ull);
+                            continue;
+                        }
+                        const double t = r.logarithm(x[i]);
+                        if (t <= kNothing) {
+                            continue;
+                        }
+                        const int part = by_size ? min(kDigits - 1, (int)((from - t) * unit)) : (int)((top - key) >> shift);
+                        const double v = power_of_two(t - highest(part)) * 0x1p31;
+                        const uint32_t whole = (uint32_t)v;
+                        atomicAdd(&lds.tally[part], (unsigned long long)whole);
+                        atomicAdd(&lds.tally[kDigits + part], (unsigned long long)(uint32_t)((v - whole) * 0x1p31));
+                        if (by_size) {
+                            atomicMax(&ends[part], key);
+                            atomicMax(&ends[kDigits + part], ~key);
                         }
                     }
                 });
-                prefix |= (~(uint32_t)cross<kDigits>([&](int b) { return (double)lds.tally[b]; }, goal * fixed, run) & mask) << to;
-                known |= mask << to;
-                shift = to;
+                auto sum = [&](int part) {
+                    return by_mass ? ((double)lds.tally[part] * 0x1p-31 + (double)lds.tally[kDigits + part] * 0x1p-62) *
+                                         power_of_two(highest(part))
+                                   : (double)lds.tally[part];
+                };
+                const int part = cross<kDigits>(sum, goal, run);
+                if (first && run + sum(part) < goal) {
+                    again = true;
+                    break;
+                }
+                first = false;
+                if (by_size) {
+                    top = ends[part];
+                    bottom = ~ends[kDigits + part];
+                } else {
+                    const uint32_t size = (1u << shift) - 1u;
+                    top -= (uint32_t)part << shift;
+                    bottom = top - bottom > size ? top - size : bottom;
+                }
             }
-            before = run / fixed;
-            w = by_mass ? r.weight(score_of(prefix)) : 1.0;
-            ties = segment_sums(per, tie);
+            if (!again) {
+                w = by_mass ? r.weight(score_of(top)) : 1.0;
+                ties = segment_sums(per, tie);
+                again = first && run + ties * w < goal;
+            }
+            low = least;
         }
-        const double take = fmax(1.0, fmin(ties, w > 0.0 ? ceil((goal - before) / w) : ties));
+        const double take = fmax(1.0, fmin(ties, w > 0.0 ? ceil((goal - run) / w) : ties));
         int64_t at;
         double one;
         locate(per, take - 0.5, tie, at, one);
         __syncthreads();
-        return r.place(prefix, (uint32_t)at);
+        return r.place(top, (uint32_t)at);
     }
 
     __device__ __forceinline__ int64_t segment_size() const
