@@ -524,12 +524,6 @@ struct Sampler {
         return total;
     }
 
-    // what weights of up to 1 are multiplied by to be integers of which n can be added up
-    __device__ __forceinline__ double fixed_point() const
-    {
-        return __builtin_ldexp(1.0, 62 - (64 - __builtin_clzll((unsigned long long)n)));
-    }
-
     // The first of BINS bins at which the running sum of value(bin), with `before` in front of the first, reaches `goal`, or the last
     // with a value; `before` becomes the sum in front of it.
     template <int BINS, typename F>
@@ -697,10 +691,11 @@ struct Sampler {
         take = max(take, min(1, m));
         // an empty list: everything above it is kept, or everything that is there
         const uint64_t place = m > 0 ? lds.list[take - 1] : before >= goal ? (uint64_t)(key_of(high) + 1) << 32 : 0;
-        // to the segments, as integers: their sums do not depend on an order
+        // to the segments, as integers: their sums do not depend on an order.  Up to kList weights of at most the first one's size.
         const int64_t columns = per * kBlock;
         const int segments = (int)((blocks() + per - 1) / per);
-        const double fixed = fixed_point();
+        const double largest = m > 0 ? r.weight(score_of((uint32_t)(lds.list[0] >> 32))) : 0.0;
+        const double fixed = largest > 0.0 ? 0x1p51 / largest : 0.0;
         __syncthreads();       // the list's sums have been read: the tallies take their place
         for (int g = tid; g < segments; g += NT) {
             lds.tally[g] = 0;
@@ -713,7 +708,7 @@ struct Sampler {
         }
         __syncthreads();
         for (int g = tid; g < segments; g += NT) {
-            lds.segment[g] += (double)lds.tally[g] / fixed;
+            lds.segment[g] += (double)lds.tally[g] * (largest * 0x1p-51);
         }
         total = segment_total(segments);
         summed = true;

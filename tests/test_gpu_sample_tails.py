@@ -69,10 +69,17 @@ def peak_and_tail(n, low, high, seed, last=True):
 @pytest.mark.parametrize("rows,n,low,high,top_p", [
     (2, 131_072, -27.75, -27.73, 1 - 2.0 ** -24), (130, 131_072, -27.75, -27.73, 1 - 2.0 ** -24), (1, 2 ** 21, -29.0, -28.9, 0.9999999),
     (1, 2 ** 22, -28.51, -28.49, 0.9999995), (1, 2 ** 24 - 3, -27.01, -26.99, 0.99999), (129, 300_001, -26.0, -25.95, 0.9999999),
-    (130, 60_000, -24.02, -24.0, 0.9999997), (2, 60_000, -24.02, -24.0, 0.9999997)])
+    (3, 1_000_003, -29.0, -25.0, 0.9999999), (130, 60_000, -24.02, -24.0, 0.9999997), (2, 60_000, -24.02, -24.0, 0.9999997)])
 @pytest.mark.parametrize("last", [True, False])
 def test_a_peak_over_a_flat_tail(lib, rows, n, low, high, top_p, last):  # noqa: F811
     check(lib, peak_and_tail(n, low, high, n, last), "f32", rows, top_p=top_p)
+
+
+@pytest.mark.parametrize("rows", [1, 130])
+def test_a_cut_in_a_short_list_of_small_weights(lib, rows):  # noqa: F811
+    """The list holds all that lie around the cut: their sums go to the segments."""
+    check(lib, peak_and_tail(2 ** 20, -36.7, -27.7, 3), "f32", rows, top_p=1 - 2.0 ** -24)
+    check(lib, peak_and_tail(131_072, -36.0, -25.0, 4), "f32", rows, top_p=1 - 2.0 ** -24)
 
 
 @pytest.mark.parametrize("rows", [2, 130])
