@@ -751,17 +751,23 @@ template <int P, int SG, bool WIDE, int W>
 void launch_stream(const GroupProductParams &p, hipStream_t s)
 {
     const bool narrow = p.n <= 32768, deep = narrow && p.steps >= 8;
+    // up to 16 rows of fewer than eight steps need no eight wavefronts: they have 56 KB of pieces at most
+    constexpr bool kShallow = W == 4;
     if (p.m <= 4) {
         if (deep) {
             launch_stream<P, 1, 1, 1, 4, 4, SG, WIDE, W>(p, s);
-        } else {
-            narrow ? launch_stream<P, 1, 1, 1, 4, 1, SG, WIDE, W>(p, s) : launch_stream<P, 1, 1, 2, 2, 1, SG, WIDE, W>(p, s);
+        } else if (!narrow) {
+            launch_stream<P, 1, 1, 2, 2, 1, SG, WIDE, W>(p, s);
+        } else if constexpr (kShallow) {
+            launch_stream<P, 1, 1, 1, 4, 1, SG, WIDE, W>(p, s);
         }
     } else if (p.m <= 16) {
         if (deep) {
             launch_stream<P, 1, 4, 1, 4, 4, SG, WIDE, W>(p, s);
-        } else {
-            narrow ? launch_stream<P, 1, 4, 1, 4, 1, SG, WIDE, W>(p, s) : launch_stream<P, 1, 4, 2, 2, 1, SG, WIDE, W>(p, s);
+        } else if (!narrow) {
+            launch_stream<P, 1, 4, 2, 2, 1, SG, WIDE, W>(p, s);
+        } else if constexpr (kShallow) {
+            launch_stream<P, 1, 4, 1, 4, 1, SG, WIDE, W>(p, s);
         }
     } else if (p.m <= 32) {
         narrow ? launch_stream<P, 2, 4, 1, 4, 1, SG, WIDE, W>(p, s) : launch_stream<P, 2, 4, 4, 1, 1, SG, WIDE, W>(p, s);
