@@ -63,13 +63,13 @@ WIDE = [("f32", 3, 9000), ("f32", 4, 4700), ("f32", 1, 16_384), ("bf16", 4, 9300
         ("f32", 33, 600), ("bf16", 40, 1000), ("f16", 64, 1024), ("bf16", 63, 897), ("bf16", 48, 768), ("f16", 48, 700)]
 # and less
 FEW = [("f32", 16, 500), ("bf16", 5, 300), ("f16", 9, 1100), ("bf16", 16, 2050), ("f32", 8, 130), ("f32", 20, 300), ("bf16", 30, 700),
-       ("f32", 50, 200), ("f16", 64, 500)]
+       ("f32", 50, 200), ("f16", 64, 500), ("bf16", 3, 1100), ("f32", 6, 1100)]
 
 
-@pytest.mark.parametrize("group,scale,zeros", [(32, "f16", True), (64, "f32", False), (128, "bf16", True), (32, "f32", False), (64, "bf16", True)])
-@pytest.mark.parametrize("n", [300, 33_003])
-@pytest.mark.parametrize("kind,m,d", WIDE + FEW)
-def test_rows_that_stay(lib, kind, m, d, n, group, scale, zeros):  # noqa: F811
+GROUPS = [(32, "f16", True), (64, "f32", False), (128, "bf16", True), (32, "f32", False), (64, "bf16", True), (128, "f32", True)]
+
+
+def compare(lib, kind, m, d, n, group, scale, zeros):  # noqa: F811
     rng = np.random.default_rng(m * n + d)
     store = Store(n, d, group, scale, zeros)
     size = n * store.ng
@@ -82,6 +82,20 @@ def test_rows_that_stay(lib, kind, m, d, n, group, scale, zeros):  # noqa: F811
     check(lib, x, kind, store)
     if n < 1000:
         check(lib, x, kind, store, "bf16")
+
+
+@pytest.mark.parametrize("group,scale,zeros", GROUPS)
+@pytest.mark.parametrize("n", [300, 33_003])
+@pytest.mark.parametrize("kind,m,d", WIDE + FEW)
+def test_rows_that_stay(lib, kind, m, d, n, group, scale, zeros):  # noqa: F811
+    compare(lib, kind, m, d, n, group, scale, zeros)
+
+
+@pytest.mark.parametrize("group,scale,zeros", GROUPS)
+@pytest.mark.parametrize("kind,m,n,d", [("f32", 64, 300, 2100), ("bf16", 50, 257, 5000), ("f16", 33, 513, 6001), ("f32", 130, 257, 200),
+                                        ("bf16", 200, 70, 1100), ("f16", 65, 300, 129)])
+def test_rows_in_tiles(lib, kind, m, n, d, group, scale, zeros):  # noqa: F811
+    compare(lib, kind, m, d, n, group, scale, zeros)
 
 
 def test_values_are_those_of_the_definition(lib):  # noqa: F811
