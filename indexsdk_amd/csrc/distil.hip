@@ -185,6 +185,21 @@ __device__ Sum sum_of(const DistilParams &p, const T *row, int64_t from, int64_t
     return joined<NT>(mine, p, box);
 }
 
+// v as 32 bits that are rounded to T next: for 16-bit types toward zero with the last bit set if anything was lost, which gives what rounding
+// v itself would.
+template <typename T>
+__device__ __forceinline__ float before_rounding(double v)
+{
+    const float f = (float)v;
+    if constexpr (sizeof(T) == 4) {
+        return f;
+    } else {
+        const double lost = v - (double)f;
+        const uint32_t bits = __float_as_uint(f);
+        return fabs(lost) > 0.0 ? __uint_as_float((bits - ((lost < 0.0) != ((int)bits < 0) ? 1u : 0u)) | 1u) : f;
+    }
+}
+
 // The teacher's entries of rows, in LDS.  A crew works on them: the first wavefront, without a barrier, while the others go on; or
 // where there are many the whole workgroup.  Its thread j has entries j, j + threads() ...
 template <int NT>
@@ -324,6 +339,7 @@ struct Entries {
     __device__ __forceinline__ bool is_first(int j, int column) const { return first[place((uint32_t)column, false)] == (uint32_t)j; }
 
     // The gradient at the labels in from ... to - 1: unit (P q - sum of p)
+    template <typename T>
     __device__ __forceinline__ void differentiate(const Buffer &b, const DistilParams &p, int64_t from, int64_t to, float reference,
                                                   float sum, double whole, double unit) const
     {
@@ -354,7 +370,7 @@ struct Entries {
                     }
                 }
                 const double q = any_power_of_two(((double)b.value[j] - (double)reference) * p.scale) * share;
-                b.value[j] = (float)(unit * (q - prob));
+                b.value[j] = before_rounding<T>(unit * (q - prob));
             }
         }
     }
@@ -481,7 +497,7 @@ __global__ __launch_bounds__(kThreads) void distil_gradient_kernel(DistilParams 
     __syncthreads();       // the scores at labels have been read: the gradient may take their place
     const Gradient<T> all(p, row, p.given_stats[row * 2], p.given_stats[row * 2 + 1], whole);
     if (entries.crew() && !all.nothing) {
-        entries.differentiate(entries.buffer(0), p, from, to, all.exponent.reference, all.sum, whole, all.unit);
+        entries.template differentiate<T>(entries.buffer(0), p, from, to, all.exponent.reference, all.sum, whole, all.unit);
     }
     for (int64_t at = from; at < to; at += kPart) {
 #pragma unroll
@@ -593,7 +609,7 @@ __global__ __launch_bounds__(NT, 4) void distil_row_kernel(DistilParams p)
             const auto buffer = entries.buffer(which);
             entries.write_loss(buffer, p, row, all);
             if (!g.nothing) {
-                entries.differentiate(buffer, p, 0, p.n, g.exponent.reference, g.sum, mass, g.unit);
+                entries.template differentiate<T>(buffer, p, 0, p.n, g.exponent.reference, g.sum, mass, g.unit);
             }
             if (next < p.rows) {
                 load_entries(next, which ^ 1);
