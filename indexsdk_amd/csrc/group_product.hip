@@ -694,7 +694,8 @@ __global__ __launch_bounds__(256, 2) void group_tile_kernel(GroupProductParams p
     }
 }
 
-// Fewer than four scales in all (up to three short rows of codes): a thread per score.
+// Fewer than four scales in all (up to three short rows of codes): a thread per score.  Sums before the scale are of x times its power of
+// two here too, or they could pass the largest number where the score does not.
 __global__ __launch_bounds__(256) void group_tiny_kernel(GroupProductParams p, int group)
 {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / p.n, col = id - row * p.n;
@@ -702,6 +703,13 @@ __global__ __launch_bounds__(256) void group_tiny_kernel(GroupProductParams p, i
         return;
     }
     const uint8_t *const x_row = static_cast<const uint8_t *>(p.x) + (size_t)row * (size_t)p.ld_x * (p.type == kTypeF32 ? 4 : 2);
+    int top = 0;
+    for (int at = 0; p.type != kTypeF16 && at < p.d; at += kEight) {
+        float v[kEight];
+        load_eight(x_row, p.type, at, p.d, v);
+        top = max(top, finite_top(v));
+    }
+    const int power = power_for(top);
     float sum = 0.f, of_group = 0.f;
     for (int at = 0; at < p.d; at += kEight) {
         const int64_t slot = col * p.groups + at / group;
@@ -711,7 +719,7 @@ __global__ __launch_bounds__(256) void group_tiny_kernel(GroupProductParams p, i
         load_eight(x_row, p.type, at, p.d, v);
 #pragma unroll
         for (int i = 0; i < kEight; i++) {
-            of_group += at + i < p.d ? v[i] * ((float)(code >> (4 * i) & 15u) - zero) : 0.f;
+            of_group += at + i < p.d ? ldexpf(v[i], power) * ((float)(code >> (4 * i) & 15u) - zero) : 0.f;
         }
         if ((at + kEight) % group == 0 || at + kEight >= p.d) {
             const float scale = p.scale_type == kTypeF32   ? static_cast<const float *>(p.scales)[slot]
@@ -724,7 +732,7 @@ __global__ __launch_bounds__(256) void group_tiny_kernel(GroupProductParams p, i
     const float sums[1] = {sum};
     float bias[1];
     load_bias(p, col, bias);
-    store_scores(p, row, 0, col, sums, bias);
+    store_scores(p, row, power, col, sums, bias);
 }
 
 int pieces_of(int type) { return type == kTypeF32 ? 2 : 1; }
