@@ -1186,6 +1186,12 @@ __device__ __forceinline__ void finish_row(Sampler<T, NT> &k, const SampleParams
     }
     const int64_t per = k.segment_size(), count = set.count;
     Row r(set.scale, score_of(set.filtered || !h.fine ? h.top : h.reference), set.min_p);
+    if (!set.filtered && h.fine) {
+        // weights count as 0 by what they are next to those of the best, not of the reference: scores of at most `border` are cut off
+        const double border = (double)score_of(h.top) + kNothing / set.scale;
+        const float nearest = (float)border;
+        r.least = (uint64_t)min(key_of(nearest) + ((double)nearest > border ? 0u : 1u), h.top) << 32;
+    }
     if (set.need_mass && !h.fine) {
         total = k.segment_sums(per, [&](float x, uint32_t) { return key_of(x) ? r.weight(x) : 0.0; });
     }
