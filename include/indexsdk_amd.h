@@ -241,8 +241,9 @@ int ixa_op_group_product(const void *x_dev, int64_t ld_x, int type, int64_t m, c
  * With weights w = exp((score - best) / T), the columns in the order of falling scores, equal ones in that of columns, are cut to
  * the first k, then to the fewest whose weights reach p of the sum of those that are left, then to those with w >= m.  The
  * draw's label is the first column, in the order of columns, at which the running sum of the weights that are left passes
- * uniform * their total; its probability w / total goes to probs [rows][draws] (may be NULL).  Weights and sums are held in 64 bits; weights below 2^-960 count as 0.  Beside a
- * score of +infinity only such columns count.  A row without a column: label -1, probability 0.
+ * uniform * their total; its probability w / total goes to probs [rows][draws] (may be NULL).  Weights and sums are held in 64 bits, right
+ * to 10^-13: a border nearer than that to a running sum may go to either side of it.  Weights below 2^-960 count as 0.  Beside a
+ * score of +infinity only such columns count.  A row without a column (n = 0 too): label -1, probability 0.
  * rows <= 2^22, n < 2^31, draws <= 2^20. */
 int ixa_sample_workspace(int64_t rows, int64_t n, int64_t *bytes);
 int ixa_op_sample(const void *scores_dev, int64_t ld, int type, int64_t rows, int64_t n, const float *temperature_dev,
@@ -258,7 +259,8 @@ int ixa_op_sample(const void *scores_dev, int64_t ld, int type, int64_t rows, in
  *         label_j = i)
  * for the weight of the row, row_weight [rows] (NULL: 1; the upstream gradient of its loss).  A label may come more than once.  Scores
  * of -infinity are columns that are masked out: gradient 0, unless a label asks for them (loss +infinity).  Rows without an entry or
- * without a score have loss and gradient 0; a NaN or a score of +infinity makes its row's NaN.
+ * without a score have loss and gradient 0, a row without an entry also beside a NaN; a NaN or a score of +infinity makes those of
+ * any other row NaN.
  * ixa_op_distil_loss writes loss [rows] and, if not NULL, stats [rows][2], the largest score and the sum of exponentials relative
  * to it, from which ixa_op_distil_gradient writes gradient [rows][ld_gradient], of the scores' type, rounded once.
  * ixa_op_distil_step does both.  The gradient may take the scores' place (same address and stride), or shares no element with

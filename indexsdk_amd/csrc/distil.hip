@@ -761,7 +761,8 @@ void run_rows(const DistilTask &t, const float *row_weight, float *loss, void *g
 
 // Rows that fit into a workgroup's registers, 256 bytes of each thread's, are read once.  From 2048 rows on a wavefront or two of
 // them take a row (4096 rows of 8192 bf16: 38.5 us, 47.2 with 256 threads; 1024 rows: 20.0 and 17.6), but not where there is more to do
-// about the labels.  A few rows of more than 8192 go in parts, as longer ones do (64 rows of 131072 bf16: 21.1 us, 23.8 in registers).
+// about the labels.  Fewer than 128 rows of more than 8192 go in parts, as longer ones do (32 rows of 131072 bf16: 18.2 us, 20.8 in registers, 64 rows
+// 20.5 and 20.4, 128 rows 30.8 and 20.3; 96 rows of 32768 fp32 16.4 and 17.6, 160 rows 19.6 and 16.6; but 64 rows of 9000 fp32 19.8 and 14.2).
 bool in_rows(const DistilTask &t, const float *row_weight, float *loss, void *gradient, int64_t ld_gradient, hipStream_t s)
 {
     const int64_t threads = (t.n + 127) / 128 * (int64_t)(element_bytes(t.type) / 2);

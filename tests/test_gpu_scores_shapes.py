@@ -36,6 +36,23 @@ def test_distillation_of_rows_in_registers(lib, kind, rows, n, k):  # noqa: F811
     assert torch.equal(both.nan_to_num(7.0), value.nan_to_num(7.0)) and torch.equal(dev.nan_to_num(7.0), out[:rows].nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", [(4, 5), (4, 300), (200, 20_000), (4, 30_000)])
+def test_rows_without_an_entry_have_no_loss_whatever_is_in_them(lib, rows, n, kind):  # noqa: F811
+    x, labels, teacher = distil.task(4, n, 3, n)
+    x[0, n // 2], x[1, 0], x[2] = np.nan, np.inf, np.nan
+    labels[:] = -1
+    of = torch.arange(rows, device="cuda") % 4
+    dev, dl = distil.rows_of(x, kind)[of], torch.from_numpy(labels).cuda()[of].contiguous()
+    dt = torch.from_numpy(teacher.astype(np.float32)).cuda()[of].contiguous()
+    out = torch.full((rows, n), 5.0, dtype=dev.dtype, device="cuda")
+    assert (distil.step(lib, dev, kind, dl, dt, None, 1.0, None, out)[:rows] == 0).all() and (out == 0).all()
+    value, stats = distil.loss(lib, dev, kind, dl, dt, None, 1.0)
+    out.fill_(5)
+    distil.gradient(lib, dev, kind, dl, dt, None, 1.0, stats, None, out)
+    assert (value[:rows] == 0).all() and (out == 0).all()
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("filters", [dict(), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.05), dict(top_k=5000, top_p=0.7)], ids=str)
 @pytest.mark.parametrize("rows,n", [(2, 40_000), (150, 33_001)])
