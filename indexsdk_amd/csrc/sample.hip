@@ -16,8 +16,8 @@
 // finds the bins around the cut, whose columns go through the list while the weights above them are added up; where these are more than it
 // holds, sums over parts of their range of scores find the part with the cut, which is divided again.
 //
-// What bounds it: one read of the scores where k cuts (1024 rows of 100003 bf16: 67 us, 3.1 TB/s), the exponentials in 64 bits where
-// all of a row's are needed (without filters 99 us, with top-p 134 us, with settings that leave every fifth row flat 190 us), and
+// What bounds it: one read of the scores where k cuts (1024 rows of 100003 bf16, four draws each: 74 us, 2.8 TB/s), the exponentials in 64 bits where
+// all of a row's are needed (without filters 105 us, with top-p 134 us, with settings that leave every fifth row flat 190 us), and
 // for a few rows the steps of one workgroup that wait for each other (a row of 32768 fp32 under all filters: 13 us).
 #include "power_of_two.h"
 #include "row_access.h"
@@ -1460,7 +1460,7 @@ __global__ __launch_bounds__(kPartThreads, 4) void sample_join_kernel(SamplePara
 }
 
 // Parts of each row where there are few rows: as many as give every CU two workgroups, of 16384 columns at least.  Rows of 131072 fp32
-// scores under top-p: one takes 26 us, 40 as a whole; 64 take 46 us, 60 as whole rows; 256 would take 67 us, 66 as whole rows.
+// scores under top-p: one takes 26 us, 40 as a whole; 64 take 46 us, 60 as whole rows; 256 would take 64 us, 61 as whole rows.
 int parts_of(int64_t rows, int64_t n)
 {
     if (rows == 0 || rows > 128 || n < 65536) {
