@@ -3,6 +3,10 @@
 #pragma once
 #include "common.h"
 
+#include <algorithm>
+#include <map>
+#include <tuple>
+
 namespace ixa {
 
 // Element types of float rows and of results.
@@ -81,5 +85,23 @@ inline void check_answer(hipError_t e)
 }
 // after a launch
 inline void check_launch() { check_answer(hipGetLastError()); }
+
+// Workgroups of a kernel that the current device runs at a time: devices and partitions differ in their CUs.
+inline int64_t resident_workgroups(const void *kern, int threads, size_t lds)
+{
+    static std::mutex mu;
+    static std::map<std::tuple<int, const void *, int, size_t>, int64_t> known;
+    int device;
+    IXA_HIP(hipGetDevice(&device));
+    std::lock_guard<std::mutex> lock(mu);
+    int64_t &count = known[std::make_tuple(device, kern, threads, lds)];
+    if (count == 0) {
+        int per_cu = 0, cus = 0;
+        IXA_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, threads, lds));
+        IXA_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
+        count = (int64_t)std::max(1, per_cu) * std::max(1, cus);
+    }
+    return count;
+}
 
 }  // namespace ixa

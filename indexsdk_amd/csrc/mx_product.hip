@@ -15,9 +15,6 @@
 #include "lowp.h"
 
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <tuple>
 #include <type_traits>
 
 namespace ixa {
@@ -801,24 +798,6 @@ __global__ __launch_bounds__(256, 1) void mx_wide_kernel(ProductParams p, int ro
 }
 
 bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-
-// Workgroups of a kernel that the current device runs at a time: devices and partitions differ in their CUs.
-int64_t resident_workgroups(const void *kern, int threads, size_t lds)
-{
-    static std::mutex mu;
-    static std::map<std::tuple<int, const void *, int, size_t>, int64_t> known;
-    int device;
-    IXA_HIP(hipGetDevice(&device));
-    std::lock_guard<std::mutex> lock(mu);
-    int64_t &count = known[std::make_tuple(device, kern, threads, lds)];
-    if (count == 0) {
-        int per_cu = 0, cus = 0;
-        IXA_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, threads, lds));
-        IXA_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
-        count = (int64_t)std::max(1, per_cu) * std::max(1, cus);
-    }
-    return count;
-}
 
 template <int FA>
 size_t stream_lds(int64_t m, int pieces, int steps)

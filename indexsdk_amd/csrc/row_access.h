@@ -3,9 +3,6 @@
 #include "lowp.h"
 
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <tuple>
 
 namespace ixa {
 
@@ -145,24 +142,6 @@ inline bool rows_collide(const void *out, int64_t ld_out, const void *in, int64_
     }
     const __int128 step = size * ld_in, apart = (a > b ? a - b : b - a) % step;
     return a != b && (apart < row || apart > step - row);
-}
-
-// Workgroups of a kernel that the current device runs at a time: devices and partitions differ in their CUs.
-inline int64_t resident_workgroups(const void *kern, int threads, size_t lds)
-{
-    static std::mutex mu;
-    static std::map<std::tuple<int, const void *, int, size_t>, int64_t> known;
-    int device;
-    IXA_HIP(hipGetDevice(&device));
-    std::lock_guard<std::mutex> lock(mu);
-    int64_t &count = known[std::make_tuple(device, kern, threads, lds)];
-    if (count == 0) {
-        int per_cu = 0, cus = 0;
-        IXA_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, threads, lds));
-        IXA_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
-        count = (int64_t)std::max(1, per_cu) * std::max(1, cus);
-    }
-    return count;
 }
 
 // A kernel for each element type.
